@@ -53,6 +53,7 @@ struct KernelStep {
 struct CopyStep {
   int src = -1, dst = -1;
   uint64_t bytes = 0;
+  bool unless_same = false;  // nothing to copy where both slots are bound to one buffer (an update in place)
 };
 
 struct Plan;
@@ -79,6 +80,8 @@ struct Plan {
   std::vector<Step> steps;
   std::vector<int> input_slots;   // per parameter
   std::vector<int> output_slots;  // per program output
+  // (input, output) positions that a caller may bind to one buffer: the output is the input updated in place.
+  std::vector<std::pair<size_t, size_t>> updates;
 };
 
 class TuningTable;

@@ -47,6 +47,7 @@ Plan Planner::run() {
   }
   match_attentions();
   mark_gemm_operands();
+  mark_custom_operands();
   for (uint32_t v = 0; v < n; ++v) {
     if (!live_[v] || done_[v]) continue;
     process(v);
@@ -80,7 +81,8 @@ void Planner::process(uint32_t v) {
     case Kind::scatter_add: scatter_add(v); break;
     case Kind::scan: scan(v); break;
     case Kind::projection: break;  // written by its scan's loop step
-    case Kind::custom_call: case Kind::sparse_cross_entropy:  // sparse_cross_entropy is expanded before planning
+    case Kind::custom_call: custom(v); break;
+    case Kind::sparse_cross_entropy:  // expanded before planning
       fail(Err::Unsupported, std::string(kind_name(op.kind)) + " is not supported by the HIP target");
     default:
       if (needed_[v]) map(v);

@@ -3,7 +3,7 @@
 // launch tuning, serial contractions and scatter_add; planner_reduce.cpp the folds and row kernels;
 // planner_views.cpp strided views and materialised transposes; planner_contraction.cpp the matrix-core
 // contractions, grouped launches and epilogues; planner_attention.cpp the fused attention matcher and
-// kernels. The fusion rules and their references are described in lower.cpp.
+// kernels; planner_mx4.cpp the custom calls of microscaled 4-bit floats. The fusion rules and their references are described in lower.cpp.
 #pragma once
 
 #include <algorithm>
@@ -598,6 +598,31 @@ class Planner {
 
   // ---- scatter_add: one pass over the table, every row's updates added in order ----
   void scatter_add(uint32_t v);
+
+  // ---- custom calls of this target: microscaled 4-bit floats (kernels/mx4.h) ----
+  //
+  // "accy.mx4.<name>", version 1; operands and results are checked against what the name takes (Unsupported with the
+  // reason otherwise, as for every other custom call).
+  void custom(uint32_t v);
+
+  // The value whose buffer holds v's elements in v's own order: v itself, or what it is a reshape of.
+  uint32_t dense_source(uint32_t v) const;
+  int dense_slot(uint32_t v);
+  // Operands of custom calls that must be in memory are materialised by the kernel that produces them.
+  void mark_custom_operands();
+
+  void mx4_quantize(uint32_t v);
+  void mx4_values(uint32_t v);
+  void mx4_contract(uint32_t v);
+  void mx4_cache_write(uint32_t v);
+  void mx4_cache_read(uint32_t v, bool value);
+  void mx4_attend(uint32_t v);
+  // The members of a cache kernel's configuration, from the cache and the rows' head dimension; fails where they do not fit.
+  struct Mx4Cache {
+    int64_t pages = 0, heads = 0, tokens = 0, dim = 0;
+    std::string members(DType d) const;
+  };
+  Mx4Cache mx4_cache(const Op& op, uint32_t cache, int64_t heads, int64_t dim) const;
 };
 
 }  // namespace planning

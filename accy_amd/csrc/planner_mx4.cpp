@@ -1,0 +1,460 @@
+// Custom calls of this target: microscaled 4-bit floats (kernels/mx4.h). A program names them "accy.mx4.<name>", version 1:
+//
+//   codes(x), scales(x)                    x [.., K] -> u8 [.., K / 2] and u8 [.., K / 32], planned as one kernel
+//   values(codes, scales)                  -> [.., K]
+//   contract(codes, scales, codes, scales) [rows .., K / 2] .. and [columns .., K / 2] .. -> [rows .., columns ..]
+//   cache_write(cache, keys, values, slots) -> the cache with the rows of the tokens' slots replaced
+//   cache_keys(cache, slots), cache_values  -> [slots .., kv_head, dim]
+//   attend(q, cache, pages, lengths)        q [seq, (query,) head, dim] -> the same
+//
+// Float operands and results are bf16, f16 or f32. The wire carries a custom call's result type, so everything about it is
+// checked here.
+#include "planner_internal.hpp"
+
+namespace accy {
+namespace planning {
+
+namespace {
+
+[[noreturn]] void refuse(const Op& op, const std::string& why) {
+  fail(Err::Unsupported, "custom_call " + op.bytes + ": " + why);
+}
+
+void require(bool ok, const Op& op, const std::string& why) {
+  if (!ok) refuse(op, why);
+}
+
+// DT of kernels/mx4.h.
+int element_type(const Op& op, DType d) {
+  switch (d) {
+    case DType::bf16: return 0;
+    case DType::f16: return 1;
+    case DType::f32: return 2;
+    default: refuse(op, std::string(dtype_name(d)) + " values (bf16, f16 or f32)");
+  }
+}
+
+int64_t last(const Type& t) { return t.rank() ? t.dims.back().extent : 0; }
+
+// The extents of a's leading axes are b's.
+bool same_rows(const Type& a, const Type& b) {
+  if (a.rank() != b.rank()) return false;
+  for (size_t i = 0; i + 1 < a.rank(); ++i)
+    if (a.dims[i].extent != b.dims[i].extent) return false;
+  return true;
+}
+
+// Codes and scales of one tensor: the elements along its blocked axis.
+int64_t blocked(const Op& op, const Type& codes, const Type& scales) {
+  require(codes.dtype == DType::u8 && scales.dtype == DType::u8, op, "codes and scales are u8");
+  require(codes.rank() >= 1 && same_rows(codes, scales), op, "codes and scales of different rows");
+  const int64_t k = last(codes) * 2;
+  require(k % 32 == 0 && last(scales) == k / 32, op, "K / 2 codes and K / 32 scales to a row, K a multiple of 32");
+  return k;
+}
+
+std::string num(int64_t n) { return std::to_string(n); }
+
+}  // namespace
+
+void Planner::custom(uint32_t v) {
+  const Op& op = g_.ops[v];
+  const std::string prefix = "accy.mx4.";
+  const std::string what = op.bytes.compare(0, prefix.size(), prefix) == 0 ? op.bytes.substr(prefix.size()) : "";
+  auto operands = [&](size_t n) { require(op.args.size() == n, op, num((int64_t)n) + " operands"); };
+  if (op.index == 1) {
+    if (what == "codes" || what == "scales") return operands(1), mx4_quantize(v);
+    if (what == "values") return operands(2), mx4_values(v);
+    if (what == "contract") return operands(4), mx4_contract(v);
+    if (what == "cache_write") return operands(4), mx4_cache_write(v);
+    if (what == "cache_keys" || what == "cache_values") return operands(2), mx4_cache_read(v, what == "cache_values");
+    if (what == "attend") return operands(4), mx4_attend(v);
+  }
+  fail(Err::Unsupported, "custom_call " + op.bytes + " version " + std::to_string(op.index) + " is not supported by the HIP target");
+}
+
+uint32_t Planner::dense_source(uint32_t v) const {
+  while (g_.ops[v].kind == Kind::reshape && slots_.slot_of[v] < 0) v = g_.ops[v].args[0];
+  return v;
+}
+
+int Planner::dense_slot(uint32_t v) { return materialize(dense_source(v)); }
+
+void Planner::mark_custom_operands() {
+  for (uint32_t v = 0; v < g_.ops.size(); ++v) {
+    const Op& op = g_.ops[v];
+    if (!live_[v] || op.kind != Kind::custom_call) continue;
+    // A quantised tensor is evaluated inside the kernel that quantises it.
+    if (op.args.size() == 1) continue;
+    for (uint32_t a : op.args) {
+      const uint32_t s = dense_source(a);
+      if (is_inlinable(g_.ops[s].kind)) needed_[s] = true;
+    }
+  }
+}
+
+// ---- codes and scales: eight values per thread, four lanes to a block ----
+
+void Planner::mx4_quantize(uint32_t v) {
+  const Op& op = g_.ops[v];
+  const uint32_t x = op.args[0];
+  const Type& t = g_.type(x);
+  element_type(op, t.dtype);
+  const int64_t K = last(t);
+  require(t.rank() >= 1 && K % 32 == 0, op, "the last axis is a multiple of 32");
+  int codes = -1, scales = -1;
+  std::vector<uint32_t> made;
+  for (uint32_t u = v; u < g_.ops.size(); ++u) {
+    const Op& uo = g_.ops[u];
+    if (!live_[u] || done_[u] || uo.kind != Kind::custom_call || uo.index != 1 || uo.args != op.args) continue;
+    const bool is_codes = uo.bytes == "accy.mx4.codes";
+    if (!is_codes && uo.bytes != "accy.mx4.scales") continue;
+    int& slot = is_codes ? codes : scales;
+    if (slot >= 0) continue;
+    require(uo.result.dtype == DType::u8 && same_rows(uo.result, t) && last(uo.result) == K / (is_codes ? 2 : 32), uo,
+            is_codes ? "u8 codes, K / 2 to a row" : "u8 scales, K / 32 to a row");
+    slot = temp_slot(u);
+    made.push_back(u);
+  }
+  const uint64_t nel = t.elements();
+  if (nel) {
+    KernelWriter w(g_, slots_, itype());
+    std::vector<Dim> outer(t.dims.begin(), t.dims.end() - 1);
+    std::ostringstream body;
+    for (int half = 0; half < 2; ++half) {
+      // Four elements at a time: a leaf read at `rest + c` is one load for the four, non-temporal when this kernel reads each
+      // of its elements once.
+      const std::string at = half ? "(i0 + 4)" : "i0";
+      std::vector<std::string> coords = outer.empty() ? std::vector<std::string>{} : delinearize("(i0 / " + num(K) + ")", outer);
+      coords.push_back("c");
+      std::string hoisted;
+      std::map<std::string, std::string> hoisted_var;
+      w.leaf_hook = [&](int s, const std::string& off, DType d, Scope& sc, std::string& out) -> bool {
+        std::optional<std::string> base = quad_base(off);
+        if (!base) return false;
+        const std::string key = num(s) + "|" + off;
+        auto hv = hoisted_var.find(key);
+        if (hv == hoisted_var.end()) {
+          const std::string q = "q" + std::to_string(hoisted_var.size());
+          const bool once = plan_.slots[(size_t)s].bytes / dtype_size(d) == nel;
+          hoisted += "      " + w.quad_load(s, q, *base, d, once) + "\n";
+          hv = hoisted_var.emplace(key, q).first;
+        }
+        out = w.tmp();
+        sc.out << sc.indent << "const " << compute_type(d) << " " << out << " = " << KernelWriter::quad_elem(hv->second, "u", d) << ";\n";
+        return true;
+      };
+      std::ostringstream inner;
+      Scope sc(inner, "        ");
+      const std::string e = w.value(x, coords, sc);
+      body << "    {\n      const I c0 = " << (outer.empty() ? at : at + " % " + num(K)) << ";\n"
+           << hoisted << "#pragma unroll\n      for (int u = 0; u < 4; ++u) {\n        const I c = c0 + u;\n"
+           << inner.str() << "        x[" << 4 * half << " + u] = " << e << ";\n      }\n    }\n";
+    }
+    w.leaf_hook = nullptr;
+    std::string stores;
+    if (codes >= 0) stores += "    *(u32_t*)(" + w.arg(codes, true) + " + i0 / 2) = accy::mx4::encode8(x, scale);\n";
+    if (scales >= 0) stores += "    if (i0 % 32 == 0) " + w.arg(scales, true) + "[i0 / 32] = (u8_t)scale;\n";
+    const std::string nm = name("mx4_quantize", v);
+    std::ostringstream src;
+    src << "#include \"mx4\"\n"
+        << "extern \"C\" __global__ void __launch_bounds__(256) " << nm << "(" << w.params() << ") {\n  typedef " << w.itype << " I;\n"
+        << w.align_hints() << "  for (I i0 = ((I)blockIdx.x * 256 + (I)threadIdx.x) * 8; i0 < (I)" << nel << "; i0 += (I)gridDim.x * 2048) {\n"
+        << "    float x[8];\n" << body.str() << "    const u32_t scale = accy::mx4::block_scale(x);\n" << stores << "  }\n}\n";
+    KernelStep k;
+    k.source = src.str();
+    k.name = nm;
+    k.grid[0] = grid_for(nel / 8, 256);
+    k.block[0] = 256;
+    k.klass = "quantize";
+    k.label = "quantize:%" + std::to_string(v);
+    push(std::move(k), w);
+  }
+  for (uint32_t u : made) finish(u);
+}
+
+void Planner::mx4_values(uint32_t v) {
+  const Op& op = g_.ops[v];
+  const Type& c = g_.type(op.args[0]);
+  const int64_t K = blocked(op, c, g_.type(op.args[1]));
+  const int dt = element_type(op, op.result.dtype);
+  require(same_rows(op.result, c) && last(op.result) == K, op, "the result has the codes' rows and two values for each of their bytes");
+  const uint64_t nel = op.result.elements();
+  const int out = temp_slot(v);
+  if (nel) {
+    const int cs = dense_slot(op.args[0]), ss = dense_slot(op.args[1]);
+    KernelWriter w(g_, slots_, itype());
+    const std::string a = w.arg(cs, false), b = w.arg(ss, false), o = w.arg(out, true), nm = name("mx4_values", v);
+    KernelStep k;
+    k.source = "#include \"mx4\"\nextern \"C\" __global__ void __launch_bounds__(256) " + nm + "(" + w.params() + ") {\n  accy::mx4::values<" +
+               num(dt) + ", " + itype() + ", " + std::to_string(nel) + ">(" + a + ", " + b + ", " + o + ");\n}\n";
+    k.name = nm;
+    k.grid[0] = grid_for(nel / 8, 256);
+    k.block[0] = 256;
+    k.klass = "quantize";
+    k.label = "values:%" + std::to_string(v);
+    push(std::move(k), w);
+  }
+  finish(v);
+}
+
+// ---- products ----
+
+void Planner::mx4_contract(uint32_t v) {
+  const Op& op = g_.ops[v];
+  const Type &at = g_.type(op.args[0]), &bt = g_.type(op.args[2]), &rt = op.result;
+  const int64_t K = blocked(op, at, g_.type(op.args[1]));
+  require(blocked(op, bt, g_.type(op.args[3])) == K, op, "operands of different K");
+  require(K > 0, op, "an empty contraction");
+  const DType d = rt.dtype;
+  const int dt = element_type(op, d);
+  const size_t ra = at.rank() - 1, rb = bt.rank() - 1;
+  bool shape = rt.rank() == ra + rb;
+  for (size_t i = 0; shape && i < rt.rank(); ++i) shape = rt.dims[i].extent == (i < ra ? at.dims[i] : bt.dims[i - ra]).extent;
+  require(shape, op, "the result has the rows of the first operand and then those of the second");
+  const int64_t M = (int64_t)prod(at.dims, 0, ra), N = (int64_t)prod(bt.dims, 0, rb);
+  if (M == 0 || N == 0) {
+    temp_slot(v);
+    finish(v);
+    return;
+  }
+  const int as = dense_slot(op.args[0]), ss = dense_slot(op.args[1]), bs = dense_slot(op.args[2]), ts = dense_slot(op.args[3]);
+  const std::string nm = name("mx4_contract", v), cidx = "m * " + num(N) + "L + n";
+  std::unique_ptr<KernelWriter> w;
+  uint32_t target = v;
+  std::ostringstream epi;
+  std::string a, sa, b, sb;
+  auto begin = [&]() {
+    w.reset(new KernelWriter(g_, slots_, "i64_t"));
+    a = w->arg(as, false), sa = w->arg(ss, false), b = w->arg(bs, false), sb = w->arg(ts, false);
+  };
+  // As for every contraction: an elementwise region that ends in one value is the epilogue (see planner_contraction.cpp).
+  if (epilogue_target(v, target)) {
+    try {
+      begin();
+      std::vector<std::string> coords = delinearize("m", std::vector<Dim>(rt.dims.begin(), rt.dims.begin() + (long)ra));
+      for (auto& c : delinearize("n", std::vector<Dim>(rt.dims.begin() + (long)ra, rt.dims.end()))) coords.push_back(c);
+      w->provide = [&](uint32_t vid, const std::vector<std::string>& c, std::string& out) -> bool {
+        if (vid != v) return false;
+        if (c != coords) throw NotFusable("contraction value read at another index");
+        out = "vv";
+        return true;
+      };
+      Scope sc(epi, "    ");
+      const std::string x = w->value(target, coords, sc);
+      epi << "    " << w->store(temp_slot(target), cidx, g_.type(target).dtype, x) << "\n";
+    } catch (const NotFusable&) {
+      target = v;
+      w.reset();
+      epi.str("");
+    }
+  }
+  if (!w) {
+    begin();
+    epi << "    " << w->arg(temp_slot(v), true) << "[" << cidx << "] = accy::mx4::to_elem<" << dt << ">(v);\n";
+  }
+  const KernelWriter::Members members = w->members();
+  const uint64_t tiles = (uint64_t)((M + 31) / 32) * (uint64_t)((N + 31) / 32);
+  require(launchable((tiles + 3) / 4, 256), op, "more tiles than a launch takes");
+  std::ostringstream src;
+  src << "#include \"mx4\"\nstruct Epi_" << nm << " {\n" << members.decls
+      << "  __device__ __forceinline__ void operator()(long, long m, long n, float v) const {\n"
+      << (target != v ? "    const float vv = accy::mx4::rounded<" + num(dt) + ">(v);\n" : "") << epi.str() << "  }\n};\n"
+      << "struct Cfg_" << nm << " {\n  static constexpr long M = " << M << ", N = " << N << ", K = " << K << ";\n};\n"
+      << "extern \"C\" __global__ void __launch_bounds__(256) " << nm << "(" << w->params() << ") {\n  accy::mx4::contract_plain<Cfg_" << nm
+      << ">(" << a << ", " << sa << ", " << b << ", " << sb << ", Epi_" << nm << "{" << members.inits << "});\n}\n";
+  KernelStep k;
+  k.source = src.str();
+  k.name = nm;
+  k.grid[0] = (uint32_t)((tiles + 3) / 4);
+  k.block[0] = 256;
+  k.klass = "gemm";
+  k.label = "mx4:%" + std::to_string(v) + (target != v ? "+%" + std::to_string(target) : "");
+  k.algorithmic_flops = 2.0 * (double)M * (double)N * (double)K;
+  push(std::move(k), *w);
+  done_[v] = true;
+  finish(target);
+}
+
+// ---- the paged cache ----
+
+Planner::Mx4Cache Planner::mx4_cache(const Op& op, uint32_t cache, int64_t heads, int64_t dim) const {
+  const Type& t = g_.type(cache);
+  require(t.dtype == DType::u8 && t.rank() == 3, op, "a cache is u8 [page, kv_head, bytes]");
+  Mx4Cache c;
+  c.pages = t.dims[0].extent;
+  c.heads = t.dims[1].extent;
+  c.dim = dim;
+  require(c.heads == heads, op, "the cache holds " + num(c.heads) + " heads, the rows " + num(heads));
+  require(dim >= 32 && dim <= 256 && dim % 32 == 0, op, "head dimensions are multiples of 32 up to 256");
+  const int64_t row = dim + dim / 16, bytes = t.dims[2].extent;
+  c.tokens = bytes / row;
+  require(bytes % row == 0 && c.tokens > 0 && c.tokens % 32 == 0, op,
+          "a page holds a multiple of 32 tokens of " + num(row) + " bytes, not " + num(bytes) + " bytes");
+  require(c.tokens < (1 << 20) && c.pages < (int64_t(1) << 31) / c.tokens, op, "a cache has fewer than 2^31 slots");
+  return c;
+}
+
+std::string Planner::Mx4Cache::members(DType d) const {
+  return "  static constexpr int DT = " + std::string(d == DType::bf16 ? "0" : d == DType::f16 ? "1" : "2") + ", HD = " + num(dim) +
+         ", H = " + num(heads) + ", T = " + num(tokens) + ", P = " + num(pages) + ";\n";
+}
+
+void Planner::mx4_cache_write(uint32_t v) {
+  const Op& op = g_.ops[v];
+  const Type &kt = g_.type(op.args[1]), &vt = g_.type(op.args[2]), &st = g_.type(op.args[3]);
+  element_type(op, kt.dtype);
+  require(kt.rank() >= 2 && kt.dtype == vt.dtype && same_rows(kt, vt) && last(kt) == last(vt), op, "keys and values of one type and shape");
+  require(st.dtype == DType::i32 && st.rank() + 2 == kt.rank(), op, "an i32 slot for every token");
+  for (size_t i = 0; i < st.rank(); ++i) require(st.dims[i].extent == kt.dims[i].extent, op, "an i32 slot for every token");
+  const Mx4Cache c = mx4_cache(op, op.args[0], kt.dims[kt.rank() - 2].extent, last(kt));
+  require(op.result == g_.type(op.args[0]), op, "the result has the cache's type");
+  const int old = dense_slot(op.args[0]), out = temp_slot(v);
+  Step copy;
+  copy.type = Step::Copy;
+  copy.copy.src = old;
+  copy.copy.dst = out;
+  copy.copy.bytes = op.result.bytes();
+  copy.copy.unless_same = true;
+  if (copy.copy.bytes) plan_.steps.push_back(copy);
+  // The cache's own buffer may be the result's where the caller hands it in, gets it back, and nothing else of the program
+  // reads what was in it.
+  const SlotInfo &from = plan_.slots[(size_t)old], &to = plan_.slots[(size_t)out];
+  if (from.role == SlotInfo::Input && to.role == SlotInfo::Output && g_.ops[op.args[0]].kind == Kind::parameter &&
+      users_[op.args[0]].size() == 1 && !is_output_[op.args[0]])
+    plan_.updates.push_back({(size_t)from.io_index, (size_t)to.io_index});
+  const uint64_t n = st.elements();
+  if (n && c.pages && c.heads) {
+    const int ks = dense_slot(op.args[1]), vs = dense_slot(op.args[2]), ss = dense_slot(op.args[3]);
+    require(n < (uint64_t(1) << 31), op, "2^31 tokens or more");
+    // Looking through the later slots costs every workgroup a pass over the list; a table of each slot's last token two launches.
+    const bool owners = n > 8192;
+    const std::string nm = name("mx4_cache_write", v);
+    const std::string head = "#include \"mx4\"\nstruct Cfg_" + nm + " {\n" + c.members(kt.dtype) + "  static constexpr long TOKENS = " +
+                             std::to_string(n) + ";\n};\n";
+    auto launch = [&](const std::string& kernel, uint64_t groups, const std::string& call, const KernelWriter& w) {
+      require(launchable(groups, 256), op, "more workgroups than a launch takes");
+      KernelStep k;
+      k.source = head + "extern \"C\" __global__ void __launch_bounds__(256) " + kernel + "(" + w.params() + ") {\n  accy::mx4::" + call + ";\n}\n";
+      k.name = kernel;
+      k.grid[0] = (uint32_t)groups;
+      k.block[0] = 256;
+      k.klass = "quantize";
+      k.label = "cache_write:%" + std::to_string(v);
+      push(std::move(k), w);
+    };
+    int owner = -1;
+    if (owners) {
+      owner = slots_.add(SlotInfo::Temp, -1, DType::i32, (uint64_t)(c.pages * c.tokens) * 4);
+      for (const bool first : {true, false}) {
+        KernelWriter w(g_, slots_, "i64_t");
+        const std::string s = w.arg(ss, false), o = w.arg(owner, true);
+        launch(name("mx4_claim", v), (n + 255) / 256, std::string("claim<Cfg_") + nm + ", " + (first ? "true" : "false") + ">(" + s + ", " + o + ")", w);
+      }
+    }
+    KernelWriter w(g_, slots_, "i64_t");
+    const std::string o = w.arg(out, true), a = w.arg(ks, false), b = w.arg(vs, false), s = w.arg(ss, false);
+    const int64_t row = c.heads * c.dim / 8, per = row >= 512 ? 1 : 512 / row;  // Write<C>::TW
+    launch(nm, (n + (uint64_t)per - 1) / (uint64_t)per, "cache_write<Cfg_" + nm + (owners ? ", true>(" : ", false>(") + o + ", " + a + ", " + b +
+               ", " + s + ", " + (owners ? w.arg(owner, false) : std::string("nullptr")) + ")", w);
+  }
+  finish(v);
+}
+
+void Planner::mx4_cache_read(uint32_t v, bool value) {
+  const Op& op = g_.ops[v];
+  const Type &rt = op.result, &st = g_.type(op.args[1]);
+  element_type(op, rt.dtype);
+  require(st.dtype == DType::i32 && st.rank() + 2 == rt.rank(), op, "i32 slots; the result is [slots .., kv_head, dim]");
+  for (size_t i = 0; i < st.rank(); ++i) require(st.dims[i].extent == rt.dims[i].extent, op, "i32 slots; the result is [slots .., kv_head, dim]");
+  const Mx4Cache c = mx4_cache(op, op.args[0], rt.dims[rt.rank() - 2].extent, last(rt));
+  const int out = temp_slot(v);
+  if (rt.elements()) {
+    const int cs = dense_slot(op.args[0]), ss = dense_slot(op.args[1]);
+    KernelWriter w(g_, slots_, "i64_t");
+    const std::string a = w.arg(cs, false), s = w.arg(ss, false), o = w.arg(out, true), nm = name("mx4_cache_read", v);
+    KernelStep k;
+    k.source = "#include \"mx4\"\nstruct Cfg_" + nm + " {\n" + c.members(rt.dtype) + "  static constexpr long TOKENS = " +
+               std::to_string(st.elements()) + ";\n};\nextern \"C\" __global__ void __launch_bounds__(256) " + nm + "(" + w.params() +
+               ") {\n  accy::mx4::cache_read<Cfg_" + nm + ", " + (value ? "true" : "false") + ">(" + a + ", " + s + ", " + o + ");\n}\n";
+    k.name = nm;
+    k.grid[0] = grid_for(rt.elements() / 8, 256);
+    k.block[0] = 256;
+    k.klass = "quantize";
+    k.label = "cache_read:%" + std::to_string(v);
+    push(std::move(k), w);
+  }
+  finish(v);
+}
+
+// ---- attention over the cache ----
+
+void Planner::mx4_attend(uint32_t v) {
+  const Op& op = g_.ops[v];
+  const Type &qt = g_.type(op.args[0]), &ct = g_.type(op.args[1]), &pt = g_.type(op.args[2]), &lt = g_.type(op.args[3]);
+  element_type(op, qt.dtype);
+  require(op.result.dtype == qt.dtype && same_rows(op.result, qt) && last(op.result) == last(qt), op, "the result has the queries' type");
+  require(qt.rank() == 3 || qt.rank() == 4, op, "queries are [seq, (query,) head, dim]");
+  require(ct.rank() == 3, op, "a cache is u8 [page, kv_head, bytes]");
+  const int64_t seqs = qt.dims[0].extent, Q = qt.rank() == 4 ? qt.dims[1].extent : 1, heads = qt.dims[qt.rank() - 2].extent;
+  const int64_t H = ct.dims[1].extent, hd = last(qt);
+  require(pt.dtype == DType::i32 && pt.rank() == 2 && pt.dims[0].extent == seqs, op, "pages are i32 [seq, page]");
+  require(lt.dtype == DType::i32 && lt.rank() == 1 && lt.dims[0].extent == seqs, op, "lengths are i32 [seq]");
+  require(H > 0 && heads % H == 0, op, num(heads) + " query heads over " + num(H) + " key-value heads");
+  const int64_t G = heads / H;
+  const Mx4Cache c = mx4_cache(op, op.args[1], H, hd);
+  const int64_t maxp = pt.dims[1].extent;
+  require(maxp < (int64_t(1) << 31) / c.tokens, op, "a sequence has fewer than 2^31 keys");
+  const int out = temp_slot(v);
+  const uint64_t nel = op.result.elements();
+  if (nel) {
+    require(Q * G < (int64_t(1) << 24), op, "2^24 query rows of a key-value head or more");
+    const int qs = dense_slot(op.args[0]), cs = dense_slot(op.args[1]), ps = dense_slot(op.args[2]), ls = dense_slot(op.args[3]);
+    const int64_t tiles = (Q * G + 15) / 16;
+    const int64_t NR = std::min<int64_t>(tiles, 2), groups = (tiles + NR - 1) / NR, wgs = seqs * H * groups;
+    const int64_t steps = (maxp * c.tokens + 31) / 32;
+    int64_t splits = 1;
+    while (opt_.allow_split && splits < 64 && wgs * splits < 1024 && steps >= 16 * splits) splits *= 2;
+    require(launchable((uint64_t)wgs, 256), op, "more workgroups than a launch takes");
+    KernelWriter w(g_, slots_, "i64_t");
+    const std::string q = w.arg(qs, false), a = w.arg(cs, false), p = w.arg(ps, false), l = w.arg(ls, false);
+    int part = -1;
+    if (splits > 1) part = slots_.add(SlotInfo::Temp, -1, DType::f32, (uint64_t)(seqs * H * Q * G * splits * (hd + 4)) * 4);
+    const std::string o = splits > 1 ? "nullptr" : w.arg(out, true), pp = splits > 1 ? w.arg(part, true) : "nullptr";
+    const std::string nm = name("mx4_attend", v);
+    char sl[64];
+    std::snprintf(sl, sizeof sl, "%af", (double)(float)(1.4426950408889634 / std::sqrt((double)hd)));
+    const std::string head = "#include \"mx4\"\nstruct Cfg_" + nm + " {\n" + c.members(qt.dtype) + "  static constexpr int Q = " + num(Q) +
+                             ", G = " + num(G) + ", MAXP = " + num(maxp) + ", NR = " + num(NR) + ", SPLITS = " + num(splits) +
+                             ";\n  static constexpr long SEQS = " + num(seqs) + ";\n  static constexpr float SL = " + sl + ";\n};\n";
+    KernelStep k;
+    k.source = head + "extern \"C\" __global__ void __launch_bounds__(256) " + nm + "(" + w.params() + ") {\n  accy::mx4::attend<Cfg_" + nm +
+               ">(" + q + ", " + a + ", " + p + ", " + l + ", " + o + ", " + pp + ");\n}\n";
+    k.name = nm;
+    k.grid[0] = (uint32_t)wgs;
+    k.grid[1] = (uint32_t)splits;
+    k.block[0] = 256;
+    k.klass = "attention";
+    k.label = "mx4_attend:%" + std::to_string(v);
+    k.algorithmic_flops = 4.0 * (double)nel * (double)(maxp * c.tokens);
+    push(std::move(k), w);
+    if (splits > 1) {
+      KernelWriter jw(g_, slots_, "i64_t");
+      const std::string jp = jw.arg(part, false), jo = jw.arg(out, true);
+      KernelStep j;
+      j.name = name("mx4_join", v);
+      j.source = head + "extern \"C\" __global__ void __launch_bounds__(256) " + j.name + "(" + jw.params() + ") {\n  accy::mx4::attend_join<Cfg_" +
+                 nm + ">(" + jp + ", " + jo + ");\n}\n";
+      require(launchable((nel + 255) / 256, 256), op, "more workgroups than a launch takes");
+      j.grid[0] = (uint32_t)((nel + 255) / 256);
+      j.block[0] = 256;
+      j.klass = "attention";
+      j.label = "mx4_join:%" + std::to_string(v);
+      push(std::move(j), jw);
+    }
+  }
+  finish(v);
+}
+
+}  // namespace planning
+}  // namespace accy

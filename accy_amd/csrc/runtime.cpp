@@ -17,6 +17,7 @@ extern const char* const kGemmDeviceSource;
 extern const char* const kAttentionDeviceSource;
 extern const char* const kScatterDeviceSource;
 extern const char* const kDecodeDeviceSource;
+extern const char* const kMx4DeviceSource;
 
 namespace {
 
@@ -62,7 +63,8 @@ std::string full_kernel_source(const std::string& body) {
   const std::pair<const char*, const char*> templates[] = {{"#include \"gemm\"\n", kGemmDeviceSource},
                                                            {"#include \"attention\"\n", kAttentionDeviceSource},
                                                            {"#include \"scatter\"\n", kScatterDeviceSource},
-                                                           {"#include \"decode\"\n", kDecodeDeviceSource}};
+                                                           {"#include \"decode\"\n", kDecodeDeviceSource},
+                                                           {"#include \"mx4\"\n", kMx4DeviceSource}};
   std::string rest = body;
   for (const auto& t : templates) {
     size_t p = rest.find(t.first);
@@ -349,6 +351,7 @@ void Executor::run_steps(hipStream_t stream, uint8_t* scratch) {
   for (size_t i = 0; i < plan_.steps.size(); ++i) {
     const Step& st = plan_.steps[i];
     if (st.type == Step::Copy) {
+      if (st.copy.unless_same && bound_[(size_t)st.copy.dst] == bound_[(size_t)st.copy.src]) continue;
       check(hipMemcpyAsync(bound_[(size_t)st.copy.dst], bound_[(size_t)st.copy.src], st.copy.bytes,
                            hipMemcpyDeviceToDevice, stream),
             "hipMemcpyAsync");
@@ -393,11 +396,13 @@ void Executor::invoke_device(const void* const* inputs, size_t n_inputs, void* c
     if (!aligned(outputs[i])) throw HipFailure(kStatusInvalidBuffer, "output " + std::to_string(i) + " not 16-byte aligned");
   // binding.zig:325-336 (expectDisjointOutputs): an output may share no byte with an input or with an
   // earlier output; kernels that read after another workgroup wrote would otherwise see its results.
-  // Inputs may alias each other (they are only read).
+  // Inputs may alias each other (they are only read). An output that is an input updated in place may be bound to
+  // that very buffer.
   for (size_t o = 0; o < n_outputs; ++o) {
     const size_t ob = plan_.slots[(size_t)plan_.output_slots[o]].bytes;
     for (size_t i = 0; i < n_inputs; ++i)
-      if (ranges_overlap(outputs[o], ob, inputs[i], plan_.slots[(size_t)plan_.input_slots[i]].bytes))
+      if (!(outputs[o] == inputs[i] && std::find(plan_.updates.begin(), plan_.updates.end(), std::make_pair(i, o)) != plan_.updates.end()) &&
+          ranges_overlap(outputs[o], ob, inputs[i], plan_.slots[(size_t)plan_.input_slots[i]].bytes))
         throw HipFailure(kStatusInvalidBuffer, "output " + std::to_string(o) + " overlaps input " + std::to_string(i));
     for (size_t j = 0; j < o; ++j)
       if (ranges_overlap(outputs[o], ob, outputs[j], plan_.slots[(size_t)plan_.output_slots[j]].bytes))

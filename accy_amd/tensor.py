@@ -384,6 +384,22 @@ class Value:
     def contract(self, rhs: "Value", axes) -> "Value":
         return self.builder.contract(self, rhs, _axes(axes))
 
+    # microscaled 4-bit floats (this target's custom calls)
+    def quantize_mx4(self, axis: str) -> "Mx4":
+        return self.builder.quantize_mx4(self, axis)
+
+    def cache_write_mx4(self, keys: "Value", values: "Value", slots: "Value") -> "Value":
+        return self.builder.cache_write_mx4(self, keys, values, slots)
+
+    def cache_keys_mx4(self, slots: "Value", dim: Dim, dtype: str) -> "Value":
+        return self.builder.cache_read_mx4("cache_keys", self, slots, dim, dtype)
+
+    def cache_values_mx4(self, slots: "Value", dim: Dim, dtype: str) -> "Value":
+        return self.builder.cache_read_mx4("cache_values", self, slots, dim, dtype)
+
+    def attend_mx4(self, cache: "Value", pages: "Value", lengths: "Value") -> "Value":
+        return self.builder.attend_mx4(self, cache, pages, lengths)
+
     def rename(self, old: str, new: str) -> "Value":
         return self.builder.rename_axis(self, old, new)
 
@@ -431,6 +447,65 @@ class Value:
 
     def is_structural_zero(self) -> bool:
         return self.builder.is_structural_zero(self.id)
+
+
+MX4_BLOCK = 32
+MX4_FLOATS = ("bf16", "f16", "f32")
+
+
+@dataclass(frozen=True)
+class Mx4:
+    """A tensor in microscaled 4-bit floats: ``codes`` u8 [.., axis / 2], two e2m1 values to a byte, the first in its low
+    half, and ``scales`` u8 [.., axis / 32], one power of two (its exponent plus 127; 255: NaN) for each 32 values along
+    ``axis``, the last one. Made by ``Value.quantize_mx4`` or, from buffers that hold them, by ``Builder.mx4``."""
+    codes: Value
+    scales: Value
+    axis: str
+
+    @property
+    def dims(self) -> Tuple[Dim, ...]:
+        return self.codes.ty.dims[:-1] + ((self.axis, 2 * self.codes.ty.dims[-1][1]),)
+
+    def dequantize(self, dtype: str) -> Value:
+        """The values, rounded to nearest even where ``dtype`` does not hold them."""
+        return self.codes.builder.dequantize_mx4(self, dtype)
+
+    def contract(self, rhs: "Mx4", dtype: str) -> Value:
+        """Sum over the blocked axis of both, which is one axis: [rows of self, rows of rhs], summed in f32 and rounded to
+        nearest even."""
+        return self.codes.builder.contract_mx4(self, rhs, dtype)
+
+
+def mx4_specs(axis: str, *dims: Dim, **named: int) -> Tuple[Spec, Spec]:
+    """The specs of codes and scales of a tensor of these dims blocked along ``axis``, its last: for ``Builder.mx4``."""
+    dims = tuple(dims) + tuple(named.items())
+    rows, blocked = _mx4_rows(dims, axis)
+    return (Spec("u8", rows + ((f"{axis}.codes", blocked // 2),)), Spec("u8", rows + ((f"{axis}.scales", blocked // MX4_BLOCK),)))
+
+
+def cache_mx4_spec(pages: int, kv_heads: int, dim: int, page: int = 64) -> Spec:
+    """A paged cache of keys and values of head dimension ``dim`` in microscaled 4-bit floats, ``page`` tokens to a page."""
+    return Spec("u8", (("page", pages), ("kv_head", kv_heads), ("byte", page * _mx4_cache_row(dim, page))))
+
+
+def _mx4_rows(dims: Sequence[Dim], axis: str) -> Tuple[Tuple[Dim, ...], int]:
+    i = _find(dims, axis)
+    if i is None:
+        raise TensorError("AxisNotFound", axis)
+    if i != len(dims) - 1:
+        raise TensorError("InvalidPermutation", f"{axis} is not the last axis")
+    if dims[i][1] % MX4_BLOCK:
+        raise TensorError("InvalidDimension", f"{axis} is not a multiple of {MX4_BLOCK}")
+    return tuple(dims[:-1]), dims[i][1]
+
+
+def _mx4_cache_row(dim: int, page: int) -> int:
+    """Bytes of a token's keys and values of one head."""
+    if dim % 32 or not 32 <= dim <= 256:
+        raise TensorError("InvalidDimension", "head dimensions are multiples of 32 up to 256")
+    if page <= 0 or page % 32:
+        raise TensorError("InvalidDimension", "pages are multiples of 32 tokens")
+    return dim + dim // 16
 
 
 def _axes(axes) -> List[str]:
@@ -900,6 +975,127 @@ class Builder:
         ty = _make_type(result.dtype, result.dims)
         return self._append(Operation("custom_call", ty, args=tuple(v.id for v in operands), index=version,
                                       payload=target.encode()))
+
+    # -- microscaled 4-bit floats: custom calls that the gfx950 target runs --
+    #
+    # Blocks of 32 values along the last axis; a block of largest magnitude A takes the scale 2^(floor(log2 A) - 2), at least
+    # 2^-127, and each value the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it (ties to the even code; larger ones 6).
+    # A block with a NaN or an infinity reads back as NaN.
+
+    def _mx4_call(self, name: str, operands: Sequence[Value], dtype: str, dims: Sequence[Dim]) -> Value:
+        return self.custom_call(f"accy.mx4.{name}", 1, operands, Type(dtype, tuple(dims)))
+
+    def _mx4_float(self, dtype: str) -> None:
+        if dtype not in MX4_FLOATS:
+            raise TensorError("DTypeMismatch", f"{dtype}: one of {', '.join(MX4_FLOATS)}")
+
+    def quantize_mx4(self, v: Value, axis: str) -> Mx4:
+        """``v`` quantised along ``axis`` (moved to the end where it is not the last). The values are evaluated inside the
+        kernel that quantises them."""
+        self._ensure(v)
+        self._mx4_float(v.ty.dtype)
+        i = _find(v.ty.dims, axis)
+        if i is None:
+            raise TensorError("AxisNotFound", axis)
+        if i != v.ty.rank - 1:
+            v = self.transpose(v, [d for d in range(v.ty.rank) if d != i] + [i])
+        rows, k = _mx4_rows(v.ty.dims, axis)
+        return self.mx4(self._mx4_call("codes", [v], "u8", rows + ((f"{axis}.codes", k // 2),)),
+                        self._mx4_call("scales", [v], "u8", rows + ((f"{axis}.scales", k // MX4_BLOCK),)), axis)
+
+    def mx4(self, codes: Value, scales: Value, axis: str) -> Mx4:
+        """A quantised tensor from its codes and scales (see ``mx4_specs``)."""
+        for x in (codes, scales):
+            self._ensure(x)
+            if x.ty.dtype != "u8":
+                raise TensorError("DTypeMismatch", "codes and scales are u8")
+        if codes.ty.rank == 0 or scales.ty.rank == 0 or codes.ty.dims[:-1] != scales.ty.dims[:-1]:
+            raise TensorError("ShapeMismatch", "codes and scales of different rows")
+        if codes.ty.dims[-1][1] * 2 != scales.ty.dims[-1][1] * MX4_BLOCK:
+            raise TensorError("AxisExtentMismatch", axis)
+        _validate_dims(codes.ty.dims[:-1] + ((axis, 2 * codes.ty.dims[-1][1]),))
+        return Mx4(codes, scales, axis)
+
+    def dequantize_mx4(self, v: Mx4, dtype: str) -> Value:
+        self._mx4_float(dtype)
+        return self._mx4_call("values", [v.codes, v.scales], dtype, v.dims)
+
+    def contract_mx4(self, lhs: Mx4, rhs: Mx4, dtype: str) -> Value:
+        self._mx4_float(dtype)
+        if lhs.axis != rhs.axis:
+            raise TensorError("AxisNotFound", rhs.axis)
+        if lhs.dims[-1] != rhs.dims[-1]:
+            raise TensorError("AxisExtentMismatch", lhs.axis)
+        if lhs.dims[-1][1] == 0:
+            raise TensorError("InvalidDimension", lhs.axis)
+        dims = lhs.dims[:-1] + rhs.dims[:-1]
+        _validate_dims(dims)  # rows that both have would be a batch: DuplicateAxis
+        return self._mx4_call("contract", [lhs.codes, lhs.scales, rhs.codes, rhs.scales], dtype, dims)
+
+    def _mx4_cache(self, cache: Value, kv_head: Dim, dim: Dim) -> None:
+        self._ensure(cache)
+        if cache.ty.dtype != "u8":
+            raise TensorError("DTypeMismatch", "a cache is u8")
+        if cache.ty.rank != 3:
+            raise TensorError("RankMismatch", "a cache is [page, kv_head, bytes]")
+        if cache.ty.dims[1] != kv_head:
+            raise TensorError("AxisExtentMismatch", f"{kv_head} against the cache's {cache.ty.dims[1]}")
+        tokens, rest = divmod(cache.ty.dims[2][1], _mx4_cache_row(dim[1], 32))
+        if rest or tokens == 0 or tokens % 32:
+            raise TensorError("AxisExtentMismatch", f"{cache.ty.dims[2][1]} bytes are no pages of head dimension {dim[1]}")
+
+    def cache_write_mx4(self, cache: Value, keys: Value, values: Value, slots: Value) -> Value:
+        """The cache with keys and values [token .., kv_head, dim] quantised into the rows of the tokens' slots: page *
+        page size + row. A slot outside the cache (-1: padding) writes nothing; of two tokens of one slot the later one in
+        order is kept. Where the cache is a parameter that nothing else reads and the result an output, a launch may bind
+        both to one buffer, which is then updated in place."""
+        for x in (keys, values, slots):
+            self._ensure(x)
+        self._mx4_float(keys.ty.dtype)
+        _same_type(keys.ty, values.ty)
+        if keys.ty.rank < 2:
+            raise TensorError("RankMismatch", "keys are [token .., kv_head, dim]")
+        self._mx4_cache(cache, keys.ty.dims[-2], keys.ty.dims[-1])
+        if slots.ty.dtype != "i32":
+            raise TensorError("DTypeMismatch", "slots are i32")
+        if slots.ty.dims != keys.ty.dims[:-2]:
+            raise TensorError("ShapeMismatch", "a slot for every token")
+        return self._mx4_call("cache_write", [cache, keys, values, slots], "u8", cache.ty.dims)
+
+    def cache_read_mx4(self, name: str, cache: Value, slots: Value, dim: Dim, dtype: str) -> Value:
+        """The keys (``cache_keys``) or values (``cache_values``) of some slots: [slots .., kv_head, dim]; zeros for a slot
+        outside the cache."""
+        self._ensure(slots)
+        self._mx4_float(dtype)
+        if cache.ty.rank != 3:
+            raise TensorError("RankMismatch", "a cache is [page, kv_head, bytes]")
+        self._mx4_cache(cache, cache.ty.dims[1], dim)
+        if slots.ty.dtype != "i32":
+            raise TensorError("DTypeMismatch", "slots are i32")
+        return self._mx4_call(name, [cache, slots], dtype, slots.ty.dims + (cache.ty.dims[1], dim))
+
+    def attend_mx4(self, q: Value, cache: Value, pages: Value, lengths: Value) -> Value:
+        """softmax(q . k / sqrt(dim)) v over a paged cache, for the newest queries of each sequence.
+
+        ``q`` [seq, head, dim] or [seq, query, head, dim]; ``pages`` i32 [seq, page slot]: key j of a sequence is row j % page
+        size of page pages[j / page size]; ``lengths`` i32 [seq]: keys of each sequence, the new tokens' among them (at most
+        what its pages hold). The last query sees all of them, each one before it one fewer. Query head h reads key-value
+        head h / (heads / kv_heads). Page numbers outside the cache hold no keys; a query that sees none gives 0."""
+        for x in (q, pages, lengths):
+            self._ensure(x)
+        self._mx4_float(q.ty.dtype)
+        if q.ty.rank not in (3, 4):
+            raise TensorError("RankMismatch", "queries are [seq, (query,) head, dim]")
+        if cache.ty.rank != 3:
+            raise TensorError("RankMismatch", "a cache is [page, kv_head, bytes]")
+        self._mx4_cache(cache, cache.ty.dims[1], q.ty.dims[-1])
+        if cache.ty.dims[1][1] == 0 or q.ty.dims[-2][1] % cache.ty.dims[1][1]:
+            raise TensorError("AxisExtentMismatch", f"{q.ty.dims[-2][1]} heads over {cache.ty.dims[1][1]} key-value heads")
+        if pages.ty.dtype != "i32" or lengths.ty.dtype != "i32":
+            raise TensorError("DTypeMismatch", "pages and lengths are i32")
+        if pages.ty.rank != 2 or pages.ty.dims[0] != q.ty.dims[0] or lengths.ty.dims != q.ty.dims[:1]:
+            raise TensorError("ShapeMismatch", "pages are [seq, page], lengths [seq]")
+        return self._mx4_call("attend", [q, cache, pages, lengths], q.ty.dtype, q.ty.dims)
 
     def scan(self, length: int, inits: Sequence[Value], body: Callable[["Builder", List[Value]], Sequence[Value]]) -> Value:
         """Repeat ``body`` ``length`` times carrying ``inits`` (builder.zig:899-990)."""
