@@ -1,4 +1,5 @@
-// Microscaled 4-bit floats on gfx950: quantisation, products, and a paged cache with the attention that reads it.
+// Microscaled 4-bit floats on gfx950: quantisation, and a paged cache with the attention that reads it (products:
+// mx4_contract.h).
 //
 // The format: blocks of 32 values along one axis; a value is e2m1 (sign, two exponent bits, one mantissa bit: 0, 0.5, 1,
 // 1.5, 2, 3, 4, 6) times its block's scale, a power of two held as its biased exponent in one byte (e8m0; 255 is NaN).
@@ -7,8 +8,7 @@
 // to the even code. A block with a NaN or an infinity takes scale 255 and reads as NaN throughout.
 //
 // v_cvt_scalef32_pk_fp4_f32 divides by the scale and rounds two values exactly so (ties, saturation and the scales 2^-127 and
-// 2^127 included), v_cvt_scalef32_pk_{f32,bf16}_fp4 is the way back, exact in both types, and
-// v_mfma_scale_f32_*_f8f6f4 takes codes and scales as they are: a lane's 16 bytes are one block, its scale byte beside it.
+// 2^127 included), v_cvt_scalef32_pk_{f32,bf16}_fp4 is the way back, exact in both types.
 #pragma once
 
 namespace accy {
@@ -17,10 +17,8 @@ namespace mx4 {
 typedef u32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef u32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -115,43 +113,6 @@ __device__ __forceinline__ void values(const u8_t* __restrict__ codes, const u8_
     float x[8];
     decode8(*(const u32_t*)(codes + i / 2), scales[i / 32], x);
     store8<DT>(out + i, x);
-  }
-}
-
-// ---------------------------------------------------------------------------------------------
-// Products: C[m, n] = sum_k A[m, k] B[n, k], both operands' rows blocked along k.
-//
-// C supplies M, N, K (K a multiple of 32); the epilogue receives (0, m, n, f32 sum) for every output.
-// ---------------------------------------------------------------------------------------------
-
-__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, int sa, int sb) {
-  const i32x8 aw = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, bw = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(aw, bw, c, 4, 4, 0, sa, 0, sb);
-}
-
-// One wave per 32 x 32 outputs, operands straight from memory. Rows past the end read the last row and are not stored; a
-// block past K (the second of the last pair where K / 32 is odd) reads the last one with the scales 2^-127 on both
-// sides, whose products vanish in f32 (below 36 x 2^-254).
-template <class C, class Epi>
-__device__ __forceinline__ void contract_plain(const u8_t* __restrict__ A, const u8_t* __restrict__ AS, const u8_t* __restrict__ B,
-                                               const u8_t* __restrict__ BS, const Epi& epi) {
-  constexpr long TN = (C::N + 31) / 32, BLOCKS = C::K / 32;
-  const int lane = threadIdx.x & 63, half = lane >> 5;
-  const long tile = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const long m0 = tile / TN * 32, n0 = tile % TN * 32;
-  if (m0 >= C::M) return;
-  const long m = m0 + (lane & 31) < C::M ? m0 + (lane & 31) : C::M - 1, n = n0 + (lane & 31) < C::N ? n0 + (lane & 31) : C::N - 1;
-  f32x16 acc = {};
-  for (long b = half; b < BLOCKS + half; b += 2) {
-    const long at = b < BLOCKS ? b : BLOCKS - 1;
-    const u32x4 a = *(const u32x4*)(A + m * (C::K / 2) + 16 * at), w = *(const u32x4*)(B + n * (C::K / 2) + 16 * at);
-    const int sa = b < BLOCKS ? AS[m * BLOCKS + at] : 0, sb = b < BLOCKS ? BS[n * BLOCKS + at] : 0;
-    acc = mfma32(a, w, acc, sa, sb);
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const long mm = m0 + (i & 3) + 8 * (i >> 2) + 4 * half, nn = n0 + (lane & 31);
-    if (mm < C::M && nn < C::N) epi(0, mm, nn, acc[i]);
   }
 }
 

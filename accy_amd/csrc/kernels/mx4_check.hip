@@ -2,7 +2,9 @@
 // microscaled 4-bit templates with shapes the planner emits, so that a host without a GPU still
 // verifies that they compile for CDNA4. Nothing calls these kernels.
 #include "common.h"
+#include "gemm.h"
 #include "mx4.h"
+#include "mx4_contract.h"
 
 struct CheckStore {
   float* c;
@@ -10,6 +12,10 @@ struct CheckStore {
 };
 struct CheckProduct {
   static constexpr long M = 300, N = 513, K = 1056;
+  static constexpr int BM = 128, BN = 128, GROUP_M = 8, SPLITS = 2, WK = 0;
+};
+struct CheckSmall : CheckProduct {
+  static constexpr int BM = 64, BN = 32, SPLITS = 1, WK = 2;
 };
 template <int D, int DIM, int QUERIES, int GROUP, int TILES, int S>
 struct CheckCache {
@@ -18,8 +24,11 @@ struct CheckCache {
   static constexpr float SL = 0x1.05p-3f;
 };
 
-extern "C" __global__ void __launch_bounds__(256) check_mx4_product(const u8_t* a, const u8_t* sa, const u8_t* b, const u8_t* sb, float* c) {
-  accy::mx4::contract_plain<CheckProduct>(a, sa, b, sb, CheckStore{c});
+extern "C" __global__ void __launch_bounds__(128) check_mx4_small(const u8_t* a, const u8_t* sa, const u8_t* b, const u8_t* sb, float* c) {
+  accy::mx4::contract_direct<CheckSmall>(a, sa, b, sb, CheckStore{c});
+}
+extern "C" __global__ void __launch_bounds__(256) check_mx4_tile(const u8_t* a, const u8_t* sa, const u8_t* b, const u8_t* sb, float* c) {
+  accy::mx4::contract_tile<CheckProduct>(a, sa, b, sb, CheckStore{c});
 }
 extern "C" __global__ void __launch_bounds__(256) check_mx4_values(const u8_t* c, const u8_t* s, u16_t* o) {
   accy::mx4::values<0, int, 4096>(c, s, o);

@@ -614,6 +614,12 @@ class Planner {
   void mx4_quantize(uint32_t v);
   void mx4_values(uint32_t v);
   void mx4_contract(uint32_t v);
+  // Outputs of a workgroup of the product, the waves that share its K (small tiles; 0: the large ones) and the workgroups along K;
+  // bm = 0: none whose grid HIP takes.
+  struct Mx4Tile {
+    int bm = 0, bn = 0, wk = 0, splits = 1;
+  };
+  Mx4Tile mx4_tile(int64_t M, int64_t N, int64_t K) const;
   void mx4_cache_write(uint32_t v);
   void mx4_cache_read(uint32_t v, bool value);
   void mx4_attend(uint32_t v);

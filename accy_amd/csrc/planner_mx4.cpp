@@ -1,4 +1,4 @@
-// Custom calls of this target: microscaled 4-bit floats (kernels/mx4.h). A program names them "accy.mx4.<name>", version 1:
+// Custom calls of this target: microscaled 4-bit floats (kernels/mx4.h, mx4_contract.h). A program names them "accy.mx4.<name>", version 1:
 //
 //   codes(x), scales(x)                    x [.., K] -> u8 [.., K / 2] and u8 [.., K / 32], planned as one kernel
 //   values(codes, scales)                  -> [.., K]
@@ -218,20 +218,46 @@ void Planner::mx4_contract(uint32_t v) {
     finish(v);
     return;
   }
-  const int as = dense_slot(op.args[0]), ss = dense_slot(op.args[1]), bs = dense_slot(op.args[2]), ts = dense_slot(op.args[3]);
+  int as = dense_slot(op.args[0]), ss = dense_slot(op.args[1]), bs = dense_slot(op.args[2]), ts = dense_slot(op.args[3]);
   const std::string nm = name("mx4_contract", v), cidx = "m * " + num(N) + "L + n";
+  const Mx4Tile tile = mx4_tile(M, N, K);
+  const bool split = tile.splits > 1;
+  require(tile.bm > 0, op, "more tiles than a launch takes");
+  if (!tile.wk && K % 128 != 0) {
+    // the tiles read scales a whole step at a time
+    const int64_t steps = (K + 127) / 128;
+    const int pa = slots_.add(SlotInfo::Temp, -1, DType::u32, (uint64_t)(M * steps) * 4);
+    const int pb = slots_.add(SlotInfo::Temp, -1, DType::u32, (uint64_t)(N * steps) * 4);
+    KernelWriter w(g_, slots_, "i64_t");
+    const std::string a = w.arg(ss, false), b = w.arg(ts, false), x = w.arg(pa, true), y = w.arg(pb, true);
+    KernelStep k;
+    k.name = name("mx4_pad", v);
+    k.source = "#include \"gemm\"\n#include \"mx4\"\n#include \"mx4_contract\"\nstruct Cfg_" + nm + " {\n  static constexpr long M = " + num(M) + ", N = " +
+               num(N) + ", K = " + num(K) + ";\n};\nextern \"C\" __global__ void __launch_bounds__(256) " + k.name + "(" + w.params() +
+               ") {\n  accy::mx4::pad_scales<Cfg_" + nm + ">(" + a + ", " + b + ", " + x + ", " + y + ");\n}\n";
+    k.grid[0] = grid_for((uint64_t)(std::max(M, N) * steps), 256);
+    k.grid[1] = 2;
+    k.block[0] = 256;
+    k.klass = "gemm";
+    k.label = "mx4_pad:%" + std::to_string(v);
+    push(std::move(k), w);
+    ss = pa;
+    ts = pb;
+  }
+  // The kernel that stores the results (the product's own, or the sum of its splits) and what it reads.
   std::unique_ptr<KernelWriter> w;
+  auto operands = [&](KernelWriter& k) {
+    std::string call;
+    for (int s : {as, ss, bs, ts}) call += "(const u8_t*)" + k.arg(s, false) + ", ";
+    return call;
+  };
   uint32_t target = v;
   std::ostringstream epi;
-  std::string a, sa, b, sb;
-  auto begin = [&]() {
-    w.reset(new KernelWriter(g_, slots_, "i64_t"));
-    a = w->arg(as, false), sa = w->arg(ss, false), b = w->arg(bs, false), sb = w->arg(ts, false);
-  };
   // As for every contraction: an elementwise region that ends in one value is the epilogue (see planner_contraction.cpp).
   if (epilogue_target(v, target)) {
     try {
-      begin();
+      w.reset(new KernelWriter(g_, slots_, "i64_t"));
+      if (!split) operands(*w);
       std::vector<std::string> coords = delinearize("m", std::vector<Dim>(rt.dims.begin(), rt.dims.begin() + (long)ra));
       for (auto& c : delinearize("n", std::vector<Dim>(rt.dims.begin() + (long)ra, rt.dims.end()))) coords.push_back(c);
       w->provide = [&](uint32_t vid, const std::vector<std::string>& c, std::string& out) -> bool {
@@ -250,30 +276,103 @@ void Planner::mx4_contract(uint32_t v) {
     }
   }
   if (!w) {
-    begin();
+    w.reset(new KernelWriter(g_, slots_, "i64_t"));
+    if (!split) operands(*w);
     epi << "    " << w->arg(temp_slot(v), true) << "[" << cidx << "] = accy::mx4::to_elem<" << dt << ">(v);\n";
   }
   const KernelWriter::Members members = w->members();
-  const uint64_t tiles = (uint64_t)((M + 31) / 32) * (uint64_t)((N + 31) / 32);
-  require(launchable((tiles + 3) / 4, 256), op, "more tiles than a launch takes");
-  std::ostringstream src;
-  src << "#include \"mx4\"\nstruct Epi_" << nm << " {\n" << members.decls
-      << "  __device__ __forceinline__ void operator()(long, long m, long n, float v) const {\n"
-      << (target != v ? "    const float vv = accy::mx4::rounded<" + num(dt) + ">(v);\n" : "") << epi.str() << "  }\n};\n"
-      << "struct Cfg_" << nm << " {\n  static constexpr long M = " << M << ", N = " << N << ", K = " << K << ";\n};\n"
-      << "extern \"C\" __global__ void __launch_bounds__(256) " << nm << "(" << w->params() << ") {\n  accy::mx4::contract_plain<Cfg_" << nm
-      << ">(" << a << ", " << sa << ", " << b << ", " << sb << ", Epi_" << nm << "{" << members.inits << "});\n}\n";
+  const std::string rounded = target != v ? "    const float vv = accy::mx4::rounded<" + num(dt) + ">(v);\n" : "";
+  std::ostringstream head;
+  head << "#include \"gemm\"\n#include \"mx4\"\n#include \"mx4_contract\"\nstruct Epi_" << nm << " {\n" << members.decls
+       << "  __device__ __forceinline__ void operator()(long, long m, long n, float v) const {\n" << rounded << epi.str() << "  }\n};\n"
+       << "struct Cfg_" << nm << " {\n  static constexpr long BATCH = 1, M = " << M << ", N = " << N << ", K = " << K << ";\n"
+       << "  static constexpr int BM = " << tile.bm << ", BN = " << tile.bn << ", GROUP_M = " << (M > N ? 4 : 8) << ", WK = " << tile.wk
+       << ", SPLITS = " << tile.splits << ";\n};\n";
+  const std::string own = "Epi_" + nm + "{" + members.inits + "}";
+  KernelWriter pw(g_, slots_, "i64_t");
+  std::string functor = own, partial_struct;
+  KernelWriter& kw = split ? pw : *w;
+  const std::string args = operands(kw);
+  int part = -1;
+  if (split) {
+    part = slots_.add(SlotInfo::Temp, -1, DType::f32, (uint64_t)tile.splits * (uint64_t)(M * N) * 4);
+    functor = "Part_" + nm + "{" + pw.arg(part, true) + "}";
+    partial_struct = "struct Part_" + nm + " {\n  float* __restrict__ p;\n  __device__ __forceinline__ void operator()(long, long m, long n, float v) const {\n    p[blockIdx.z * " +
+                     num(M * N) + "L + " + cidx + "] = v;\n  }\n};\n";
+  }
   KernelStep k;
-  k.source = src.str();
+  k.block[0] = tile.wk ? 64u * (uint32_t)tile.wk : 256u;
+  k.source = head.str() + partial_struct + "extern \"C\" __global__ void __launch_bounds__(" + std::to_string(k.block[0]) + ") " + nm + "(" + kw.params() + ") {\n  accy::mx4::" +
+             (tile.wk ? "contract_direct" : "contract_tile") + "<Cfg_" + nm + ">(" + args + functor + ");\n}\n";
   k.name = nm;
-  k.grid[0] = (uint32_t)((tiles + 3) / 4);
-  k.block[0] = 256;
+  const uint64_t groups = (uint64_t)((M + tile.bm - 1) / tile.bm) * (uint64_t)((N + tile.bn - 1) / tile.bn);
+  k.grid[0] = (uint32_t)groups;
+  k.grid[2] = (uint32_t)tile.splits;
   k.klass = "gemm";
   k.label = "mx4:%" + std::to_string(v) + (target != v ? "+%" + std::to_string(target) : "");
   k.algorithmic_flops = 2.0 * (double)M * (double)N * (double)K;
-  push(std::move(k), *w);
+  push(std::move(k), kw);
+  if (split) {
+    KernelStep sum;
+    sum.name = name("mx4_sum", v);
+    const std::string p = w->arg(part, false);
+    sum.source = head.str() + "extern \"C\" __global__ void __launch_bounds__(256) " + sum.name + "(" + w->params() + ") {\n  accy::split::sum<Cfg_" + nm +
+                 ">(" + p + ", " + own + ");\n}\n";
+    sum.grid[0] = grid_for((uint64_t)(M * N), 256);
+    sum.block[0] = 256;
+    sum.klass = "gemm";
+    sum.label = "mx4_sum:%" + std::to_string(target);
+    push(std::move(sum), *w);
+  }
   done_[v] = true;
   finish(target);
+}
+
+// The kernel, tile and K split of a product: the least of the times estimated for each, in us (kernels/mx4_contract.h). Small
+// tiles are bound by the bytes that a CU takes; a workgroup of a large one takes a time per step of 128 values that grows with the
+// workgroups at work (two of 128 x 128 to a CU, one of 256 x 256) and the time to store its results.
+// Measured (us back to back, 2.4 of them a launch; 128 x 128 / 256 x 256): 512 x 8192 x 2048 8.4 / 17.0, 1024 x 8192 x 2048 16.0 /
+// 19.6, 1536 x 8192 x 2048 21.8 / 21.6, 2048 x 8192 x 2048 28.3 / 24.5, 3000 x 8192 x 2048 42 / 48, 4096 x 4096 x 1024 19.4 /
+// 18.1, 8192^3 377 / 276; small / 128 x 128: 16 x 8192 x 2048 3.2 / 6.3, 64 x 8192 x 2048 5.3 / 6.4, 128 x 8192 x 2048 8 / 6.3.
+Planner::Mx4Tile Planner::mx4_tile(int64_t M, int64_t N, int64_t K) const {
+  auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const int64_t steps = up(K, 128), groups = up(steps, 4);
+  Mx4Tile best;
+  double least = 0;
+  auto offer = [&](const Mx4Tile& t, double cost) {
+    if (!launchable((uint64_t)(up(M, t.bm) * up(N, t.bn)), t.wk ? 64u * (unsigned)t.wk : 256u)) return;
+    if (best.bm && cost >= least) return;
+    best = t;
+    least = cost;
+  };
+  const int bm = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+  for (const int bn : {16, 32, 64}) {
+    if (bm == 64 && bn == 64) continue;  // 160 KB of LDS hold four stages of two waves' (64, 32)
+    Mx4Tile t;
+    t.bm = bm;
+    t.bn = bn;
+    const int64_t wgs = up(M, bm) * up(N, bn);
+    t.wk = bm + bn <= 48 && wgs <= 256 ? 4 : 2;
+    offer(t, 1.2 + (double)up(wgs, 256) * (double)((bm + bn) * K) * 0.53 / 42e3);
+  }
+  for (const int size : {128, 256}) {
+    const int64_t tiles = up(M, size) * up(N, size), most = size == 128 ? 512 : 256;
+    for (int splits = 1; splits <= (opt_.allow_split && size == 128 ? 8 : 1); splits *= 2) {
+      if (splits > 1 && up(groups, up(groups, splits)) != splits) continue;
+      const double share = (double)(splits > 1 ? up(groups, splits) * 4 : steps);
+      auto round = [&](double n) {
+        if (size == 128) return 0.3 + 1.8 * std::min(1.0, n / 256) + share * (0.25 + 0.45 * std::max(0.0, n - 256) / 256);
+        return 1.0 + 4.0 * n / 256 + share * (0.65 + 0.4 * n / 256);
+      };
+      const int64_t all = tiles * splits;
+      Mx4Tile t;
+      t.bm = t.bn = size;
+      t.splits = splits;
+      offer(t, (double)(all / most) * round((double)most) + (all % most ? round((double)(all % most)) : 0.0) + (K % 128 ? 2.6 : 0.0) +
+                   (splits > 1 ? 3.0 + (double)splits * (double)(M * N) * 8.0 / 4e6 : 0.0));
+    }
+  }
+  return best;
 }
 
 // ---- the paged cache ----

@@ -18,6 +18,7 @@ extern const char* const kAttentionDeviceSource;
 extern const char* const kScatterDeviceSource;
 extern const char* const kDecodeDeviceSource;
 extern const char* const kMx4DeviceSource;
+extern const char* const kMx4ContractDeviceSource;
 
 namespace {
 
@@ -64,7 +65,8 @@ std::string full_kernel_source(const std::string& body) {
                                                            {"#include \"attention\"\n", kAttentionDeviceSource},
                                                            {"#include \"scatter\"\n", kScatterDeviceSource},
                                                            {"#include \"decode\"\n", kDecodeDeviceSource},
-                                                           {"#include \"mx4\"\n", kMx4DeviceSource}};
+                                                           {"#include \"mx4\"\n", kMx4DeviceSource},
+                                                           {"#include \"mx4_contract\"\n", kMx4ContractDeviceSource}};
   std::string rest = body;
   for (const auto& t : templates) {
     size_t p = rest.find(t.first);

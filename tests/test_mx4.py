@@ -317,8 +317,22 @@ def test_contract(m, n, k, dtype):
     _check_product(hip_run(_product(m, n, k, dtype), ops)[0], ops, dtype)
 
 
+# the large tiles, ragged: 128 x 128 and 256 x 256, K in whole steps of 512, of 128 and neither, K split
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,k", [(3, 40, 96), (130, 300, 544), (600, 600, 1056)])
+@pytest.mark.parametrize("m,n,k,dtype,tile,splits", [
+    (1100, 4100, 672, "bf16", 128, 1), (260, 4100, 1280, "f16", 128, 1), (100, 8192, 128, "f32", 128, 1), (2500, 4100, 1184, "f32", 256, 1),
+    (2100, 4200, 1664, "bf16", 256, 1), (2100, 4200, 2048, "f16", 256, 1), (200, 1000, 8192, "bf16", 128, 4), (1024, 1000, 8320, "f32", 128, 1)])
+def test_contract_large(m, n, k, dtype, tile, splits):
+    prog = _product(m, n, k, dtype)
+    src = hip.plan_source(prog)
+    assert f"BM = {tile}, BN = {tile}" in src and f"SPLITS = {splits};" in src
+    ops = _operands(m, n, k, m + n + k)
+    say(f"contract {m} {n} {k} {dtype}")
+    _check_product(hip_run(prog, ops)[0], ops, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(3, 40, 96), (130, 300, 544), (600, 2600, 1056)])
 def test_contract_keeps_nan_blocks_to_their_rows(m, n, k):
     """A NaN scale makes the sums it is in NaN and no others, whatever the other scales are."""
     ops = _operands(m, n, k, 5)
@@ -334,7 +348,7 @@ def test_contract_keeps_nan_blocks_to_their_rows(m, n, k):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,k", [(4, 48, 64), (70, 300, 1024), (520, 512, 512)])
+@pytest.mark.parametrize("m,n,k", [(4, 48, 64), (70, 300, 1024), (520, 2512, 512), (200, 1000, 8192)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_contract_with_a_fused_epilogue(m, n, k, dtype):
     """An elementwise region after the product runs in its kernel: a bias, an activation and a residual."""
