@@ -215,17 +215,22 @@ __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const
 // key is 0. Scores, softmax and sums are f32.
 //
 // The Q x G rows that share a key-value head are the columns of 16-wide matrix instructions, NR sixteens of them per wave, so
-// the cache is read once for all of them. Per 32 keys a wave computes S^T = K Q^T (two v_mfma_f32_16x16x32_bf16 tiles of 16
-// keys per 32 dims): lane l holds row l % 16 and, g = l / 16, keys 4 g + i and 16 + 4 g + i, which is how the B operand of
-// O^T = V^T P^T wants them when its k index 8 g + j means key 4 g + j (j < 4) or 12 + 4 g + j, so P never leaves the lane. K's
-// codes go from memory to the A operand's lanes as they lie: lane l's HD / 4 dims of key l % 16 (g HD / 4 on) are
-// contiguous, and step s takes eight of them. V's rows are keys while its A operand wants eight keys of one dim: its codes
-// pass through LDS, where ds_read_b64_tr_b8 hands a lane one byte (two dims) of eight rows.
+// the cache is read once for all of them. Per 32 keys (a step) a wave computes S^T = K Q^T (two v_mfma_f32_16x16x32_bf16 tiles of
+// 16 keys per 32 dims): lane l holds row l % 16 and, g = l / 16, keys 4 g + i and 16 + 4 g + i, which is how the B operand of
+// O^T = V^T P^T wants them when its k index 8 g + j means key 4 g + j (j < 4) or 12 + 4 g + j, so P never leaves the lane. Of
+// K's dims, of which any order will do, lane l takes the HD / 4 from g HD / 4 on of key l % 16: they are contiguous. V's rows are
+// keys while its A operand wants eight keys of one dim: ds_read_b64_tr_b8 hands a lane one byte (two dims) of eight rows.
 //
 // fp4 with its scale is exact in bf16. Queries are split into PARTS bf16 parts (bf16 1, f16 2, f32 3: exact, or 24 bits), and the
-// probabilities likewise (PPARTS), one matrix instruction each: the sums keep f32's accuracy whatever the type.
+// probabilities likewise (PP), one matrix instruction each: the sums keep f32's accuracy whatever the type. A row's running
+// maximum follows the scores only where one exceeds it by 2^8: till then probabilities are at most 2^8 and sums need no
+// rescaling, nor the maximum its way through the lanes.
 //
-// Each wave takes every fourth 32 keys of the workgroup's range; the waves join through LDS, the SPLITS workgroups of a
+// A step's codes (32 HD bytes) and scales go straight to LDS, three stages of them per wave, each wave on its own: loads that
+// are in order, and 8 KB in flight per wave without a register. Rows of a power of two of 16-byte chunks are
+// swizzled so that the reads above meet every bank once.
+//
+// Each wave takes every fourth step of the workgroup's range; the waves join through LDS, the SPLITS workgroups of a
 // sequence and head through memory (m, l, O per row) and a second kernel. A range is a share of the sequence's own length.
 //
 // C supplies, besides the cache's, Q, G, MAXP (pages per sequence), SEQS, NR, SPLITS and SL = log2(e) / sqrt(HD).
@@ -235,7 +240,7 @@ __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const
 
 template <int DT> constexpr int query_parts() { return DT + 1; }
 
-// x as `PARTS` bf16 numbers whose sum is x (to 8 bits a part): the part, and what is left.
+// x as bf16 numbers whose sum is x (to 8 bits a part): the next part; x becomes what is left.
 __device__ __forceinline__ __bf16 take_part(float& x) {
   const __bf16 h = (__bf16)x;
   x -= (float)h;
@@ -249,6 +254,28 @@ template <class C> struct Rows {
   static constexpr int R = C::Q * C::G, TILES = (R + 15) / 16, GROUPS = (TILES + C::NR - 1) / C::NR;
 };
 
+// Where 16-byte chunk c of key's row lies within the row's chunks in LDS: 16 rows that are read at one chunk (keys; 32 lanes of
+// values read 16 rows, four of each eight) fall into different banks.
+template <int CH> __device__ __forceinline__ int key_chunk(int key, int c) {
+  if constexpr (CH == 2 || CH == 4 || CH == 8) return c ^ (key / (16 / CH) & (CH - 1));
+  else return c;
+}
+template <int CH> __device__ __forceinline__ int value_chunk(int key, int c) {
+  if constexpr (CH == 2) return c ^ (key >> 4 & 1);
+  else if constexpr (CH == 4) return c ^ ((key >> 2 & 1) | (key >> 3 & 2));
+  else if constexpr (CH == 8) return c ^ ((key >> 1 & 3) | (key >> 2 & 4));
+  else return c;
+}
+
+// Four bf16 pairs as the eight elements of a matrix operand.
+__device__ __forceinline__ bf16x8 eight(bf16x2 a, bf16x2 b, bf16x2 c, bf16x2 d) { return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
+
+template <int I> __device__ __forceinline__ bf16x2 pair_of_byte(u32_t w, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, I);
+}
+
+template <int N> struct Number { static constexpr int value = N; };
+
 template <class C>
 __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restrict__ Q, const u8_t* __restrict__ cache,
                                        const int* __restrict__ pages, const int* __restrict__ lengths,
@@ -256,18 +283,21 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   typedef Page<C> P;
   typedef Rows<C> RS;
   constexpr int HD = C::HD, NB = HD / 32, PARTS = query_parts<C::DT>(), PP = C::DT == 2 ? 3 : 2, NR = C::NR;
-  constexpr int KB = HD / 8;             // bytes of a lane's share of a key
-  constexpr int VPITCH = HD / 2 + 8;     // LDS pitch of a value row
-  constexpr int VCH = (32 * HD / 2 + 1023) / 1024;  // 16-byte chunks per lane of 32 value rows
-  __shared__ __attribute__((aligned(16))) u8_t vs[4][32 * VPITCH];
-  __shared__ float joined[2][16 * (HD + 4)];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, r = lane & 15;
+  constexpr int CODES = 16 * HD, SCALES = 32 * NB;  // bytes of a step's keys, or values, in LDS
+  constexpr int DC = 2 * HD / 64, DS = (16 * NB + 63) / 64, PER = DC + DS;  // load instructions of a step
+  constexpr int STAGE = 2 * CODES + 256 * DS;
+  __shared__ __attribute__((aligned(1024))) u8_t l0[4][STAGE], l1[4][STAGE], l2[4][STAGE];
+  __shared__ __attribute__((aligned(16))) float joined[2][16 * (HD + 4)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
+  u8_t* const stage[3] = {l0[wave], l1[wave], l2[wave]};
   const long bh = blockIdx.x / RS::GROUPS, b = bh / C::H, h = bh % C::H;
   const int row0 = (int)(blockIdx.x % RS::GROUPS) * NR * 16;
-  int len = lengths[b];
+  int len = C::P > 0 ? lengths[b] : 0;
   len = len < 0 ? 0 : len > C::MAXP * C::T ? C::MAXP * C::T : len;
+  len = __builtin_amdgcn_readfirstlane(len);
   const int steps = (len + 31) / 32, per = (steps + C::SPLITS - 1) / C::SPLITS;
   const int first = (int)blockIdx.y * per, end = first + per < steps ? first + per : steps;
+  const int sure = len - (C::Q - 1);  // keys below it are seen by every row
 
   // queries: the B operand of S^T, row r of each tile, dims g HD / 4 + 8 s + j at step s
   bf16x8 q[NR][NB][PARTS];
@@ -287,8 +317,6 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
         for (int j = 0; j < 8; ++j) q[t][s][p][j] = take_part(x[j]);
     }
   }
-  const int sure = len - (C::Q - 1);  // keys below it are seen by every row
-
   f32x4 o[NR][NB][2];
   float m[NR], l[NR];
 #pragma unroll
@@ -299,132 +327,169 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     for (int d = 0; d < NB; ++d) o[t][d][0] = o[t][d][1] = f32x4{0, 0, 0, 0};
   }
 
-  for (int step = first + wave; step < end; step += 4) {
-    const int k0 = step * 32, page = pages[b * C::MAXP + k0 / C::T];
-    if (page < 0 || page >= C::P) continue;
-    const u8_t* const head = P::head(cache, page, h);
-    const int in = k0 % C::T;
-    // values into LDS
+  // Loads: chunk x = 64 i + lane of a step's LDS, keys and then values; then the scales, a word a lane.
+  int from[DC], sfrom[DS];
 #pragma unroll
-    for (int c = 0; c < VCH; ++c) {
-      const int chunk = c * 64 + lane;
-      if (32 * HD / 2 % 1024 == 0 || chunk < 32 * HD / 32) {
-        const u32x4 w = *(const u32x4*)(head + P::codes(true, in) + 16 * chunk);
-        u8_t* const p = &vs[wave][chunk / (HD / 32) * VPITCH + chunk % (HD / 32) * 16];
-        *(u32x2*)p = u32x2{w[0], w[1]};
-        *(u32x2*)(p + 8) = u32x2{w[2], w[3]};
-      }
-    }
-    // other lanes' rows are read below: no access may move across
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    // scores
+  for (int i = 0; i < DC; ++i) {
+    const int x = 64 * i + lane, value = x >= HD, y = value ? x - HD : x, row = y / NB, c = y % NB;
+    from[i] = value ? (int)P::CODES + row * (HD / 2) + 16 * value_chunk<NB>(row, c) : row * (HD / 2) + 16 * key_chunk<NB>(row, c);
+  }
+#pragma unroll
+  for (int i = 0; i < DS; ++i) {
+    const int x = 64 * i + lane < 16 * NB ? 64 * i + lane : 16 * NB - 1, value = x >= 8 * NB;
+    sfrom[i] = (int)(2 * P::CODES) + (value ? (int)P::SCALES + 4 * (x - 8 * NB) : 4 * x);
+  }
+  auto page_of = [&](int step) { return step < end ? __builtin_amdgcn_readfirstlane(pages[b * C::MAXP + step * 32 / C::T]) : 0; };
+  auto load = [&](int s, int step, int page) {
+    const int in = step * 32 % C::T;
+    const u8_t* const head = P::head(cache, page >= 0 && page < C::P ? page : 0, h);
+    const u8_t *const codes = head + in * (HD / 2), *const scales = head + in * NB;
+#pragma unroll
+    for (int i = 0; i < DC; ++i) __builtin_amdgcn_global_load_lds(codes + from[i], (ACCY_MX4_LDS void*)(stage[s] + 1024 * i), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < DS; ++i)
+      __builtin_amdgcn_global_load_lds(scales + sfrom[i], (ACCY_MX4_LDS void*)(stage[s] + 2 * CODES + 256 * i), 4, 0, 0);
+  };
+  auto wait = [&](auto left) {
+    constexpr int N = decltype(left)::value;
+    static_assert(N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));  // vmcnt(N)
+    asm volatile("" ::: "memory");
+  };
+
+  auto compute = [&](int s, int step, int page, auto tail_) {
+    constexpr bool TAIL = decltype(tail_)::value != 0;
+    const int k0 = step * 32;
+    const u8_t *const ks = stage[s], *const vs = ks + CODES, *const kscale = vs + CODES, *const vscale = kscale + SCALES;
     f32x4 sc[NR][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int key = in + 16 * u + r;
+      const int key = 16 * u + r;
       u32_t kw[NB];
-      const u8_t* const kp = head + P::codes(false, key) + g * KB;
+      if constexpr (NB % 4 == 0) {
 #pragma unroll
-      for (int s = 0; s < NB; ++s) kw[s] = *(const u32_t*)(kp + 4 * s);
+        for (int c = 0; c < NB / 4; ++c) {
+          const u32x4 w = *(const u32x4*)(ks + key * (HD / 2) + 16 * key_chunk<NB>(key, g * (NB / 4) + c));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) kw[4 * c + e] = w[e];
+        }
+      } else if constexpr (NB == 2) {
+        const u32x2 w = *(const u32x2*)(ks + key * (HD / 2) + 16 * key_chunk<NB>(key, g >> 1) + 8 * (g & 1));
+        kw[0] = w[0], kw[1] = w[1];
+      } else {
+#pragma unroll
+        for (int e = 0; e < NB; ++e) kw[e] = *(const u32_t*)(ks + key * (HD / 2) + g * (HD / 8) + 4 * e);
+      }
 #pragma unroll
       for (int t = 0; t < NR; ++t) sc[t][u] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int s = 0; s < NB; ++s) {
-        const float scale = scale_of(head[P::scales(false, key) + (g * (HD / 4) + 8 * s) / 32]);
-        bf16x8 a;
-        const bf16x2 a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(kw[s], scale, 0), a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(kw[s], scale, 1);
-        const bf16x2 a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(kw[s], scale, 2), a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(kw[s], scale, 3);
-        a[0] = a0[0], a[1] = a0[1], a[2] = a1[0], a[3] = a1[1], a[4] = a2[0], a[5] = a2[1], a[6] = a3[0], a[7] = a3[1];
+      for (int e = 0; e < NB; ++e) {
+        const float x = scale_of(kscale[key * NB + (g * (HD / 4) + 8 * e) / 32]);
+        const bf16x8 a = eight(pair_of_byte<0>(kw[e], x), pair_of_byte<1>(kw[e], x), pair_of_byte<2>(kw[e], x), pair_of_byte<3>(kw[e], x));
 #pragma unroll
         for (int t = 0; t < NR; ++t)
 #pragma unroll
-          for (int p = 0; p < PARTS; ++p) sc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[t][s][p], sc[t][u], 0, 0, 0);
+          for (int p = 0; p < PARTS; ++p) sc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[t][e][p], sc[t][u], 0, 0, 0);
       }
     }
-    // softmax: lane's keys are k0 + 16 u + 4 g + i
+    // The scores' maximum over the lane's keys k0 + 16 u + 4 g + i, those that the row does not see left out.
+    float top[NR];
+    bool above = false;
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
-      float top = m[t];
+      top[t] = -__builtin_inff();
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float s = sc[t][u][i] * C::SL;
-          sc[t][u][i] = k0 + 16 * u + 4 * g + i < limit[t] ? s : -__builtin_inff();
-          top = fmaxf(top, sc[t][u][i]);
+          if constexpr (TAIL) sc[t][u][i] = k0 + 16 * u + 4 * g + i < limit[t] && page >= 0 && page < C::P ? sc[t][u][i] : -__builtin_inff();
+          top[t] = fmaxf(top[t], sc[t][u][i]);
         }
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float base = base_of(top), alpha = __builtin_amdgcn_exp2f(m[t] - base);
-      m[t] = top;
-      l[t] *= alpha;
-#pragma unroll
-      for (int d = 0; d < NB; ++d)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[t][d][e][i] *= alpha;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sc[t][u][i] = __builtin_amdgcn_exp2f(sc[t][u][i] - base);
-          l[t] += sc[t][u][i];
-        }
+      top[t] *= C::SL;
+      above |= top[t] > m[t] + 8.0f;  // also where m is -inf and a key is seen
     }
-    // scale bytes of the lane's eight keys
-    u8_t vb[8][NB];
-    bool nan = false;
+    if (__builtin_amdgcn_ballot_w64(above) != 0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int key = 4 * g + (j & 3) + (j >> 2) * 16;
+      for (int t = 0; t < NR; ++t) {
+        top[t] = fmaxf(top[t], __shfl_xor(top[t], 16, 64));
+        top[t] = fmaxf(top[t], __shfl_xor(top[t], 32, 64));
+        top[t] = fmaxf(top[t], m[t]);
+        const float alpha = __builtin_amdgcn_exp2f(m[t] - base_of(top[t]));
+        m[t] = top[t];
+        l[t] *= alpha;
 #pragma unroll
-      for (int d = 0; d < NB; ++d) {
-        vb[j][d] = head[P::scales(true, in + key) + d];
-        nan |= k0 + key >= sure && k0 + key < len && vb[j][d] == 255;
+        for (int d = 0; d < NB; ++d)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][d][e][i] *= alpha;
       }
     }
+    bf16x8 pr[NR][PP];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+      const float base = base_of(m[t]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], C::SL, -base));
+        l[t] += p;
+#pragma unroll
+        for (int e = 0; e < PP; ++e) pr[t][e][j] = take_part(p);
+      }
+    }
+    // scale bytes of the lane's eight keys: four rows of NB bytes, twice
+    u32_t vw[2][NB];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < NB; ++e) vw[u][e] = *(const u32_t*)(vscale + (16 * u + 4 * g) * NB + 4 * e);
+    auto vbyte = [&](int j, int d) { const int at = (j & 3) * NB + d; return vw[j >> 2][at >> 2] >> (8 * (at & 3)) & 255; };
     // A key that only some rows see must not reach the others where it is NaN (0 x NaN): then one query at a time, with
     // what that query does not see left out. Keys past the end are left out always.
-    const bool apart = C::Q > 1 && __builtin_amdgcn_ballot_w64(nan) != 0;
-#pragma unroll 1
-    for (int only = apart ? 0 : C::Q - 1; only < C::Q; ++only) {
-      const int seen = len - (C::Q - 1 - only);
+    bool apart = false;
+    if constexpr (TAIL && C::Q > 1) {
+      bool nan = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = k0 + 4 * g + (j & 3) + (j >> 2) * 16;
+#pragma unroll
+        for (int d = 0; d < NB; ++d) nan |= key >= sure && key < len && vbyte(j, d) == 255;
+      }
+      apart = __builtin_amdgcn_ballot_w64(nan) != 0;
+    }
+    auto weigh = [&](int only) {
+      const int seen = page >= 0 && page < C::P ? len - (C::Q - 1 - only) : 0;
 #pragma unroll
       for (int d = 0; d < NB; ++d) {
         // lanes 2 t and 2 t + 1 of sixteen address the block's bytes of their t-th key
-        const int t = r >> 1, key = 4 * g + (t & 3) + (t >> 2) * 16;
-        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((ACCY_MX4_LDS i32x2*)&vs[wave][key * VPITCH + 16 * d + 8 * (r & 1)]);
+        const int tk = r >> 1, at = 4 * g + (tk & 3) + (tk >> 2) * 16;
+        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((ACCY_MX4_LDS i32x2*)(vs + at * (HD / 2) + 16 * value_chunk<NB>(at, d) + 8 * (r & 1)));
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          u32_t byte = vbyte(j, d);
+          if constexpr (TAIL) byte = k0 + 4 * g + (j & 3) + (j >> 2) * 16 < seen ? byte : 0;
+          x[j] = scale_of(byte);
+        }
+        const bf16x2 y[8] = {pair_of_byte<0>((u32_t)w[0], x[0]), pair_of_byte<1>((u32_t)w[0], x[1]), pair_of_byte<2>((u32_t)w[0], x[2]),
+                             pair_of_byte<3>((u32_t)w[0], x[3]), pair_of_byte<0>((u32_t)w[1], x[4]), pair_of_byte<1>((u32_t)w[1], x[5]),
+                             pair_of_byte<2>((u32_t)w[1], x[6]), pair_of_byte<3>((u32_t)w[1], x[7])};
         bf16x8 even, odd;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int key = 4 * g + (j & 3) + (j >> 2) * 16;
-          const float scale = scale_of(k0 + key < seen ? vb[j][d] : 0);
-          const u32_t word = (u32_t)w[j >> 2];
-          bf16x2 x;
-          if ((j & 3) == 0) x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0);
-          else if ((j & 3) == 1) x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1);
-          else if ((j & 3) == 2) x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2);
-          else x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3);
-          even[j] = x[0];
-          odd[j] = x[1];
+          even[j] = y[j][0];
+          odd[j] = y[j][1];
         }
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
-          const bool mine = !apart || (row0 + 16 * t + r) / C::G == only;
           const f32x4 before[2] = {o[t][d][0], o[t][d][1]};
-          float x[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = sc[t][j >> 2][j & 3];
 #pragma unroll
           for (int p = 0; p < PP; ++p) {
-            bf16x8 pr;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) pr[j] = take_part(x[j]);
-            o[t][d][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, pr, o[t][d][0], 0, 0, 0);
-            o[t][d][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, pr, o[t][d][1], 0, 0, 0);
+            o[t][d][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, pr[t][p], o[t][d][0], 0, 0, 0);
+            o[t][d][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, pr[t][p], o[t][d][1], 0, 0, 0);
           }
-          if constexpr (C::Q > 1) {
+          if constexpr (TAIL && C::Q > 1) {
+            const bool mine = !apart || (row0 + 16 * t + r) / C::G == only;
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -432,8 +497,41 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
           }
         }
       }
+    };
+    if constexpr (TAIL && C::Q > 1) {
+#pragma unroll 1
+      for (int only = apart ? 0 : C::Q - 1; only < C::Q; ++only) weigh(only);
+    } else {
+      weigh(C::Q - 1);
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+
+  {
+    int step = first + wave, page[3] = {page_of(step), page_of(step + 4), 0}, ahead = page_of(step + 8);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (step + 4 * s < end) load(s, step + 4 * s, page[s]);
+    for (; step < end; step += 12) {
+#pragma unroll
+      for (int s = 0; s < 3; ++s) {
+        const int now = step + 4 * s;
+        if (now >= end) break;
+        // This stage has landed when no more than the next one's and the one's after are outstanding; where no more follow, when
+        // nothing is.
+        if (now + 8 < end) {
+          page[(s + 2) % 3] = ahead;
+          load((s + 2) % 3, now + 8, ahead);
+          ahead = page_of(now + 12);
+          wait(Number<2 * PER>());
+        } else {
+          wait(Number<0>());
+        }
+        if (now * 32 + 32 <= sure && page[s] >= 0 && page[s] < C::P) compute(s, now, page[s], Number<0>());
+        else compute(s, now, page[s], Number<1>());
+        __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0): the stage may be overwritten
+        asm volatile("" ::: "memory");
+      }
+    }
   }
 
   // The waves: 2 and 3 hand theirs to 0 and 1, then 1 to 0. Lane (r, g) holds dims 32 d + 8 g .. + 7 of row r: even ones in
