@@ -286,10 +286,18 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   constexpr int CODES = 16 * HD, SCALES = 32 * NB;  // bytes of a step's keys, or values, in LDS
   constexpr int DC = 2 * HD / 64, DS = (16 * NB + 63) / 64, PER = DC + DS;  // load instructions of a step
   constexpr int STAGE = 2 * CODES + 256 * DS;
-  __shared__ __attribute__((aligned(1024))) u8_t l0[4][STAGE], l1[4][STAGE], l2[4][STAGE];
-  __shared__ __attribute__((aligned(16))) float joined[2][16 * (HD + 4)];
+  // One array per stage: the compiler can then tell a stage's reads from the loads still on their way into the others.
+  __shared__ __attribute__((aligned(1024))) u8_t l0[4 * STAGE], l1[4 * STAGE], l2[4 * STAGE];
+  // the waves' meeting place, once the steps are done (every load has landed by then): two waves' rows
+  constexpr int JOIN = 16 * (HD + 4) * 4;
+  static_assert(JOIN <= 4 * STAGE, "a stage of the four waves holds a wave's rows");
+  auto joined = [&](int w) { return (float*)(w ? l1 : l0); };
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
-  u8_t* const stage[3] = {l0[wave], l1[wave], l2[wave]};
+  auto stage = [&](auto s) -> u8_t* {
+    if constexpr (decltype(s)::value == 0) return l0;
+    else if constexpr (decltype(s)::value == 1) return l1;
+    else return l2;
+  };
   const long bh = blockIdx.x / RS::GROUPS, b = bh / C::H, h = bh % C::H;
   const int row0 = (int)(blockIdx.x % RS::GROUPS) * NR * 16;
   int len = C::P > 0 ? lengths[b] : 0;
@@ -328,27 +336,27 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   }
 
   // Loads: chunk x = 64 i + lane of a step's LDS, keys and then values; then the scales, a word a lane.
-  int from[DC], sfrom[DS];
+  u32_t from[DC], sfrom[DS];
 #pragma unroll
   for (int i = 0; i < DC; ++i) {
     const int x = 64 * i + lane, value = x >= HD, y = value ? x - HD : x, row = y / NB, c = y % NB;
-    from[i] = value ? (int)P::CODES + row * (HD / 2) + 16 * value_chunk<NB>(row, c) : row * (HD / 2) + 16 * key_chunk<NB>(row, c);
+    from[i] = value ? (u32_t)P::CODES + row * (HD / 2) + 16 * value_chunk<NB>(row, c) : row * (HD / 2) + 16 * key_chunk<NB>(row, c);
   }
 #pragma unroll
   for (int i = 0; i < DS; ++i) {
     const int x = 64 * i + lane < 16 * NB ? 64 * i + lane : 16 * NB - 1, value = x >= 8 * NB;
-    sfrom[i] = (int)(2 * P::CODES) + (value ? (int)P::SCALES + 4 * (x - 8 * NB) : 4 * x);
+    sfrom[i] = (u32_t)(2 * P::CODES) + (value ? (u32_t)P::SCALES + 4 * (x - 8 * NB) : 4 * x);
   }
   auto page_of = [&](int step) { return step < end ? __builtin_amdgcn_readfirstlane(pages[b * C::MAXP + step * 32 / C::T]) : 0; };
-  auto load = [&](int s, int step, int page) {
+  auto load = [&](auto s, int step, int page) {
     const int in = step * 32 % C::T;
     const u8_t* const head = P::head(cache, page >= 0 && page < C::P ? page : 0, h);
     const u8_t *const codes = head + in * (HD / 2), *const scales = head + in * NB;
 #pragma unroll
-    for (int i = 0; i < DC; ++i) __builtin_amdgcn_global_load_lds(codes + from[i], (ACCY_MX4_LDS void*)(stage[s] + 1024 * i), 16, 0, 0);
+    for (int i = 0; i < DC; ++i) __builtin_amdgcn_global_load_lds(codes + from[i], (ACCY_MX4_LDS void*)(stage(s) + wave * STAGE + 1024 * i), 16, 0, 0);
 #pragma unroll
     for (int i = 0; i < DS; ++i)
-      __builtin_amdgcn_global_load_lds(scales + sfrom[i], (ACCY_MX4_LDS void*)(stage[s] + 2 * CODES + 256 * i), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds(scales + sfrom[i], (ACCY_MX4_LDS void*)(stage(s) + wave * STAGE + 2 * CODES + 256 * i), 4, 0, 0);
   };
   auto wait = [&](auto left) {
     constexpr int N = decltype(left)::value;
@@ -357,34 +365,48 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     asm volatile("" ::: "memory");
   };
 
-  auto compute = [&](int s, int step, int page, auto tail_) {
+  // Where in a stage the lane reads: its share of key r's codes (of key 16 + r 8 HD bytes on) and key r's scales; a block's bytes of
+  // its value row, which lanes 2 t and 2 t + 1 of sixteen have for their t-th key; the scales of values 4 g .. (16 on: those of 16 + 4 g).
+  constexpr int KC = NB % 4 == 0 ? NB / 4 : 1;
+  u32_t kat[KC], vat[NB];
+#pragma unroll
+  for (int c = 0; c < KC; ++c)
+    kat[c] = wave * STAGE + r * (HD / 2) +
+             (NB % 4 == 0 ? 16 * key_chunk<NB>(r, g * KC + c) : NB == 2 ? 16 * key_chunk<NB>(r, g >> 1) + 8 * (g & 1) : g * (HD / 8));
+  const u32_t ksat = wave * STAGE + 2 * CODES + r * NB, vsat = wave * STAGE + 2 * CODES + SCALES + 4 * g * NB;
+#pragma unroll
+  for (int d = 0; d < NB; ++d) {
+    const int tk = r >> 1, key = 4 * g + (tk & 3) + (tk >> 2) * 16;
+    vat[d] = wave * STAGE + CODES + key * (HD / 2) + 16 * value_chunk<NB>(key, d) + 8 * (r & 1);
+  }
+
+  auto compute = [&](auto s, int step, int page, auto tail_) {
     constexpr bool TAIL = decltype(tail_)::value != 0;
     const int k0 = step * 32;
-    const u8_t *const ks = stage[s], *const vs = ks + CODES, *const kscale = vs + CODES, *const vscale = kscale + SCALES;
+    const u8_t* const lds = stage(s);
     f32x4 sc[NR][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int key = 16 * u + r;
       u32_t kw[NB];
       if constexpr (NB % 4 == 0) {
 #pragma unroll
-        for (int c = 0; c < NB / 4; ++c) {
-          const u32x4 w = *(const u32x4*)(ks + key * (HD / 2) + 16 * key_chunk<NB>(key, g * (NB / 4) + c));
+        for (int c = 0; c < KC; ++c) {
+          const u32x4 w = *(const u32x4*)(lds + kat[c] + u * 8 * HD);
 #pragma unroll
           for (int e = 0; e < 4; ++e) kw[4 * c + e] = w[e];
         }
       } else if constexpr (NB == 2) {
-        const u32x2 w = *(const u32x2*)(ks + key * (HD / 2) + 16 * key_chunk<NB>(key, g >> 1) + 8 * (g & 1));
+        const u32x2 w = *(const u32x2*)(lds + kat[0] + u * 8 * HD);
         kw[0] = w[0], kw[1] = w[1];
       } else {
 #pragma unroll
-        for (int e = 0; e < NB; ++e) kw[e] = *(const u32_t*)(ks + key * (HD / 2) + g * (HD / 8) + 4 * e);
+        for (int e = 0; e < NB; ++e) kw[e] = *(const u32_t*)(lds + kat[0] + u * 8 * HD + 4 * e);
       }
 #pragma unroll
       for (int t = 0; t < NR; ++t) sc[t][u] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int e = 0; e < NB; ++e) {
-        const float x = scale_of(kscale[key * NB + (g * (HD / 4) + 8 * e) / 32]);
+        const float x = scale_of(lds[ksat + u * 16 * NB + (g * (HD / 4) + 8 * e) / 32]);
         const bf16x8 a = eight(pair_of_byte<0>(kw[e], x), pair_of_byte<1>(kw[e], x), pair_of_byte<2>(kw[e], x), pair_of_byte<3>(kw[e], x));
 #pragma unroll
         for (int t = 0; t < NR; ++t)
@@ -442,8 +464,13 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int e = 0; e < NB; ++e) vw[u][e] = *(const u32_t*)(vscale + (16 * u + 4 * g) * NB + 4 * e);
+      for (int e = 0; e < NB; ++e) vw[u][e] = *(const u32_t*)(lds + vsat + 16 * u * NB + 4 * e);
     auto vbyte = [&](int j, int d) { const int at = (j & 3) * NB + d; return vw[j >> 2][at >> 2] >> (8 * (at & 3)) & 255; };
+    // The conversions take the scale's exponent bits alone, so its other bits may be the neighbouring bytes'.
+    auto vscale = [&](int j, int d) {
+      const int at = (j & 3) * NB + d, by = 23 - 8 * (at & 3);
+      return by >= 0 ? vw[j >> 2][at >> 2] << by : vw[j >> 2][at >> 2] >> -by;
+    };
     // A key that only some rows see must not reach the others where it is NaN (0 x NaN): then one query at a time, with
     // what that query does not see left out. Keys past the end are left out always.
     bool apart = false;
@@ -461,15 +488,13 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
       const int seen = page >= 0 && page < C::P ? len - (C::Q - 1 - only) : 0;
 #pragma unroll
       for (int d = 0; d < NB; ++d) {
-        // lanes 2 t and 2 t + 1 of sixteen address the block's bytes of their t-th key
-        const int tk = r >> 1, at = 4 * g + (tk & 3) + (tk >> 2) * 16;
-        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((ACCY_MX4_LDS i32x2*)(vs + at * (HD / 2) + 16 * value_chunk<NB>(at, d) + 8 * (r & 1)));
+        const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((ACCY_MX4_LDS i32x2*)(lds + vat[d]));
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          u32_t byte = vbyte(j, d);
-          if constexpr (TAIL) byte = k0 + 4 * g + (j & 3) + (j >> 2) * 16 < seen ? byte : 0;
-          x[j] = scale_of(byte);
+          u32_t scale = vscale(j, d);
+          if constexpr (TAIL) scale = k0 + 4 * g + (j & 3) + (j >> 2) * 16 < seen ? scale : 0;
+          x[j] = __builtin_bit_cast(float, scale);
         }
         const bf16x2 y[8] = {pair_of_byte<0>((u32_t)w[0], x[0]), pair_of_byte<1>((u32_t)w[0], x[1]), pair_of_byte<2>((u32_t)w[0], x[2]),
                              pair_of_byte<3>((u32_t)w[0], x[3]), pair_of_byte<0>((u32_t)w[1], x[4]), pair_of_byte<1>((u32_t)w[1], x[5]),
@@ -507,30 +532,32 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   };
 
   {
-    int step = first + wave, page[3] = {page_of(step), page_of(step + 4), 0}, ahead = page_of(step + 8);
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (step + 4 * s < end) load(s, step + 4 * s, page[s]);
-    for (; step < end; step += 12) {
-#pragma unroll
-      for (int s = 0; s < 3; ++s) {
-        const int now = step + 4 * s;
-        if (now >= end) break;
-        // This stage has landed when no more than the next one's and the one's after are outstanding; where no more follow, when
-        // nothing is.
-        if (now + 8 < end) {
-          page[(s + 2) % 3] = ahead;
-          load((s + 2) % 3, now + 8, ahead);
-          ahead = page_of(now + 12);
-          wait(Number<2 * PER>());
-        } else {
-          wait(Number<0>());
-        }
-        if (now * 32 + 32 <= sure && page[s] >= 0 && page[s] < C::P) compute(s, now, page[s], Number<0>());
-        else compute(s, now, page[s], Number<1>());
-        __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0): the stage may be overwritten
-        asm volatile("" ::: "memory");
+    int step = first + wave, p0 = page_of(step), p1 = page_of(step + 4), p2 = page_of(step + 8);
+    // Stage S holds step `now` of page `mine`; the step two stages on goes to stage S + 2, its page into `mine`.
+    auto turn = [&](auto s, auto two, int now, int& mine, int next) {
+      // This stage has landed when no more than the next one's and the one's after are outstanding; where no more follow, when
+      // nothing is.
+      const int page = mine;
+      if (now + 8 < end) {
+        load(two, now + 8, next);
+        mine = page_of(now + 12);
+        wait(Number<2 * PER>());
+      } else {
+        wait(Number<0>());
       }
+      if (now * 32 + 32 <= sure && page >= 0 && page < C::P) compute(s, now, page, Number<0>());
+      else compute(s, now, page, Number<1>());
+      __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0): the stage may be overwritten
+      asm volatile("" ::: "memory");
+    };
+    if (step < end) load(Number<0>(), step, p0);
+    if (step + 4 < end) load(Number<1>(), step + 4, p1);
+    for (; step < end; step += 12) {
+      turn(Number<0>(), Number<2>(), step, p0, p2);
+      if (step + 4 >= end) break;
+      turn(Number<1>(), Number<0>(), step + 4, p1, p0);
+      if (step + 8 >= end) break;
+      turn(Number<2>(), Number<1>(), step + 8, p2, p1);
     }
   }
 
@@ -544,7 +571,7 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     for (int from = 2; from > 0; from >>= 1) {
       __syncthreads();
       if (wave >= from && wave < 2 * from) {
-        float* const p = &joined[wave - from][r * (HD + 4)];
+        float* const p = joined(wave - from) + r * (HD + 4);
 #pragma unroll
         for (int d = 0; d < NB; ++d)
 #pragma unroll
@@ -559,7 +586,7 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
       }
       __syncthreads();
       if (wave < from) {
-        const float* const p = &joined[wave][r * (HD + 4)];
+        const float* const p = joined(wave) + r * (HD + 4);
         const float top = fmaxf(m[t], p[HD]), base = base_of(top);
         const float mine = __builtin_amdgcn_exp2f(m[t] - base), theirs = __builtin_amdgcn_exp2f(p[HD] - base);
         m[t] = top;

@@ -514,6 +514,7 @@ void Planner::mx4_attend(uint32_t v) {
     const int64_t steps = (maxp * c.tokens + 31) / 32;
     int64_t splits = 1;
     while (opt_.allow_split && splits < 64 && wgs * splits < 1024 && steps >= 16 * splits) splits *= 2;
+    if (std::getenv("MX4_SPLITS")) splits = std::atoi(std::getenv("MX4_SPLITS"));
     require(launchable((uint64_t)wgs, 256), op, "more workgroups than a launch takes");
     KernelWriter w(g_, slots_, "i64_t");
     const std::string q = w.arg(qs, false), a = w.arg(cs, false), p = w.arg(ps, false), l = w.arg(ls, false);
@@ -527,7 +528,7 @@ void Planner::mx4_attend(uint32_t v) {
                              ", G = " + num(G) + ", MAXP = " + num(maxp) + ", NR = " + num(NR) + ", SPLITS = " + num(splits) +
                              ";\n  static constexpr long SEQS = " + num(seqs) + ";\n  static constexpr float SL = " + sl + ";\n};\n";
     KernelStep k;
-    k.source = head + "extern \"C\" __global__ void __launch_bounds__(256) " + nm + "(" + w.params() + ") {\n  accy::mx4::attend<Cfg_" + nm +
+    k.source = head + "extern \"C\" __global__ void __launch_bounds__(" + std::string(std::getenv("MX4_LB") ? std::getenv("MX4_LB") : "256, 2") + ") " + nm + "(" + w.params() + ") {\n  accy::mx4::attend<Cfg_" + nm +
                ">(" + q + ", " + a + ", " + p + ", " + l + ", " + o + ", " + pp + ");\n}\n";
     k.name = nm;
     k.grid[0] = (uint32_t)wgs;
