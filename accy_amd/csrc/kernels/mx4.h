@@ -134,7 +134,8 @@ template <class C> struct Page {
 // The rows of TOKENS tokens, keys and values [token, head, dim], quantised into their slots: TW tokens per workgroup, eight
 // values of both per thread and step. A slot outside the cache writes nothing, and of two tokens of one slot the later
 // one is kept, so that codes and scales are always one token's. With few tokens every workgroup looks through the slots
-// after its own for them; with OWNERS, `owner` holds the last token of each slot (claim, before).
+// after its own for them, eight loads at a time and its first rows already on their way; with OWNERS, `owner` holds the last
+// token of each slot (claim, before).
 template <class C> struct Write {
   static constexpr int ROW = C::H * C::HD / 8, TW = ROW >= 512 ? 1 : 512 / ROW;
 };
@@ -146,6 +147,16 @@ __device__ __forceinline__ void cache_write(u8_t* __restrict__ cache, const type
   __shared__ int place[TW];
   const int tid = threadIdx.x;
   const long t0 = (long)blockIdx.x * TW;
+  float k[2][8], v[2][8];
+  auto fetch = [&](int u, int i) {
+    const long at = t0 * C::H * C::HD + (long)i * 8;
+    if (i < TW * ROW && t0 + i / ROW < C::TOKENS) {
+      load8<C::DT>(keys + at, k[u]);
+      load8<C::DT>(values + at, v[u]);
+    }
+  };
+  fetch(0, tid);
+  fetch(1, 256 + tid);
   if (tid < TW) {
     int s = t0 + tid < C::TOKENS ? slots[t0 + tid] : -1;
     if (s < 0 || s >= C::P * C::T) s = -1;
@@ -156,27 +167,33 @@ __device__ __forceinline__ void cache_write(u8_t* __restrict__ cache, const type
   }
   __syncthreads();
   if constexpr (!OWNERS) {
-    for (long j = t0 + 1 + tid; j < C::TOKENS; j += 256) {
-      const int s = slots[j];
-      for (int w = 0; w < TW && t0 + w < j; ++w)
-        if (place[w] == s) place[w] = -1;
+    for (long j0 = t0 + 1 + tid; j0 < C::TOKENS; j0 += 2048) {
+      int s[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s[u] = slots[j0 + 256 * u < C::TOKENS ? j0 + 256 * u : C::TOKENS - 1];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        for (int w = 0; w < TW && t0 + w < (j0 + 256 * u < C::TOKENS ? j0 + 256 * u : C::TOKENS - 1); ++w)
+          if (place[w] == s[u]) place[w] = -1;
     }
     __syncthreads();
   }
-  for (int i = tid; i < TW * ROW; i += 256) {
-    const int w = i / ROW, h = i % ROW / (C::HD / 8), c = i % (C::HD / 8) * 8, s = place[w];
-    if (s < 0) continue;
-    const long at = (t0 + w) * C::H * C::HD + h * C::HD + c;
-    float k[8], v[8];
-    load8<C::DT>(keys + at, k);
-    load8<C::DT>(values + at, v);
-    u8_t* const page = cache + ((long)(s / C::T) * C::H + h) * Page<C>::BYTES;
-    const u32_t ks = block_scale(k), vs = block_scale(v);
-    *(u32_t*)(page + Page<C>::codes(false, s % C::T) + c / 2) = encode8(k, ks);
-    *(u32_t*)(page + Page<C>::codes(true, s % C::T) + c / 2) = encode8(v, vs);
-    if (c % 32 == 0) {
-      page[Page<C>::scales(false, s % C::T) + c / 32] = (u8_t)ks;
-      page[Page<C>::scales(true, s % C::T) + c / 32] = (u8_t)vs;
+  for (int i0 = 0; i0 < TW * ROW; i0 += 512) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = i0 + 256 * u + tid;
+      if (i0 > 0) fetch(u, i);
+      if (i >= TW * ROW) continue;
+      const int w = i / ROW, h = i % ROW / (C::HD / 8), c = i % (C::HD / 8) * 8, s = place[w];
+      if (s < 0) continue;
+      u8_t* const page = cache + ((long)(s / C::T) * C::H + h) * Page<C>::BYTES;
+      const u32_t ks = block_scale(k[u]), vs = block_scale(v[u]);
+      *(u32_t*)(page + Page<C>::codes(false, s % C::T) + c / 2) = encode8(k[u], ks);
+      *(u32_t*)(page + Page<C>::codes(true, s % C::T) + c / 2) = encode8(v[u], vs);
+      if (c % 32 == 0) {
+        page[Page<C>::scales(false, s % C::T) + c / 32] = (u8_t)ks;
+        page[Page<C>::scales(true, s % C::T) + c / 32] = (u8_t)vs;
+      }
     }
   }
 }
@@ -192,20 +209,26 @@ __device__ __forceinline__ void claim(const int* __restrict__ slots, int* __rest
   else atomicMax(&owner[s], (int)t);
 }
 
-// The keys or values of N slots; zeros for a slot outside the cache.
-template <class C, bool VALUE>
+// The keys, the values or both of N slots (none: nullptr); zeros for a slot outside the cache.
+template <class C>
 __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const int* __restrict__ slots,
-                                           typename Elem<C::DT>::type* __restrict__ out) {
+                                           typename Elem<C::DT>::type* __restrict__ keys, typename Elem<C::DT>::type* __restrict__ values) {
   constexpr long N = (long)C::TOKENS * C::H * C::HD;
   for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8; i < N; i += (long)gridDim.x * 2048) {
     const long row = i / C::HD, h = row % C::H, c = i % C::HD;
     const int slot = slots[row / C::H];
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (slot >= 0 && slot < C::P * C::T) {
-      const u8_t* const page = Page<C>::head(cache, slot / C::T, h);
-      decode8(*(const u32_t*)(page + Page<C>::codes(VALUE, slot % C::T) + c / 2), page[Page<C>::scales(VALUE, slot % C::T) + c / 32], x);
+#pragma unroll
+    for (int value = 0; value < 2; ++value) {
+      typename Elem<C::DT>::type* const out = value ? values : keys;
+      if (!out) continue;
+      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (slot >= 0 && slot < C::P * C::T) {
+        const u8_t* const page = Page<C>::head(cache, slot / C::T, h);
+        decode8(*(const u32_t*)(page + Page<C>::codes(value != 0, slot % C::T) + c / 2),
+                page[Page<C>::scales(value != 0, slot % C::T) + c / 32], x);
+      }
+      store8<C::DT>(out + i, x);
     }
-    store8<C::DT>(out + i, x);
   }
 }
 
@@ -214,17 +237,21 @@ __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const
 // key-value head h / G; key j is row j % T of page pages[b, j / T]. Pages outside the cache hold no keys, and a row that sees no
 // key is 0. Scores, softmax and sums are f32.
 //
-// The Q x G rows that share a key-value head are the columns of 16-wide matrix instructions, NR sixteens of them per wave, so
-// the cache is read once for all of them. Per 32 keys (a step) a wave computes S^T = K Q^T (two v_mfma_f32_16x16x32_bf16 tiles of
-// 16 keys per 32 dims): lane l holds row l % 16 and, g = l / 16, keys 4 g + i and 16 + 4 g + i, which is how the B operand of
-// O^T = V^T P^T wants them when its k index 8 g + j means key 4 g + j (j < 4) or 12 + 4 g + j, so P never leaves the lane. Of
-// K's dims, of which any order will do, lane l takes the HD / 4 from g HD / 4 on of key l % 16: they are contiguous. V's rows are
-// keys while its A operand wants eight keys of one dim: ds_read_b64_tr_b8 hands a lane one byte (two dims) of eight rows.
-//
-// fp4 with its scale is exact in bf16. Queries are split into PARTS bf16 parts (bf16 1, f16 2, f32 3: exact, or 24 bits), and the
-// probabilities likewise (PP), one matrix instruction each: the sums keep f32's accuracy whatever the type. A row's running
-// maximum follows the scores only where one exceeds it by 2^8: till then probabilities are at most 2^8 and sums need no
-// rescaling, nor the maximum its way through the lanes.
+// The Q x G rows that share a key-value head are the columns of 16-wide matrix instructions, 16 rows to a workgroup (two sixteens to
+// a wave, so that the cache is read once for 32 rows, run out of registers: 8 heads of 128 x 32 rows bf16 over 8 x 4096 keys take 94
+// us where twice the workgroups and reads take 65). Per 32 keys (a step) a wave computes S^T = K Q^T, two tiles of 16 keys, on
+// v_mfma_scale_f32_16x16x128_f8f6f4, whose A operand is K as it lies: a lane's 16 bytes are a block of one key, its scale beside
+// it. The queries are its B operand, in e4m3 with a scale per block: four bits of them at a time, PARTS times (f32 6, else 3).
+// That is all bits of a query down to 2^-11 of its block's largest in bf16, 2^-8 in f16 and 2^-7 in f32; what lies below is off by
+// 2^-19 (f32 2^-31) of the largest at most. (Two parts for bf16 take 113 us where three take 115, 8 x 16 x 4096 keys 15.0 and 16.2, but they
+// lose queries 2^-13 of the largest altogether. K widened to bf16 as V is: 40 of the 241 VALU instructions of a step, which bound it.)
+// Lane l then holds row l % 16 and, g = l / 16, keys 4 g + i and 16 + 4 g + i, which is how the B operand of O^T = V^T P^T
+// (v_mfma_f32_16x16x32_bf16) wants them when its k index 8 g + j means key 4 g + j (j < 4) or 12 + 4 g + j, so P never leaves
+// the lane. V's blocks lie along its dims and not along the keys that are summed, so V is widened to bf16, in which fp4 with its
+// scale is exact; its rows are keys while the A operand wants eight keys of one dim: ds_read_b64_tr_b8 hands a lane one byte (two
+// dims) of eight rows. The probabilities are split into PP bf16 numbers, one matrix instruction each: the sums keep f32's
+// accuracy whatever the type. A row's running maximum follows the scores only where one exceeds it by 2^8: till then
+// probabilities are at most 2^8 and sums need no rescaling, nor the maximum its way through the lanes.
 //
 // A step's codes (32 HD bytes) and scales go straight to LDS, three stages of them per wave, each wave on its own: loads that
 // are in order, and 8 KB in flight per wave without a register. Rows of a power of two of 16-byte chunks are
@@ -233,12 +260,37 @@ __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const
 // Each wave takes every fourth step of the workgroup's range; the waves join through LDS, the SPLITS workgroups of a
 // sequence and head through memory (m, l, O per row) and a second kernel. A range is a share of the sequence's own length.
 //
-// C supplies, besides the cache's, Q, G, MAXP (pages per sequence), SEQS, NR, SPLITS and SL = log2(e) / sqrt(HD).
+// C supplies, besides the cache's, Q, G, MAXP (pages per sequence), SEQS, SPLITS and SL = log2(e) / sqrt(HD).
 // ---------------------------------------------------------------------------------------------
 
 #define ACCY_MX4_LDS __attribute__((address_space(3)))
 
-template <int DT> constexpr int query_parts() { return DT + 1; }
+template <int DT> constexpr int query_parts() { return DT == 2 ? 6 : 3; }
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// 32 values below 256 as e4m3 numbers, four bits of each; x becomes what is left, 16 times over (under a scale four less). The
+// instruction adds a block's products exactly only where they lie close enough together (with eighths up to 256 it does; with all of
+// e4m3, sums were off by 2^-11 of the largest product), so what is below an eighth is left to the next part.
+__device__ __forceinline__ i32x8 take_e4m3(float (&x)[32]) {
+  constexpr float EIGHTHS = 1572864.0f;  // 1.5 2^20: adding and subtracting it rounds to a multiple of 1/8
+  i32x8 w;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = (x[4 * i + j] + EIGHTHS) - EIGHTHS;
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    v = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], v, true);
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(v, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
+    x[4 * i] = (x[4 * i] - a[0]) * 16.0f;
+    x[4 * i + 1] = (x[4 * i + 1] - a[1]) * 16.0f;
+    x[4 * i + 2] = (x[4 * i + 2] - b[0]) * 16.0f;
+    x[4 * i + 3] = (x[4 * i + 3] - b[1]) * 16.0f;
+    w[i] = v;
+  }
+  return w;
+}
 
 // x as bf16 numbers whose sum is x (to 8 bits a part): the next part; x becomes what is left.
 __device__ __forceinline__ __bf16 take_part(float& x) {
@@ -251,7 +303,7 @@ __device__ __forceinline__ __bf16 take_part(float& x) {
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
 template <class C> struct Rows {
-  static constexpr int R = C::Q * C::G, TILES = (R + 15) / 16, GROUPS = (TILES + C::NR - 1) / C::NR;
+  static constexpr int R = C::Q * C::G, GROUPS = (R + 15) / 16;
 };
 
 // Where 16-byte chunk c of key's row lies within the row's chunks in LDS: 16 rows that are read at one chunk (keys; 32 lanes of
@@ -267,9 +319,6 @@ template <int CH> __device__ __forceinline__ int value_chunk(int key, int c) {
   else return c;
 }
 
-// Four bf16 pairs as the eight elements of a matrix operand.
-__device__ __forceinline__ bf16x8 eight(bf16x2 a, bf16x2 b, bf16x2 c, bf16x2 d) { return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
-
 template <int I> __device__ __forceinline__ bf16x2 pair_of_byte(u32_t w, float scale) {
   return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, I);
 }
@@ -282,58 +331,35 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
                                        typename Elem<C::DT>::type* __restrict__ out, float* __restrict__ part) {
   typedef Page<C> P;
   typedef Rows<C> RS;
-  constexpr int HD = C::HD, NB = HD / 32, PARTS = query_parts<C::DT>(), PP = C::DT == 2 ? 3 : 2, NR = C::NR;
+  constexpr int HD = C::HD, NB = HD / 32, KI = (NB + 3) / 4, PARTS = query_parts<C::DT>(), PP = C::DT == 2 ? 3 : 2;
   constexpr int CODES = 16 * HD, SCALES = 32 * NB;  // bytes of a step's keys, or values, in LDS
   constexpr int DC = 2 * HD / 64, DS = (16 * NB + 63) / 64, PER = DC + DS;  // load instructions of a step
   constexpr int STAGE = 2 * CODES + 256 * DS;
+  // A cache that one workgroup alone reads streams by with the non-temporal hint (6.0 TB/s of loads alone against 5.2).
+  constexpr int ONCE = RS::GROUPS == 1 ? 2 : 0;
   // One array per stage: the compiler can then tell a stage's reads from the loads still on their way into the others.
   __shared__ __attribute__((aligned(1024))) u8_t l0[4 * STAGE], l1[4 * STAGE], l2[4 * STAGE];
-  // the waves' meeting place, once the steps are done (every load has landed by then): two waves' rows
-  constexpr int JOIN = 16 * (HD + 4) * 4;
-  static_assert(JOIN <= 4 * STAGE, "a stage of the four waves holds a wave's rows");
-  auto joined = [&](int w) { return (float*)(w ? l1 : l0); };
+  // where the waves meet, once the steps are done (every load has landed by then): two waves' rows to a stage
+  constexpr int JOIN = 16 * (HD + 4);
+  static_assert(2 * JOIN * 4 <= 4 * STAGE, "a stage of the four waves holds two waves' rows");
+  auto joined = [&](int k) { return (float*)(k < 2 ? l0 : l1) + (k & 1) * JOIN; };
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
   auto stage = [&](auto s) -> u8_t* {
     if constexpr (decltype(s)::value == 0) return l0;
     else if constexpr (decltype(s)::value == 1) return l1;
     else return l2;
   };
-  const long bh = blockIdx.x / RS::GROUPS, b = bh / C::H, h = bh % C::H;
-  const int row0 = (int)(blockIdx.x % RS::GROUPS) * NR * 16;
+  // A head's groups of rows lie eight workgroups apart, on one XCD: its cache comes through that one's L2.
+  const int set = blockIdx.x / (8 * RS::GROUPS), in = blockIdx.x % (8 * RS::GROUPS);
+  const int wide = C::SEQS * C::H - 8 * set < 8 ? (int)(C::SEQS * C::H - 8 * set) : 8;
+  const long bh = 8 * set + in % wide, b = bh / C::H, h = bh % C::H;
+  const int row0 = in / wide * 16;
   int len = C::P > 0 ? lengths[b] : 0;
   len = len < 0 ? 0 : len > C::MAXP * C::T ? C::MAXP * C::T : len;
   len = __builtin_amdgcn_readfirstlane(len);
   const int steps = (len + 31) / 32, per = (steps + C::SPLITS - 1) / C::SPLITS;
   const int first = (int)blockIdx.y * per, end = first + per < steps ? first + per : steps;
   const int sure = len - (C::Q - 1);  // keys below it are seen by every row
-
-  // queries: the B operand of S^T, row r of each tile, dims g HD / 4 + 8 s + j at step s
-  bf16x8 q[NR][NB][PARTS];
-  int limit[NR];
-#pragma unroll
-  for (int t = 0; t < NR; ++t) {
-    const int row = row0 + 16 * t + r, i = row / C::G;
-    limit[t] = row < RS::R ? len - (C::Q - 1 - i) : 0;
-    const long at = ((b * C::Q + i) * C::H * C::G + h * C::G + row % C::G) * HD + g * (HD / 4);
-#pragma unroll
-    for (int s = 0; s < NB; ++s) {
-      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (row < RS::R) load8<C::DT>(Q + at + 8 * s, x);
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q[t][s][p][j] = take_part(x[j]);
-    }
-  }
-  f32x4 o[NR][NB][2];
-  float m[NR], l[NR];
-#pragma unroll
-  for (int t = 0; t < NR; ++t) {
-    m[t] = -__builtin_inff();
-    l[t] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < NB; ++d) o[t][d][0] = o[t][d][1] = f32x4{0, 0, 0, 0};
-  }
 
   // Loads: chunk x = 64 i + lane of a step's LDS, keys and then values; then the scales, a word a lane.
   u32_t from[DC], sfrom[DS];
@@ -353,11 +379,63 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     const u8_t* const head = P::head(cache, page >= 0 && page < C::P ? page : 0, h);
     const u8_t *const codes = head + in * (HD / 2), *const scales = head + in * NB;
 #pragma unroll
-    for (int i = 0; i < DC; ++i) __builtin_amdgcn_global_load_lds(codes + from[i], (ACCY_MX4_LDS void*)(stage(s) + wave * STAGE + 1024 * i), 16, 0, 0);
+    for (int i = 0; i < DC; ++i) __builtin_amdgcn_global_load_lds(codes + from[i], (ACCY_MX4_LDS void*)(stage(s) + wave * STAGE + 1024 * i), 16, 0, ONCE);
 #pragma unroll
     for (int i = 0; i < DS; ++i)
-      __builtin_amdgcn_global_load_lds(scales + sfrom[i], (ACCY_MX4_LDS void*)(stage(s) + wave * STAGE + 2 * CODES + 256 * i), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds(scales + sfrom[i], (ACCY_MX4_LDS void*)(stage(s) + wave * STAGE + 2 * CODES + 256 * i), 4, 0, ONCE);
   };
+  int step = first + wave, p0 = page_of(step), p1 = page_of(step + 4), p2 = page_of(step + 8);
+  // The queries are asked for before the steps' loads, which would have to land first otherwise, and worked on after.
+  float x[KI][32];
+  const int row = row0 + r;
+  const long at = ((b * C::Q + row / C::G) * C::H * C::G + h * C::G + row % C::G) * HD;
+#pragma unroll
+  for (int c = 0; c < KI; ++c)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int dim = 128 * c + 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+      float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (row < RS::R && dim < HD) load8<C::DT>(Q + at + dim, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[c][8 * s + j] = y[j];
+    }
+  __builtin_amdgcn_sched_barrier(0);
+  if (step < end) load(Number<0>(), step, p0);
+  if (step + 4 < end) load(Number<1>(), step + 4, p1);
+
+  // Queries: the B operand of S^T, row r, as PARTS e4m3 numbers each, four bits apart. Of 128 dims lane group g holds 16
+  // from 16 g on and 16 from 64 + 16 g on, halves of blocks g / 2 and 2 + g / 2, and the scale of block g. A block's largest
+  // value is scaled to [128, 256): e4m3 goes to 448, and its steps are 2^-9 at the least.
+  i32x8 q[KI][PARTS];
+  u32_t qscale[KI];
+  const int limit = row < RS::R ? len - (C::Q - 1 - row / C::G) : 0;
+#pragma unroll
+  for (int c = 0; c < KI; ++c) {
+    u32_t byte[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      u32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const u32_t bits = __builtin_bit_cast(u32_t, x[c][16 * half + j]) & 0x7fffffffu;
+        top = top > bits ? top : bits;
+      }
+      const u32_t other = (u32_t)__shfl_xor((int)top, 16, 64), e = (top > other ? top : other) >> 23;
+      // at least 2^-96: values below lose bits, and a scale is left for every part
+      byte[half] = e == 255 ? 255 : e < 38 ? 31 : e - 7;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[c][16 * half + j] = e == 255 ? 0.0f : x[c][16 * half + j] * scale_of(254 - byte[half]);
+    }
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) q[c][p] = take_e4m3(x[c]);
+    const int first = __shfl((int)byte[0], r + 32 * (g & 1), 64), second = __shfl((int)byte[1], r + 32 * (g & 1), 64);
+    qscale[c] = (u32_t)(g < 2 ? first : second);
+  }
+  f32x4 o[NB][2];
+  float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < NB; ++d) o[d][0] = o[d][1] = f32x4{0, 0, 0, 0};
+
   auto wait = [&](auto left) {
     constexpr int N = decltype(left)::value;
     static_assert(N < 64, "vmcnt range");
@@ -365,15 +443,17 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     asm volatile("" ::: "memory");
   };
 
-  // Where in a stage the lane reads: its share of key r's codes (of key 16 + r 8 HD bytes on) and key r's scales; a block's bytes of
-  // its value row, which lanes 2 t and 2 t + 1 of sixteen have for their t-th key; the scales of values 4 g .. (16 on: those of 16 + 4 g).
-  constexpr int KC = NB % 4 == 0 ? NB / 4 : 1;
-  u32_t kat[KC], vat[NB];
+  // Where in a stage the lane reads: block 4 c + g of key r (of key 16 + r 8 HD bytes on; past the last block one of the others, which
+  // meets zeros) and its scale; a block's bytes of its value row, which lanes 2 t and 2 t + 1 of sixteen have for their t-th key; the
+  // scales of values 4 g .. (16 on: those of 16 + 4 g).
+  u32_t kat[KI], ksat[KI], vat[NB];
 #pragma unroll
-  for (int c = 0; c < KC; ++c)
-    kat[c] = wave * STAGE + r * (HD / 2) +
-             (NB % 4 == 0 ? 16 * key_chunk<NB>(r, g * KC + c) : NB == 2 ? 16 * key_chunk<NB>(r, g >> 1) + 8 * (g & 1) : g * (HD / 8));
-  const u32_t ksat = wave * STAGE + 2 * CODES + r * NB, vsat = wave * STAGE + 2 * CODES + SCALES + 4 * g * NB;
+  for (int c = 0; c < KI; ++c) {
+    const int block = 4 * c + g < NB ? 4 * c + g : (4 * c + g) % NB;
+    kat[c] = wave * STAGE + r * (HD / 2) + 16 * key_chunk<NB>(r, block);
+    ksat[c] = wave * STAGE + 2 * CODES + r * NB + block;
+  }
+  const u32_t vsat = wave * STAGE + 2 * CODES + SCALES + 4 * g * NB;
 #pragma unroll
   for (int d = 0; d < NB; ++d) {
     const int tk = r >> 1, key = 4 * g + (tk & 3) + (tk >> 2) * 16;
@@ -384,80 +464,54 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     constexpr bool TAIL = decltype(tail_)::value != 0;
     const int k0 = step * 32;
     const u8_t* const lds = stage(s);
-    f32x4 sc[NR][2];
+    f32x4 sc[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      u32_t kw[NB];
-      if constexpr (NB % 4 == 0) {
+      sc[u] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const u32x4 w = *(const u32x4*)(lds + kat[c] + u * 8 * HD);
+      for (int c = 0; c < KI; ++c) {
+        const u32x4 w = *(const u32x4*)(lds + kat[c] + u * 8 * HD);
+        const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+        const int scale = lds[ksat[c] + u * 16 * NB];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) kw[4 * c + e] = w[e];
+        for (int p = 0; p < PARTS; ++p) {
+          const int by = qscale[c] == 255 ? 255 : (int)qscale[c] - 4 * p;
+          sc[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[c][p], sc[u], 4, 0, 0, scale, 0, by);
         }
-      } else if constexpr (NB == 2) {
-        const u32x2 w = *(const u32x2*)(lds + kat[0] + u * 8 * HD);
-        kw[0] = w[0], kw[1] = w[1];
-      } else {
-#pragma unroll
-        for (int e = 0; e < NB; ++e) kw[e] = *(const u32_t*)(lds + kat[0] + u * 8 * HD + 4 * e);
-      }
-#pragma unroll
-      for (int t = 0; t < NR; ++t) sc[t][u] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < NB; ++e) {
-        const float x = scale_of(lds[ksat + u * 16 * NB + (g * (HD / 4) + 8 * e) / 32]);
-        const bf16x8 a = eight(pair_of_byte<0>(kw[e], x), pair_of_byte<1>(kw[e], x), pair_of_byte<2>(kw[e], x), pair_of_byte<3>(kw[e], x));
-#pragma unroll
-        for (int t = 0; t < NR; ++t)
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p) sc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[t][e][p], sc[t][u], 0, 0, 0);
       }
     }
     // The scores' maximum over the lane's keys k0 + 16 u + 4 g + i, those that the row does not see left out.
-    float top[NR];
-    bool above = false;
+    float top = -__builtin_inff();
 #pragma unroll
-    for (int t = 0; t < NR; ++t) {
-      top[t] = -__builtin_inff();
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (TAIL) sc[t][u][i] = k0 + 16 * u + 4 * g + i < limit[t] && page >= 0 && page < C::P ? sc[t][u][i] : -__builtin_inff();
-          top[t] = fmaxf(top[t], sc[t][u][i]);
-        }
-      top[t] *= C::SL;
-      above |= top[t] > m[t] + 8.0f;  // also where m is -inf and a key is seen
-    }
-    if (__builtin_amdgcn_ballot_w64(above) != 0) {
-#pragma unroll
-      for (int t = 0; t < NR; ++t) {
-        top[t] = fmaxf(top[t], __shfl_xor(top[t], 16, 64));
-        top[t] = fmaxf(top[t], __shfl_xor(top[t], 32, 64));
-        top[t] = fmaxf(top[t], m[t]);
-        const float alpha = __builtin_amdgcn_exp2f(m[t] - base_of(top[t]));
-        m[t] = top[t];
-        l[t] *= alpha;
-#pragma unroll
-        for (int d = 0; d < NB; ++d)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[t][d][e][i] *= alpha;
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (TAIL) sc[u][i] = k0 + 16 * u + 4 * g + i < limit && page >= 0 && page < C::P ? sc[u][i] : -__builtin_inff();
+        top = fmaxf(top, sc[u][i]);
       }
+    top *= C::SL;
+    if (__builtin_amdgcn_ballot_w64(top > m + 8.0f) != 0) {  // also where m is -inf and a key is seen
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      top = fmaxf(top, m);
+      const float alpha = __builtin_amdgcn_exp2f(m - base_of(top));
+      m = top;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < NB; ++d)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[d][e][i] *= alpha;
     }
-    bf16x8 pr[NR][PP];
+    bf16x8 pr[PP];
+    const float base = base_of(m);
 #pragma unroll
-    for (int t = 0; t < NR; ++t) {
-      const float base = base_of(m[t]);
+    for (int j = 0; j < 8; ++j) {
+      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j >> 2][j & 3], C::SL, -base));
+      l += p;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j >> 2][j & 3], C::SL, -base));
-        l[t] += p;
-#pragma unroll
-        for (int e = 0; e < PP; ++e) pr[t][e][j] = take_part(p);
-      }
+      for (int e = 0; e < PP; ++e) pr[e][j] = take_part(p);
     }
     // scale bytes of the lane's eight keys: four rows of NB bytes, twice
     u32_t vw[2][NB];
@@ -505,21 +559,18 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
           even[j] = y[j][0];
           odd[j] = y[j][1];
         }
+        const f32x4 before[2] = {o[d][0], o[d][1]};
 #pragma unroll
-        for (int t = 0; t < NR; ++t) {
-          const f32x4 before[2] = {o[t][d][0], o[t][d][1]};
+        for (int p = 0; p < PP; ++p) {
+          o[d][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, pr[p], o[d][0], 0, 0, 0);
+          o[d][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, pr[p], o[d][1], 0, 0, 0);
+        }
+        if constexpr (TAIL && C::Q > 1) {
+          const bool mine = !apart || (row0 + r) / C::G == only;
 #pragma unroll
-          for (int p = 0; p < PP; ++p) {
-            o[t][d][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, pr[t][p], o[t][d][0], 0, 0, 0);
-            o[t][d][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, pr[t][p], o[t][d][1], 0, 0, 0);
-          }
-          if constexpr (TAIL && C::Q > 1) {
-            const bool mine = !apart || (row0 + 16 * t + r) / C::G == only;
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[t][d][e][i] = mine ? o[t][d][e][i] : before[e][i];
-          }
+            for (int i = 0; i < 4; ++i) o[d][e][i] = mine ? o[d][e][i] : before[e][i];
         }
       }
     };
@@ -532,7 +583,6 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   };
 
   {
-    int step = first + wave, p0 = page_of(step), p1 = page_of(step + 4), p2 = page_of(step + 8);
     // Stage S holds step `now` of page `mine`; the step two stages on goes to stage S + 2, its page into `mine`.
     auto turn = [&](auto s, auto two, int now, int& mine, int next) {
       // This stage has landed when no more than the next one's and the one's after are outstanding; where no more follow, when
@@ -550,8 +600,6 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
       __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0): the stage may be overwritten
       asm volatile("" ::: "memory");
     };
-    if (step < end) load(Number<0>(), step, p0);
-    if (step + 4 < end) load(Number<1>(), step + 4, p1);
     for (; step < end; step += 12) {
       turn(Number<0>(), Number<2>(), step, p0, p2);
       if (step + 4 >= end) break;
@@ -561,71 +609,51 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     }
   }
 
-  // The waves: 2 and 3 hand theirs to 0 and 1, then 1 to 0. Lane (r, g) holds dims 32 d + 8 g .. + 7 of row r: even ones in
-  // [0], odd ones in [1]. A row in LDS: HD outputs, m, then l per lane group.
+  // The waves meet: lane (r, g) holds dims 32 d + 8 g .. + 7 of row r, even ones in [0], odd ones in [1]. A row in LDS is HD
+  // outputs, m and l; then every thread joins the four waves' four dims of a row.
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  __syncthreads();
+  float* const p = joined(wave) + r * (HD + 4);
 #pragma unroll
-  for (int t = 0; t < NR; ++t) {
-    l[t] += __shfl_xor(l[t], 16, 64);
-    l[t] += __shfl_xor(l[t], 32, 64);
-#pragma unroll
-    for (int from = 2; from > 0; from >>= 1) {
-      __syncthreads();
-      if (wave >= from && wave < 2 * from) {
-        float* const p = joined(wave - from) + r * (HD + 4);
-#pragma unroll
-        for (int d = 0; d < NB; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[32 * d + 8 * g + 2 * i] = o[t][d][0][i];
-            p[32 * d + 8 * g + 2 * i + 1] = o[t][d][1][i];
-          }
-        if (g == 0) {
-          p[HD] = m[t];
-          p[HD + 1] = l[t];
-        }
-      }
-      __syncthreads();
-      if (wave < from) {
-        const float* const p = joined(wave) + r * (HD + 4);
-        const float top = fmaxf(m[t], p[HD]), base = base_of(top);
-        const float mine = __builtin_amdgcn_exp2f(m[t] - base), theirs = __builtin_amdgcn_exp2f(p[HD] - base);
-        m[t] = top;
-        l[t] = l[t] * mine + p[HD + 1] * theirs;
-#pragma unroll
-        for (int d = 0; d < NB; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            o[t][d][0][i] = o[t][d][0][i] * mine + p[32 * d + 8 * g + 2 * i] * theirs;
-            o[t][d][1][i] = o[t][d][1][i] * mine + p[32 * d + 8 * g + 2 * i + 1] * theirs;
-          }
-      }
-    }
+  for (int d = 0; d < NB; ++d) {
+    *(f32x4*)(p + 32 * d + 8 * g) = f32x4{o[d][0][0], o[d][1][0], o[d][0][1], o[d][1][1]};
+    *(f32x4*)(p + 32 * d + 8 * g + 4) = f32x4{o[d][0][2], o[d][1][2], o[d][0][3], o[d][1][3]};
   }
-  if (wave != 0) return;
-#pragma unroll
-  for (int t = 0; t < NR; ++t) {
-    const int row = row0 + 16 * t + r;
+  if (g == 0) {
+    p[HD] = m;
+    p[HD + 1] = l;
+  }
+  __syncthreads();
+  for (int at = tid; at < 16 * HD / 4; at += 256) {
+    const int rr = at / (HD / 4), d = at % (HD / 4) * 4, row = row0 + rr;
     if (row >= RS::R) continue;
+    const int from = rr * (HD + 4);
+    float top = joined(0)[from + HD], sum = 0.0f;
+#pragma unroll
+    for (int k = 1; k < 4; ++k) top = fmaxf(top, joined(k)[from + HD]);
+    const float base = base_of(top);
+    f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float* const w = joined(k) + from;
+      const float scale = __builtin_amdgcn_exp2f(w[HD] - base);
+      const f32x4 y = *(const f32x4*)(w + d);
+      sum += w[HD + 1] * scale;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += y[i] * scale;
+    }
     if constexpr (C::SPLITS == 1) {
-      const long at = ((b * C::Q + row / C::G) * C::H * C::G + h * C::G + row % C::G) * HD;
-      const float by = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+      const long to = ((b * C::Q + row / C::G) * C::H * C::G + h * C::G + row % C::G) * HD + d;
+      const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-      for (int d = 0; d < NB; ++d) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = o[t][d][i & 1][i >> 1] * by;
-        store8<C::DT>(out + at + 32 * d + 8 * g, x);
-      }
+      for (int i = 0; i < 4; ++i) out[to + i] = to_elem<C::DT>(v[i] * by);
     } else {
-      float* const p = part + ((bh * RS::R + row) * C::SPLITS + blockIdx.y) * (HD + 4);
-#pragma unroll
-      for (int d = 0; d < NB; ++d) {
-        *(f32x4*)(p + 32 * d + 8 * g) = f32x4{o[t][d][0][0], o[t][d][1][0], o[t][d][0][1], o[t][d][1][1]};
-        *(f32x4*)(p + 32 * d + 8 * g + 4) = f32x4{o[t][d][0][2], o[t][d][1][2], o[t][d][0][3], o[t][d][1][3]};
-      }
-      if (g == 0) {
-        p[HD] = m[t];
-        p[HD + 1] = l[t];
+      float* const to = part + ((bh * RS::R + row) * C::SPLITS + blockIdx.y) * (HD + 4);
+      *(f32x4*)(to + d) = v;
+      if (d == 0) {
+        to[HD] = top;
+        to[HD + 1] = sum;
       }
     }
   }

@@ -17,9 +17,9 @@ struct CheckProduct {
 struct CheckSmall : CheckProduct {
   static constexpr int BM = 64, BN = 32, SPLITS = 1, WK = 2;
 };
-template <int D, int DIM, int QUERIES, int GROUP, int TILES, int S>
+template <int D, int DIM, int QUERIES, int GROUP, int S>
 struct CheckCache {
-  static constexpr int DT = D, HD = DIM, H = 8, T = 64, P = 512, Q = QUERIES, G = GROUP, MAXP = 64, NR = TILES, SPLITS = S;
+  static constexpr int DT = D, HD = DIM, H = 8, T = 64, P = 512, Q = QUERIES, G = GROUP, MAXP = 64, SPLITS = S;
   static constexpr long SEQS = 8, TOKENS = 100;
   static constexpr float SL = 0x1.05p-3f;
 };
@@ -34,17 +34,17 @@ extern "C" __global__ void __launch_bounds__(256) check_mx4_values(const u8_t* c
   accy::mx4::values<0, int, 4096>(c, s, o);
 }
 extern "C" __global__ void __launch_bounds__(256) check_mx4_write(u8_t* c, const float* k, const float* v, const int* s) {
-  accy::mx4::cache_write<CheckCache<2, 96, 1, 1, 1, 1>, false>(c, k, v, s, nullptr);
+  accy::mx4::cache_write<CheckCache<2, 96, 1, 1, 1>, false>(c, k, v, s, nullptr);
 }
-extern "C" __global__ void __launch_bounds__(256) check_mx4_read(const u8_t* c, const int* s, u16_t* o) {
-  accy::mx4::cache_read<CheckCache<1, 96, 1, 1, 1, 1>, true>(c, s, o);
+extern "C" __global__ void __launch_bounds__(256) check_mx4_read(const u8_t* c, const int* s, u16_t* k, u16_t* v) {
+  accy::mx4::cache_read<CheckCache<1, 96, 1, 1, 1>>(c, s, k, v);
 }
 extern "C" __global__ void __launch_bounds__(256) check_mx4_attend_bf16(const u16_t* q, const u8_t* c, const int* p, const int* l, u16_t* o, float* part) {
-  accy::mx4::attend<CheckCache<0, 128, 1, 8, 1, 4>>(q, c, p, l, o, part);
+  accy::mx4::attend<CheckCache<0, 128, 1, 8, 4>>(q, c, p, l, o, part);
 }
 extern "C" __global__ void __launch_bounds__(256) check_mx4_attend_f32(const float* q, const u8_t* c, const int* p, const int* l, float* o, float* part) {
-  accy::mx4::attend<CheckCache<2, 96, 5, 4, 2, 1>>(q, c, p, l, o, part);
+  accy::mx4::attend<CheckCache<2, 96, 5, 4, 1>>(q, c, p, l, o, part);
 }
 extern "C" __global__ void __launch_bounds__(256) check_mx4_join(const float* part, u16_t* o) {
-  accy::mx4::attend_join<CheckCache<0, 128, 1, 8, 1, 4>>(part, o);
+  accy::mx4::attend_join<CheckCache<0, 128, 1, 8, 4>>(part, o);
 }

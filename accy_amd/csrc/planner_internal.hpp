@@ -621,7 +621,7 @@ class Planner {
   };
   Mx4Tile mx4_tile(int64_t M, int64_t N, int64_t K) const;
   void mx4_cache_write(uint32_t v);
-  void mx4_cache_read(uint32_t v, bool value);
+  void mx4_cache_read(uint32_t v);
   void mx4_attend(uint32_t v);
   // The members of a cache kernel's configuration, from the cache and the rows' head dimension; fails where they do not fit.
   struct Mx4Cache {

@@ -67,7 +67,7 @@ void Planner::custom(uint32_t v) {
     if (what == "values") return operands(2), mx4_values(v);
     if (what == "contract") return operands(4), mx4_contract(v);
     if (what == "cache_write") return operands(4), mx4_cache_write(v);
-    if (what == "cache_keys" || what == "cache_values") return operands(2), mx4_cache_read(v, what == "cache_values");
+    if (what == "cache_keys" || what == "cache_values") return operands(2), mx4_cache_read(v);
     if (what == "attend") return operands(4), mx4_attend(v);
   }
   fail(Err::Unsupported, "custom_call " + op.bytes + " version " + std::to_string(op.index) + " is not supported by the HIP target");
@@ -426,8 +426,9 @@ void Planner::mx4_cache_write(uint32_t v) {
   if (n && c.pages && c.heads) {
     const int ks = dense_slot(op.args[1]), vs = dense_slot(op.args[2]), ss = dense_slot(op.args[3]);
     require(n < (uint64_t(1) << 31), op, "2^31 tokens or more");
-    // Looking through the later slots costs every workgroup a pass over the list; a table of each slot's last token two launches.
-    const bool owners = n > 8192;
+    // Looking through the later slots costs every workgroup a pass over the list; a table of each slot's last token two launches
+    // (8 heads of 128 bf16: 1000 tokens 4.8 us by the list and 7.7 by the table, 4000 8.1 and 10.1, 8192 17.5 and 14.8, 65536 324 and 92).
+    const bool owners = n > 6000;
     const std::string nm = name("mx4_cache_write", v);
     const std::string head = "#include \"mx4\"\nstruct Cfg_" + nm + " {\n" + c.members(kt.dtype) + "  static constexpr long TOKENS = " +
                              std::to_string(n) + ";\n};\n";
@@ -460,22 +461,35 @@ void Planner::mx4_cache_write(uint32_t v) {
   finish(v);
 }
 
-void Planner::mx4_cache_read(uint32_t v, bool value) {
+// Keys and values of the same slots are one kernel, whichever is asked for first.
+void Planner::mx4_cache_read(uint32_t v) {
   const Op& op = g_.ops[v];
   const Type &rt = op.result, &st = g_.type(op.args[1]);
   element_type(op, rt.dtype);
   require(st.dtype == DType::i32 && st.rank() + 2 == rt.rank(), op, "i32 slots; the result is [slots .., kv_head, dim]");
   for (size_t i = 0; i < st.rank(); ++i) require(st.dims[i].extent == rt.dims[i].extent, op, "i32 slots; the result is [slots .., kv_head, dim]");
   const Mx4Cache c = mx4_cache(op, op.args[0], rt.dims[rt.rank() - 2].extent, last(rt));
-  const int out = temp_slot(v);
+  int out[2] = {-1, -1};  // keys, values
+  std::vector<uint32_t> made;
+  for (uint32_t u = v; u < g_.ops.size(); ++u) {
+    const Op& uo = g_.ops[u];
+    if (!live_[u] || done_[u] || uo.kind != Kind::custom_call || uo.index != 1 || uo.args != op.args || !(uo.result == rt)) continue;
+    if (uo.bytes != "accy.mx4.cache_keys" && uo.bytes != "accy.mx4.cache_values") continue;
+    int& slot = out[uo.bytes == "accy.mx4.cache_values"];
+    if (slot >= 0) continue;
+    slot = temp_slot(u);
+    made.push_back(u);
+  }
   if (rt.elements()) {
     const int cs = dense_slot(op.args[0]), ss = dense_slot(op.args[1]);
     KernelWriter w(g_, slots_, "i64_t");
-    const std::string a = w.arg(cs, false), s = w.arg(ss, false), o = w.arg(out, true), nm = name("mx4_cache_read", v);
+    const std::string a = w.arg(cs, false), s = w.arg(ss, false), nm = name("mx4_cache_read", v);
+    std::string to[2];
+    for (int i = 0; i < 2; ++i) to[i] = out[i] >= 0 ? w.arg(out[i], true) : "nullptr";
     KernelStep k;
     k.source = "#include \"mx4\"\nstruct Cfg_" + nm + " {\n" + c.members(rt.dtype) + "  static constexpr long TOKENS = " +
                std::to_string(st.elements()) + ";\n};\nextern \"C\" __global__ void __launch_bounds__(256) " + nm + "(" + w.params() +
-               ") {\n  accy::mx4::cache_read<Cfg_" + nm + ", " + (value ? "true" : "false") + ">(" + a + ", " + s + ", " + o + ");\n}\n";
+               ") {\n  accy::mx4::cache_read<Cfg_" + nm + ">(" + a + ", " + s + ", " + to[0] + ", " + to[1] + ");\n}\n";
     k.name = nm;
     k.grid[0] = grid_for(rt.elements() / 8, 256);
     k.block[0] = 256;
@@ -483,7 +497,7 @@ void Planner::mx4_cache_read(uint32_t v, bool value) {
     k.label = "cache_read:%" + std::to_string(v);
     push(std::move(k), w);
   }
-  finish(v);
+  for (uint32_t u : made) finish(u);
 }
 
 // ---- attention over the cache ----
@@ -509,12 +523,14 @@ void Planner::mx4_attend(uint32_t v) {
   if (nel) {
     require(Q * G < (int64_t(1) << 24), op, "2^24 query rows of a key-value head or more");
     const int qs = dense_slot(op.args[0]), cs = dense_slot(op.args[1]), ps = dense_slot(op.args[2]), ls = dense_slot(op.args[3]);
-    const int64_t tiles = (Q * G + 15) / 16;
-    const int64_t NR = std::min<int64_t>(tiles, 2), groups = (tiles + NR - 1) / NR, wgs = seqs * H * groups;
-    const int64_t steps = (maxp * c.tokens + 31) / 32;
-    int64_t splits = 1;
-    while (opt_.allow_split && splits < 64 && wgs * splits < 1024 && steps >= 16 * splits) splits *= 2;
-    if (std::getenv("MX4_SPLITS")) splits = std::atoi(std::getenv("MX4_SPLITS"));
+    // Outputs and queries are registers of the whole run: two workgroups of a CU where they leave half of 256, else one.
+    const int64_t groups = (Q * G + 15) / 16, wgs = seqs * H * groups, parts = qt.dtype == DType::f32 ? 6 : 3;
+    const int bounds = hd / 4 + (hd + 127) / 128 * parts * 8 <= 128 ? 2 : 1;
+    // Three workgroups share a CU. Fewer sequences and heads than that are split along their keys till half of the chip's places are
+    // taken (8 x 16 heads x 4096 keys of 128 bf16: 17.4 us in 2, 14.7 in 4, 15.2 in 6, 16.8 in 8 splits), more of them till
+    // uneven lengths even out (48 x 8 x 16000: 140 in 1, 115 in 2, 112 in 4, 117 in 8), each split with four steps of every wave at least.
+    const int64_t steps = (maxp * c.tokens + 31) / 32, want = wgs >= 256 ? 1024 : 512;
+    const int64_t splits = opt_.allow_split ? std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, steps / 16, 64})) : 1;
     require(launchable((uint64_t)wgs, 256), op, "more workgroups than a launch takes");
     KernelWriter w(g_, slots_, "i64_t");
     const std::string q = w.arg(qs, false), a = w.arg(cs, false), p = w.arg(ps, false), l = w.arg(ls, false);
@@ -525,10 +541,10 @@ void Planner::mx4_attend(uint32_t v) {
     char sl[64];
     std::snprintf(sl, sizeof sl, "%af", (double)(float)(1.4426950408889634 / std::sqrt((double)hd)));
     const std::string head = "#include \"mx4\"\nstruct Cfg_" + nm + " {\n" + c.members(qt.dtype) + "  static constexpr int Q = " + num(Q) +
-                             ", G = " + num(G) + ", MAXP = " + num(maxp) + ", NR = " + num(NR) + ", SPLITS = " + num(splits) +
+                             ", G = " + num(G) + ", MAXP = " + num(maxp) + ", SPLITS = " + num(splits) +
                              ";\n  static constexpr long SEQS = " + num(seqs) + ";\n  static constexpr float SL = " + sl + ";\n};\n";
     KernelStep k;
-    k.source = head + "extern \"C\" __global__ void __launch_bounds__(" + std::string(std::getenv("MX4_LB") ? std::getenv("MX4_LB") : "256, 2") + ") " + nm + "(" + w.params() + ") {\n  accy::mx4::attend<Cfg_" + nm +
+    k.source = head + "extern \"C\" __global__ void __launch_bounds__(256, " + num(bounds) + ") " + nm + "(" + w.params() + ") {\n  accy::mx4::attend<Cfg_" + nm +
                ">(" + q + ", " + a + ", " + p + ", " + l + ", " + o + ", " + pp + ");\n}\n";
     k.name = nm;
     k.grid[0] = (uint32_t)wgs;

@@ -538,9 +538,10 @@ def _check_attend(q, cache, pages, lengths, dtype, got=None):
     # A score errs by its sum's (3 dim) 2^-23 and three roundings, of the sum of |q k| at most, which is also a bound of its
     # largest distance to the running maximum; a probability by that, 2^-21 of the hardware's exponential and the parts it is
     # split into (2^-17 for two, less for three); the sums over n keys by n 2^-23, the joins' scalings by 2^-18 of 64 or fewer. Numerator and
-    # denominator both.
+    # denominator both. An f16 result below 2^-14 is off by half of f16's smallest step, 2^-24, and no longer by a share of itself.
     rel = 2 * ((3 * dim + 4) * 2.0 ** -23 * most + 2.0 ** -21 + 2.0 ** -17 * (dtype != "f32") + (n + 64) * 2.0 ** -23 * 3)
-    assert_within(wide(got, dtype), want, HALF_STEP[dtype] * np.abs(want) + (1 + HALF_STEP[dtype]) * rel * mass + 1e-37)
+    least = 2.0 ** -25 if dtype == "f16" else 1e-37
+    assert_within(wide(got, dtype), want, HALF_STEP[dtype] * np.abs(want) + (1 + HALF_STEP[dtype]) * rel * mass + least)
     return got
 
 
@@ -611,6 +612,24 @@ def test_attend_with_very_different_scores(dtype):
     kc[pages[0, 3], 0, 60], ks[pages[0, 3], 0, 60] = encoded(wide(q, dtype)[0, 0, 0] * 4)
     kc[pages[1, 0], 0, 0], ks[pages[1, 0], 0, 0] = encoded(wide(q, dtype)[1, 0, 1] * 4)
     _check_attend(q, cache, pages, np.array([256, 250], np.int32), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("below", [2, 8, 13])
+def test_attend_small_queries_beside_large_ones(dtype, below):
+    """One dim of each block is 2^below or more times the others; every key has the same large value there, so what tells
+    the keys apart is the small ones' part of the score."""
+    rng = np.random.default_rng(15)
+    cache = finite_cache(4, 2, 64, 32, rng)
+    kc, ks, vc, vs = cache_parts(cache, 64)
+    kc[...] |= 0x11  # no zeros
+    kc[..., 0::16] |= 7
+    ks[...] = 127
+    q = rng.uniform(1, 2, (2, 3, 4, 64)) * 2.0 ** -below
+    q[..., 0::32] = 1.9
+    pages = np.arange(4).reshape(2, 2).astype(np.int32)
+    _check_attend(floats(q * 8, dtype), cache, pages, np.array([64, 40], np.int32), dtype)
 
 
 @pytest.mark.gpu
