@@ -14,6 +14,9 @@ C3 gemm     A[m,k], B[k,n] ~ U(-1,1); C = A.contract(B, k) or A.mul(B).sum(k)
 C4 attn     Q,K,V f16[head, query|key, dim] ~ N(0,1); softmax(Q K^T * c) V, c = f16(1/sqrt(dim))
 C5 decoder  pre-RMSNorm block: RMSNorm -> QKV -> causal attention -> out-proj -> residual ->
             RMSNorm -> W1 -> GELU(tanh) -> W2 -> residual, all bf16
+
+``decoder_step_mx4_program`` is such a block in service: one token per sequence, weights and a paged
+cache in microscaled 4-bit floats. It is not one of the measured configurations.
 """
 from __future__ import annotations
 
@@ -299,6 +302,34 @@ def decoder_inputs(batch: int = 4, seq: int = 2048, model: int = 2048, heads: in
     ones = lambda n: to_dtype(np.ones(n), dtype)
     return [w(0, batch, seq, model, std=1.0), ones(model), w(1, model, heads, hd), w(2, model, heads, hd),
             w(3, model, heads, hd), w(4, heads, hd, model), ones(model), w(5, model, ffn), w(6, ffn, model)]
+
+
+def decoder_step_mx4_program(seqs: int = 64, model: int = 2048, heads: int = 16, kv_heads: int = 4, hd: int = 128, ffn: int = 8192,
+                             pages: int = 4096, page: int = 64, pages_per_seq: int = 64, dtype: str = "bf16") -> T.Program:
+    """One token of each of ``seqs`` sequences through a decoder block served in microscaled 4-bit floats: weights [out, in]
+    and the paged cache are held in them, activations are quantised before each product. Inputs: x, the first norm's gains,
+    Wq, Wk, Wv, Wo, the second norm's gains, W1, W2 (codes and scales each), the cache, the tokens' slots, the
+    sequences' pages and their lengths with this token. Outputs: the block's output and the cache, which may be the
+    input cache's buffer."""
+    def body(b: T.Builder, args: List[T.Value]) -> List[T.Value]:
+        x, g1, g2, cache, slots, pages_of, lengths = args[:1] + args[1:2] + args[10:11] + args[15:]
+        wq, wk, wv = (b.mx4(args[i], args[i + 1], "model") for i in (2, 4, 6))
+        wo, w1, w2 = b.mx4(args[8], args[9], "att"), b.mx4(args[11], args[12], "model"), b.mx4(args[13], args[14], "ffn")
+        h = rms_norm(b, x, g1, "model", dtype).quantize_mx4("model")
+        q = h.contract(wq, dtype)                              # [seq, head, dim]
+        cache = cache.cache_write_mx4(h.contract(wk, dtype), h.contract(wv, dtype), slots)
+        o = q.attend_mx4(cache, pages_of, lengths)
+        y = o.merge(("head", "dim"), "att").quantize_mx4("att").contract(wo, dtype)
+        x1 = x.add(y)
+        f = gelu(b, rms_norm(b, x1, g2, "model", dtype).quantize_mx4("model").contract(w1, dtype), dtype)
+        return [x1.add(f.quantize_mx4("ffn").contract(w2, dtype)), cache]
+    kv = T.mx4_specs("model", kv_head=kv_heads, dim=hd, model=model)
+    specs = [T.spec(dtype, seq=seqs, model=model), T.spec(dtype, model=model), *T.mx4_specs("model", head=heads, dim=hd, model=model),
+             *kv, *kv, *T.mx4_specs("att", model=model, att=heads * hd), T.spec(dtype, model=model),
+             *T.mx4_specs("model", ffn=ffn, model=model), *T.mx4_specs("ffn", model=model, ffn=ffn),
+             T.cache_mx4_spec(pages, kv_heads, hd, page), T.spec("i32", seq=seqs), T.spec("i32", seq=seqs, at=pages_per_seq),
+             T.spec("i32", seq=seqs)]
+    return T.define("decoder_step_mx4", specs, body)
 
 
 CONFIGS: Dict[str, dict] = {

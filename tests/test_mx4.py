@@ -15,6 +15,7 @@ from accy_amd import hip
 from accy_amd import tensor as T
 from accy_amd import workloads as W
 from conftest import hip_run, to_f32
+from test_zz_no_alloc import _Bound, _capture, _hip_runtime, _same
 
 GRID = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
 HALF_STEP = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}
@@ -642,3 +643,193 @@ def test_attend_without_sequences_pages_or_cache():
         assert got.shape == q.shape and not got.any()
     none = hip_run(_attend_program(q[:0], cache, np.zeros((0, 4), np.int32), "f32"), [q[:0], cache, np.zeros((0, 4), np.int32), np.zeros(0, np.int32)])[0]
     assert none.shape == (0, 1, 2, 64)
+
+
+# ---- the operators together: one token of every sequence through a decoder block ----
+
+STEPS = [  # seqs, model, heads, kv, hd, ffn, page, pages per sequence, dtype
+    (5, 256, 4, 2, 64, 512, 32, 4, "bf16"), (33, 160, 6, 1, 96, 288, 64, 3, "f16"), (1, 128, 2, 2, 32, 256, 32, 1, "f32"),
+    (8, 512, 8, 2, 128, 1024, 64, 40, "bf16")]
+
+
+def _step(seqs, model, heads, kv, hd, ffn, page, per, dtype, seed=20):
+    """The program and its inputs; each sequence's own pages in some order, its new token the last of its length."""
+    rng = np.random.default_rng(seed)
+    pages = seqs * per + 1
+    prog = W.decoder_step_mx4_program(seqs, model, heads, kv, hd, ffn, pages, page, per, dtype)
+
+    def weight(*shape):
+        return list(encoded(rng.standard_normal(shape) * shape[-1] ** -0.5))
+
+    def gains():
+        return floats(1 + 0.1 * rng.standard_normal(model), dtype)
+    x = floats(rng.standard_normal((seqs, model)), dtype)
+    table = rng.permutation(pages)[:seqs * per].reshape(seqs, per).astype(np.int32)
+    lengths = rng.integers(1, per * page + 1, seqs).astype(np.int32)
+    lengths[-1] = per * page
+    slots = (table[np.arange(seqs), (lengths - 1) // page] * page + (lengths - 1) % page).astype(np.int32)
+    ins = ([x, gains()] + weight(heads, hd, model) + weight(kv, hd, model) + weight(kv, hd, model) + weight(model, heads * hd) + [gains()] +
+           weight(ffn, model) + weight(model, ffn) + [finite_cache(pages, kv, hd, page, rng), slots, table, lengths])
+    for v, t in zip(ins, prog.input_types()):
+        assert v.shape == t.shape and v.dtype == T.NUMPY_DTYPE[t.dtype]
+    return prog, ins
+
+
+def _alone(body, specs, ins):
+    return hip_run(T.define("alone", specs, body), ins)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", STEPS)
+def test_decoder_step_is_its_operators_one_by_one(sizes):
+    """The program, with what it fuses, against programs of one operator each, bit for bit; and its attention and products
+    against 64 bits on the way."""
+    seqs, model, heads, kv, hd, ffn, page, per, dtype = sizes
+    prog, ins = _step(*sizes)
+    x, g1, g2, cache, slots, table, lengths = ins[0], ins[1], ins[10], ins[15], ins[16], ins[17], ins[18]
+    say(f"decoder step {sizes}")
+    y, after = hip_run(prog, ins)
+    S, M = ("seq", seqs), ("model", model)
+
+    def codes(v, axis, n):
+        return _alone(lambda b, a: list(_pair(a[0].quantize_mx4(axis))), [T.spec(dtype, S, (axis, n))], [v])
+
+    def normed(v, g):
+        return codes(_alone(lambda b, a: W.rms_norm(b, a[0], a[1], "model", dtype), [T.spec(dtype, S, M), T.spec(dtype, M)], [v, g])[0], "model", model)
+
+    def product(v, w, axis, n, *rows):
+        specs = [*T.mx4_specs(axis, S, (axis, n)), *T.mx4_specs(axis, *rows, (axis, n))]
+        got = _alone(lambda b, a: b.mx4(a[0], a[1], axis).contract(b.mx4(a[2], a[3], axis), dtype), specs, v + w)[0]
+        p, q = decoded(*v), decoded(*w).reshape(-1, n)
+        want, mass = p @ q.T, np.abs(p) @ np.abs(q).T
+        assert_within(wide(got, dtype).reshape(seqs, -1), want, HALF_STEP[dtype] * np.abs(want) + 2 * n * 2.0 ** -23 * mass + (2.0 ** -25 if dtype == "f16" else 0))
+        return got
+    h = normed(x, g1)
+    q = product(h, ins[2:4], "model", model, ("head", heads), ("dim", hd))
+    k, v = (product(h, ins[i:i + 2], "model", model, ("kv_head", kv), ("dim", hd)) for i in (4, 6))
+    row = T.spec(dtype, S, ("kv_head", kv), ("dim", hd))
+    filled = _alone(lambda b, a: a[0].cache_write_mx4(a[1], a[2], a[3]),
+                    [T.cache_mx4_spec(len(cache), kv, hd, page), row, row, T.spec("i32", S)], [cache, k, v, slots])[0]
+    assert np.array_equal(filled, after) and np.array_equal(filled, written(cache, wide(k, dtype), wide(v, dtype), slots))
+    o = _alone(lambda b, a: a[0].attend_mx4(a[1], a[2], a[3]), [T.spec(dtype, S, ("head", heads), ("dim", hd)),
+               T.cache_mx4_spec(len(cache), kv, hd, page), T.spec("i32", S, ("at", per)), T.spec("i32", S)], [q, filled, table, lengths])[0]
+    _check_attend(q[:, None], filled, table, lengths, dtype, o[:, None])
+    back = product(codes(o.reshape(seqs, -1), "att", heads * hd), ins[8:10], "att", heads * hd, M)
+    two = [T.spec(dtype, S, M)] * 2
+    x1 = _alone(lambda b, a: a[0].add(a[1]), two, [x, back])[0]
+    f = product(normed(x1, g2), ins[11:13], "model", model, ("ffn", ffn))
+    f = _alone(lambda b, a: W.gelu(b, a[0], dtype), [T.spec(dtype, S, ("ffn", ffn))], [f])[0]
+    last = product(codes(f, "ffn", ffn), ins[13:15], "ffn", ffn, M)
+    want = _alone(lambda b, a: a[0].add(a[1]), two, [x1, last])[0]
+    assert np.array_equal(y.view(np.uint8), want.view(np.uint8))
+
+
+def _pair(q):
+    return q.codes, q.scales
+
+
+def test_decoder_step_plan():
+    """Elementwise work is part of the operators' kernels: norms' sums, codes, products, the cache, attention and nothing else;
+    the cache may be updated in place."""
+    source = hip.plan_source(_step(*STEPS[0])[0])
+    labels = [line.split()[1].split(":")[0] for line in source.splitlines() if line.startswith("// ") and " grid " in line]
+    assert labels == ["row", "quantize", "mx4", "mx4", "mx4", "cache_write", "mx4_attend", "quantize", "mx4", "row", "quantize", "mx4", "quantize", "mx4"]
+
+
+CACHE = 15  # the step's input; its second output
+
+
+def _step_bound(prog, ins, in_place):
+    bound = _Bound(prog, ins)
+    if in_place:
+        bound.op[1] = bound.ip[CACHE]
+
+    def restore():
+        """The outputs cleared, the cache as it came in."""
+        bound.clear()
+        bound.dins[CACHE].upload(ins[CACHE])
+
+    def outputs():
+        y, cache = bound.read()
+        return [y, bound.dins[CACHE].download(np.empty_like(ins[CACHE])) if in_place else cache]
+    return bound, restore, outputs
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scratch", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_decoder_step_captured_into_hip_graphs(scratch, in_place):
+    """The steps of two models captured on a stream of their own and replayed in turn, with eager steps of the other between the
+    replays; the cache in a buffer of its own and in place. Every replay equals run_hip bit for bit."""
+    rt, s, stream = _hip_runtime(), hip.Session(), hip.Stream()
+    progs = [_step(*STEPS[0]), _step(*STEPS[3], seed=21)]
+    refs = [hip_run(*p) for p in progs]
+    handles = [s.compile(p) for p, _ in progs]
+    bounds = [_step_bound(*p, in_place) for p in progs]
+    graphs, exes = [], []
+    try:
+        for h, (bound, restore, outputs), ref in zip(handles, bounds, refs):
+            bound.call(h, scratch, stream)
+            stream.synchronize()
+            _same(outputs(), ref)
+            graphs.append(_capture(rt, stream, lambda: bound.call(h, scratch, stream)))
+            exes.append(ctypes.c_void_p())
+            assert rt.hipGraphInstantiate(ctypes.byref(exes[-1]), graphs[-1], None, None, 0) == 0
+        for r in range(3):
+            for i in (0, 1):
+                say(f"replay {r} of {i}, scratch={scratch}, in place={in_place}")
+                bounds[i][1]()
+                assert rt.hipGraphLaunch(exes[i], ctypes.c_void_p(stream.handle)) == 0
+                stream.synchronize()
+                _same(bounds[i][2](), refs[i])
+                bounds[1 - i][1]()
+                bounds[1 - i][0].call(handles[1 - i], scratch, stream)
+                stream.synchronize()
+                _same(bounds[1 - i][2](), refs[1 - i])
+        for exe, graph in zip(exes, graphs):
+            rt.hipGraphExecDestroy(exe)
+            rt.hipGraphDestroy(graph)
+    finally:
+        for b, _, _ in bounds:
+            b.free()
+        for h in handles:
+            s.release(h)
+        stream.destroy()
+
+
+@pytest.mark.gpu
+def test_decoder_steps_on_two_streams_at_once():
+    """Two executors of one program on two streams, their steps submitted in turn without waiting; then every step of both has
+    run: the caches hold the tokens of all, the outputs the last step's."""
+    sizes = STEPS[0]
+    prog, ins = _step(*sizes)
+    rng = np.random.default_rng(22)
+    tokens = [floats(rng.standard_normal(ins[0].shape), sizes[-1]) for _ in range(3)]
+    want = []
+    for order in ((0, 1, 2), (2, 1, 0)):
+        cache = ins[CACHE]
+        for t in order:
+            y, cache = hip_run(prog, [tokens[t]] + ins[1:CACHE] + [cache] + ins[CACHE + 1:])
+        want.append([y, cache])
+    s, streams = hip.Session(), [hip.Stream(), hip.Stream()]
+    handles = [s.compile(prog) for _ in streams]
+    bounds = [_step_bound(prog, ins, True) for _ in streams]
+    xs = [hip.DeviceBuffer.from_array(t) for t in tokens]
+    try:
+        for again in range(3):
+            for _, restore, _ in bounds:
+                restore()
+            for step in range(3):
+                for i, (bound, _, _) in enumerate(bounds):
+                    bound.ip[0] = xs[step if i == 0 else 2 - step].ptr
+                    bound.call(handles[i], False, streams[i])
+            for i in (0, 1):
+                streams[i].synchronize()
+                _same(bounds[i][2](), want[i])
+    finally:
+        for b in [b for b, _, _ in bounds] + xs:
+            b.free()
+        for h in handles:
+            s.release(h)
+        for st in streams:
+            st.destroy()
