@@ -15,7 +15,7 @@ struct CheckProduct {
   static constexpr int BM = 128, BN = 128, GROUP_M = 8, SPLITS = 2, WK = 0;
 };
 struct CheckSmall : CheckProduct {
-  static constexpr int BM = 64, BN = 32, SPLITS = 1, WK = 2;
+  static constexpr int BM = 32, BN = 32, WK = 4;
 };
 template <int D, int DIM, int QUERIES, int GROUP, int S>
 struct CheckCache {
@@ -24,7 +24,7 @@ struct CheckCache {
   static constexpr float SL = 0x1.05p-3f;
 };
 
-extern "C" __global__ void __launch_bounds__(128) check_mx4_small(const u8_t* a, const u8_t* sa, const u8_t* b, const u8_t* sb, float* c) {
+extern "C" __global__ void __launch_bounds__(256) check_mx4_small(const u8_t* a, const u8_t* sa, const u8_t* b, const u8_t* sb, float* c) {
   accy::mx4::contract_direct<CheckSmall>(a, sa, b, sb, CheckStore{c});
 }
 extern "C" __global__ void __launch_bounds__(256) check_mx4_tile(const u8_t* a, const u8_t* sa, const u8_t* b, const u8_t* sb, float* c) {

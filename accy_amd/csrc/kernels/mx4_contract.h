@@ -24,10 +24,10 @@ __device__ __forceinline__ void settle(f32x16& acc) { asm volatile("" : "+a"(acc
 
 // Small tiles, BM x BN outputs (multiples of 16) of a workgroup whose WK waves share K, each keeping sums of the whole tile, which
 // meet in LDS at the end: for few rows, where every weight is read once, and for products too small to fill the chip with
-// larger tiles. Bound by the operands' bytes, of which a CU takes about 45 KB a us (tile (16, 32): 16 x 8192 x 8192 6.7
+// larger tiles. Bound by the operands' bytes, of which a CU takes about 52 KB a us (tile (16, 32): 16 x 8192 x 8192 6.7
 // us, 2.4 of them a launch; 16 x 28672 x 8192, from HBM, 22.5).
 //
-// A wave takes 256 values of every row at a time (every WK-th 256), four stages ahead, on its own: its codes go straight to
+// A wave takes 256 values of every row at a time (every WK-th 256), up to four stages ahead, on its own: its codes go straight to
 // its own part of LDS, an instruction 128 bytes of eight rows, and its scales through registers, eight bytes a row. (Operands
 // straight to registers in the matrix instruction's order, whose neighbouring lanes are rows apart, take a cache access
 // per lane: 10.3 and 29.5 us for the above.) v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds row l % 16 and, of the eight
@@ -35,7 +35,7 @@ __device__ __forceinline__ void settle(f32x16& acc) { asm volatile("" : "+a"(acc
 // row and are not stored. A block past K reads the last one with the scales 2^-127 on both sides, whose products vanish in f32
 // (below 36 x 2^-254).
 //
-// C supplies M, N, K, BM, BN, WK and SPLITS (workgroups along K, blockIdx.z).
+// C supplies M, N, K, BM, BN and WK.
 template <int S>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c, u32_t sa, u32_t sb) {
   const i32x8 aw = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, bw = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
@@ -57,13 +57,15 @@ __device__ __forceinline__ u32x2 scale_eight(const u8_t* __restrict__ row, long 
 template <class C, class Epi>
 __device__ __forceinline__ void contract_direct(const u8_t* __restrict__ A, const u8_t* __restrict__ AS, const u8_t* __restrict__ B,
                                                 const u8_t* __restrict__ BS, const Epi& epi) {
-  constexpr int TM = C::BM / 16, TN = C::BN / 16, WK = C::WK, S = 4, ROWS = C::BM + C::BN, D = ROWS / 8, E = (ROWS + 63) / 64;
-  constexpr long TILES_N = (C::N + C::BN - 1) / C::BN, BLOCKS = C::K / 32, ITERS = (BLOCKS + 7) / 8, STRIDE = (long)WK * C::SPLITS;
+  constexpr int TM = C::BM / 16, TN = C::BN / 16, WK = C::WK, ROWS = C::BM + C::BN, D = ROWS / 8, E = (ROWS + 63) / 64;
+  constexpr long TILES_N = (C::N + C::BN - 1) / C::BN, BLOCKS = C::K / 32, ITERS = (BLOCKS + 7) / 8;
+  constexpr int S = ITERS >= 4 * WK ? 4 : (int)((ITERS + WK - 1) / WK);  // no more stages than a wave has steps
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   const long m0 = (long)blockIdx.x / TILES_N * C::BM, n0 = (long)blockIdx.x % TILES_N * C::BN;
-  __shared__ __attribute__((aligned(1024))) u8_t c0[WK][ROWS * 128], c1[WK][ROWS * 128], c2[WK][ROWS * 128], c3[WK][ROWS * 128];
+  __shared__ __attribute__((aligned(1024))) u8_t c0[WK][ROWS * 128], c1[S > 1 ? WK : 1][S > 1 ? ROWS * 128 : 16],
+      c2[S > 2 ? WK : 1][S > 2 ? ROWS * 128 : 16], c3[S > 3 ? WK : 1][S > 3 ? ROWS * 128 : 16];
   __shared__ __attribute__((aligned(16))) u8_t words[WK][ROWS * 8];
-  u8_t* const stage[4] = {c0[wave], c1[wave], c2[wave], c3[wave]};
+  u8_t* const stage[4] = {c0[wave], c1[S > 1 ? wave : 0], c2[S > 2 ? wave : 0], c3[S > 3 ? wave : 0]};
   // codes: an instruction moves 128 bytes of eight rows, lane l the chunk l % 8 ^ (row / 2 mod 8) of row l / 8
   const u8_t* src[D];
   int chunk[D];
@@ -102,14 +104,14 @@ __device__ __forceinline__ void contract_direct(const u8_t* __restrict__ A, cons
     const int r = row0 + (lane & 15);
     return *(const u32x4*)(stage[s] + r * 128 + 16 * ((2 * g + e) ^ ((r >> 1) & 7)));
   };
-  long it = C::SPLITS > 1 ? (long)blockIdx.z * WK + wave : wave;
+  long it = wave;
 #pragma unroll
   for (int s = 0; s < S - 1; ++s)
-    if (it + s * STRIDE < ITERS) load(s, it + s * STRIDE);
-  for (; it < ITERS; it += S * STRIDE) {
+    if (it + s * WK < ITERS) load(s, it + s * WK);
+  for (; it < ITERS; it += S * WK) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const long now = it + s * STRIDE, ahead = now + (S - 1) * STRIDE;
+      const long now = it + s * WK, ahead = now + (S - 1) * WK;
       if (now >= ITERS) break;
       // The stage's codes have landed when no more is outstanding than the three stages after it (their scales not counted);
       // where no stage follows, when nothing is.
@@ -147,18 +149,20 @@ __device__ __forceinline__ void contract_direct(const u8_t* __restrict__ A, cons
     }
   }
   // Element e of lane l of tile (i, j) is output (16 i + 4 (l / 16) + e, 16 j + l % 16).
+  // A wave's sums take the place of its first stage, which every load has reached and every read has left.
   constexpr int ALL = C::BM * C::BN;
-  __shared__ float sums[WK * ALL];
+  static_assert(ALL * 4 <= ROWS * 128, "a wave's sums fit its stage");
+  float* const mine = (float*)c0[wave];
 #pragma unroll
   for (int t = 0; t < TM * TN; ++t)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sums[wave * ALL + (t * 4 + e) * 64 + lane] = acc[t / TN][t % TN][e];
+    for (int e = 0; e < 4; ++e) mine[(t * 4 + e) * 64 + lane] = acc[t / TN][t % TN][e];
   __syncthreads();
   for (int x = tid; x < ALL; x += 64 * WK) {
     const int m = x / C::BN, n = x % C::BN, at = (((m >> 4) * TN + (n >> 4)) * 4 + (m & 3)) * 64 + ((m >> 2) & 3) * 16 + (n & 15);
-    float v = sums[at];
+    float v = ((const float*)c0[0])[at];
 #pragma unroll
-    for (int w = 1; w < WK; ++w) v += sums[w * ALL + at];
+    for (int w = 1; w < WK; ++w) v += ((const float*)c0[w])[at];
     if ((C::M % C::BM == 0 || m0 + m < C::M) && (C::N % C::BN == 0 || n0 + n < C::N)) epi(0, m0 + m, n0 + n, v);
   }
 }

@@ -328,12 +328,13 @@ void Planner::mx4_contract(uint32_t v) {
   finish(target);
 }
 
-// The kernel, tile and K split of a product: the least of the times estimated for each, in us (kernels/mx4_contract.h). Small
-// tiles are bound by the bytes that a CU takes; a workgroup of a large one takes a time per step of 128 values that grows with the
-// workgroups at work (two of 128 x 128 to a CU, one of 256 x 256) and the time to store its results.
+// The kernel, tile and K split of a product: the least of the times estimated for each, in us without a launch (kernels/mx4_contract.h).
+// Small tiles are bound by the bytes that a CU takes, 52 KB a us and 0.1 us a workgroup; a workgroup of a large one takes a time per
+// step of 128 values that grows with the workgroups at work (two of 128 x 128 to a CU, one of 256 x 256) and the time to store its results.
 // Measured (us back to back, 2.4 of them a launch; 128 x 128 / 256 x 256): 512 x 8192 x 2048 8.4 / 17.0, 1024 x 8192 x 2048 16.0 /
 // 19.6, 1536 x 8192 x 2048 21.8 / 21.6, 2048 x 8192 x 2048 28.3 / 24.5, 3000 x 8192 x 2048 42 / 48, 4096 x 4096 x 1024 19.4 /
-// 18.1, 8192^3 377 / 276; small / 128 x 128: 16 x 8192 x 2048 3.2 / 6.3, 64 x 8192 x 2048 5.3 / 6.4, 128 x 8192 x 2048 8 / 6.3.
+// 18.1, 8192^3 377 / 276; 32 x 32 / 128 x 128: 64 x 8192 x 2048 4.6 / 6.5, 500 x 1000 x 2048 5.0 / 7.0, 200 x 1000 x 8192 7.0 / 15.8,
+// 1000 x 1000 x 1024 5.3 / 5.6, 2000 x 1000 x 1024 8.7 / 6.1, 1000 x 4096 x 256 7.9 / 5.7.
 Planner::Mx4Tile Planner::mx4_tile(int64_t M, int64_t N, int64_t K) const {
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t steps = up(K, 128), groups = up(steps, 4);
@@ -345,15 +346,18 @@ Planner::Mx4Tile Planner::mx4_tile(int64_t M, int64_t N, int64_t K) const {
     best = t;
     least = cost;
   };
-  const int bm = M <= 16 ? 16 : M <= 32 ? 32 : 64;
-  for (const int bn : {16, 32, 64}) {
-    if (bm == 64 && bn == 64) continue;  // 160 KB of LDS hold four stages of two waves' (64, 32)
+  // Four waves along K where their stages leave room for two workgroups on a CU or there is but one for each (1000 x 1000 x 1024 in 32 x
+  // 32: four 5.3, two 5.4, one 6.2; 300 x 1000 x 16384 19.7 and 17.4). Larger tiles read less, but fewer of them do (64 x 8192 x 2048: 32 x
+  // 32 4.6, 32 x 64 5.3, 64 x 64 7.1).
+  const int bm = M <= 16 ? 16 : 32;
+  for (const int bn : {16, 32}) {
     Mx4Tile t;
     t.bm = bm;
     t.bn = bn;
-    const int64_t wgs = up(M, bm) * up(N, bn);
-    t.wk = bm + bn <= 48 && wgs <= 256 ? 4 : 2;
-    offer(t, 1.2 + (double)up(wgs, 256) * (double)((bm + bn) * K) * 0.53 / 42e3);
+    const int64_t wgs = up(M, bm) * up(N, bn), lds = std::min<int64_t>(4, up(K, 1024)) * 4 * (bm + bn) * 128;
+    t.wk = wgs > 256 && lds > 80 * 1024 ? 2 : 4;
+    const double per_cu = std::max(1.0, (double)wgs / 256);
+    offer(t, 0.3 + per_cu * (0.1 + (double)((bm + bn) * K) * 0.53 / 52e3));
   }
   for (const int size : {128, 256}) {
     const int64_t tiles = up(M, size) * up(N, size), most = size == 128 ? 512 : 256;
@@ -361,7 +365,7 @@ Planner::Mx4Tile Planner::mx4_tile(int64_t M, int64_t N, int64_t K) const {
       if (splits > 1 && up(groups, up(groups, splits)) != splits) continue;
       const double share = (double)(splits > 1 ? up(groups, splits) * 4 : steps);
       auto round = [&](double n) {
-        if (size == 128) return 0.3 + 1.8 * std::min(1.0, n / 256) + share * (0.25 + 0.45 * std::max(0.0, n - 256) / 256);
+        if (size == 128) return 0.9 + 1.8 * std::min(1.0, n / 256) + share * (0.2 + 0.5 * std::max(0.0, n - 256) / 256);
         return 1.0 + 4.0 * n / 256 + share * (0.65 + 0.4 * n / 256);
       };
       const int64_t all = tiles * splits;

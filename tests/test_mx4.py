@@ -321,8 +321,8 @@ def test_contract(m, n, k, dtype):
 # the large tiles, ragged: 128 x 128 and 256 x 256, K in whole steps of 512, of 128 and neither, K split
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k,dtype,tile,splits", [
-    (1100, 4100, 672, "bf16", 128, 1), (260, 4100, 1280, "f16", 128, 1), (100, 8192, 128, "f32", 128, 1), (2500, 4100, 1184, "f32", 256, 1),
-    (2100, 4200, 1664, "bf16", 256, 1), (2100, 4200, 2048, "f16", 256, 1), (200, 1000, 8192, "bf16", 128, 4), (1024, 1000, 8320, "f32", 128, 1)])
+    (1100, 4100, 672, "bf16", 128, 1), (260, 4100, 1280, "f16", 128, 1), (1000, 4100, 128, "f32", 256, 1), (1000, 4000, 256, "f32", 128, 1), (2500, 4100, 1184, "f32", 256, 1),
+    (2100, 4200, 1664, "bf16", 256, 1), (2100, 4200, 2048, "f16", 256, 1), (200, 1000, 28672, "bf16", 128, 8), (1024, 1000, 8320, "f32", 128, 1)])
 def test_contract_large(m, n, k, dtype, tile, splits):
     prog = _product(m, n, k, dtype)
     src = hip.plan_source(prog)
