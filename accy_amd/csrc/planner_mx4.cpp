@@ -359,7 +359,9 @@ Planner::Mx4Tile Planner::mx4_tile(int64_t M, int64_t N, int64_t K) const {
     const double per_cu = std::max(1.0, (double)wgs / 256);
     offer(t, 0.3 + per_cu * (0.1 + (double)((bm + bn) * K) * 0.53 / 52e3));
   }
+  // (a tile's scales are addressed in 32 bits)
   for (const int size : {128, 256}) {
+    if (K > (int64_t(1) << 28)) continue;
     const int64_t tiles = up(M, size) * up(N, size), most = size == 128 ? 512 : 256;
     for (int splits = 1; splits <= (opt_.allow_split && size == 128 ? 8 : 1); splits *= 2) {
       if (splits > 1 && up(groups, up(groups, splits)) != splits) continue;

@@ -7,6 +7,7 @@ most an ulp, truncating ones included). Quantised values are exact: codes and sc
 """
 import ctypes
 import itertools
+import random
 
 import numpy as np
 import pytest
@@ -15,6 +16,7 @@ from accy_amd import hip
 from accy_amd import tensor as T
 from accy_amd import workloads as W
 from conftest import hip_run, to_f32
+from test_mutated_programs import _mutate, _plan_status
 from test_zz_no_alloc import _Bound, _capture, _hip_runtime, _same
 
 GRID = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
@@ -645,6 +647,94 @@ def test_attend_without_sequences_pages_or_cache():
     assert none.shape == (0, 1, 2, 64)
 
 
+@pytest.mark.gpu
+def test_cache_beyond_32_bits():
+    """A cache of 4.5 GB, its last pages in use, against a small one that holds the same tokens."""
+    rng = np.random.default_rng(16)
+    pages, kv, dim, page, tokens, dtype = 64000, 8, 128, 64, 100, "f16"
+    keys, values = (floats(rng.standard_normal((tokens, kv, dim)), dtype) for _ in range(2))
+    q = floats(rng.standard_normal((1, 1, 16, dim)), dtype)
+    row = T.spec(dtype, token=tokens, kv_head=kv, dim=dim)
+
+    def body(b, a):
+        cache = a[0].cache_write_mx4(a[1], a[2], a[3])
+        return [cache, cache.cache_keys_mx4(a[3], ("dim", dim), dtype), cache.cache_values_mx4(a[3], ("dim", dim), dtype),
+                a[4].attend_mx4(cache, a[5], a[6])]
+    out = []
+    for n in (2, pages):
+        prog = T.define("far", [T.cache_mx4_spec(n, kv, dim, page), row, row, T.spec("i32", token=tokens), T.spec(dtype, seq=1, query=1, head=16, dim=dim),
+                                T.spec("i32", seq=1, at=2), T.spec("i32", seq=1)], body)
+        table = np.array([[n - 1, n - 2]], np.int32)
+        at = np.arange(tokens)
+        slots = (table[0, at // page] * page + at % page).astype(np.int32)
+        say(f"{n} pages")
+        stream = hip.Stream()
+        cache = hip.DeviceBuffer(n * kv * page * (dim + dim // 16))
+        ins = [cache] + [hip.DeviceBuffer.from_array(x) for x in (keys, values, slots, q, table, np.array([tokens], np.int32))]
+        got = [np.zeros_like(keys), np.zeros_like(keys), np.zeros_like(q)]
+        outs = [hip.DeviceBuffer(x.nbytes) for x in got]
+        _device_run(prog, ins, [cache] + outs, stream)
+        out.append([o.download(x) for o, x in zip(outs, got)])
+        for x in ins + outs:
+            x.free()
+        stream.destroy()
+    _same(out[1], out[0])
+    for got, want in zip(out[0], (keys, values)):
+        assert np.array_equal(wide(got, dtype), quantized(wide(want, dtype))[2])
+
+
+@pytest.mark.gpu
+def test_operands_used_twice():
+    """One quantised tensor on both sides of a product; one tensor as keys and values."""
+    rng = np.random.default_rng(17)
+    x = floats(rng.standard_normal((70, 96)), "f32")
+
+    def gram(b, a):
+        m = a[0].quantize_mx4("k")
+        return m.contract(b.mx4(m.codes.rename("m", "n"), m.scales.rename("m", "n"), "k"), "f32")
+    got = hip_run(T.define("gram", [T.spec("f32", m=70, k=96)], gram), [x])[0]
+    v = quantized(wide(x, "f32"))[2]
+    assert_within(got.astype(np.float64), v @ v.T, 2 * 96 * 2.0 ** -23 * (np.abs(v) @ np.abs(v).T))
+    cache = finite_cache(2, 3, 32, 32, rng)
+    slots = np.array([63, 0, 5], np.int32)
+    prog = T.define("both", [T.cache_mx4_spec(2, 3, 32, 32), T.spec("f32", token=3, kv_head=3, dim=32), T.spec("i32", token=3)],
+                    lambda b, a: a[0].cache_write_mx4(a[1], a[1], a[2]))
+    rows = x.reshape(-1)[:3 * 3 * 32].reshape(3, 3, 32)
+    assert np.array_equal(hip_run(prog, [cache, rows, slots])[0], written(cache, wide(rows, "f32"), wide(rows, "f32"), slots))
+
+
+@pytest.mark.gpu
+def test_cache_grows_in_a_scan():
+    """Tokens made one after the other inside a scan, each from the attention over those before: as single programs."""
+    rng = np.random.default_rng(18)
+    S, H, D, page, per, dtype = 3, 2, 64, 32, 2, "bf16"
+    cache = finite_cache(S * per, H, D, page, rng)
+    table = rng.permutation(S * per).reshape(S, per).astype(np.int32)
+    lengths = np.array([5, 31, 32], np.int32)
+    x = floats(rng.standard_normal((S, H, D)), dtype)
+    specs = [T.spec(dtype, seq=S, head=H, dim=D), T.cache_mx4_spec(S * per, H, D, page), T.spec("i32", seq=S, at=per), T.spec("i32", seq=S)]
+
+    def step(b, c):
+        x, cache, table, lengths = c
+        one, width = b.full("i32", 1, ("seq", S)), b.full("i32", page, ("seq", S))
+        at = lengths.div(width)
+        second = at.compare("ge", one)
+        pages = [table.mul(b.iota("i32", "at", ("seq", S), ("at", per)).compare("eq", b.full("i32", i, ("seq", S), ("at", per))).select(
+            b.full("i32", 1, ("seq", S), ("at", per)), b.full("i32", 0, ("seq", S), ("at", per)))).sum("at") for i in range(per)]
+        slots = second.select(pages[1], pages[0]).mul(width).add(lengths.sub(at.mul(width)))
+        rows = x.rename("head", "kv_head")
+        cache = cache.cache_write_mx4(rows, rows, slots)
+        return [x.attend_mx4(cache, table, lengths.add(one)).add(x), cache, table, lengths.add(one)]
+    ins = [x, cache, table, lengths]
+    loop = T.define("loop", specs, lambda b, a: (lambda l: [l, b.projection(l, 1)])(b.scan(4, a, step)))
+    one = T.define("one", specs, lambda b, a: step(b, a))
+    want = ins
+    for _ in range(4):
+        want = hip_run(one, want)
+    got = hip_run(loop, ins)
+    _same(got, want[:2])
+
+
 # ---- the operators together: one token of every sequence through a decoder block ----
 
 STEPS = [  # seqs, model, heads, kv, hd, ffn, page, pages per sequence, dtype
@@ -833,3 +923,11 @@ def test_decoder_steps_on_two_streams_at_once():
             s.release(h)
         for st in streams:
             st.destroy()
+
+
+def test_every_mutated_program_gets_a_status():
+    lib, rng = hip.library(), random.Random(1)
+    bases = [p.encode() for p in (_step(*STEPS[0])[0], _step(*STEPS[1])[0], _product(1000, 4000, 256, "bf16"), _product(40, 50, 96, "f32"),
+                                  _write_program(4, 2, 64, 32, 9000, "f16"))]
+    seen = {_plan_status(lib, _mutate(rng.choice(bases), rng)) for _ in range(1500)}
+    assert seen <= set(range(9)) and {0, 1} <= seen
