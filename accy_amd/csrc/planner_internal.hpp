@@ -71,9 +71,9 @@ inline uint64_t prod(const std::vector<Dim>& dims, size_t b, size_t e) {
   return n;
 }
 
-// 32-bit indices while every element index plus one grid stride (at most 2^20 workgroups x 256
-// threads = 2^28) stays below 2^31, so that no grid-stride loop's increment overflows.
-inline std::string index_type(uint64_t max_elems) { return max_elems < (1ull << 31) - (1ull << 28) ? "i32_t" : "i64_t"; }
+// 32-bit indices while every element index plus one grid stride (of 2^20 workgroups x 256 threads x the four or eight elements of
+// each, but not beyond the elements rounded up to a workgroup's) stays below 2^31, so that no grid-stride loop's increment overflows.
+inline std::string index_type(uint64_t max_elems) { return max_elems <= (1ull << 30) ? "i32_t" : "i64_t"; }
 
 inline uint32_t grid_for(uint64_t work_items, uint32_t block, uint64_t cap = 1u << 20) {
   uint64_t g = (work_items + block - 1) / block;
@@ -218,7 +218,7 @@ class Planner {
   int counter_ = 0;
   uint64_t max_elems_ = 1;
 
-  // Index arithmetic is 32-bit unless some value of the program has 2^31 or more elements.
+  // Index arithmetic is 32-bit unless some value of the program has more than 2^30 elements.
   std::string itype() const { return index_type(max_elems_); }
 
   void process(uint32_t v);

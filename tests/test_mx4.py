@@ -8,6 +8,7 @@ most an ulp, truncating ones included). Quantised values are exact: codes and sc
 import ctypes
 import itertools
 import random
+import re
 
 import numpy as np
 import pytest
@@ -265,6 +266,35 @@ def test_quantize_evaluates_its_operand_and_moves_the_axis():
     codes, scales = hip_run(T.define("p", [T.spec("f32", k=64, m=9), T.spec("f32", k=64)], body), [x, g])
     want = encoded((x * g[:, None]).T.astype(np.float64))
     assert np.array_equal(codes, want[0]) and np.array_equal(scales, want[1])
+
+
+def test_index_width():
+    """Beyond 2^30 elements an index and a grid's stride no longer fit 32 bits together."""
+    def body(b, a):
+        m = a[0].quantize_mx4("c")
+        return [m.codes, m.scales, m.dequantize("f16"), a[0].add(a[0])]
+    for rows, index in ((1 << 15, "i32_t"), ((1 << 15) + 1, "i64_t")):
+        source = hip.plan_source(T.define("p", [T.spec("bf16", r=rows, c=1 << 15)], body))
+        assert set(re.findall(r"typedef (i\d\d_t) I;", source)) == {index} and f"values<1, {index}," in source
+
+
+@pytest.mark.gpu
+def test_quantize_more_than_2_to_the_30():
+    """1.1 G values, rows that repeat: so do codes, scales and values."""
+    rows, cols = 33600, 1 << 15
+    row = floats(np.random.default_rng(19).standard_normal((25, cols)), "bf16")
+    spec = T.spec("bf16", g=rows // 25, r=25, c=cols)
+    x = np.broadcast_to(row, (rows // 25, 25, cols))
+
+    def body(b, a):
+        m = a[0].quantize_mx4("c")
+        return [m.codes, m.scales, m.dequantize("bf16")]
+    say("quantize 1.1 G")
+    got = hip_run(T.define("p", [spec], body), [np.ascontiguousarray(x)])
+    want = hip_run(T.define("p", [T.spec("bf16", g=1, r=25, c=cols)], body), [row[None]])
+    for g, w in zip(got, want):
+        for i in range(len(g)):
+            assert np.array_equal(g[i], w[0])
 
 
 @pytest.mark.gpu
