@@ -961,3 +961,26 @@ def test_every_mutated_program_gets_a_status():
                                   _write_program(4, 2, 64, 32, 9000, "f16"))]
     seen = {_plan_status(lib, _mutate(rng.choice(bases), rng)) for _ in range(1500)}
     assert seen <= set(range(9)) and {0, 1} <= seen
+
+
+@pytest.mark.gpu
+def test_decoder_step_tuned_and_profiled():
+    """Launch tuning of a program with custom calls keeps its results; profiling names their kernels."""
+    prog, ins = _step(*STEPS[1])
+    want = hip_run(prog, ins)
+    hip.tuning_clear()
+    try:
+        hip.tune(prog, ins, repeats=2)
+        _same(hip_run(prog, ins), want)
+    finally:
+        hip.tuning_clear()
+    bound, _, outputs = _step_bound(prog, ins, False)
+    stream = hip.Stream()
+    with hip.Hip(prog) as ex:
+        ex.set_profiling(True)
+        ex.launch_device(list(bound.ip), list(bound.op), stream.handle)
+        kernels = ex.kernels()
+        assert {"quantize", "gemm", "attention", "row"} == {k.klass for k in kernels} and all(k.last_ms > 0 for k in kernels)
+        _same(outputs(), want)
+    bound.free()
+    stream.destroy()
