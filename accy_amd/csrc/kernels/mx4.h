@@ -167,14 +167,27 @@ __device__ __forceinline__ void cache_write(u8_t* __restrict__ cache, const type
   }
   __syncthreads();
   if constexpr (!OWNERS) {
-    for (long j0 = t0 + 1 + tid; j0 < C::TOKENS; j0 += 2048) {
+    // token t0 + j against t0 + w, j > w; none has the slot -2
+    constexpr int W = TW < 4 ? TW : 4;
+    for (int j0 = 1 + tid; j0 < C::TOKENS - t0; j0 += 2048) {
       int s[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) s[u] = slots[j0 + 256 * u < C::TOKENS ? j0 + 256 * u : C::TOKENS - 1];
+      for (int u = 0; u < 8; ++u) s[u] = j0 + 256 * u < C::TOKENS - t0 ? slots[t0 + j0 + 256 * u] : -2;
+      for (int w0 = 0; w0 < TW; w0 += W) {
+        int mine[W];
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        for (int w = 0; w < TW && t0 + w < (j0 + 256 * u < C::TOKENS ? j0 + 256 * u : C::TOKENS - 1); ++w)
-          if (place[w] == s[u]) place[w] = -1;
+        for (int w = 0; w < W; ++w) mine[w] = w0 + w < TW ? place[w0 + w] : -1;
+        u32_t lost = 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+          for (int w = 0; w < W; ++w) lost |= s[u] == mine[w] && j0 + 256 * u > w0 + w ? 1u << w : 0;
+        if (lost != 0) {
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            if (lost >> w & 1) place[w0 + w] = -1;
+        }
+      }
     }
     __syncthreads();
   }

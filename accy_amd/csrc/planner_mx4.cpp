@@ -433,8 +433,8 @@ void Planner::mx4_cache_write(uint32_t v) {
     const int ks = dense_slot(op.args[1]), vs = dense_slot(op.args[2]), ss = dense_slot(op.args[3]);
     require(n < (uint64_t(1) << 31), op, "2^31 tokens or more");
     // Looking through the later slots costs every workgroup a pass over the list; a table of each slot's last token two launches
-    // (8 heads of 128 bf16: 1000 tokens 4.8 us by the list and 7.7 by the table, 4000 8.1 and 10.1, 8192 17.5 and 14.8, 65536 324 and 92).
-    const bool owners = n > 6000;
+    // (8 heads of 128 bf16: 1000 tokens 3.9 us by the list and 7.7 by the table, 4000 7.0 and 10.1, 8192 13.9 and 14.7, 16384 27.2 and 23.9).
+    const bool owners = n > 8192;
     const std::string nm = name("mx4_cache_write", v);
     const std::string head = "#include \"mx4\"\nstruct Cfg_" + nm + " {\n" + c.members(kt.dtype) + "  static constexpr long TOKENS = " +
                              std::to_string(n) + ";\n};\n";
