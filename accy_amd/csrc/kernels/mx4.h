@@ -251,12 +251,12 @@ __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const
 // key is 0. Scores, softmax and sums are f32.
 //
 // The Q x G rows that share a key-value head are the columns of 16-wide matrix instructions, 16 rows to a workgroup (two sixteens to
-// a wave, so that the cache is read once for 32 rows, run out of registers: 8 heads of 128 x 32 rows bf16 over 8 x 4096 keys take 94
-// us where twice the workgroups and reads take 65). Per 32 keys (a step) a wave computes S^T = K Q^T, two tiles of 16 keys, on
+// a wave, so that the cache is read once for 32 rows, run out of registers: 24 x 8 heads x 8000 keys of 128, 32 rows, bf16, take 94 us
+// where twice the workgroups and reads take 65). Per 32 keys (a step) a wave computes S^T = K Q^T, two tiles of 16 keys, on
 // v_mfma_scale_f32_16x16x128_f8f6f4, whose A operand is K as it lies: a lane's 16 bytes are a block of one key, its scale beside
 // it. The queries are its B operand, in e4m3 with a scale per block: four bits of them at a time, PARTS times (f32 6, else 3).
 // That is all bits of a query down to 2^-11 of its block's largest in bf16, 2^-8 in f16 and 2^-7 in f32; what lies below is off by
-// 2^-19 (f32 2^-31) of the largest at most. (Two parts for bf16 take 113 us where three take 115, 8 x 16 x 4096 keys 15.0 and 16.2, but they
+// 2^-19 (f32 2^-31) of the largest at most. (Two parts for bf16 take 113 us where three take 115 for 48 x 8 heads x 16000 keys, 15.0 and 16.2 for 8 x 16 x 4096, but they
 // lose queries 2^-13 of the largest altogether. K widened to bf16 as V is: 40 of the 241 VALU instructions of a step, which bound it.)
 // Lane l then holds row l % 16 and, g = l / 16, keys 4 g + i and 16 + 4 g + i, which is how the B operand of O^T = V^T P^T
 // (v_mfma_f32_16x16x32_bf16) wants them when its k index 8 g + j means key 4 g + j (j < 4) or 12 + 4 g + j, so P never leaves
@@ -362,7 +362,8 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     else if constexpr (decltype(s)::value == 1) return l1;
     else return l2;
   };
-  // A head's groups of rows lie eight workgroups apart, on one XCD: its cache comes through that one's L2.
+  // A head's groups of rows lie eight workgroups apart, on one XCD: its cache comes through that one's L2 (24 x 8 heads x 8000 keys
+  // of 128, 32 rows: 66.9 us side by side, 64.3 so).
   const int set = blockIdx.x / (8 * RS::GROUPS), in = blockIdx.x % (8 * RS::GROUPS);
   const int wide = C::SEQS * C::H - 8 * set < 8 ? (int)(C::SEQS * C::H - 8 * set) : 8;
   const long bh = 8 * set + in % wide, b = bh / C::H, h = bh % C::H;
