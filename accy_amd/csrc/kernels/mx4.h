@@ -70,19 +70,19 @@ template <int DT> __device__ __forceinline__ void store8(typename Elem<DT>::type
   }
 }
 
-// The scale byte of the block that four adjacent lanes hold eight values each of (all four call it), and the codes of
-// this lane's eight. The exponent of the largest magnitude comes from its bits: the unsigned order of the bits without
+// The scale byte of the block that 32 / V adjacent lanes hold V values each of (all of them call it), and the codes of
+// this lane's. The exponent of the largest magnitude comes from its bits: the unsigned order of the bits without
 // the sign is the order of the magnitudes, with infinity and NaN above all of them. The scale's exponent is 2 less, and
 // 2^-127 (byte 0) for everything below 2^-125, subnormals and zero among it.
-__device__ __forceinline__ u32_t block_scale(const float (&x)[8]) {
+template <int V> __device__ __forceinline__ u32_t block_scale(const float (&x)[V]) {
   u32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < V; ++i) {
     const u32_t b = __builtin_bit_cast(u32_t, x[i]) & 0x7fffffffu;
     top = top > b ? top : b;
   }
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
+  for (int o = 1; o < 32 / V; o <<= 1) {
     const u32_t b = (u32_t)__shfl_xor((int)top, o, 64);
     top = top > b ? top : b;
   }
@@ -103,6 +103,24 @@ __device__ __forceinline__ void decode8(u32_t w, u32_t byte, float (&x)[8]) {
   const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
   const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
   x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1], x[4] = c[0], x[5] = c[1], x[6] = d[0], x[7] = d[1];
+}
+// The same of four values, codes in the low half.
+__device__ __forceinline__ u32_t encode4(const float (&x)[4], u32_t byte) {
+  const float s = scale_of(byte);
+  const u32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[0], x[1], s, 0);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+}
+__device__ __forceinline__ void decode4(u32_t w, u32_t byte, float (&x)[4]) {
+  const float s = scale_of(byte);
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+  x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1];
+}
+template <int DT> __device__ __forceinline__ void store4(typename Elem<DT>::type* __restrict__ p, const float (&x)[4]) {
+  if constexpr (DT == 2) {
+    *(f32x4*)p = f32x4{x[0], x[1], x[2], x[3]};
+  } else {
+    *(u32x2*)p = u32x2{(u32_t)to_elem<DT>(x[0]) | ((u32_t)to_elem<DT>(x[1]) << 16), (u32_t)to_elem<DT>(x[2]) | ((u32_t)to_elem<DT>(x[3]) << 16)};
+  }
 }
 
 // The values of codes and scales, eight per thread: N values, a multiple of 32.

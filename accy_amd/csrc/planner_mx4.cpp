@@ -102,30 +102,59 @@ void Planner::mx4_quantize(uint32_t v) {
   element_type(op, t.dtype);
   const int64_t K = last(t);
   require(t.rank() >= 1 && K % 32 == 0, op, "the last axis is a multiple of 32");
-  int codes = -1, scales = -1;
+  // codes, scales: the first of each
+  bool have[2] = {false, false};
+  uint32_t id[2] = {0, 0};
   std::vector<uint32_t> made;
   for (uint32_t u = v; u < g_.ops.size(); ++u) {
     const Op& uo = g_.ops[u];
     if (!live_[u] || done_[u] || uo.kind != Kind::custom_call || uo.index != 1 || uo.args != op.args) continue;
     const bool is_codes = uo.bytes == "accy.mx4.codes";
     if (!is_codes && uo.bytes != "accy.mx4.scales") continue;
-    int& slot = is_codes ? codes : scales;
-    if (slot >= 0) continue;
+    if (have[!is_codes]) continue;
     require(uo.result.dtype == DType::u8 && same_rows(uo.result, t) && last(uo.result) == K / (is_codes ? 2 : 32), uo,
             is_codes ? "u8 codes, K / 2 to a row" : "u8 scales, K / 32 to a row");
-    slot = temp_slot(u);
+    have[!is_codes] = true;
+    id[!is_codes] = u;
     made.push_back(u);
+  }
+  // Their values, where the program reads them back, are stored by the same kernel; what only they read is not stored.
+  std::vector<std::pair<int, uint32_t>> values;  // element type, operation
+  for (uint32_t u = v; have[0] && have[1] && u < g_.ops.size(); ++u) {
+    const Op& uo = g_.ops[u];
+    if (!live_[u] || done_[u] || uo.kind != Kind::custom_call || uo.index != 1 || uo.bytes != "accy.mx4.values") continue;
+    if (uo.args.size() != 2 || uo.args[0] != id[0] || uo.args[1] != id[1]) continue;
+    require(same_rows(uo.result, t) && last(uo.result) == K, uo, "the result has the codes' rows and two values for each of their bytes");
+    values.push_back({element_type(uo, uo.result.dtype), u});
+  }
+  auto stored = [&](int which) {
+    if (!have[which]) return false;
+    if (values.empty() || is_output_[id[which]]) return true;
+    for (const uint32_t u : users_[id[which]])
+      if (std::none_of(values.begin(), values.end(), [&](const std::pair<int, uint32_t>& x) { return x.second == u; })) return true;
+    return false;
+  };
+  const int codes = stored(0) ? temp_slot(id[0]) : -1, scales = stored(1) ? temp_slot(id[1]) : -1;
+  std::vector<int> value_slots;
+  for (const auto& x : values) {
+    value_slots.push_back(temp_slot(x.second));
+    made.push_back(x.second);
   }
   const uint64_t nel = t.elements();
   if (nel) {
+    // A thread takes eight values of a workgroup's 2048, next to each other where they are 16 bits wide, else four and, 1024 further on,
+    // four more: 16 bytes a lane and whole lines a wave (8192 x 8192 f32 with its values: 91 us, and eight together 110).
+    bool apart = t.dtype == DType::f32;
+    for (const auto& x : values) apart |= x.first == 2;
     KernelWriter w(g_, slots_, itype());
     std::vector<Dim> outer(t.dims.begin(), t.dims.end() - 1);
     std::ostringstream body;
     for (int half = 0; half < 2; ++half) {
       // Four elements at a time: a leaf read at `rest + c` is one load for the four, non-temporal when this kernel reads each
       // of its elements once.
-      const std::string at = half ? "(i0 + 4)" : "i0";
-      std::vector<std::string> coords = outer.empty() ? std::vector<std::string>{} : delinearize("(i0 / " + num(K) + ")", outer);
+      const std::string at = !half ? "i0" : apart ? "i1" : "(i0 + 4)";
+      std::vector<std::string> coords =
+          outer.empty() ? std::vector<std::string>{} : delinearize(std::string("(") + (half && apart ? "i1" : "i0") + " / " + num(K) + ")", outer);
       coords.push_back("c");
       std::string hoisted;
       std::map<std::string, std::string> hoisted_var;
@@ -149,18 +178,36 @@ void Planner::mx4_quantize(uint32_t v) {
       const std::string e = w.value(x, coords, sc);
       body << "    {\n      const I c0 = " << (outer.empty() ? at : at + " % " + num(K)) << ";\n"
            << hoisted << "#pragma unroll\n      for (int u = 0; u < 4; ++u) {\n        const I c = c0 + u;\n"
-           << inner.str() << "        x[" << 4 * half << " + u] = " << e << ";\n      }\n    }\n";
+           << inner.str() << "        " << (apart ? "x[" + num(half) + "][u]" : "x[" + num(4 * half) + " + u]") << " = " << e << ";\n      }\n    }\n";
     }
     w.leaf_hook = nullptr;
-    std::string stores;
-    if (codes >= 0) stores += "    *(u32_t*)(" + w.arg(codes, true) + " + i0 / 2) = accy::mx4::encode8(x, scale);\n";
-    if (scales >= 0) stores += "    if (i0 % 32 == 0) " + w.arg(scales, true) + "[i0 / 32] = (u8_t)scale;\n";
-    const std::string nm = name("mx4_quantize", v);
+    // x's codes, scale and values at element i
+    auto store = [&](const std::string& x, const std::string& i) {
+      const std::string v = apart ? "4" : "8";
+      std::string o = "      const u32_t scale = accy::mx4::block_scale(" + x + "), codes = accy::mx4::encode" + v + "(" + x + ", scale);\n";
+      if (codes >= 0) o += "      *(" + std::string(apart ? "u16_t" : "u32_t") + "*)(" + w.arg(codes, true) + " + " + i + " / 2) = codes;\n";
+      if (scales >= 0) o += "      if (" + i + " % 32 == 0) " + w.arg(scales, true) + "[" + i + " / 32] = (u8_t)scale;\n";
+      if (!values.empty()) o += "      accy::mx4::decode" + v + "(codes, scale, " + x + ");\n";
+      for (size_t k = 0; k < values.size(); ++k)
+        o += "      accy::mx4::store" + v + "<" + num(values[k].first) + ">(" + w.arg(value_slots[k], true) + " + " + i + ", " + x + ");\n";
+      return "    {\n" + o + "    }\n";
+    };
+    const std::string nm = name("mx4_quantize", v), n = "(I)" + std::to_string(nel);
+    std::string loop;
+    if (apart) {
+      // whole blocks (eight lanes) pass the end or do not
+      const bool whole = nel % 2048 == 0;
+      loop = "  for (I i0 = (I)blockIdx.x * 2048 + (I)threadIdx.x * 4; i0 < " + n + "; i0 += (I)gridDim.x * 2048) {\n    const I i1 = " +
+             (whole ? "i0 + 1024" : "i0 + 1024 < " + n + " ? i0 + 1024 : i0") + ";\n    float x[2][4];\n" + body.str() + store("x[0]", "i0") +
+             (whole ? "" : "    if (i1 != i0)\n") + store("x[1]", "i1");
+    } else {
+      loop = "  for (I i0 = ((I)blockIdx.x * 256 + (I)threadIdx.x) * 8; i0 < " + n + "; i0 += (I)gridDim.x * 2048) {\n    float x[8];\n" + body.str() +
+             store("x", "i0");
+    }
     std::ostringstream src;
     src << "#include \"mx4\"\n"
         << "extern \"C\" __global__ void __launch_bounds__(256) " << nm << "(" << w.params() << ") {\n  typedef " << w.itype << " I;\n"
-        << w.align_hints() << "  for (I i0 = ((I)blockIdx.x * 256 + (I)threadIdx.x) * 8; i0 < (I)" << nel << "; i0 += (I)gridDim.x * 2048) {\n"
-        << "    float x[8];\n" << body.str() << "    const u32_t scale = accy::mx4::block_scale(x);\n" << stores << "  }\n}\n";
+        << w.align_hints() << loop << "  }\n}\n";
     KernelStep k;
     k.source = src.str();
     k.name = nm;

@@ -197,6 +197,26 @@ def test_codes_and_scales_are_one_kernel_that_evaluates_its_operand():
     assert src.count("__global__") == 1
 
 
+def test_values_of_new_codes_are_stored_by_their_kernel():
+    def source(body):
+        return hip.plan_source(T.define("p", [T.spec("bf16", m=8, k=64), T.spec("f32", m=8, k=64)], body), compile=True)
+
+    def both(b, a):
+        q = a[0].quantize_mx4("k")
+        return [q.codes, q.scales, q.dequantize("bf16"), q.dequantize("f32")]
+    assert source(both).count("__global__") == 1
+
+    def back(b, a):
+        return [a[1].quantize_mx4("k").dequantize("f16")]  # nobody else reads codes and scales
+    src = source(back)
+    assert src.count("__global__") == 1 and "i0 / 2)" not in src and "[i0 / 32]" not in src
+
+    def mixed(b, a):  # codes of one tensor with scales of another are no tensor's own
+        q, r = a[0].quantize_mx4("k"), a[1].quantize_mx4("k")
+        return [b.mx4(q.codes, r.scales, "k").dequantize("bf16"), q.scales, r.codes]
+    assert source(mixed).count("__global__") == 3
+
+
 # ---- quantisation ----
 
 def _roundtrip(shape, dtype):
@@ -272,10 +292,34 @@ def test_index_width():
     """Beyond 2^30 elements an index and a grid's stride no longer fit 32 bits together."""
     def body(b, a):
         m = a[0].quantize_mx4("c")
-        return [m.codes, m.scales, m.dequantize("f16"), a[0].add(a[0])]
+        return [m.codes, m.scales, b.mx4(a[1], a[2], "c").dequantize("f16"), a[0].add(a[0])]
     for rows, index in ((1 << 15, "i32_t"), ((1 << 15) + 1, "i64_t")):
-        source = hip.plan_source(T.define("p", [T.spec("bf16", r=rows, c=1 << 15)], body))
+        source = hip.plan_source(T.define("p", [T.spec("bf16", r=rows, c=1 << 15), *T.mx4_specs("c", r=rows, c=1 << 15)], body))
         assert set(re.findall(r"typedef (i\d\d_t) I;", source)) == {index} and f"values<1, {index}," in source
+
+
+@pytest.mark.gpu
+def test_values_read_back_in_other_types():
+    """Values of new codes in three types, alone and beside the codes; codes of one tensor under another's scales."""
+    rng = np.random.default_rng(23)
+    x, y = floats(rng.standard_normal((7, 96)) * 3, "bf16"), floats(rng.standard_normal((7, 96)), "bf16")
+    x[3, 40] = floats(np.array(np.nan), "bf16")
+    specs = [T.spec("bf16", m=7, k=96)] * 2
+
+    def three(b, a):
+        q = a[0].quantize_mx4("k")
+        return [q.dequantize(t) for t in ("bf16", "f16", "f32")]
+
+    def mixed(b, a):
+        q, r = a[0].quantize_mx4("k"), a[1].quantize_mx4("k")
+        return [q.codes, r.scales, b.mx4(q.codes, r.scales, "k").dequantize("f32"), r.dequantize("f32"), q.scales]
+    want = quantized(wide(x, "bf16"))[2]
+    for got, t in zip(hip_run(T.define("p", specs, three), [x, y]), ("bf16", "f16", "f32")):
+        assert np.array_equal(wide(got, t), want, equal_nan=True)
+    codes, scales, got, back, own = hip_run(T.define("p", specs, mixed), [x, y])
+    assert np.array_equal(got.astype(np.float64), decoded(codes, scales), equal_nan=True)
+    assert np.array_equal(back.astype(np.float64), quantized(wide(y, "bf16"))[2]) and np.array_equal(scales, quantized(wide(y, "bf16"))[1])
+    assert np.array_equal(own, quantized(wide(x, "bf16"))[1])
 
 
 @pytest.mark.gpu
