@@ -330,7 +330,7 @@ bool Planner::gemm_eligible(const Op& op, GemmShape& gs, bool rows) const {
   DType d = op.result.dtype;
   if (d != DType::bf16 && d != DType::f16 && d != DType::f32) return false;
   if (!gemm_shape(op, gs)) return false;
-  if (gs.m == 0 || gs.n == 0 || gs.k == 0) return false;
+  if (gs.m == 0 || gs.n == 0 || gs.k == 0 || gs.batch == 0) return false;
   if (gs.batch > 65535) return false;  // the batch index is gridDim.y, at most 65535 on gfx950
   if (d == DType::f32) {
     bool akc, bkc;

@@ -999,6 +999,14 @@ def test_decoder_steps_on_two_streams_at_once():
             st.destroy()
 
 
+@pytest.mark.parametrize("program", [
+    lambda: W.decoder_step_mx4_program(0, 256, 4, 2, 64, 512, 24, 32, 4), lambda: W.decoder_program(0, 32, 64, 2, 32, 128),
+    lambda: T.define("sums", [T.spec("bf16", m=0, k=64)] * 2, lambda b, a: a[0].mul(a[1]).sum("k"))])
+def test_no_sequences_are_planned(program):
+    """Nothing to compute for a batch of none."""
+    hip.plan_source(program())
+
+
 def test_every_mutated_program_gets_a_status():
     lib, rng = hip.library(), random.Random(1)
     bases = [p.encode() for p in (_step(*STEPS[0])[0], _step(*STEPS[1])[0], _product(1000, 4000, 256, "bf16"), _product(40, 50, 96, "f32"),
@@ -1028,3 +1036,11 @@ def test_decoder_step_tuned_and_profiled():
         _same(outputs(), want)
     bound.free()
     stream.destroy()
+
+
+@pytest.mark.gpu
+def test_decoder_step_of_no_sequences():
+    prog, ins = _step(*STEPS[0])
+    none = W.decoder_step_mx4_program(0, *STEPS[0][1:6], len(ins[CACHE]), *STEPS[0][6:])
+    y, cache = hip_run(none, [x[:0] if i in (0, 16, 17, 18) else x for i, x in enumerate(ins)])
+    assert y.shape == (0, STEPS[0][1]) and np.array_equal(cache, ins[CACHE])
