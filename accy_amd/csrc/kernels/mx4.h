@@ -275,7 +275,8 @@ __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const
 // it. The queries are its B operand, in e4m3 with a scale per block: four bits of them at a time, PARTS times (f32 6, else 3).
 // That is all bits of a query down to 2^-11 of its block's largest in bf16, 2^-8 in f16 and 2^-7 in f32; what lies below is off by
 // 2^-19 (f32 2^-31) of the largest at most. (Two parts for bf16 take 113 us where three take 115 for 48 x 8 heads x 16000 keys, 15.0 and 16.2 for 8 x 16 x 4096, but they
-// lose queries 2^-13 of the largest altogether. K widened to bf16 as V is: 40 of the 241 VALU instructions of a step, which bound it.)
+// lose queries 2^-13 of the largest altogether. K widened to bf16 as V is would add 40 VALU
+// instructions to the 160 of a step, which bound it together with the loads.)
 // Lane l then holds row l % 16 and, g = l / 16, keys 4 g + i and 16 + 4 g + i, which is how the B operand of O^T = V^T P^T
 // (v_mfma_f32_16x16x32_bf16) wants them when its k index 8 g + j means key 4 g + j (j < 4) or 12 + 4 g + j, so P never leaves
 // the lane. V's blocks lie along its dims and not along the keys that are summed, so V is widened to bf16, in which fp4 with its
@@ -323,11 +324,12 @@ __device__ __forceinline__ i32x8 take_e4m3(float (&x)[32]) {
   return w;
 }
 
-// x as bf16 numbers whose sum is x (to 8 bits a part): the next part; x becomes what is left.
-__device__ __forceinline__ __bf16 take_part(float& x) {
-  const __bf16 h = (__bf16)x;
-  x -= (float)h;
-  return h;
+// Two values as bf16 numbers whose sums they are (to 8 bits a part): the next part of both; x becomes what is left.
+__device__ __forceinline__ u32_t take_parts(f32x2& x) {
+  const u32_t w = __builtin_bit_cast(u32_t, __builtin_convertvector(x, bf16x2));
+  x[0] -= __builtin_bit_cast(float, w << 16);
+  x[1] -= __builtin_bit_cast(float, w & 0xffff0000u);
+  return w;
 }
 
 // Nothing is subtracted while a row has seen no key.
@@ -536,14 +538,16 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[d][e][i] *= alpha;
     }
-    bf16x8 pr[PP];
+    u32x4 pr[PP];
     const float base = base_of(m);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j >> 2][j & 3], C::SL, -base));
-      l += p;
+    for (int j = 0; j < 8; j += 2) {
+      f32x2 p = {__builtin_amdgcn_exp2f(__builtin_fmaf(sc[j >> 2][j & 3], C::SL, -base)),
+                 __builtin_amdgcn_exp2f(__builtin_fmaf(sc[(j + 1) >> 2][(j + 1) & 3], C::SL, -base))};
+      l += p[0];
+      l += p[1];
 #pragma unroll
-      for (int e = 0; e < PP; ++e) pr[e][j] = take_part(p);
+      for (int e = 0; e < PP; ++e) pr[e][j >> 1] = take_parts(p);
     }
     // scale bytes of the lane's eight keys: four rows of NB bytes, twice
     u32_t vw[2][NB];
@@ -594,8 +598,8 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
         const f32x4 before[2] = {o[d][0], o[d][1]};
 #pragma unroll
         for (int p = 0; p < PP; ++p) {
-          o[d][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, pr[p], o[d][0], 0, 0, 0);
-          o[d][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, pr[p], o[d][1], 0, 0, 0);
+          o[d][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, __builtin_bit_cast(bf16x8, pr[p]), o[d][0], 0, 0, 0);
+          o[d][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, __builtin_bit_cast(bf16x8, pr[p]), o[d][1], 0, 0, 0);
         }
         if constexpr (TAIL && C::Q > 1) {
           const bool mine = !apart || (row0 + r) / C::G == only;
