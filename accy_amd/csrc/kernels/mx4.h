@@ -274,8 +274,8 @@ __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const
 // v_mfma_scale_f32_16x16x128_f8f6f4, whose A operand is K as it lies: a lane's 16 bytes are a block of one key, its scale beside
 // it. The queries are its B operand, in e4m3 with a scale per block: four bits of them at a time, PARTS times (f32 6, else 3).
 // That is all bits of a query down to 2^-11 of its block's largest in bf16, 2^-8 in f16 and 2^-7 in f32; what lies below is off by
-// 2^-19 (f32 2^-31) of the largest at most. (Two parts for bf16 take 113 us where three take 115 for 48 x 8 heads x 16000 keys, 15.0 and 16.2 for 8 x 16 x 4096, but they
-// lose queries 2^-13 of the largest altogether. K widened to bf16 as V is would add 40 VALU
+// 2^-19 (f32 2^-31) of the largest at most. (Two parts for bf16 take 113 us where three take 115 for 48 x 8 heads x 16000 keys, 15.0
+// and 16.2 for 8 x 16 x 4096, but they lose queries 2^-13 of the largest altogether. K widened to bf16 as V is would add 40 VALU
 // instructions to the 160 of a step, which bound it together with the loads.)
 // Lane l then holds row l % 16 and, g = l / 16, keys 4 g + i and 16 + 4 g + i, which is how the B operand of O^T = V^T P^T
 // (v_mfma_f32_16x16x32_bf16) wants them when its k index 8 g + j means key 4 g + j (j < 4) or 12 + 4 g + j, so P never leaves

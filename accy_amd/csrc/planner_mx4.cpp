@@ -381,7 +381,8 @@ void Planner::mx4_contract(uint32_t v) {
 // Measured (us back to back, 2.4 of them a launch; 128 x 128 / 256 x 256): 512 x 8192 x 2048 8.4 / 17.0, 1024 x 8192 x 2048 16.0 /
 // 19.6, 1536 x 8192 x 2048 21.8 / 21.6, 2048 x 8192 x 2048 28.3 / 24.5, 3000 x 8192 x 2048 42 / 48, 4096 x 4096 x 1024 19.4 /
 // 18.1, 8192^3 377 / 276; 32 x 32 / 128 x 128: 64 x 8192 x 2048 4.6 / 6.5, 500 x 1000 x 2048 5.0 / 7.0, 200 x 1000 x 8192 7.0 / 15.8,
-// 1000 x 1000 x 1024 5.3 / 5.6, 2000 x 1000 x 1024 8.7 / 6.1, 1000 x 4096 x 256 7.9 / 5.7.
+// 1000 x 1000 x 1024 5.3 / 5.6, 2000 x 1000 x 1024 8.7 / 6.1, 1000 x 4096 x 256 7.9 / 5.7; 128 x 128 in one / split along K (with the
+// sum) / 32 x 32: 512 x 2048 x 28672 58 / 33 / 65, 256 x 2048 x 16384 31 / 16.6 / 19.7, 200 x 1000 x 28672 54 / 15.7 / 18.1.
 Planner::Mx4Tile Planner::mx4_tile(int64_t M, int64_t N, int64_t K) const {
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t steps = up(K, 128), groups = up(steps, 4);
