@@ -271,14 +271,14 @@ __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const
 // The Q x G rows that share a key-value head are the columns of 16-wide matrix instructions, 16 rows to a workgroup (two sixteens to
 // a wave, so that the cache is read once for 32 rows, run out of registers: 24 x 8 heads x 8000 keys of 128, 32 rows, bf16, take 94 us
 // where twice the workgroups and reads take 65). Per 32 keys (a step) a wave computes S^T = K Q^T, two tiles of 16 keys, on
-// v_mfma_scale_f32_16x16x128_f8f6f4, whose A operand is K as it lies: a lane's 16 bytes are a block of one key, its scale beside
-// it. The queries are its B operand, in e4m3 with a scale per block: four bits of them at a time, PARTS times (f32 6, else 3).
-// That is all bits of a query down to 2^-11 of its block's largest in bf16, 2^-8 in f16 and 2^-7 in f32; what lies below is off by
-// 2^-19 (f32 2^-31) of the largest at most. (Two parts for bf16 take 113 us where three take 115 for 48 x 8 heads x 16000 keys, 15.0
-// and 16.2 for 8 x 16 x 4096, but they lose queries 2^-13 of the largest altogether. K widened to bf16 as V is would add 40 VALU
-// instructions to the 160 of a step, which bound it together with the loads.)
+// v_mfma_f32_16x16x32_bf16, with K widened to bf16, in which fp4 with its scale is exact, and the queries as QP bf16 numbers whose
+// sum they are, all bits of them (bf16 1, f16 2, f32 3). Lane group g of four holds dims g HD / 4 .. of a key and of a
+// row, so that a lane's codes are adjacent, and of an instruction's eight dims one block's. (The scaled 4-bit instruction takes
+// keys as they lie and saves 32 VALU instructions a step of 128 dims, but queries as three e4m3 numbers on their block's scale
+// lose what lies 2^-20 below its largest, and it is no faster: 48 x 8 x 8 heads x 16000 keys 116 us either way, 8 x 16 x 4096 18.3 against
+// 16.7.)
 // Lane l then holds row l % 16 and, g = l / 16, keys 4 g + i and 16 + 4 g + i, which is how the B operand of O^T = V^T P^T
-// (v_mfma_f32_16x16x32_bf16) wants them when its k index 8 g + j means key 4 g + j (j < 4) or 12 + 4 g + j, so P never leaves
+// (the same instruction) wants them when its k index 8 g + j means key 4 g + j (j < 4) or 12 + 4 g + j, so P never leaves
 // the lane. V's blocks lie along its dims and not along the keys that are summed, so V is widened to bf16, in which fp4 with its
 // scale is exact; its rows are keys while the A operand wants eight keys of one dim: ds_read_b64_tr_b8 hands a lane one byte (two
 // dims) of eight rows. The probabilities are split into PP bf16 numbers, one matrix instruction each: the sums keep f32's
@@ -297,31 +297,13 @@ __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const
 
 #define ACCY_MX4_LDS __attribute__((address_space(3)))
 
-template <int DT> constexpr int query_parts() { return DT == 2 ? 6 : 3; }
+template <int DT> constexpr int query_parts() { return DT + 1; }
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-// 32 values below 256 as e4m3 numbers, four bits of each; x becomes what is left, 16 times over (under a scale four less). The
-// instruction adds a block's products exactly only where they lie close enough together (with eighths up to 256 it does; with all of
-// e4m3, sums were off by 2^-11 of the largest product), so what is below an eighth is left to the next part.
-__device__ __forceinline__ i32x8 take_e4m3(float (&x)[32]) {
-  constexpr float EIGHTHS = 1572864.0f;  // 1.5 2^20: adding and subtracting it rounds to a multiple of 1/8
-  i32x8 w;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float y[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = (x[4 * i + j] + EIGHTHS) - EIGHTHS;
-    int v = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-    v = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], v, true);
-    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(v, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
-    x[4 * i] = (x[4 * i] - a[0]) * 16.0f;
-    x[4 * i + 1] = (x[4 * i + 1] - a[1]) * 16.0f;
-    x[4 * i + 2] = (x[4 * i + 2] - b[0]) * 16.0f;
-    x[4 * i + 3] = (x[4 * i + 3] - b[1]) * 16.0f;
-    w[i] = v;
-  }
-  return w;
+// The upper eight bits of a number's significand, as a bf16 number; x becomes what is left, exactly.
+__device__ __forceinline__ u32_t take_top(float& x) {
+  const u32_t w = __builtin_bit_cast(u32_t, x) & 0xffff0000u;
+  x -= __builtin_bit_cast(float, w);
+  return w >> 16;
 }
 
 // Two values as bf16 numbers whose sums they are (to 8 bits a part): the next part of both; x becomes what is left.
@@ -364,7 +346,8 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
                                        typename Elem<C::DT>::type* __restrict__ out, float* __restrict__ part) {
   typedef Page<C> P;
   typedef Rows<C> RS;
-  constexpr int HD = C::HD, NB = HD / 32, KI = (NB + 3) / 4, PARTS = query_parts<C::DT>(), PP = C::DT == 2 ? 3 : 2;
+  constexpr int HD = C::HD, NB = HD / 32, QP = query_parts<C::DT>(), PP = C::DT == 2 ? 3 : 2;
+  constexpr int W = NB % 4 == 0 ? 4 : NB % 2 == 0 ? 2 : 1;  // eights of a key's dims to a read, all of one block
   constexpr int CODES = 16 * HD, SCALES = 32 * NB;  // bytes of a step's keys, or values, in LDS
   constexpr int DC = 2 * HD / 64, DS = (16 * NB + 63) / 64, PER = DC + DS;  // load instructions of a step
   constexpr int STAGE = 2 * CODES + 256 * DS;
@@ -420,51 +403,33 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   };
   int step = first + wave, p0 = page_of(step), p1 = page_of(step + 4), p2 = page_of(step + 8);
   // The queries are asked for before the steps' loads, which would have to land first otherwise, and worked on after.
-  float x[KI][32];
+  float x[NB][8];
   const int row = row0 + r;
   const long at = ((b * C::Q + row / C::G) * C::H * C::G + h * C::G + row % C::G) * HD;
 #pragma unroll
-  for (int c = 0; c < KI; ++c)
+  for (int t = 0; t < NB; ++t) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int dim = 128 * c + 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-      float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (row < RS::R && dim < HD) load8<C::DT>(Q + at + dim, y);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[c][8 * s + j] = y[j];
-    }
+    for (int j = 0; j < 8; ++j) x[t][j] = 0;
+    if (row < RS::R) load8<C::DT>(Q + at + 8 * (g * NB + t), x[t]);
+  }
   __builtin_amdgcn_sched_barrier(0);
   if (step < end) load(Number<0>(), step, p0);
   if (step + 4 < end) load(Number<1>(), step + 4, p1);
 
-  // Queries: the B operand of S^T, row r, as PARTS e4m3 numbers each, four bits apart. Of 128 dims lane group g holds 16
-  // from 16 g on and 16 from 64 + 16 g on, halves of blocks g / 2 and 2 + g / 2, and the scale of block g. A block's largest
-  // value is scaled to [128, 256): e4m3 goes to 448, and its steps are 2^-9 at the least.
-  i32x8 q[KI][PARTS];
-  u32_t qscale[KI];
+  // Queries: the B operand of S^T, row r, eight dims to an instruction. Infinities become NaN, as their scores do.
+  u32x4 q[NB][QP];
   const int limit = row < RS::R ? len - (C::Q - 1 - row / C::G) : 0;
 #pragma unroll
-  for (int c = 0; c < KI; ++c) {
-    u32_t byte[2];
+  for (int t = 0; t < NB; ++t)
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      u32_t top = 0;
+    for (int j = 0; j < 4; ++j) {
+      float y[2] = {x[t][2 * j] + (x[t][2 * j] - x[t][2 * j]), x[t][2 * j + 1] + (x[t][2 * j + 1] - x[t][2 * j + 1])};
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const u32_t bits = __builtin_bit_cast(u32_t, x[c][16 * half + j]) & 0x7fffffffu;
-        top = top > bits ? top : bits;
+      for (int p = 0; p < QP; ++p) {
+        const u32_t first = take_top(y[0]);
+        q[t][p][j] = first | take_top(y[1]) << 16;
       }
-      const u32_t other = (u32_t)__shfl_xor((int)top, 16, 64), e = (top > other ? top : other) >> 23;
-      // at least 2^-96: values below lose bits, and a scale is left for every part
-      byte[half] = e == 255 ? 255 : e < 38 ? 31 : e - 7;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) x[c][16 * half + j] = e == 255 ? 0.0f : x[c][16 * half + j] * scale_of(254 - byte[half]);
     }
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p) q[c][p] = take_e4m3(x[c]);
-    const int first = __shfl((int)byte[0], r + 32 * (g & 1), 64), second = __shfl((int)byte[1], r + 32 * (g & 1), 64);
-    qscale[c] = (u32_t)(g < 2 ? first : second);
-  }
   f32x4 o[NB][2];
   float m = -__builtin_inff(), l = 0.0f;
 #pragma unroll
@@ -477,15 +442,15 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     asm volatile("" ::: "memory");
   };
 
-  // Where in a stage the lane reads: block 4 c + g of key r (of key 16 + r 8 HD bytes on; past the last block one of the others, which
-  // meets zeros) and its scale; a block's bytes of its value row, which lanes 2 t and 2 t + 1 of sixteen have for their t-th key; the
-  // scales of values 4 g .. (16 on: those of 16 + 4 g).
-  u32_t kat[KI], ksat[KI], vat[NB];
+  // Where in a stage the lane reads: W eights of key r (of key 16 + r 8 HD bytes on) and their block's scale; a block's bytes
+  // of its value row, which lanes 2 t and 2 t + 1 of sixteen have for their t-th key; the scales of values 4 g .. (16 on: those
+  // of 16 + 4 g).
+  u32_t kat[NB / W], ksat[NB / W], vat[NB];
 #pragma unroll
-  for (int c = 0; c < KI; ++c) {
-    const int block = 4 * c + g < NB ? 4 * c + g : (4 * c + g) % NB;
-    kat[c] = wave * STAGE + r * (HD / 2) + 16 * key_chunk<NB>(r, block);
-    ksat[c] = wave * STAGE + 2 * CODES + r * NB + block;
+  for (int c = 0; c < NB / W; ++c) {
+    const int eight = g * NB + c * W;
+    kat[c] = wave * STAGE + r * (HD / 2) + 16 * key_chunk<NB>(r, eight / 4) + eight % 4 * 4;
+    ksat[c] = wave * STAGE + 2 * CODES + r * NB + eight / 4;
   }
   const u32_t vsat = wave * STAGE + 2 * CODES + SCALES + 4 * g * NB;
 #pragma unroll
@@ -494,26 +459,43 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     vat[d] = wave * STAGE + CODES + key * (HD / 2) + 16 * value_chunk<NB>(key, d) + 8 * (r & 1);
   }
 
-  auto compute = [&](auto s, int step, int page, auto tail_) {
+  // sc[u][i]: key 16 u + 4 g + i of the stage against row r.
+  auto scores = [&](auto s, f32x4 (&sc)[2]) {
+    const u8_t* const lds = stage(s);
+    sc[0] = sc[1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < NB / W; ++c) {
+      typedef u32_t codes_t __attribute__((ext_vector_type(W)));
+      codes_t w[2];
+      float scale[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        w[u] = *(const codes_t*)(lds + kat[c] + u * 8 * HD);
+        scale[u] = scale_of(lds[ksat[c] + u * 16 * NB]);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const bf16x2 y[4] = {pair_of_byte<0>(w[u][e], scale[u]), pair_of_byte<1>(w[u][e], scale[u]), pair_of_byte<2>(w[u][e], scale[u]),
+                               pair_of_byte<3>(w[u][e], scale[u])};
+          bf16x8 k;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) k[j] = y[j >> 1][j & 1];
+#pragma unroll
+          for (int p = 0; p < QP; ++p)
+            sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8, q[c * W + e][p]), sc[u], 0, 0, 0);
+        }
+        // a block's widened codes at a time: the registers of more would cost a CU its third workgroup
+        if ((c + 1) * W % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+
+  auto compute = [&](auto s, f32x4 (&sc)[2], int step, int page, auto tail_) {
     constexpr bool TAIL = decltype(tail_)::value != 0;
     const int k0 = step * 32;
     const u8_t* const lds = stage(s);
-    f32x4 sc[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      sc[u] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int c = 0; c < KI; ++c) {
-        const u32x4 w = *(const u32x4*)(lds + kat[c] + u * 8 * HD);
-        const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-        const int scale = lds[ksat[c] + u * 16 * NB];
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-          const int by = qscale[c] == 255 ? 255 : (int)qscale[c] - 4 * p;
-          sc[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[c][p], sc[u], 4, 0, 0, scale, 0, by);
-        }
-      }
-    }
     // The scores' maximum over the lane's keys k0 + 16 u + 4 g + i, those that the row does not see left out.
     float top = -__builtin_inff();
 #pragma unroll
@@ -631,8 +613,10 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
       } else {
         wait(Number<0>());
       }
-      if (now * 32 + 32 <= sure && page >= 0 && page < C::P) compute(s, now, page, Number<0>());
-      else compute(s, now, page, Number<1>());
+      f32x4 sc[2];
+      scores(s, sc);
+      if (now * 32 + 32 <= sure && page >= 0 && page < C::P) compute(s, sc, now, page, Number<0>());
+      else compute(s, sc, now, page, Number<1>());
       __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0): the stage may be overwritten
       asm volatile("" ::: "memory");
     };

@@ -1,0 +1,50 @@
+"""Microscaled 4-bit floats where their values lie far apart and where a kernel's rarer paths run, against float64 (helpers and
+tolerances: test_mx4.py)."""
+import numpy as np
+import pytest
+
+from test_mx4 import _check_attend, cache_parts, finite_cache, floats
+
+
+# ---- attention: queries of any spread ----
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,apart", [("bf16", 13), ("bf16", 17), ("bf16", 20), ("bf16", 60), ("f16", 13), ("f16", 15), ("f32", 24), ("f32", 40)])
+def test_attend_small_queries_beside_large_ones_that_meet_zeros(dtype, apart):
+    """Two dims of each block are 2^apart times the others, and every key is 0 there: the small ones are all of the score."""
+    rng = np.random.default_rng(31)
+    cache = finite_cache(4, 2, 64, 32, rng)
+    cache_parts(cache, 64)[0][..., 0::8] &= 0xf0
+    q = rng.uniform(1, 2, (2, 3, 4, 64)) * rng.choice([-1.0, 1.0], (2, 3, 4, 64))
+    q[..., 0::16] = 2.0 ** apart
+    pages = np.arange(4).reshape(2, 2).astype(np.int32)
+    _check_attend(floats(q, dtype), cache, pages, np.array([64, 40], np.int32), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attend_tiny_queries_and_huge_keys(dtype):
+    """Queries around 2^-105 against keys as much above 1: scores of ordinary size."""
+    rng = np.random.default_rng(32)
+    cache = finite_cache(4, 2, 96, 32, rng)
+    cache_parts(cache, 96)[1][...] += 100
+    q = rng.standard_normal((2, 2, 4, 96)) * 2.0 ** -100
+    pages = np.arange(4).reshape(2, 2).astype(np.int32)
+    _check_attend(floats(q, dtype), cache, pages, np.array([64, 40], np.int32), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("below", [2, 8, 13])
+def test_attend_small_queries_beside_a_large_one_that_all_keys_share(dtype, below):
+    """One dim of each block is 2^below or more times the others; every key is 6 there, so only the small ones tell keys apart."""
+    rng = np.random.default_rng(15)
+    cache = finite_cache(4, 2, 64, 32, rng)
+    kc, ks, vc, vs = cache_parts(cache, 64)
+    kc[...] |= 0x11  # no zeros
+    kc[..., 0::16] = kc[..., 0::16] & 0xf0 | 7
+    ks[...] = 127
+    q = rng.uniform(1, 2, (2, 3, 4, 64)) * 2.0 ** -below
+    q[..., 0::32] = 1.9
+    pages = np.arange(4).reshape(2, 2).astype(np.int32)
+    _check_attend(floats(q * 8, dtype), cache, pages, np.array([64, 40], np.int32), dtype)
