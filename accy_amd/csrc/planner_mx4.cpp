@@ -579,9 +579,11 @@ void Planner::mx4_attend(uint32_t v) {
     const int qs = dense_slot(op.args[0]), cs = dense_slot(op.args[1]), ps = dense_slot(op.args[2]), ls = dense_slot(op.args[3]);
     // Outputs and queries are registers of the whole run, and with several queries the outputs before a step as well: two workgroups of a CU
     // where they leave half of 256, else one, whose kernel may take 512 (24 x 8 heads x 4096 keys, four rows of 192 f16 39 us in two, 47 in one,
-    // five queries of 160 bf16 34 and 44; five of 192 would spill in two).
+    // five queries of 160 bf16 34 and 44; five of 192 would spill in two). Three, whose LDS there is up to 128 dims, where one query's kernel
+    // fits 168 (a row of 128 f16, which takes 169 unasked, 26.9 us in three and 28.7 in two).
     const int64_t groups = (Q * G + 15) / 16, wgs = seqs * H * groups, parts = qt.dtype == DType::f32 ? 3 : qt.dtype == DType::f16 ? 2 : 1;
-    const int bounds = hd / 4 * (Q > 1 ? 2 : 1) + hd / 8 * parts < 120 ? 2 : 1;
+    const int64_t held = hd / 4 * (Q > 1 ? 2 : 1) + hd / 8 * parts;
+    const int bounds = Q == 1 && hd <= 128 && held <= 64 ? 3 : held < 120 ? 2 : 1;
     // Three workgroups share a CU. Fewer sequences and heads than that are split along their keys till half of the chip's places are
     // taken (8 x 16 heads x 4096 keys of 128 bf16: 17.8 us in 2, 16.0 in 4, 16.4 in 6, 17.6 in 8 splits), more of them till
     // uneven lengths even out (48 x 8 x 16000: 144 in 1, 115 in 2, 114 in 4, 117 in 8), each split with four steps of every wave at least.

@@ -3,7 +3,8 @@ tolerances: test_mx4.py)."""
 import numpy as np
 import pytest
 
-from test_mx4 import _check_attend, cache_parts, finite_cache, floats
+from conftest import hip_run
+from test_mx4 import _attend_program, _check_attend, cache_parts, finite_cache, floats, wide
 
 
 # ---- attention: queries of any spread ----
@@ -48,3 +49,18 @@ def test_attend_small_queries_beside_a_large_one_that_all_keys_share(dtype, belo
     q[..., 0::32] = 1.9
     pages = np.arange(4).reshape(2, 2).astype(np.int32)
     _check_attend(floats(q * 8, dtype), cache, pages, np.array([64, 40], np.int32), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("seqs,query,heads,kv,dim,page,slots", [(3, 1, 8, 2, 128, 64, 20), (2, 3, 6, 2, 96, 32, 5), (1, 1, 4, 4, 32, 32, 2), (2, 1, 16, 1, 256, 32, 12)])
+def test_attend_in_16_bits_is_rounded_once(seqs, query, heads, kv, dim, page, slots, dtype):
+    """Scores, probabilities and sums are f32's whatever the type: results are the bits of the f32 ones, rounded."""
+    rng = np.random.default_rng(dim)
+    cache = finite_cache(seqs * slots, kv, dim, page, rng)
+    q = floats(rng.standard_normal((seqs, query, heads, dim)) * 2, dtype)
+    pages = rng.permutation(seqs * slots).reshape(seqs, slots).astype(np.int32)
+    lengths = rng.integers(1, slots * page + 1, seqs).astype(np.int32)
+    full = wide(q, dtype).astype(np.float32)
+    got, want = (hip_run(_attend_program(x, cache, pages, t), [x, cache, pages, lengths])[0] for x, t in ((q, dtype), (full, "f32")))
+    assert np.array_equal(got, floats(want, dtype))
