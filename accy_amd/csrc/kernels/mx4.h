@@ -149,6 +149,33 @@ template <class C> struct Page {
   static __device__ __forceinline__ long scales(bool value, long row) { return 2 * CODES + (value ? SCALES : 0) + row * (C::HD / 32); }
 };
 
+// place[w], the slot of token w of TW or -1, becomes -1 where a later one of `left` tokens has the same: the part of thread tid of 256.
+template <int TW>
+__device__ __forceinline__ void leave_to_later(int* place, const int* __restrict__ slots, int left, int tid) {
+  constexpr int W = TW < 4 ? TW : 4;
+  for (int j0 = 1 + tid; j0 < left; j0 += 2048) {
+    int s[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s[u] = j0 + 256 * u < left ? slots[j0 + 256 * u] : -1;
+    for (int w0 = 0; w0 < TW; w0 += W) {
+      int mine[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) mine[w] = w0 + w < TW ? place[w0 + w] : -1;
+      u32_t lost = 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int w = 0; w < W; ++w) lost |= s[u] == mine[w] && j0 + 256 * u > w0 + w ? 1u << w : 0;
+      if (lost != 0) {
+        // (a token without a slot has nothing to lose, and past TW there is none)
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          if ((lost >> w & 1) && mine[w] >= 0) place[w0 + w] = -1;
+      }
+    }
+  }
+}
+
 // The rows of TOKENS tokens, keys and values [token, head, dim], quantised into their slots: TW tokens per workgroup, eight
 // values of both per thread and step. A slot outside the cache writes nothing, and of two tokens of one slot the later
 // one is kept, so that codes and scales are always one token's. With few tokens every workgroup looks through the slots
@@ -185,28 +212,7 @@ __device__ __forceinline__ void cache_write(u8_t* __restrict__ cache, const type
   }
   __syncthreads();
   if constexpr (!OWNERS) {
-    // token t0 + j against t0 + w, j > w; none has the slot -2
-    constexpr int W = TW < 4 ? TW : 4;
-    for (int j0 = 1 + tid; j0 < C::TOKENS - t0; j0 += 2048) {
-      int s[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) s[u] = j0 + 256 * u < C::TOKENS - t0 ? slots[t0 + j0 + 256 * u] : -2;
-      for (int w0 = 0; w0 < TW; w0 += W) {
-        int mine[W];
-#pragma unroll
-        for (int w = 0; w < W; ++w) mine[w] = w0 + w < TW ? place[w0 + w] : -1;
-        u32_t lost = 0;
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-#pragma unroll
-          for (int w = 0; w < W; ++w) lost |= s[u] == mine[w] && j0 + 256 * u > w0 + w ? 1u << w : 0;
-        if (lost != 0) {
-#pragma unroll
-          for (int w = 0; w < W; ++w)
-            if (lost >> w & 1) place[w0 + w] = -1;
-        }
-      }
-    }
+    leave_to_later<TW>(place, slots + t0, (int)(C::TOKENS - t0), tid);
     __syncthreads();
   }
   for (int i0 = 0; i0 < TW * ROW; i0 += 512) {

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from conftest import hip_run
-from test_mx4 import _attend_program, _check_attend, cache_parts, finite_cache, floats, wide
+from test_mx4 import _attend_program, _check_attend, _write_program, cache_parts, empty_cache, finite_cache, floats, wide, written
 
 
 # ---- attention: queries of any spread ----
@@ -64,3 +64,19 @@ def test_attend_in_16_bits_is_rounded_once(seqs, query, heads, kv, dim, page, sl
     full = wide(q, dtype).astype(np.float32)
     got, want = (hip_run(_attend_program(x, cache, pages, t), [x, cache, pages, lengths])[0] for x, t in ((q, dtype), (full, "f32")))
     assert np.array_equal(got, floats(want, dtype))
+
+
+# ---- the cache ----
+
+# tokens per workgroup of 5, 10, 21, 12 and 1
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,dim,dtype", [(8, 96, "bf16"), (4, 96, "f16"), (2, 96, "f32"), (5, 64, "bf16"), (5, 128, "f32"), (17, 256, "bf16")])
+def test_cache_write_of_a_padded_batch(heads, dim, dtype):
+    """Most tokens are padding, some slots come twice; workgroups whose tokens are no multiple of the four searched at a time."""
+    rng = np.random.default_rng(heads + dim)
+    pages, page, tokens = 3, 32, 333
+    cache = empty_cache(pages, heads, dim, page, rng)
+    keys, values = (floats(rng.standard_normal((tokens, heads, dim)), dtype) for _ in range(2))
+    slots = np.where(rng.random(tokens) < 0.7, -1, rng.integers(0, pages * page, tokens)).astype(np.int32)
+    got = hip_run(_write_program(pages, heads, dim, page, tokens, dtype), [cache, keys, values, slots])[0]
+    assert np.array_equal(got, written(cache, wide(keys, dtype), wide(values, dtype), slots))
