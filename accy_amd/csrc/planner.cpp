@@ -212,10 +212,11 @@ void Planner::map_into(uint32_t v, int slot) {
   if (nel == 0) return;
   View pv;
   if (resolve_view(v, pv) && permute_copy(v, slot, pv)) return;
-  KernelWriter w(g_, slots_, itype());
+  const int64_t inner = t.rank() ? t.dims.back().extent : 1;
+  const bool vectors = t.rank() >= 1 && inner % 4 == 0;
+  KernelWriter w(g_, slots_, itype(vectors ? nel : 0));
   std::ostringstream body;
   const uint32_t B = 256;
-  const int64_t inner = t.rank() ? t.dims.back().extent : 1;
   std::string nm = name("map", v);
   std::ostringstream src;
   // The kernel's parameters are known once its body is written.
@@ -224,7 +225,7 @@ void Planner::map_into(uint32_t v, int slot) {
            ") {\n  typedef " + w.itype + " I;\n";
   };
   KernelStep k;
-  if (t.rank() >= 1 && inner % 4 == 0) {
+  if (vectors) {
     // Four consecutive elements per thread (the innermost extent is a multiple of 4, so they share
     // their outer coordinates): c0 is the innermost coordinate of the first, c = c0 + u. A leaf read
     // at `rest + c` is loaded once for the four as one vector load at the top of the iteration,

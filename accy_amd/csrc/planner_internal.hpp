@@ -71,9 +71,12 @@ inline uint64_t prod(const std::vector<Dim>& dims, size_t b, size_t e) {
   return n;
 }
 
-// 32-bit indices while every element index plus one grid stride (of 2^20 workgroups x 256 threads x the four or eight elements of
-// each, but not beyond the elements rounded up to a workgroup's) stays below 2^31, so that no grid-stride loop's increment overflows.
-inline std::string index_type(uint64_t max_elems) { return max_elems <= (1ull << 30) ? "i32_t" : "i64_t"; }
+// 32-bit indices while every element index plus one grid stride (at most 2^20 workgroups x 256
+// threads = 2^28) stays below 2^31, so that no grid-stride loop's increment overflows. A kernel of four or
+// eight elements a thread has a stride of up to `vectors`, its elements, and takes 32 bits up to 2^30 of them.
+inline std::string index_type(uint64_t max_elems, uint64_t vectors = 0) {
+  return max_elems < (1ull << 31) - (1ull << 28) && vectors <= (1ull << 30) ? "i32_t" : "i64_t";
+}
 
 inline uint32_t grid_for(uint64_t work_items, uint32_t block, uint64_t cap = 1u << 20) {
   uint64_t g = (work_items + block - 1) / block;
@@ -202,7 +205,9 @@ inline std::string serial_fold_step(DType d, Reducer r, const std::string& acc, 
 class Planner {
  public:
   Planner(const Graph& g, const LowerOptions& o) : g_(g), opt_(o), slots_(g, plan_) {
-    for (const Op& op : g.ops) max_elems_ = std::max<uint64_t>(max_elems_, op.result.elements());
+    const std::vector<bool> opaque = opaque_caches();
+    for (size_t v = 0; v < g.ops.size(); ++v)
+      if (!opaque[v]) max_elems_ = std::max<uint64_t>(max_elems_, g.ops[v].result.elements());
   }
 
   Plan run();
@@ -218,8 +223,9 @@ class Planner {
   int counter_ = 0;
   uint64_t max_elems_ = 1;
 
-  // Index arithmetic is 32-bit unless some value of the program has more than 2^30 elements.
-  std::string itype() const { return index_type(max_elems_); }
+  // Index arithmetic is 32-bit unless some value that a generated kernel indexes has about 2^31 elements, or this kernel
+  // takes more than 2^30 by vectors.
+  std::string itype(uint64_t vectors = 0) const { return index_type(max_elems_, vectors); }
 
   void process(uint32_t v);
 
@@ -608,6 +614,8 @@ class Planner {
   // The value whose buffer holds v's elements in v's own order: v itself, or what it is a reshape of.
   uint32_t dense_source(uint32_t v) const;
   int dense_slot(uint32_t v);
+  // Caches that only cache calls (whose own indices are 64 bits wide), scans and outputs take.
+  std::vector<bool> opaque_caches() const;
   // Operands of custom calls that must be in memory are materialised by the kernel that produces them.
   void mark_custom_operands();
 

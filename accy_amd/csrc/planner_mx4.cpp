@@ -80,6 +80,20 @@ uint32_t Planner::dense_source(uint32_t v) const {
 
 int Planner::dense_slot(uint32_t v) { return materialize(dense_source(v)); }
 
+std::vector<bool> Planner::opaque_caches() const {
+  auto call = [](const Op& op, const char* name) { return op.kind == Kind::custom_call && op.bytes == std::string("accy.mx4.") + name; };
+  std::vector<bool> opaque(g_.ops.size());
+  for (size_t v = 0; v < g_.ops.size(); ++v) {
+    const Op& op = g_.ops[v];
+    opaque[v] = op.kind == Kind::parameter || op.kind == Kind::scan || op.kind == Kind::projection || call(op, "cache_write");
+    for (size_t i = 0; i < op.args.size(); ++i) {
+      const bool cache = (i == 0 && (call(op, "cache_write") || call(op, "cache_keys") || call(op, "cache_values"))) || (i == 1 && call(op, "attend"));
+      if (!cache && op.kind != Kind::scan && op.kind != Kind::projection) opaque[op.args[i]] = false;
+    }
+  }
+  return opaque;
+}
+
 void Planner::mark_custom_operands() {
   for (uint32_t v = 0; v < g_.ops.size(); ++v) {
     const Op& op = g_.ops[v];
@@ -146,7 +160,7 @@ void Planner::mx4_quantize(uint32_t v) {
     // four more: 16 bytes a lane and whole lines a wave (8192 x 8192 f32 with its values: 91 us, and eight together 110).
     bool apart = t.dtype == DType::f32;
     for (const auto& x : values) apart |= x.first == 2;
-    KernelWriter w(g_, slots_, itype());
+    KernelWriter w(g_, slots_, itype(nel));
     std::vector<Dim> outer(t.dims.begin(), t.dims.end() - 1);
     std::ostringstream body;
     for (int half = 0; half < 2; ++half) {
@@ -230,11 +244,11 @@ void Planner::mx4_values(uint32_t v) {
   const int out = temp_slot(v);
   if (nel) {
     const int cs = dense_slot(op.args[0]), ss = dense_slot(op.args[1]);
-    KernelWriter w(g_, slots_, itype());
+    KernelWriter w(g_, slots_, itype(nel));
     const std::string a = w.arg(cs, false), b = w.arg(ss, false), o = w.arg(out, true), nm = name("mx4_values", v);
     KernelStep k;
     k.source = "#include \"mx4\"\nextern \"C\" __global__ void __launch_bounds__(256) " + nm + "(" + w.params() + ") {\n  accy::mx4::values<" +
-               num(dt) + ", " + itype() + ", " + std::to_string(nel) + ">(" + a + ", " + b + ", " + o + ");\n}\n";
+               num(dt) + ", " + w.itype + ", " + std::to_string(nel) + ">(" + a + ", " + b + ", " + o + ");\n}\n";
     k.name = nm;
     k.grid[0] = grid_for(nel / 8, 256);
     k.block[0] = 256;

@@ -1,10 +1,15 @@
 """Microscaled 4-bit floats where their values lie far apart and where a kernel's rarer paths run, against float64 (helpers and
 tolerances: test_mx4.py)."""
+import re
+
 import numpy as np
 import pytest
 
+from accy_amd import hip
+from accy_amd import tensor as T
+from accy_amd import workloads as W
 from conftest import hip_run
-from test_mx4 import _attend_program, _check_attend, _write_program, cache_parts, empty_cache, finite_cache, floats, wide, written
+from test_mx4 import _attend_program, _check_attend, _write_program, cache_parts, empty_cache, finite_cache, floats, say, wide, written
 
 
 # ---- attention: queries of any spread ----
@@ -80,3 +85,46 @@ def test_cache_write_of_a_padded_batch(heads, dim, dtype):
     slots = np.where(rng.random(tokens) < 0.7, -1, rng.integers(0, pages * page, tokens)).astype(np.int32)
     got = hip_run(_write_program(pages, heads, dim, page, tokens, dtype), [cache, keys, values, slots])[0]
     assert np.array_equal(got, written(cache, wide(keys, dtype), wide(values, dtype), slots))
+
+
+# ---- 32-bit and 64-bit indices ----
+
+def _index_types(program):
+    return set(re.findall(r"typedef (i\d\d_t) I;", hip.plan_source(program)))
+
+
+def test_a_large_cache_leaves_other_kernels_their_indices():
+    """A cache that only cache calls take is indexed by none of the generated kernels: a step over 1.3 GB of it, and a scan of steps,
+    index their norms and codes in 32 bits; arithmetic on the cache itself does not."""
+    assert _index_types(W.decoder_step_mx4_program(pages=40000)) == {"i32_t"}
+    row = T.spec("bf16", token=4, kv_head=4, dim=128)
+    specs = [T.cache_mx4_spec(80000, 4, 128), row, T.spec("i32", token=4)]
+
+    def step(b, c):
+        cache = c[0].cache_write_mx4(c[1], c[1], c[2])
+        return [cache, c[1].add(cache.cache_keys_mx4(c[2], ("dim", 128), "bf16")), c[2]]
+    assert _index_types(T.define("loop", specs, lambda b, a: (lambda l: [l, b.projection(l, 1).add(a[1])])(b.scan(4, a, step)))) == {"i32_t"}
+    assert _index_types(T.define("sum", specs, lambda b, a: [step(b, a)[1], a[0].add(a[0])])) == {"i64_t"}
+
+
+def test_row_kernels_and_folds_of_more_than_2_to_the_30():
+    """Kernels whose grids stride by rows or single elements take 32 bits up to 1.75 x 2^30 elements."""
+    def body(b, a):
+        return [a[0].max("c"), a[0].max("r")]
+    for rows, index in (((1 << 15) + 32, "i32_t"), (57000, "i32_t"), (57400, "i64_t")):
+        assert _index_types(T.define("p", [T.spec("bf16", r=rows, c=1 << 15)], body)) == {index}
+
+
+@pytest.mark.gpu
+def test_row_kernel_and_fold_more_than_2_to_the_30():
+    """1.8 G values in rows that repeat, indexed in 32 bits: the largest of each row and of each column."""
+    group, cols = 25, 1 << 15
+    groups = 2276  # 1.736 x 2^30
+    row = floats(np.random.default_rng(33).standard_normal((group, cols)), "bf16")
+
+    prog = T.define("p", [T.spec("bf16", r=groups * group, c=cols)], lambda b, a: [a[0].max("c"), a[0].max("r")])
+    assert _index_types(prog) == {"i32_t"}
+    say("rows of 1.8 G")
+    top, columns = hip_run(prog, [np.tile(row, (groups, 1))])
+    want = wide(row, "bf16")
+    assert np.array_equal(wide(top, "bf16"), np.tile(want.max(1), groups)) and np.array_equal(wide(columns, "bf16"), want.max(0))
