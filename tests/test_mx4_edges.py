@@ -9,7 +9,8 @@ from accy_amd import hip
 from accy_amd import tensor as T
 from accy_amd import workloads as W
 from conftest import hip_run
-from test_mx4 import _attend_program, _check_attend, _write_program, cache_parts, empty_cache, finite_cache, floats, say, wide, written
+from test_mx4 import (HALF_STEP, _attend_program, _check_attend, _operands, _product, _write_program, assert_within, cache_parts, decoded,
+                      empty_cache, finite_cache, floats, say, wide, written)
 
 
 # ---- attention: queries of any spread ----
@@ -71,6 +72,29 @@ def test_attend_in_16_bits_is_rounded_once(seqs, query, heads, kv, dim, page, sl
     assert np.array_equal(got, floats(want, dtype))
 
 
+# ---- attention: paths that only some sizes take ----
+
+# head dims whose scales take two load instructions, and others, over more steps than a wave has stages; several queries over splits;
+# more than eight sequences and heads with more than one group of rows, the last set of eight not full
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,query,heads,kv,dim,page,slots,dtype,splits", [
+    (2, 1, 3, 1, 160, 64, 30, "bf16", 3), (1, 1, 2, 1, 224, 32, 50, "f32", 3), (1, 1, 4, 2, 256, 64, 26, "bf16", 3), (2, 1, 2, 2, 96, 32, 60, "f16", 3),
+    (1, 3, 2, 1, 192, 32, 48, "f16", 3), (2, 4, 6, 2, 64, 64, 24, "f16", 3), (1, 5, 8, 2, 128, 32, 40, "f32", 2), (1, 40, 2, 1, 64, 32, 36, "bf16", 2),
+    (3, 5, 16, 4, 64, 32, 6, "bf16", 1), (5, 3, 28, 4, 64, 32, 33, "f32", 2)])
+def test_attend_long_ranges_splits_and_sets(seqs, query, heads, kv, dim, page, slots, dtype, splits):
+    rng = np.random.default_rng(dim + slots)
+    P = seqs * slots + 1
+    cache = finite_cache(P, kv, dim, page, rng)
+    q = floats(rng.standard_normal((seqs, query, heads, dim)) * 2, dtype)
+    pages = rng.permutation(P)[:seqs * slots].reshape(seqs, slots).astype(np.int32)
+    lengths = rng.integers(slots * page // 2, slots * page + 1, seqs).astype(np.int32)
+    lengths[0] = slots * page - 3
+    prog = _attend_program(q, cache, pages, dtype)
+    assert f"SPLITS = {splits};" in hip.plan_source(prog)
+    say(f"attend {seqs} {query} {heads} {kv} {dim} {page} {slots} {dtype}")
+    _check_attend(q, cache, pages, lengths, dtype, hip_run(prog, [q, cache, pages, lengths])[0])
+
+
 # ---- the cache ----
 
 # tokens per workgroup of 5, 10, 21, 12 and 1
@@ -128,3 +152,85 @@ def test_row_kernel_and_fold_more_than_2_to_the_30():
     top, columns = hip_run(prog, [np.tile(row, (groups, 1))])
     want = wide(row, "bf16")
     assert np.array_equal(wide(top, "bf16"), np.tile(want.max(1), groups)) and np.array_equal(wide(columns, "bf16"), want.max(0))
+
+
+# ---- products ----
+
+def _tile(program):
+    """(rows of a tile, waves along K or 0, workgroups along K)."""
+    return tuple(int(x) for x in re.search(r"BM = (\d+), BN = \d+, GROUP_M = \d+, WK = (\d+), SPLITS = (\d+);", hip.plan_source(program)).groups())
+
+
+# K split into 8, 4 and 2: the last share one group of four steps, shorter than the others or not, ending in one to three steps; K in
+# whole steps of 128 and not
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,dtype,splits", [(200, 1000, 18048, "f32", 8), (390, 1000, 24832, "bf16", 4), (257, 1500, 20000, "f16", 4), (513, 2048, 13152, "f32", 2)])
+def test_contract_split_along_k(m, n, k, dtype, splits):
+    prog = _product(m, n, k, dtype)
+    assert _tile(prog) == (128, 0, splits)
+    ops = _operands(m, n, k, m + n + k)
+    say(f"contract {m} {n} {k} {dtype}")
+    got = wide(hip_run(prog, ops)[0], dtype)
+    a, b = decoded(*ops[:2]), decoded(*ops[2:])
+    want, mass = a @ b.T, np.abs(a) @ np.abs(b).T
+    tol = HALF_STEP[dtype] * np.abs(want) + (1 + HALF_STEP[dtype]) * k * 2.0 ** -23 * mass
+    # f16 rounds to infinity from 65520 on (65504 and half of its step of 32)
+    over = np.abs(got) == np.inf
+    assert np.all(np.abs(want)[over] >= (65520.0 if dtype == "f16" else np.inf) - tol[over]) and np.array_equal(np.sign(got[over]), np.sign(want[over]))
+    assert_within(np.where(over, 0, got), np.where(over, 0, want), tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,splits", [(300, 2048, 8192, 4), (257, 1500, 20000, 4), (1100, 4100, 672, 1), (2500, 4100, 1184, 1)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_contract_of_large_tiles_with_a_fused_epilogue(m, n, k, splits, dtype):
+    """A bias, an activation and a residual in the kernel of a split product's sum, and in those of 128 x 128 and 256 x 256 tiles."""
+    rng = np.random.default_rng(3)
+    ops = _operands(m, n, k, 4, 1)
+    bias, res = floats(rng.standard_normal(n), dtype), floats(rng.standard_normal((m, n)) * 4, dtype)
+
+    def tail(b, y, a):
+        return y.add(a[0]).max(b.full_float(T.Type(dtype, ()), 0.0)).add(a[1])
+    rows = [T.spec(dtype, n=n), T.spec(dtype, m=m, n=n)]
+    prog = _product(m, n, k, dtype, tail, rows)
+    bm, wk, s = _tile(prog)
+    assert bm >= 128 and not wk and s == splits
+    say(f"contract {m} {n} {k} {dtype} with an epilogue")
+    y = hip_run(_product(m, n, k, dtype), ops)[0]
+    want = hip_run(T.define("tail", [T.spec(dtype, m=m, n=n)] + rows, lambda b, a: tail(b, a[0], a[1:])), [y, bias, res])[0]
+    got = hip_run(prog, ops + [bias, res])[0]
+    assert np.array_equal(got.view(np.uint8), want.view(np.uint8))
+    assert "map" not in {line.split()[1].split(":")[0] for line in hip.plan_source(prog).splitlines() if line.startswith("// ") and " grid " in line}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,tile", [(1100, 4100, 672, (128, 0, 1)), (1024, 1000, 8320, (128, 0, 1)), (2500, 4100, 1184, (256, 0, 1)), (2100, 4200, 1664, (256, 0, 1)),
+                                        (300, 2048, 8192, (128, 0, 4)), (513, 2048, 13152, (128, 0, 2))])
+def test_contract_of_large_tiles_keeps_nan_blocks_to_their_rows(m, n, k, tile):
+    """NaN scales in the first and the last block of a row, beside rows of scales near both ends of the range."""
+    prog = _product(m, n, k, "f32")
+    assert _tile(prog) == tile
+    ops = _operands(m, n, k, 5)
+    ops[1][0, :], ops[3][0, :] = 20, 230
+    ops[1][m // 2, k // 32 - 1], ops[3][n - 1, 0], ops[3][n // 3, k // 32 - 1] = 255, 255, 255
+    say(f"contract {m} {n} {k} with NaN")
+    got = wide(hip_run(prog, ops)[0], "f32")
+    nan = np.zeros((m, n), bool)
+    nan[m // 2, :], nan[:, n - 1], nan[:, n // 3] = True, True, True
+    assert np.array_equal(np.isnan(got), nan)
+    a, b = (np.nan_to_num(decoded(*ops[i:i + 2])) for i in (0, 2))
+    assert_within(np.where(nan, 0, got), np.where(nan, 0, a @ b.T), k * 2.0 ** -23 * (np.abs(a) @ np.abs(b).T))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,tile", [(5, 40, 64, 16), (33, 65, 128, 32), (130, 300, 256, 32), (1000, 4000, 256, 128), (1000, 4100, 128, 256), (2500, 4100, 256, 256)])
+def test_contract_of_blocks_far_apart(m, n, k, tile):
+    """Scales 2^20 apart within a row, so that an instruction's blocks are up to 2^40 apart. A block's 32 products are multiples of a
+    quarter of its scale below 2^11 of it and so is their sum, exact in f32; a sum over B blocks then errs by an ulp of each of its B additions, and
+    of those of up to 4 waves."""
+    prog = _product(m, n, k, "f32")
+    assert _tile(prog)[0] == tile
+    ops = _operands(m, n, k, 7, 10)
+    a, b = decoded(*ops[:2]), decoded(*ops[2:])
+    tol = (k // 32 + 4) * 2.0 ** -23 * (np.abs(a) @ np.abs(b).T)
+    assert_within(wide(hip_run(prog, ops)[0], "f32"), a @ b.T, tol)
