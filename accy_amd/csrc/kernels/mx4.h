@@ -275,8 +275,8 @@ __device__ __forceinline__ void cache_read(const u8_t* __restrict__ cache, const
 // key is 0. Scores, softmax and sums are f32.
 //
 // The Q x G rows that share a key-value head are the columns of 16-wide matrix instructions, 16 rows to a workgroup (two sixteens to
-// a wave, so that the cache is read once for 32 rows, run out of registers: 24 x 8 heads x 8000 keys of 128, 32 rows, bf16, take 94 us
-// where twice the workgroups and reads take 65). Per 32 keys (a step) a wave computes S^T = K Q^T, two tiles of 16 keys, on
+// a wave, so that the cache is read once for 32 rows, run out of registers: with keys unwidened and probabilities in 17 bits 24 x 8 heads x
+// 8000 keys of 128, 32 rows, bf16, took 94 us so, and 65 in twice the workgroups). Per 32 keys (a step) a wave computes S^T = K Q^T, two tiles of 16 keys, on
 // v_mfma_f32_16x16x32_bf16, with K widened to bf16, in which fp4 with its scale is exact, and the queries as QP bf16 numbers whose
 // sum they are, all bits of them (bf16 1, f16 2, f32 3). Lane group g of four holds dims g HD / 4 .. of a key and of a
 // row, so that a lane's codes are adjacent, and of an instruction's eight dims one block's. (The scaled 4-bit instruction takes
@@ -356,7 +356,8 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   constexpr int CODES = 16 * HD, SCALES = 32 * NB;  // bytes of a step's keys, or values, in LDS
   constexpr int DC = 2 * HD / 64, DS = (16 * NB + 63) / 64, PER = DC + DS;  // load instructions of a step
   constexpr int STAGE = 2 * CODES + 256 * DS;
-  // A cache that one workgroup alone reads streams by with the non-temporal hint (6.0 TB/s of loads alone against 5.2).
+  // A cache that one workgroup alone reads streams by with the non-temporal hint (48 x 8 x 8 heads x 16000 keys of 128 bf16 122 us,
+  // 138 without).
   constexpr int ONCE = RS::GROUPS == 1 ? 2 : 0;
   // One array per stage: the compiler can then tell a stage's reads from the loads still on their way into the others.
   __shared__ __attribute__((aligned(1024))) u8_t l0[4 * STAGE], l1[4 * STAGE], l2[4 * STAGE];
@@ -371,7 +372,7 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     else return l2;
   };
   // A head's groups of rows lie eight workgroups apart, on one XCD: its cache comes through that one's L2 (24 x 8 heads x 8000 keys
-  // of 128, 32 rows: 66.9 us side by side, 64.3 so).
+  // of 128, 32 rows bf16: 70 us side by side, 68 so).
   const int set = blockIdx.x / (8 * RS::GROUPS), in = blockIdx.x % (8 * RS::GROUPS);
   const int wide = C::SEQS * C::H - 8 * set < 8 ? (int)(C::SEQS * C::H - 8 * set) : 8;
   const long bh = 8 * set + in % wide, b = bh / C::H, h = bh % C::H;

@@ -598,9 +598,9 @@ void Planner::mx4_attend(uint32_t v) {
     const int64_t groups = (Q * G + 15) / 16, wgs = seqs * H * groups, parts = qt.dtype == DType::f32 ? 3 : qt.dtype == DType::f16 ? 2 : 1;
     const int64_t held = hd / 4 * (Q > 1 ? 2 : 1) + hd / 8 * parts;
     const int bounds = Q == 1 && hd <= 128 && held <= 64 ? 3 : held < 120 ? 2 : 1;
-    // Three workgroups share a CU. Fewer sequences and heads than that are split along their keys till half of the chip's places are
-    // taken (8 x 16 heads x 4096 keys of 128 bf16: 17.8 us in 2, 16.0 in 4, 16.4 in 6, 17.6 in 8 splits), more of them till
-    // uneven lengths even out (48 x 8 x 16000: 144 in 1, 115 in 2, 114 in 4, 117 in 8), each split with four steps of every wave at least.
+    // Up to three workgroups share a CU. Fewer sequences and heads than 256 are split along their keys till 512 workgroups are at
+    // work (8 x 16 heads x 4096 keys of 128 bf16: 31.5 us in 1, 20.9 in 2, 18.5 in 4, 18.7 in 6 and 8 splits), more of them till
+    // uneven lengths even out (48 x 8 x 16000: 155 in 1, 119 to 125 in 2 to 8), each split with four steps of every wave at least.
     const int64_t steps = (maxp * c.tokens + 31) / 32, want = wgs >= 256 ? 1024 : 512;
     const int64_t splits = opt_.allow_split ? std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, steps / 16, 64})) : 1;
     require(launchable((uint64_t)wgs, 256), op, "more workgroups than a launch takes");

@@ -41,6 +41,56 @@ def test_attend_tiny_queries_and_huge_keys(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attend_huge_queries_and_tiny_keys(dtype):
+    """Keys of the four smallest scales, 2^-127 on, many of them below the smallest normal number."""
+    rng = np.random.default_rng(34)
+    cache = finite_cache(4, 2, 64, 32, rng)
+    ks = cache_parts(cache, 64)[1]
+    ks[...] = rng.integers(0, 4, ks.shape)
+    q = rng.standard_normal((2, 2, 4, 64)) * 2.0 ** 124
+    _check_attend(floats(q, dtype), cache, np.arange(4).reshape(2, 2).astype(np.int32), np.array([64, 40], np.int32), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_attend_of_queries_that_are_no_numbers(dtype):
+    """A NaN or an infinity in a query makes its own outputs NaN, and 0 where it sees no key."""
+    rng = np.random.default_rng(35)
+    cache = finite_cache(6, 2, 64, 32, rng)
+    lengths = np.array([64, 40, 1], np.int32)
+    x = rng.standard_normal((3, 2, 4, 64))
+    f = floats(x, dtype)
+    bad = [(0, 0, 1, 5, np.nan), (0, 1, 2, 63, np.inf), (1, 1, 3, 0, -np.inf), (2, 0, 0, 7, np.nan)]
+    for *at, v in bad:
+        f[tuple(at)] = floats(np.array(v), dtype) if dtype != "bf16" else (0x7fc0 if np.isnan(v) else 0x7f80 if v > 0 else 0xff80)
+    pages = np.arange(6).reshape(3, 2).astype(np.int32)
+    got = wide(hip_run(_attend_program(f, cache, pages, dtype), [f, cache, pages, lengths])[0], dtype)
+    nan = np.isnan(got)
+    for b, i, h in np.ndindex(3, 2, 4):
+        assert nan[b, i, h].all() if (b, i, h) in [(0, 0, 1), (0, 1, 2), (1, 1, 3)] else not nan[b, i, h].any()
+    assert not got[2, 0].any()
+    for *at, v in bad:
+        f[tuple(at)] = 0
+    clean = hip_run(_attend_program(f, cache, pages, dtype), [f, cache, pages, lengths])[0]
+    assert np.array_equal(got[~nan], wide(_check_attend(f, cache, pages, lengths, dtype, clean), dtype)[~nan])
+
+
+@pytest.mark.gpu
+def test_attend_to_one_key_is_its_value():
+    """Of every code under scales at both ends of the range, the smallest values below the smallest normal number."""
+    scales = np.array([0, 1, 2, 3, 100, 127, 251, 252], np.uint8)
+    cache = np.zeros((8, 1, 32 * 34), np.uint8)
+    kc, ks, vc, vs = cache_parts(cache, 32)
+    vc[:, 0, 0] = [0x10, 0x32, 0x54, 0x76, 0x98, 0xba, 0xdc, 0xfe, 0x01, 0x23, 0x45, 0x67, 0x89, 0xab, 0xcd, 0xef]
+    vs[:, 0, 0, 0] = scales
+    ks[...] = 127
+    q = np.ones((8, 1, 1, 32), np.float32)
+    got = hip_run(_attend_program(q, cache, np.zeros((8, 1)), "f32"), [q, cache, np.arange(8, dtype=np.int32)[:, None], np.ones(8, np.int32)])[0]
+    assert np.array_equal(got[:, 0, 0].astype(np.float64), decoded(vc[:, 0, 0], vs[:, 0, 0]))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("below", [2, 8, 13])
 def test_attend_small_queries_beside_a_large_one_that_all_keys_share(dtype, below):
