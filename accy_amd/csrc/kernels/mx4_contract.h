@@ -171,8 +171,8 @@ __device__ __forceinline__ void contract_direct(const u8_t* __restrict__ A, cons
 // the codes as its 16-bit elements (K / 4 of them to a row; a K step of 128 values is 64 bytes of a row, four stages of
 // them), a fragment's 16 bytes one block of the row. A step's 2 x TM x TN matrix instructions take 32 clocks each against
 // (BM + BN) x 64 bytes of LDS written and twice that read, at 128 bytes a clock: with 256 x 256 tiles three quarters of the
-// LDS's rate. At that size random codes are bound by the board's power: registers alone reach 6.2-6.6 PFLOP/s of them (8.3-8.8 of
-// zeros), this kernel 4.0 (5.2 of zeros).
+// LDS's rate. At that size registers alone reach 6.2-6.6 PFLOP/s of random codes and 8.3-8.8 of
+// zeros, this kernel 4.0 and 5.2: the board's power takes a quarter of either, the structure over a third.
 //
 // A row's scales are four bytes to a step. Fetched 16 bytes a row and four steps, straight to registers, they take a line of
 // the row each time (8192^3: 297 us; without any scales 255), so 64 bytes of each row go to LDS at once, for 16 steps, in

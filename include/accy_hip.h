@@ -104,7 +104,8 @@ int accy_hip_invoke(accy_hip_handle h, const void* const* inputs, const size_t* 
  * count that does not match, or an output whose descriptor-sized range overlaps an input or an earlier
  * output (binding.zig:325-336) returns ACCY_HIP_INVALID_BUFFER before anything is launched. One overlap is
  * allowed: an output that is a cache_write (custom call accy.mx4.cache_write) of an input that nothing else in
- * the program reads may be bound to that input's buffer, which is then updated in place. */
+ * the program reads may be bound to that input's buffer, which is then updated in place. A program's
+ * intermediates are the executor's own: calls of one handle, captured or not, may not overlap on different streams. */
 int accy_hip_invoke_device(accy_hip_handle h, const void* const* inputs, size_t n_inputs, void* const* outputs,
                            size_t n_outputs, void* stream);
 
