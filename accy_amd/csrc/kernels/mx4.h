@@ -549,8 +549,8 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
       const int at = (j & 3) * NB + d, by = 23 - 8 * (at & 3);
       return by >= 0 ? vw[j >> 2][at >> 2] << by : vw[j >> 2][at >> 2] >> -by;
     };
-    // A key that only some rows see must not reach the others where it is NaN (0 x NaN): then one query at a time, with
-    // what that query does not see left out. Keys past the end are left out always.
+    // A key that only some rows see must not reach the others where it is NaN (0 x NaN): then one query of the workgroup's rows at
+    // a time, with what that query does not see left out. Keys past the end are left out always.
     bool apart = false;
     if constexpr (TAIL && C::Q > 1) {
       bool nan = false;
@@ -599,8 +599,9 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
       }
     };
     if constexpr (TAIL && C::Q > 1) {
+      const int most = (row0 + 15) / C::G < C::Q ? (row0 + 15) / C::G : C::Q - 1;  // the last query of the workgroup's rows
 #pragma unroll 1
-      for (int only = apart ? 0 : C::Q - 1; only < C::Q; ++only) weigh(only);
+      for (int only = apart ? row0 / C::G : C::Q - 1; only <= (apart ? most : C::Q - 1); ++only) weigh(only);
     } else {
       weigh(C::Q - 1);
     }

@@ -145,6 +145,46 @@ def test_attend_long_ranges_splits_and_sets(seqs, query, heads, kv, dim, page, s
     _check_attend(q, cache, pages, lengths, dtype, hip_run(prog, [q, cache, pages, lengths])[0])
 
 
+@pytest.mark.gpu
+def test_attend_of_a_prompt_with_nan_values():
+    """Each of 2048 queries among 2048 keys, eight of whose values are NaN: the queries from a NaN on are NaN in its block's dims, those
+    before it as without it, and the call takes a few times as long, not as many times as there are queries."""
+    rng = np.random.default_rng(36)
+    n, dim, page = 2048, 64, 64
+    cache = finite_cache(n // page, 1, dim, page, rng)
+    q = floats(rng.standard_normal((1, n, 1, dim)), "bf16")
+    pages, lengths = np.arange(n // page, dtype=np.int32)[None], np.array([n], np.int32)
+    prog = _attend_program(q, cache, pages, "bf16")
+    at = np.sort(rng.choice(n, 8, replace=False))
+    dirty = cache.copy()
+    for j in at:
+        cache_parts(dirty, dim)[3][j // page, 0, j % page, 1] = 255
+    got, took, stream = [], [], hip.Stream()
+    with hip.Hip(prog) as ex:
+        for c in (cache, dirty):
+            bufs = [hip.DeviceBuffer.from_array(x) for x in (q, c, pages, lengths)]
+            out = hip.DeviceBuffer(q.nbytes)
+            times = []
+            for _ in range(3):
+                a, b = hip.Event(), hip.Event()
+                a.record(stream)
+                ex.launch_device([x.ptr for x in bufs], [out.ptr], stream.handle)
+                b.record(stream)
+                stream.synchronize()
+                times.append(a.elapsed_ms(b))
+            got.append(wide(out.download(np.empty_like(q)), "bf16")[0, :, 0])
+            took.append(min(times))
+            for x in bufs + [out]:
+                x.free()
+    stream.destroy()
+    say(f"{took[0]:.3f} ms without, {took[1]:.3f} ms with NaN")
+    nan = np.zeros((n, dim), bool)
+    nan[at[0]:, 32:] = True
+    assert np.array_equal(np.isnan(got[1]), nan) and np.array_equal(got[1][~nan], got[0][~nan])
+    # a workgroup's sixteen queries weigh one after the other in the steps that hold a NaN
+    assert took[1] < 20 * took[0]
+
+
 # ---- the cache ----
 
 # tokens per workgroup of 5, 10, 21, 12 and 1
