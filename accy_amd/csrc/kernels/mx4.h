@@ -549,7 +549,8 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
       const int at = (j & 3) * NB + d, by = 23 - 8 * (at & 3);
       return by >= 0 ? vw[j >> 2][at >> 2] << by : vw[j >> 2][at >> 2] >> -by;
     };
-    // A key that only some rows see must not reach the others where it is NaN (0 x NaN): then one query of the workgroup's rows at
+    // A key that only some rows see must not reach the others where its value is NaN or, with the two scales whose larger codes are
+    // beyond f32, infinite (0 x NaN): then one query of the workgroup's rows at
     // a time, with what that query does not see left out. Keys past the end are left out always.
     bool apart = false;
     if constexpr (TAIL && C::Q > 1) {
@@ -558,7 +559,7 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
       for (int j = 0; j < 8; ++j) {
         const int key = k0 + 4 * g + (j & 3) + (j >> 2) * 16;
 #pragma unroll
-        for (int d = 0; d < NB; ++d) nan |= key >= sure && key < len && vbyte(j, d) == 255;
+        for (int d = 0; d < NB; ++d) nan |= key >= sure && key < len && vbyte(j, d) >= 253;
       }
       apart = __builtin_amdgcn_ballot_w64(nan) != 0;
     }

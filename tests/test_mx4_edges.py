@@ -185,6 +185,26 @@ def test_attend_of_a_prompt_with_nan_values():
     assert took[1] < 20 * took[0]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("byte", [253, 254, 255])
+def test_attend_keeps_values_beyond_f32_to_the_queries_that_see_them(dtype, byte):
+    """The newest value is infinite (6 under the largest scales) or NaN: the last of three queries sees it, the others are as without it."""
+    rng = np.random.default_rng(37)
+    cache = finite_cache(2, 1, 64, 32, rng)
+    q = floats(rng.standard_normal((1, 3, 4, 64)), dtype)
+    pages, lengths = np.array([[1, 0]], np.int32), np.array([50], np.int32)
+    prog = _attend_program(q, cache, pages, dtype)
+    kc, ks, vc, vs = cache_parts(cache, 64)
+    vc[0, 0, 17] = 0x77
+    clean = wide(hip_run(prog, [q, cache, pages, lengths])[0], dtype)
+    vs[0, 0, 17, 0] = byte
+    got = wide(hip_run(prog, [q, cache, pages, lengths])[0], dtype)
+    same = got == clean
+    assert same[0, :2].all() and same[0, 2, :, 32:].all()
+    assert not np.isfinite(got[0, 2, :, :32]).any(), got[0, 2, 0, :4]
+
+
 # ---- the cache ----
 
 # tokens per workgroup of 5, 10, 21, 12 and 1
