@@ -215,7 +215,7 @@ def _inputs(case, seed):
         if seqs > 8:
             of[seqs // 2] = -1  # a sequence without a shared prompt
         q = normal(seqs, case["queries"], case["kv_heads"] * case["group"], case["dim"])
-        return [q, _random_cache(gen, pages, case["kv_heads"], case["dim"]), table.contiguous(), lengths, prefix_table.contiguous(), prefix_lengths, of]
+        return [q, _random_cache(gen, pages, case["kv_heads"], case["dim"]), table.clone(), lengths, prefix_table.clone(), prefix_lengths, of]
     if kind in ("fork", "compact"):
         seqs, slots, pages = case["seqs"], case["slots"], case["pages"]
         held = torch.rand(pages, generator=gen, device="cuda") < 0.02
