@@ -225,7 +225,7 @@ def _inputs(case, seed):
         table = torch.full((seqs, slots), -1, dtype=torch.int32, device="cuda")
         mine = torch.arange(seqs * each, device="cuda").view(seqs, each) % pages
         table[:, :each] = order[mine]
-        table[:, :each // 2] = table[0, :each // 2]
+        table[:, :each // 2] = table[0, :each // 2].clone()
         lengths = whole(each * PAGE // 2, each * PAGE + 1, seqs)
         if kind == "compact":
             return [table, held, _random_cache(gen, pages, case["kv_heads"], case["dim"])]
