@@ -25,12 +25,14 @@ ORACLE_LIB = ROOT / "oracle" / "build" / "liboracle.so"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
 HOST_SOURCES = ["ir.cpp", "wire.cpp", "lower.cpp", "planner.cpp", "planner_reduce.cpp", "planner_views.cpp",
-                "planner_contraction.cpp", "planner_attention.cpp", "planner_mx4.cpp", "runtime.cpp", "tuning.cpp", "tune.cpp", "capi.cpp"]
+                "planner_contraction.cpp", "planner_attention.cpp", "planner_custom.cpp", "planner_mx4.cpp",
+                "planner_heads.cpp", "planner_pages.cpp", "planner_logits.cpp", "runtime.cpp", "tuning.cpp", "tune.cpp", "capi.cpp"]
 # Device sources embedded as text: (C++ symbol, file under csrc/kernels).
 EMBEDDED = [("kCommonDeviceSource", "common.h"), ("kGemmDeviceSource", "gemm.h"),
             ("kAttentionDeviceSource", "attention.h"), ("kScatterDeviceSource", "scatter.h"),
             ("kDecodeDeviceSource", "decode.h"), ("kMx4DeviceSource", "mx4.h"),
-            ("kMx4ContractDeviceSource", "mx4_contract.h")]
+            ("kMx4ContractDeviceSource", "mx4_contract.h"), ("kHeadsDeviceSource", "heads.h"),
+            ("kPagesDeviceSource", "pages.h"), ("kLogitsDeviceSource", "logits.h")]
 # Packed-f32 instructions stay off in every device build; loops marked `#pragma unroll` unroll
 # whatever their size (as for the kernels compiled at run time).
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-mllvm", "-pragma-unroll-threshold=65536"]

@@ -345,22 +345,89 @@ template <int I> __device__ __forceinline__ bf16x2 pair_of_byte(u32_t w, float s
 
 template <int N> struct Number { static constexpr int value = N; };
 
-template <class C>
-__device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restrict__ Q, const u8_t* __restrict__ cache,
-                                       const int* __restrict__ pages, const int* __restrict__ lengths,
-                                       typename Elem<C::DT>::type* __restrict__ out, float* __restrict__ part) {
+// Shared keys: C::PREFIXES, PSPLITS (workgroups along a prefix), PREFIX_MAXP (pages of one); without them 0. The rows of a prefix are those of
+// its sequences, one sequence after the other, sixteen to a workgroup: at most so many groups.
+template <class C, class = void> struct Shared {
+  static constexpr int N = 0, SPLITS = 0, MAXP = 0;
+};
+template <class C> struct Shared<C, decltype((void)C::PREFIXES)> {
+  static constexpr int N = C::PREFIXES, SPLITS = C::PSPLITS, MAXP = C::PREFIX_MAXP;
+};
+template <class C> constexpr int PREFIXES = Shared<C>::N;
+template <class C> constexpr int PSPLITS = Shared<C>::SPLITS;
+template <class C> constexpr int PREFIX_PAGES = Shared<C>::MAXP;
+template <class C> constexpr int PREFIX_GROUPS = (int)(C::SEQS * Rows<C>::R / 16) + Shared<C>::N;
+
+// The prefix that group `group` of the prefixes' rows belongs to (-1: there is no such group), the group's first row of the prefix's, and how
+// many those are. The sequences of the group's rows go to `list`, in order. All threads; `list` has room for 16 and the counts.
+struct Members {
+  int prefix, row0, rows;
+};
+template <class C> __device__ __forceinline__ Members members_of(const int* __restrict__ of, int group, int* list) {
+  constexpr int R = Rows<C>::R, N = PREFIXES<C>;
+  int* const count = list + 16;
+  int* const waves = count + N;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < N; i += 256) count[i] = 0;
+  __syncthreads();
+  for (long s = tid; s < C::SEQS; s += 256) {
+    const int p = of[s];
+    if (p >= 0 && p < N) atomicAdd(&count[p], 1);
+  }
+  __syncthreads();
+  Members m = {-1, 0, 0};
+  for (int p = 0; p < N; ++p) {
+    const int groups = (count[p] * R + 15) / 16;
+    if (group < groups) {
+      m = {p, group * 16, count[p] * R};
+      break;
+    }
+    group -= groups;
+  }
+  if (m.prefix < 0) return m;
+  // its sequences number first .. last in order
+  const int first = m.row0 / R, last = (m.row0 + 15) / R;
+  int before = 0;
+  for (long s0 = 0; s0 < C::SEQS && before <= last; s0 += 256) {
+    const bool mine = s0 + tid < C::SEQS && of[s0 + tid] == m.prefix;
+    const u64_t ballot = __builtin_amdgcn_ballot_w64(mine);
+    if (lane == 0) waves[wave] = __builtin_popcountll(ballot);
+    __syncthreads();
+    int k = before + __builtin_popcountll(ballot & ((1ull << lane) - 1));
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) k += waves[w];
+      before += waves[w];
+    }
+    if (mine && k >= first && k <= last) list[k - first] = (int)(s0 + tid);
+    __syncthreads();
+  }
+  return m;
+}
+
+// What a workgroup's keys are: all of its sequence's, or with shared keys its sequence's own or those of a prefix.
+enum Keys { ALL, OWN, PREFIX };
+
+// What the stages of a workgroup's loads take, and the numbers that follow from C.
+template <class C> struct Stages {
+  static constexpr int NB = C::HD / 32, CODES = 16 * C::HD, SCALES = 32 * NB;  // bytes of a step's keys, or values, in LDS
+  static constexpr int DC = 2 * C::HD / 64, DS = (16 * NB + 63) / 64, PER = DC + DS;  // load instructions of a step
+  static constexpr int STAGE = 2 * CODES + 256 * DS;
+};
+
+template <class C, Keys KEYS>
+__device__ __forceinline__ void attend_keys(const typename Elem<C::DT>::type* __restrict__ Q, const u8_t* __restrict__ cache,
+                                            const int* __restrict__ pages, const int* __restrict__ lengths, const int* __restrict__ of,
+                                            typename Elem<C::DT>::type* __restrict__ out, float* __restrict__ part, const int block, const int split,
+                                            u8_t (&l0)[4 * Stages<C>::STAGE], u8_t (&l1)[4 * Stages<C>::STAGE], u8_t (&l2)[4 * Stages<C>::STAGE]) {
   typedef Page<C> P;
   typedef Rows<C> RS;
-  constexpr int HD = C::HD, NB = HD / 32, QP = C::DT + 1, PP = 3;
+  typedef Stages<C> ST;
+  constexpr int HD = C::HD, NB = ST::NB, QP = C::DT + 1, PP = 3;
   constexpr int W = NB % 4 == 0 ? 4 : NB % 2 == 0 ? 2 : 1;  // eights of a key's dims to a read, all of one block
-  constexpr int CODES = 16 * HD, SCALES = 32 * NB;  // bytes of a step's keys, or values, in LDS
-  constexpr int DC = 2 * HD / 64, DS = (16 * NB + 63) / 64, PER = DC + DS;  // load instructions of a step
-  constexpr int STAGE = 2 * CODES + 256 * DS;
+  constexpr int CODES = ST::CODES, SCALES = ST::SCALES, DC = ST::DC, DS = ST::DS, PER = ST::PER, STAGE = ST::STAGE;
   // A cache that one workgroup alone reads streams by with the non-temporal hint (48 x 8 x 8 heads x 16000 keys of 128 bf16 122 us,
   // 138 without).
-  constexpr int ONCE = RS::GROUPS == 1 ? 2 : 0;
-  // One array per stage: the compiler can then tell a stage's reads from the loads still on their way into the others.
-  __shared__ __attribute__((aligned(1024))) u8_t l0[4 * STAGE], l1[4 * STAGE], l2[4 * STAGE];
+  constexpr int ONCE = KEYS != PREFIX && RS::GROUPS == 1 ? 2 : 0;
   // where the waves meet, once the steps are done (every load has landed by then): two waves' rows to a stage
   constexpr int JOIN = 16 * (HD + 4);
   static_assert(2 * JOIN * 4 <= 4 * STAGE, "a stage of the four waves holds two waves' rows");
@@ -373,16 +440,31 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   };
   // A head's groups of rows lie eight workgroups apart, on one XCD: its cache comes through that one's L2 (24 x 8 heads x 8000 keys
   // of 128, 32 rows bf16: 70 us side by side, 68 so).
-  const int set = blockIdx.x / (8 * RS::GROUPS), in = blockIdx.x % (8 * RS::GROUPS);
-  const int wide = C::SEQS * C::H - 8 * set < 8 ? (int)(C::SEQS * C::H - 8 * set) : 8;
-  const long bh = 8 * set + in % wide, b = bh / C::H, h = bh % C::H;
-  const int row0 = in / wide * 16;
+  constexpr int SETS = KEYS == PREFIX ? C::H * PSPLITS<C> : (int)(C::SEQS * C::H), GROUPS = KEYS == PREFIX ? PREFIX_GROUPS<C> : RS::GROUPS;
+  const int set = block / (8 * GROUPS), in = block % (8 * GROUPS);
+  const int wide = SETS - 8 * set < 8 ? SETS - 8 * set : 8;
+  // b: the sequence or the prefix; row0: the first of the workgroup's rows among those of its head and sequence or prefix, `rows` in all.
+  long bh = 8 * set + in % wide, b = bh / C::H, h = bh % C::H;
+  int row0 = in / wide * 16, rows = RS::R, share = split;
+  int member = 0;
+  if constexpr (KEYS == PREFIX) {
+    h = bh % C::H;
+    share = (int)(bh / C::H);
+    const Members m = members_of<C>(of, in / wide, (int*)l0);
+    if (m.prefix < 0) return;  // (there are fewer groups than there could be)
+    b = m.prefix;
+    row0 = m.row0;
+    rows = m.rows;
+    member = row0 + (lane & 15) < rows ? ((const int*)l0)[(row0 + (lane & 15)) / RS::R - row0 / RS::R] : 0;
+    __syncthreads();  // the list's place is a stage's
+  }
+  constexpr int MAXP = KEYS == PREFIX ? PREFIX_PAGES<C> : C::MAXP, SHARES = KEYS == PREFIX ? PSPLITS<C> : C::SPLITS;
   int len = C::P > 0 ? lengths[b] : 0;
-  len = len < 0 ? 0 : len > C::MAXP * C::T ? C::MAXP * C::T : len;
+  len = len < 0 ? 0 : len > MAXP * C::T ? MAXP * C::T : len;
   len = __builtin_amdgcn_readfirstlane(len);
-  const int steps = (len + 31) / 32, per = (steps + C::SPLITS - 1) / C::SPLITS;
-  const int first = (int)blockIdx.y * per, end = first + per < steps ? first + per : steps;
-  const int sure = len - (C::Q - 1);  // keys below it are seen by every row
+  const int steps = (len + 31) / 32, per = (steps + SHARES - 1) / SHARES;
+  const int first = share * per, end = first + per < steps ? first + per : steps;
+  const int sure = KEYS == PREFIX ? len : len - (C::Q - 1);  // keys below it are seen by every row
 
   // Loads: chunk x = 64 i + lane of a step's LDS, keys and then values; then the scales, a word a lane.
   u32_t from[DC], sfrom[DS];
@@ -396,7 +478,7 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     const int x = 64 * i + lane < 16 * NB ? 64 * i + lane : 16 * NB - 1, value = x >= 8 * NB;
     sfrom[i] = (u32_t)(2 * P::CODES) + (value ? (u32_t)P::SCALES + 4 * (x - 8 * NB) : 4 * x);
   }
-  auto page_of = [&](int step) { return step < end ? __builtin_amdgcn_readfirstlane(pages[b * C::MAXP + step * 32 / C::T]) : 0; };
+  auto page_of = [&](int step) { return step < end ? __builtin_amdgcn_readfirstlane(pages[b * MAXP + step * 32 / C::T]) : 0; };
   auto load = [&](auto s, int step, int page) {
     const int in = step * 32 % C::T;
     const u8_t* const head = P::head(cache, page >= 0 && page < C::P ? page : 0, h);
@@ -410,13 +492,15 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   int step = first + wave, p0 = page_of(step), p1 = page_of(step + 4), p2 = page_of(step + 8);
   // The queries are asked for before the steps' loads, which would have to land first otherwise, and worked on after.
   float x[NB][8];
-  const int row = row0 + r;
-  const long at = ((b * C::Q + row / C::G) * C::H * C::G + h * C::G + row % C::G) * HD;
+  // (a row of a prefix is one of its sequences' rows, one sequence after the other)
+  const int row = row0 + r, inner = KEYS == PREFIX ? row % RS::R : row;
+  const long seq = KEYS == PREFIX ? (long)member : b;
+  const long at = ((seq * C::Q + inner / C::G) * C::H * C::G + h * C::G + inner % C::G) * HD;
 #pragma unroll
   for (int t = 0; t < NB; ++t) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[t][j] = 0;
-    if (row < RS::R) load8<C::DT>(Q + at + 8 * (g * NB + t), x[t]);
+    if (row < rows) load8<C::DT>(Q + at + 8 * (g * NB + t), x[t]);
   }
   __builtin_amdgcn_sched_barrier(0);
   if (step < end) load(Number<0>(), step, p0);
@@ -424,7 +508,7 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
 
   // Queries: the B operand of S^T, row r, eight dims to an instruction. Infinities become NaN, as their scores do.
   u32x4 q[NB][QP];
-  const int limit = row < RS::R ? len - (C::Q - 1 - row / C::G) : 0;
+  const int limit = row < rows ? len - (KEYS == PREFIX ? 0 : C::Q - 1 - row / C::G) : 0;
 #pragma unroll
   for (int t = 0; t < NB; ++t)
 #pragma unroll
@@ -553,7 +637,7 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
     // beyond f32, infinite (0 x NaN): then one query of the workgroup's rows at
     // a time, with what that query does not see left out. Keys past the end are left out always.
     bool apart = false;
-    if constexpr (TAIL && C::Q > 1) {
+    if constexpr (TAIL && C::Q > 1 && KEYS != PREFIX) {
       bool nan = false;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -590,7 +674,7 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
           o[d][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, __builtin_bit_cast(bf16x8, pr[p]), o[d][0], 0, 0, 0);
           o[d][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, __builtin_bit_cast(bf16x8, pr[p]), o[d][1], 0, 0, 0);
         }
-        if constexpr (TAIL && C::Q > 1) {
+        if constexpr (TAIL && C::Q > 1 && KEYS != PREFIX) {
           const bool mine = !apart || (row0 + r) / C::G == only;
 #pragma unroll
           for (int e = 0; e < 2; ++e)
@@ -599,7 +683,7 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
         }
       }
     };
-    if constexpr (TAIL && C::Q > 1) {
+    if constexpr (TAIL && C::Q > 1 && KEYS != PREFIX) {
       const int most = (row0 + 15) / C::G < C::Q ? (row0 + 15) / C::G : C::Q - 1;  // the last query of the workgroup's rows
 #pragma unroll 1
       for (int only = apart ? row0 / C::G : C::Q - 1; only <= (apart ? most : C::Q - 1); ++only) weigh(only);
@@ -651,11 +735,12 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   if (g == 0) {
     p[HD] = m;
     p[HD + 1] = l;
+    if (KEYS == PREFIX && wave == 0) p[HD + 2] = __builtin_bit_cast(float, member);
   }
   __syncthreads();
   for (int at = tid; at < 16 * HD / 4; at += 256) {
     const int rr = at / (HD / 4), d = at % (HD / 4) * 4, row = row0 + rr;
-    if (row >= RS::R) continue;
+    if (row >= rows) continue;
     const int from = rr * (HD + 4);
     float top = joined(0)[from + HD], sum = 0.0f;
 #pragma unroll
@@ -671,13 +756,16 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] += y[i] * scale;
     }
-    if constexpr (C::SPLITS == 1) {
+    if constexpr (KEYS == ALL && C::SPLITS == 1) {
       const long to = ((b * C::Q + row / C::G) * C::H * C::G + h * C::G + row % C::G) * HD + d;
       const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
       for (int i = 0; i < 4; ++i) out[to + i] = to_elem<C::DT>(v[i] * by);
     } else {
-      float* const to = part + ((bh * RS::R + row) * C::SPLITS + blockIdx.y) * (HD + 4);
+      // a row's parts: those of its prefix, then those of its own keys
+      constexpr int PARTS = KEYS == ALL ? C::SPLITS : C::SPLITS + PSPLITS<C>;
+      const long whose = KEYS == PREFIX ? ((long)__builtin_bit_cast(int, joined(0)[from + HD + 2]) * C::H + h) * RS::R + row % RS::R : bh * RS::R + row;
+      float* const to = part + (whose * PARTS + (KEYS == OWN ? PSPLITS<C> : 0) + share) * (HD + 4);
       *(f32x4*)(to + d) = v;
       if (d == 0) {
         to[HD] = top;
@@ -687,20 +775,49 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
   }
 }
 
-// The rows' outputs from their splits' parts, in split order; one thread per output.
 template <class C>
-__device__ __forceinline__ void attend_join(const float* __restrict__ part, typename Elem<C::DT>::type* __restrict__ out) {
+__device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restrict__ Q, const u8_t* __restrict__ cache,
+                                       const int* __restrict__ pages, const int* __restrict__ lengths,
+                                       typename Elem<C::DT>::type* __restrict__ out, float* __restrict__ part) {
+  // One array per stage: the compiler can then tell a stage's reads from the loads still on their way into the others.
+  __shared__ __attribute__((aligned(1024))) u8_t l0[4 * Stages<C>::STAGE], l1[4 * Stages<C>::STAGE], l2[4 * Stages<C>::STAGE];
+  attend_keys<C, ALL>(Q, cache, pages, lengths, nullptr, out, part, (int)blockIdx.x, (int)blockIdx.y, l0, l1, l2);
+}
+
+// With keys that sequences share: the first workgroups take the prefixes, the rows of all of a prefix's sequences together, the others
+// each sequence's own keys. Every row's parts are joined by the next kernel.
+template <class C>
+__device__ __forceinline__ void attend_shared(const typename Elem<C::DT>::type* __restrict__ Q, const u8_t* __restrict__ cache,
+                                              const int* __restrict__ pages, const int* __restrict__ lengths, const int* __restrict__ prefix_pages,
+                                              const int* __restrict__ prefix_lengths, const int* __restrict__ of, float* __restrict__ part) {
+  __shared__ __attribute__((aligned(1024))) u8_t l0[4 * Stages<C>::STAGE], l1[4 * Stages<C>::STAGE], l2[4 * Stages<C>::STAGE];
+  constexpr int FIRST = PREFIX_GROUPS<C> * C::H * PSPLITS<C>, EACH = (int)(C::SEQS * C::H * Rows<C>::GROUPS);
+  const int block = (int)blockIdx.x - FIRST;
+  if (block < 0) attend_keys<C, PREFIX>(Q, cache, prefix_pages, prefix_lengths, of, nullptr, part, (int)blockIdx.x, 0, l0, l1, l2);
+  else attend_keys<C, OWN>(Q, cache, pages, lengths, of, nullptr, part, block % EACH, block / EACH, l0, l1, l2);
+}
+
+// The rows' outputs from their splits' parts, in split order; one thread per output. `of`: with shared keys, whose parts come first and
+// are not there for a sequence without a prefix.
+template <class C>
+__device__ __forceinline__ void attend_join(const float* __restrict__ part, typename Elem<C::DT>::type* __restrict__ out, const int* __restrict__ of = nullptr) {
   constexpr long R = Rows<C>::R, N = (long)C::SEQS * C::H * R * C::HD;
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= N) return;
   const long bhr = i / C::HD, d = i % C::HD, row = bhr % R, bh = bhr / R;
-  const float* const p = part + bhr * C::SPLITS * (C::HD + 4);
+  constexpr int PARTS = C::SPLITS + PSPLITS<C>;
+  const float* const p = part + bhr * PARTS * (C::HD + 4);
   float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
+  int from = 0;
+  if constexpr (PSPLITS<C> > 0) {
+    const int x = of[bh / C::H];
+    if (x < 0 || x >= PREFIXES<C>) from = PSPLITS<C>;
+  }
 #pragma unroll 8
-  for (int s = 0; s < C::SPLITS; ++s) m = fmaxf(m, p[s * (C::HD + 4) + C::HD]);
+  for (int s = from; s < PARTS; ++s) m = fmaxf(m, p[s * (C::HD + 4) + C::HD]);
   const float base = base_of(m);
 #pragma unroll 8
-  for (int s = 0; s < C::SPLITS; ++s) {
+  for (int s = from; s < PARTS; ++s) {
     const float* const x = p + s * (C::HD + 4);
     const float scale = __builtin_amdgcn_exp2f(x[C::HD] - base);
     l += x[C::HD + 1] * scale;

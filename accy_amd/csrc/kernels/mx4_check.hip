@@ -48,3 +48,13 @@ extern "C" __global__ void __launch_bounds__(256) check_mx4_attend_f32(const flo
 extern "C" __global__ void __launch_bounds__(256) check_mx4_join(const float* part, u16_t* o) {
   accy::mx4::attend_join<CheckCache<0, 128, 1, 8, 4>>(part, o);
 }
+struct CheckShared : CheckCache<0, 128, 2, 4, 2> {
+  static constexpr int PREFIXES = 3, PSPLITS = 4, PREFIX_MAXP = 128;
+};
+extern "C" __global__ void __launch_bounds__(256) check_mx4_attend_shared(const u16_t* q, const u8_t* c, const int* p, const int* l, const int* sp, const int* sl,
+                                                                          const int* of, float* part) {
+  accy::mx4::attend_shared<CheckShared>(q, c, p, l, sp, sl, of, part);
+}
+extern "C" __global__ void __launch_bounds__(256) check_mx4_join_shared(const float* part, u16_t* o, const int* of) {
+  accy::mx4::attend_join<CheckShared>(part, o, of);
+}

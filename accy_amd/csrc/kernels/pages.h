@@ -1,0 +1,418 @@
+// Page tables of a cache, and copies of its pages.
+//
+// fork and compact are counting: which pages are in use is a bitmap (a bit a page), the k-th free page the k-th bit that is clear, found by
+// the words' running counts. One workgroup of 1024 threads does either in a few passes over the tables, the bitmaps in LDS (beyond
+// LDS_PAGES pages in memory), so that a call is one launch; what bounds it is the way to memory and back of each pass and what one
+// CU reads and writes, the tables. No order of atomics shows: bits are set, and ties go to the lowest row or page.
+//
+// copies are bound by HBM. Source and target pages of fork and compact differ from each other and are all different, so that their
+// copies need no check (C::CHECK false); of other lists the last copy to a page counts, and in place a page that is the source of one
+// copy and the target of another is kept aside first.
+#pragma once
+
+namespace accy {
+namespace pages {
+
+constexpr int THREADS = 1024, WAVES = THREADS / 64;
+constexpr long LDS_PAGES = 1 << 17;
+
+// ---- bitmaps: in LDS, or in memory, where other threads' bits come from the coherent level ----
+template <bool LDS> __device__ __forceinline__ u32_t word(const u32_t* map, long w) {
+  if constexpr (LDS) return map[w];
+  else return __hip_atomic_load(map + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <bool LDS> __device__ __forceinline__ void put_word(u32_t* map, long w, u32_t v) {
+  if constexpr (LDS) map[w] = v;
+  else __hip_atomic_store(map + w, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <bool LDS> __device__ __forceinline__ bool bit(const u32_t* map, long p) { return word<LDS>(map, p >> 5) >> (p & 31) & 1; }
+// A barrier after which the other threads' stores and bits are seen, in LDS or in memory.
+template <bool LDS> __device__ __forceinline__ void meet() {
+  if constexpr (!LDS) __threadfence();
+  __syncthreads();
+}
+__device__ __forceinline__ void set_bit(u32_t* map, long p) { atomicOr(map + (p >> 5), 1u << (p & 31)); }
+
+// The running sum of the threads' values before this one's; total: of all. `lds` holds WAVES + 1 elements.
+__device__ __forceinline__ int before_me(int v, int* lds, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int sum = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int below = __shfl_up(sum, o, 64);
+    if (lane >= o) sum += below;
+  }
+  __syncthreads();
+  if (lane == 63) lds[wave] = sum;
+  __syncthreads();
+  int start = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const int n = lds[w];
+    if (w < wave) start += n;
+    total += n;
+  }
+  return start + sum - v;
+}
+
+// The words of a bitmap as each thread's share of them, in order.
+__device__ __forceinline__ void my_words(long words, long& from, long& to) {
+  const long per = (words + THREADS - 1) / THREADS;
+  from = (long)threadIdx.x * per < words ? threadIdx.x * per : words;
+  to = from + per < words ? from + per : words;
+}
+
+// The position of the k-th bit that is set in w (it has more than k).
+__device__ __forceinline__ int nth_bit(u32_t w, int k) {
+  int at = 0;
+#pragma unroll
+  for (int half = 16; half > 0; half >>= 1) {
+    const int below = __builtin_popcount(w & ((1u << half) - 1));
+    if (k >= below) {
+      k -= below;
+      w >>= half;
+      at += half;
+    }
+  }
+  return at;
+}
+
+// Pages held as the first word of a bitmap: bytes of `held` that are not 0. Bits past the last page are set: no page either.
+template <long P> __device__ __forceinline__ u32_t held_word(const u8_t* __restrict__ held, long w) {
+  u32_t bits = 0;
+  if (w * 32 + 32 <= P) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const u32_t four = *(const u32_t*)(held + w * 32 + 4 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bits |= (four >> (8 * j) & 255u) ? 1u << (4 * i + j) : 0u;
+    }
+  } else {
+    for (int i = 0; i < 32; ++i) bits |= w * 32 + i >= P || held[w * 32 + i] ? 1u << i : 0u;
+  }
+  return bits;
+}
+
+// ---------------------------------------------------------------------------------------------
+// fork: C supplies SEQS, ROWS, SLOTS, P (pages), T (tokens of a page).
+// ---------------------------------------------------------------------------------------------
+
+// What row r becomes: its parent (-1: empty), the parent's length, the slots that its tokens take and those that it is to have.
+struct Fork {
+  int parent, length, kept, want;
+  bool partial;
+};
+template <class C>
+__device__ __forceinline__ Fork fork_of(const int* __restrict__ lengths, const int* __restrict__ parents, const int* __restrict__ room, long r) {
+  Fork f = {-1, 0, 0, 0, false};
+  constexpr long MOST = C::SLOTS * C::T;
+  const int p = parents[r];
+  if (p < 0 || p >= C::SEQS) return f;
+  f.parent = p;
+  const int n = lengths[p], more = room[r];
+  const long length = n < 0 ? 0 : n > MOST ? MOST : n, all = length + (more < 0 ? 0 : more);
+  f.length = (int)length;
+  f.kept = (int)((length + C::T - 1) / C::T);
+  f.want = (int)(((all > MOST ? MOST : all) + C::T - 1) / C::T);
+  f.partial = length % C::T != 0;
+  return f;
+}
+// The page in a slot, -1 for none.
+template <class C> __device__ __forceinline__ int page_at(const int* __restrict__ table, int parent, int slot) {
+  const int p = table[(long)parent * C::SLOTS + slot];
+  return p >= 0 && p < C::P ? p : -1;
+}
+
+// `map` and `counts`: (P + 31) / 32 words each; `firsts` [P]: work space where there are more than THREADS rows.
+template <class C, bool LDS>
+__device__ __forceinline__ void fork_with(u32_t* map, int* counts, const int* __restrict__ table, const int* __restrict__ lengths,
+                                          const int* __restrict__ parents, const int* __restrict__ room, const u8_t* __restrict__ held,
+                                          int* __restrict__ out_table, int* __restrict__ out_lengths, int* __restrict__ source,
+                                          int* __restrict__ target, int* __restrict__ left, int* __restrict__ firsts) {
+  constexpr long WORDS = (C::P + 31) / 32;
+  constexpr int SLOTS = C::SLOTS > 0 ? (int)C::SLOTS : 1;
+  __shared__ int parent[THREADS], kept[THREADS], place[THREADS], sums[WAVES + 1];
+  const int tid = threadIdx.x;
+  for (long w = tid; w < WORDS; w += THREADS) put_word<LDS>(map, w, held_word<C::P>(held, w));
+  meet<LDS>();
+  // Pages that a row has filled.
+  for (long r0 = 0; r0 < C::ROWS; r0 += THREADS) {
+    if (r0 + tid < C::ROWS) {
+      const Fork f = fork_of<C>(lengths, parents, room, r0 + tid);
+      parent[tid] = f.parent;
+      kept[tid] = f.kept - (f.partial ? 1 : 0);
+    }
+    __syncthreads();
+    const int n = (int)((C::ROWS - r0 < THREADS ? C::ROWS - r0 : THREADS) * C::SLOTS);
+#pragma unroll 4
+    for (int i = tid; i < n; i += THREADS) {
+      const int r = i / SLOTS, j = i % SLOTS;
+      if (j >= kept[r]) continue;
+      const int p = page_at<C>(table, parent[r], j);
+      if (p >= 0) set_bit(map, p);
+    }
+    meet<LDS>();
+  }
+  // Pages that a row has filled in part: whose they are. `source` says which rows copy theirs.
+  auto partly = [&](long r) {
+    const Fork f = fork_of<C>(lengths, parents, room, r);
+    return f.partial ? page_at<C>(table, f.parent, f.kept - 1) : -1;
+  };
+  if constexpr (C::ROWS <= THREADS) {
+    const int mine = tid < C::ROWS ? partly(tid) : -1;
+    place[tid] = mine;
+    __syncthreads();
+    bool copied = false;
+    if (mine >= 0) {
+      copied = bit<LDS>(map, mine);
+      for (int r = 0; r < tid; ++r) copied |= place[r] == mine;
+    }
+    if (tid < C::ROWS) source[tid] = copied ? mine : -1;
+    __syncthreads();
+    if (mine >= 0) set_bit(map, mine);
+  } else {
+    for (long r = tid; r < C::ROWS; r += THREADS) {
+      const int mine = partly(r);
+      if (mine >= 0) __hip_atomic_store(firsts + mine, (int)C::ROWS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    meet<false>();
+    for (long r = tid; r < C::ROWS; r += THREADS) {
+      const int mine = partly(r);
+      if (mine >= 0) atomicMin(firsts + mine, (int)r);
+    }
+    meet<false>();
+    for (long r = tid; r < C::ROWS; r += THREADS) {
+      const int mine = partly(r);
+      source[r] = mine >= 0 && (bit<LDS>(map, mine) || __hip_atomic_load(firsts + mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != (int)r) ? mine : -1;
+    }
+    __syncthreads();
+    for (long r = tid; r < C::ROWS; r += THREADS) {
+      const int mine = partly(r);
+      if (mine >= 0) set_bit(map, mine);
+    }
+  }
+  meet<LDS>();
+  // Free pages before each word.
+  long from, to;
+  my_words(WORDS, from, to);
+  int mine = 0, all;
+  for (long w = from; w < to; ++w) mine += __builtin_popcount(~word<LDS>(map, w));
+  int so_far = before_me(mine, sums, all);
+  for (long w = from; w < to; ++w) {
+    put_word<LDS>((u32_t*)counts, w, (u32_t)so_far);
+    so_far += __builtin_popcount(~word<LDS>(map, w));
+  }
+  meet<LDS>();
+  auto fresh = [&](long k) {
+    if (k >= all) return -1;
+    long lo = 0, hi = WORDS;  // the last word with at most k free pages before it
+    while (hi - lo > 1) {
+      const long mid = (lo + hi) / 2;
+      if ((int)word<LDS>((const u32_t*)counts, mid) <= k) lo = mid;
+      else hi = mid;
+    }
+    return (int)(lo * 32) + nth_bit(~word<LDS>(map, lo), (int)(k - (int)word<LDS>((const u32_t*)counts, lo)));
+  };
+  // The rows: their copies, and then what they are to have.
+  long asked = 0;
+  for (long r0 = 0; r0 < C::ROWS; r0 += THREADS) {
+    __syncthreads();
+    const long r = r0 + tid;
+    Fork f = {-1, 0, 0, 0, false};
+    int old = -1, wanted = 0;
+    if (r < C::ROWS) {
+      f = fork_of<C>(lengths, parents, room, r);
+      old = source[r];
+      wanted = (old >= 0) + (f.want - f.kept);
+    }
+    int total;
+    const long first = asked + before_me(wanted, sums, total);
+    if (r < C::ROWS) {
+      parent[tid] = f.parent;
+      // (the last kept slot of a row that copies is one of those to be filled)
+      kept[tid] = f.kept - (old >= 0);
+      place[tid] = (int)(first - asked);
+      out_lengths[r] = f.length;
+      const int page = old >= 0 ? fresh(first) : -1;
+      source[r] = page >= 0 ? old : -1;
+      target[r] = page;
+    }
+    __syncthreads();
+    const int n = (int)((C::ROWS - r0 < THREADS ? C::ROWS - r0 : THREADS) * C::SLOTS);
+#pragma unroll 4
+    for (int i = tid; i < n; i += THREADS) {
+      const int row = i / SLOTS, j = i % SLOTS, k = j - kept[row];
+      const int mine = (row + 1 < THREADS && r0 + row + 1 < C::ROWS ? place[row + 1] : total) - place[row];
+      int p = -1;
+      if (k < 0) p = page_at<C>(table, parent[row], j);
+      else if (k < mine) p = fresh(asked + place[row] + k);
+      out_table[r0 * C::SLOTS + i] = p;
+    }
+    asked += total;
+  }
+  if (tid == 0) left[0] = (int)(all - asked);
+}
+template <class C>
+__device__ __forceinline__ void fork(const int* __restrict__ table, const int* __restrict__ lengths, const int* __restrict__ parents,
+                                     const int* __restrict__ room, const u8_t* __restrict__ held, int* __restrict__ out_table,
+                                     int* __restrict__ out_lengths, int* __restrict__ source, int* __restrict__ target, int* __restrict__ left,
+                                     int* __restrict__ work) {
+  constexpr long WORDS = (C::P + 31) / 32;
+  constexpr bool LDS = C::P <= LDS_PAGES;
+  __shared__ u32_t map[LDS ? WORDS + 1 : 1];
+  __shared__ int counts[LDS ? WORDS + 1 : 1];
+  int* const firsts = LDS ? work : work + 2 * WORDS;
+  fork_with<C, LDS>(LDS ? map : (u32_t*)work, LDS ? counts : work + WORDS, table, lengths, parents, room, held, out_table, out_lengths, source, target,
+                    left, firsts);
+}
+
+// ---------------------------------------------------------------------------------------------
+// compact: C supplies ENTRIES (of the tables), P, MOVES.
+// ---------------------------------------------------------------------------------------------
+
+template <class C, bool LDS>
+__device__ __forceinline__ void compact_with(u32_t* used, u32_t* busy, int* counts, const int* __restrict__ table, const u8_t* __restrict__ held,
+                                             int* __restrict__ out_table, int* __restrict__ source, int* __restrict__ target) {
+  constexpr long WORDS = (C::P + 31) / 32;
+  __shared__ int sums[WAVES + 1];
+  const int tid = threadIdx.x;
+  for (long w = tid; w < WORDS; w += THREADS) put_word<LDS>(used, w, 0);
+  meet<LDS>();
+#pragma unroll 8
+  for (long i = tid; i < C::ENTRIES; i += THREADS) {
+    const int p = table[i];
+    if (p >= 0 && p < C::P) set_bit(used, p);
+  }
+  meet<LDS>();
+  // Pages in use, `used` or held, are n; what is in use and not held from n on moves into what is free below. `used` becomes those that move.
+  long from, to;
+  my_words(WORDS, from, to);
+  int mine = 0, n;
+  for (long w = from; w < to; ++w) {
+    const u32_t h = held_word<C::P>(held, w), u = word<LDS>(used, w);
+    put_word<LDS>(busy, w, h | u);
+    put_word<LDS>(used, w, u & ~h);
+    mine += __builtin_popcount(h | u);
+  }
+  before_me(mine, sums, n);
+  n -= (int)(WORDS * 32 - C::P);  // (what lies past the last page counts as held)
+  auto below = [&](long w) { return n <= w * 32 ? 0u : n >= w * 32 + 32 ? ~0u : (1u << (n - w * 32)) - 1; };
+  int movers = 0, holes = 0, all;
+  for (long w = from; w < to; ++w) {
+    const u32_t m = word<LDS>(used, w) & ~below(w);
+    put_word<LDS>(used, w, m);
+    movers += __builtin_popcount(m);
+    holes += __builtin_popcount(~word<LDS>(busy, w) & below(w));
+  }
+  int hole = before_me(holes, sums, all), mover = before_me(movers, sums, all);
+  const int moves = all < C::MOVES ? all : (int)C::MOVES;
+  for (long w = from; w < to; ++w) {
+    put_word<LDS>((u32_t*)counts, w, (u32_t)mover);
+    for (u32_t m = word<LDS>(used, w); m; m &= m - 1, ++mover)
+      if (mover < moves) source[mover] = (int)(w * 32) + __builtin_ctz(m);
+    for (u32_t h = ~word<LDS>(busy, w) & below(w); h; h &= h - 1, ++hole)
+      if (hole < moves) target[hole] = (int)(w * 32) + __builtin_ctz(h);
+  }
+  for (long i = moves + tid; i < C::MOVES; i += THREADS) source[i] = target[i] = -1;
+  meet<false>();
+#pragma unroll 8
+  for (long i = tid; i < C::ENTRIES; i += THREADS) {
+    int p = table[i];
+    if (p < 0 || p >= C::P) {
+      p = -1;
+    } else {
+      const u32_t m = word<LDS>(used, p >> 5);
+      if (m >> (p & 31) & 1) {
+        const int k = (int)word<LDS>((const u32_t*)counts, p >> 5) + __builtin_popcount(m & ((1u << (p & 31)) - 1));
+        if (k < moves) p = __hip_atomic_load(target + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+    out_table[i] = p;
+  }
+}
+template <class C>
+__device__ __forceinline__ void compact(const int* __restrict__ table, const u8_t* __restrict__ held, int* __restrict__ out_table,
+                                        int* __restrict__ source, int* __restrict__ target, int* __restrict__ work) {
+  constexpr long WORDS = (C::P + 31) / 32;
+  constexpr bool LDS = C::P <= LDS_PAGES;
+  __shared__ u32_t used[LDS ? WORDS + 1 : 1], busy[LDS ? WORDS + 1 : 1];
+  __shared__ int counts[LDS ? WORDS + 1 : 1];
+  compact_with<C, LDS>(LDS ? used : (u32_t*)work, LDS ? busy : (u32_t*)work + WORDS, LDS ? counts : work + 2 * WORDS, table, held, out_table, source, target);
+}
+
+// ---------------------------------------------------------------------------------------------
+// copies: C supplies N (copies), P, BYTES (of a page), PER (bytes of a workgroup), W (bytes of an access), CHECK, OWNERS (the last copy to each
+// page is in a table).
+// ---------------------------------------------------------------------------------------------
+
+template <int W> struct alignas(W) Piece { u8_t v[W]; };
+
+template <class C> __device__ __forceinline__ bool pair_of(const int* __restrict__ source, const int* __restrict__ target, long i, int& s, int& t) {
+  s = source[i];
+  t = target[i];
+  return s >= 0 && s < C::P && t >= 0 && t < C::P;
+}
+
+// The last copy to each page that copies name: FIRST puts -1 there, then the largest copy's number is taken.
+template <class C, bool FIRST>
+__device__ __forceinline__ void claim(const int* __restrict__ source, const int* __restrict__ target, int* __restrict__ owner) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  int s, t;
+  if (i >= C::N || !pair_of<C>(source, target, i, s, t)) return;
+  if constexpr (FIRST) owner[s] = owner[t] = -1;
+  else atomicMax(&owner[t], (int)i);
+}
+
+// Whether some copy from number `from` on goes to page p. All threads of the workgroup.
+template <class C> __device__ __forceinline__ bool goes_to(const int* __restrict__ source, const int* __restrict__ target, long from, int p) {
+  int found = 0;
+  for (long j = from + threadIdx.x; j < C::N; j += 256) {
+    int s, t;
+    if (pair_of<C>(source, target, j, s, t)) found |= t == p;
+  }
+  return __syncthreads_or(found) != 0;
+}
+
+// The part blockIdx.y of a page.
+template <class C> __device__ __forceinline__ void move(const u8_t* from, u8_t* to) {
+  typedef Piece<C::W> V;
+  const long begin = (long)blockIdx.y * C::PER, end = begin + C::PER < C::BYTES ? begin + C::PER : C::BYTES;
+#pragma unroll 4
+  for (long b = begin + threadIdx.x * C::W; b < end; b += 256 * C::W) *(V*)(to + b) = *(const V*)(from + b);
+}
+
+// In place: sources that are a target too, aside. aside [N][BYTES], flags [N]: whether a copy's source is there.
+template <class C>
+__device__ __forceinline__ void put_aside(const u8_t* from, const u8_t* to, const int* __restrict__ source, const int* __restrict__ target,
+                                          const int* __restrict__ owner, u8_t* __restrict__ aside, int* __restrict__ flags) {
+  if (from != to) return;
+  const long i = blockIdx.x;
+  int s, t;
+  if (!pair_of<C>(source, target, i, s, t)) return;
+  bool hit;
+  if constexpr (C::OWNERS) hit = owner[s] >= 0;
+  else hit = goes_to<C>(source, target, 0, s);
+  if (blockIdx.y == 0 && threadIdx.x == 0) flags[i] = hit;
+  if (hit) move<C>(from + (long)s * C::BYTES, aside + i * C::BYTES);
+}
+
+template <class C>
+__device__ __forceinline__ void copy(const u8_t* from, u8_t* to, const int* __restrict__ source, const int* __restrict__ target,
+                                     const int* __restrict__ owner, const u8_t* __restrict__ aside, const int* __restrict__ flags) {
+  const long i = blockIdx.x;
+  int s, t;
+  if (!pair_of<C>(source, target, i, s, t)) return;
+  const u8_t* page = from + (long)s * C::BYTES;
+  if constexpr (C::CHECK) {
+    bool last;
+    if constexpr (C::OWNERS) last = owner[t] == (int)i;
+    else last = !goes_to<C>(source, target, i + 1, t);
+    if (!last) return;
+    if (from == to && flags[i]) page = aside + i * C::BYTES;
+  }
+  move<C>(page, to + (long)t * C::BYTES);
+}
+
+}  // namespace pages
+}  // namespace accy

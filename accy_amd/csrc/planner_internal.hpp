@@ -3,7 +3,8 @@
 // launch tuning, serial contractions and scatter_add; planner_reduce.cpp the folds and row kernels;
 // planner_views.cpp strided views and materialised transposes; planner_contraction.cpp the matrix-core
 // contractions, grouped launches and epilogues; planner_attention.cpp the fused attention matcher and
-// kernels; planner_mx4.cpp the custom calls of microscaled 4-bit floats. The fusion rules and their references are described in lower.cpp.
+// kernels; planner_custom.cpp the custom calls of this target, planner_mx4.cpp those of microscaled 4-bit floats, planner_heads.cpp,
+// planner_pages.cpp and planner_logits.cpp the others. The fusion rules and their references are described in lower.cpp.
 #pragma once
 
 #include <algorithm>
@@ -605,9 +606,9 @@ class Planner {
   // ---- scatter_add: one pass over the table, every row's updates added in order ----
   void scatter_add(uint32_t v);
 
-  // ---- custom calls of this target: microscaled 4-bit floats (kernels/mx4.h) ----
+  // ---- custom calls of this target ----
   //
-  // "accy.mx4.<name>", version 1; operands and results are checked against what the name takes (Unsupported with the
+  // "accy.<set>.<name>", version 1; operands and results are checked against what the name takes (Unsupported with the
   // reason otherwise, as for every other custom call).
   void custom(uint32_t v);
 
@@ -618,6 +619,22 @@ class Planner {
   std::vector<bool> opaque_caches() const;
   // Operands of custom calls that must be in memory are materialised by the kernel that produces them.
   void mark_custom_operands();
+
+  void group(uint32_t v);
+  std::vector<uint32_t> grouped(const Op& op, uint32_t a, size_t least, size_t most) const;
+  std::map<std::string, uint32_t> siblings(uint32_t v, const std::string& prefix, const std::string& suffix = "") const;
+  int updated_cache(uint32_t v);
+
+  bool heads(uint32_t v);
+  void pages_copy(uint32_t v);
+  void pages_fork(uint32_t v);
+  void pages_compact(uint32_t v);
+  void logits_log_probs(uint32_t v);
+  void logits_grad(uint32_t v);
+  int64_t logit_chunks(int64_t vocab, DType d) const;
+  int64_t logit_splits(uint64_t rows, int64_t chunks, int64_t k) const;
+  uint64_t logit_part(int64_t k) const;
+  std::string logit_config(const std::string& nm, int dt, uint64_t rows, int64_t vocab, int64_t k, int64_t splits, int64_t threads, int64_t u) const;
 
   void mx4_quantize(uint32_t v);
   void mx4_values(uint32_t v);

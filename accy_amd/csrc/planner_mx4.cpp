@@ -6,43 +6,15 @@
 //   cache_write(cache, keys, values, slots) -> the cache with the rows of the tokens' slots replaced
 //   cache_keys(cache, slots), cache_values  -> [slots .., kv_head, dim]
 //   attend(q, cache, pages, lengths)        q [seq, (query,) head, dim] -> the same
+//   attend_shared(q, cache, group(pages, lengths), group(prefix pages, prefix lengths, prefix of each sequence))
 //
-// Float operands and results are bf16, f16 or f32. The wire carries a custom call's result type, so everything about it is
-// checked here.
-#include "planner_internal.hpp"
+// Float operands and results are bf16, f16 or f32.
+#include "planner_custom.hpp"
 
 namespace accy {
 namespace planning {
 
 namespace {
-
-[[noreturn]] void refuse(const Op& op, const std::string& why) {
-  fail(Err::Unsupported, "custom_call " + op.bytes + ": " + why);
-}
-
-void require(bool ok, const Op& op, const std::string& why) {
-  if (!ok) refuse(op, why);
-}
-
-// DT of kernels/mx4.h.
-int element_type(const Op& op, DType d) {
-  switch (d) {
-    case DType::bf16: return 0;
-    case DType::f16: return 1;
-    case DType::f32: return 2;
-    default: refuse(op, std::string(dtype_name(d)) + " values (bf16, f16 or f32)");
-  }
-}
-
-int64_t last(const Type& t) { return t.rank() ? t.dims.back().extent : 0; }
-
-// The extents of a's leading axes are b's.
-bool same_rows(const Type& a, const Type& b) {
-  if (a.rank() != b.rank()) return false;
-  for (size_t i = 0; i + 1 < a.rank(); ++i)
-    if (a.dims[i].extent != b.dims[i].extent) return false;
-  return true;
-}
 
 // Codes and scales of one tensor: the elements along its blocked axis.
 int64_t blocked(const Op& op, const Type& codes, const Type& scales) {
@@ -53,59 +25,7 @@ int64_t blocked(const Op& op, const Type& codes, const Type& scales) {
   return k;
 }
 
-std::string num(int64_t n) { return std::to_string(n); }
-
 }  // namespace
-
-void Planner::custom(uint32_t v) {
-  const Op& op = g_.ops[v];
-  const std::string prefix = "accy.mx4.";
-  const std::string what = op.bytes.compare(0, prefix.size(), prefix) == 0 ? op.bytes.substr(prefix.size()) : "";
-  auto operands = [&](size_t n) { require(op.args.size() == n, op, num((int64_t)n) + " operands"); };
-  if (op.index == 1) {
-    if (what == "codes" || what == "scales") return operands(1), mx4_quantize(v);
-    if (what == "values") return operands(2), mx4_values(v);
-    if (what == "contract") return operands(4), mx4_contract(v);
-    if (what == "cache_write") return operands(4), mx4_cache_write(v);
-    if (what == "cache_keys" || what == "cache_values") return operands(2), mx4_cache_read(v);
-    if (what == "attend") return operands(4), mx4_attend(v);
-  }
-  fail(Err::Unsupported, "custom_call " + op.bytes + " version " + std::to_string(op.index) + " is not supported by the HIP target");
-}
-
-uint32_t Planner::dense_source(uint32_t v) const {
-  while (g_.ops[v].kind == Kind::reshape && slots_.slot_of[v] < 0) v = g_.ops[v].args[0];
-  return v;
-}
-
-int Planner::dense_slot(uint32_t v) { return materialize(dense_source(v)); }
-
-std::vector<bool> Planner::opaque_caches() const {
-  auto call = [](const Op& op, const char* name) { return op.kind == Kind::custom_call && op.bytes == std::string("accy.mx4.") + name; };
-  std::vector<bool> opaque(g_.ops.size());
-  for (size_t v = 0; v < g_.ops.size(); ++v) {
-    const Op& op = g_.ops[v];
-    opaque[v] = op.kind == Kind::parameter || op.kind == Kind::scan || op.kind == Kind::projection || call(op, "cache_write");
-    for (size_t i = 0; i < op.args.size(); ++i) {
-      const bool cache = (i == 0 && (call(op, "cache_write") || call(op, "cache_keys") || call(op, "cache_values"))) || (i == 1 && call(op, "attend"));
-      if (!cache && op.kind != Kind::scan && op.kind != Kind::projection) opaque[op.args[i]] = false;
-    }
-  }
-  return opaque;
-}
-
-void Planner::mark_custom_operands() {
-  for (uint32_t v = 0; v < g_.ops.size(); ++v) {
-    const Op& op = g_.ops[v];
-    if (!live_[v] || op.kind != Kind::custom_call) continue;
-    // A quantised tensor is evaluated inside the kernel that quantises it.
-    if (op.args.size() == 1) continue;
-    for (uint32_t a : op.args) {
-      const uint32_t s = dense_source(a);
-      if (is_inlinable(g_.ops[s].kind)) needed_[s] = true;
-    }
-  }
-}
 
 // ---- codes and scales: eight values per thread, four lanes to a block ----
 
@@ -476,20 +396,7 @@ void Planner::mx4_cache_write(uint32_t v) {
   for (size_t i = 0; i < st.rank(); ++i) require(st.dims[i].extent == kt.dims[i].extent, op, "an i32 slot for every token");
   const Mx4Cache c = mx4_cache(op, op.args[0], kt.dims[kt.rank() - 2].extent, last(kt));
   require(op.result == g_.type(op.args[0]), op, "the result has the cache's type");
-  const int old = dense_slot(op.args[0]), out = temp_slot(v);
-  Step copy;
-  copy.type = Step::Copy;
-  copy.copy.src = old;
-  copy.copy.dst = out;
-  copy.copy.bytes = op.result.bytes();
-  copy.copy.unless_same = true;
-  if (copy.copy.bytes) plan_.steps.push_back(copy);
-  // The cache's own buffer may be the result's where the caller hands it in, gets it back, and nothing else of the program
-  // reads what was in it.
-  const SlotInfo &from = plan_.slots[(size_t)old], &to = plan_.slots[(size_t)out];
-  if (from.role == SlotInfo::Input && to.role == SlotInfo::Output && g_.ops[op.args[0]].kind == Kind::parameter &&
-      users_[op.args[0]].size() == 1 && !is_output_[op.args[0]])
-    plan_.updates.push_back({(size_t)from.io_index, (size_t)to.io_index});
+  const int out = updated_cache(v);
   const uint64_t n = st.elements();
   if (n && c.pages && c.heads) {
     const int ks = dense_slot(op.args[1]), vs = dense_slot(op.args[2]), ss = dense_slot(op.args[3]);
@@ -572,7 +479,10 @@ void Planner::mx4_cache_read(uint32_t v) {
 
 void Planner::mx4_attend(uint32_t v) {
   const Op& op = g_.ops[v];
-  const Type &qt = g_.type(op.args[0]), &ct = g_.type(op.args[1]), &pt = g_.type(op.args[2]), &lt = g_.type(op.args[3]);
+  const bool shared = op.bytes == "accy.mx4.attend_shared";
+  const std::vector<uint32_t> own = shared ? grouped(op, op.args[2], 2, 2) : std::vector<uint32_t>{op.args[2], op.args[3]};
+  const std::vector<uint32_t> prefix = shared ? grouped(op, op.args[3], 3, 3) : std::vector<uint32_t>();
+  const Type &qt = g_.type(op.args[0]), &ct = g_.type(op.args[1]), &pt = g_.type(own[0]), &lt = g_.type(own[1]);
   element_type(op, qt.dtype);
   require(op.result.dtype == qt.dtype && same_rows(op.result, qt) && last(op.result) == last(qt), op, "the result has the queries' type");
   require(qt.rank() == 3 || qt.rank() == 4, op, "queries are [seq, (query,) head, dim]");
@@ -586,11 +496,22 @@ void Planner::mx4_attend(uint32_t v) {
   const Mx4Cache c = mx4_cache(op, op.args[1], H, hd);
   const int64_t maxp = pt.dims[1].extent;
   require(maxp < (int64_t(1) << 31) / c.tokens, op, "a sequence has fewer than 2^31 keys");
+  int64_t prefixes = 0, prefix_maxp = 0;
+  if (shared) {
+    const Type &spt = g_.type(prefix[0]), &slt = g_.type(prefix[1]), &oft = g_.type(prefix[2]);
+    require(spt.dtype == DType::i32 && spt.rank() == 2, op, "shared pages are i32 [prefix, page]");
+    prefixes = spt.dims[0].extent;
+    prefix_maxp = spt.dims[1].extent;
+    require(slt.dtype == DType::i32 && slt.rank() == 1 && slt.dims[0].extent == prefixes, op, "shared lengths are i32 [prefix]");
+    require(oft.dtype == DType::i32 && oft.rank() == 1 && oft.dims[0].extent == seqs, op, "prefixes of sequences are i32 [seq]");
+    require(prefix_maxp < (int64_t(1) << 31) / c.tokens, op, "a prefix has fewer than 2^31 keys");
+    require(prefixes >= 1 && prefixes <= 1024, op, "1 to 1024 prefixes");  // their counts lie in a stage of LDS
+  }
   const int out = temp_slot(v);
   const uint64_t nel = op.result.elements();
   if (nel) {
     require(Q * G < (int64_t(1) << 24), op, "2^24 query rows of a key-value head or more");
-    const int qs = dense_slot(op.args[0]), cs = dense_slot(op.args[1]), ps = dense_slot(op.args[2]), ls = dense_slot(op.args[3]);
+    const int qs = dense_slot(op.args[0]), cs = dense_slot(op.args[1]), ps = dense_slot(own[0]), ls = dense_slot(own[1]);
     // Outputs and queries are registers of the whole run, and with several queries the outputs before a step as well: two workgroups of a CU
     // where they leave half of 256, else one, whose kernel may take 512 (24 x 8 heads x 4096 keys, four rows of 192 f16 39 us in two, 47 in one,
     // five queries of 160 bf16 34 and 44; five of 192 would spill in two). Three, whose LDS there is up to 128 dims, where one query's kernel
@@ -604,35 +525,49 @@ void Planner::mx4_attend(uint32_t v) {
     const int64_t steps = (maxp * c.tokens + 31) / 32, want = wgs >= 256 ? 1024 : 512;
     const int64_t splits = opt_.allow_split ? std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, steps / 16, 64})) : 1;
     require(launchable((uint64_t)wgs, 256), op, "more workgroups than a launch takes");
+    // A prefix's rows, sixteen to a workgroup, against its keys: split till two workgroups are at work on every CU.
+    const int64_t prefix_groups = shared ? seqs * Q * G / 16 + prefixes : 0, prefix_steps = (prefix_maxp * c.tokens + 31) / 32;
+    const int64_t rows = std::max<int64_t>(1, (seqs * Q * G + 15) / 16);
+    const int64_t prefix_splits = !shared ? 0 : opt_.allow_split ? std::max<int64_t>(1, std::min<int64_t>({(512 + H * rows - 1) / (H * rows), prefix_steps / 16, 64})) : 1;
+    const int64_t all_parts = splits + prefix_splits;
     KernelWriter w(g_, slots_, "i64_t");
     const std::string q = w.arg(qs, false), a = w.arg(cs, false), p = w.arg(ps, false), l = w.arg(ls, false);
+    std::string more;
+    for (const uint32_t x : prefix) more += w.arg(dense_slot(x), false) + ", ";
     int part = -1;
-    if (splits > 1) part = slots_.add(SlotInfo::Temp, -1, DType::f32, (uint64_t)(seqs * H * Q * G * splits * (hd + 4)) * 4);
-    const std::string o = splits > 1 ? "nullptr" : w.arg(out, true), pp = splits > 1 ? w.arg(part, true) : "nullptr";
+    if (all_parts > 1) part = slots_.add(SlotInfo::Temp, -1, DType::f32, (uint64_t)(seqs * H * Q * G * all_parts * (hd + 4)) * 4);
+    const std::string o = all_parts > 1 ? "nullptr" : w.arg(out, true), pp = all_parts > 1 ? w.arg(part, true) : "nullptr";
     const std::string nm = name("mx4_attend", v);
     char sl[64];
     std::snprintf(sl, sizeof sl, "%af", (double)(float)(1.4426950408889634 / std::sqrt((double)hd)));
     const std::string head = "#include \"mx4\"\nstruct Cfg_" + nm + " {\n" + c.members(qt.dtype) + "  static constexpr int Q = " + num(Q) +
                              ", G = " + num(G) + ", MAXP = " + num(maxp) + ", SPLITS = " + num(splits) +
+                             (shared ? ", PREFIXES = " + num(prefixes) + ", PSPLITS = " + num(prefix_splits) + ", PREFIX_MAXP = " + num(prefix_maxp) : std::string()) +
                              ";\n  static constexpr long SEQS = " + num(seqs) + ";\n  static constexpr float SL = " + sl + ";\n};\n";
     KernelStep k;
-    k.source = head + "extern \"C\" __global__ void __launch_bounds__(256, " + num(bounds) + ") " + nm + "(" + w.params() + ") {\n  accy::mx4::attend<Cfg_" + nm +
-               ">(" + q + ", " + a + ", " + p + ", " + l + ", " + o + ", " + pp + ");\n}\n";
+    k.source = head + "extern \"C\" __global__ void __launch_bounds__(256, " + num(bounds) + ") " + nm + "(" + w.params() + ") {\n  accy::mx4::" +
+               (shared ? "attend_shared" : "attend") + "<Cfg_" + nm + ">(" + q + ", " + a + ", " + p + ", " + l + ", " + (shared ? more : o + ", ") + pp + ");\n}\n";
     k.name = nm;
-    k.grid[0] = (uint32_t)wgs;
-    k.grid[1] = (uint32_t)splits;
+    if (shared) {
+      const uint64_t groups_of_all = (uint64_t)(prefix_groups * H * prefix_splits) + (uint64_t)(wgs * splits);
+      require(launchable(groups_of_all, 256) && groups_of_all < (uint64_t(1) << 31), op, "more workgroups than a launch takes");
+      k.grid[0] = (uint32_t)groups_of_all;
+    } else {
+      k.grid[0] = (uint32_t)wgs;
+      k.grid[1] = (uint32_t)splits;
+    }
     k.block[0] = 256;
     k.klass = "attention";
     k.label = "mx4_attend:%" + std::to_string(v);
-    k.algorithmic_flops = 4.0 * (double)nel * (double)(maxp * c.tokens);
+    k.algorithmic_flops = 4.0 * (double)nel * (double)((maxp + prefix_maxp) * c.tokens);
     push(std::move(k), w);
-    if (splits > 1) {
+    if (all_parts > 1) {
       KernelWriter jw(g_, slots_, "i64_t");
-      const std::string jp = jw.arg(part, false), jo = jw.arg(out, true);
+      const std::string jp = jw.arg(part, false), jo = jw.arg(out, true), jf = shared ? ", " + jw.arg(dense_slot(prefix[2]), false) : std::string();
       KernelStep j;
       j.name = name("mx4_join", v);
       j.source = head + "extern \"C\" __global__ void __launch_bounds__(256) " + j.name + "(" + jw.params() + ") {\n  accy::mx4::attend_join<Cfg_" +
-                 nm + ">(" + jp + ", " + jo + ");\n}\n";
+                 nm + ">(" + jp + ", " + jo + jf + ");\n}\n";
       require(launchable((nel + 255) / 256, 256), op, "more workgroups than a launch takes");
       j.grid[0] = (uint32_t)((nel + 255) / 256);
       j.block[0] = 256;

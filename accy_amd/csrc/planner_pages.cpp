@@ -1,0 +1,189 @@
+// Custom calls on the pages of a cache (kernels/pages.h), "accy.pages.<name>":
+//
+//   fork_table, fork_lengths, fork_source, fork_target, fork_left(group(table, lengths), group(parents, room), held, page)
+//       table i32 [seq, slot], lengths i32 [seq], parents, room i32 [row], held i1 [page], page an i32 constant -> i32 [row, slot], [row], [row],
+//       [row], []: planned as one kernel
+//   compact_table, compact_source, compact_target(table, held)   table i32 [seq, slot], held i1 [page] -> as the table, i32 [move] twice
+//   copy(cache, source, target)   cache [page, ..], i32 [copy] twice -> the cache
+#include "planner_custom.hpp"
+
+namespace accy {
+namespace planning {
+
+namespace {
+
+constexpr int64_t kMostPages = int64_t(1) << 24;
+constexpr int64_t kLdsPages = int64_t(1) << 17;  // LDS_PAGES of kernels/pages.h
+
+bool whole_numbers(const Type& t, size_t rank) { return t.dtype == DType::i32 && t.rank() == rank; }
+
+}  // namespace
+
+void Planner::pages_fork(uint32_t v) {
+  const Op& op = g_.ops[v];
+  const std::vector<uint32_t> now = grouped(op, op.args[0], 2, 2), next = grouped(op, op.args[1], 2, 2);
+  const Type &tt = g_.type(now[0]), &lt = g_.type(now[1]), &pt = g_.type(next[0]), &rt = g_.type(next[1]), &ht = g_.type(op.args[2]);
+  require(whole_numbers(tt, 2) && whole_numbers(lt, 1) && lt.dims[0].extent == tt.dims[0].extent, op, "tables are i32 [seq, slot], lengths i32 [seq]");
+  require(whole_numbers(pt, 1) && whole_numbers(rt, 1) && pt.dims[0].extent == rt.dims[0].extent, op, "parents and room are i32 [row]");
+  require(ht.dtype == DType::i1 && ht.rank() == 1, op, "held pages are i1 [page]");
+  const Op& size = g_.ops[op.args[3]];
+  int32_t page = 0;
+  if (size.kind == Kind::constant && size.result.dtype == DType::i32 && size.result.rank() == 0 && size.bytes.size() >= 4) std::memcpy(&page, size.bytes.data(), 4);
+  require(page >= 1 && page < (1 << 20), op, "the size of a page is an i32 constant of 1 to 2^20");
+  const int64_t seqs = tt.dims[0].extent, slots = tt.dims[1].extent, rows = pt.dims[0].extent, pages = ht.dims[0].extent;
+  require(pages <= kMostPages, op, "more than 2^24 pages");
+  require(slots < (int64_t(1) << 31) && rows < (int64_t(1) << 31) && rows * std::max<int64_t>(1, slots) < (int64_t(1) << 31), op, "2^31 entries or more");
+  const auto calls = siblings(v, "accy.pages.fork_");
+  const char* const names[] = {"table", "lengths", "source", "target", "left"};
+  std::vector<int> out(5, -1);
+  std::vector<uint32_t> made;
+  for (size_t i = 0; i < 5; ++i) {
+    const auto call = calls.find(names[i]);
+    const uint64_t bytes = i == 0 ? (uint64_t)(rows * slots) * 4 : i == 4 ? 4 : (uint64_t)rows * 4;
+    if (call == calls.end()) {
+      out[i] = slots_.add(SlotInfo::Temp, -1, DType::i32, bytes);  // what nobody reads is written all the same
+      continue;
+    }
+    const Type& t = g_.ops[call->second].result;
+    const bool fits = i == 0 ? whole_numbers(t, 2) && t.dims[0].extent == rows && t.dims[1].extent == slots
+                             : i == 4 ? whole_numbers(t, 0) : whole_numbers(t, 1) && t.dims[0].extent == rows;
+    require(fits, g_.ops[call->second], i == 0 ? "the result is i32 [row, slot]" : i == 4 ? "the result is i32 []" : "the result is i32 [row]");
+    out[i] = temp_slot(call->second);
+    made.push_back(call->second);
+  }
+  require(!made.empty(), op, "no result of that name");
+  const uint64_t words = (uint64_t)(pages + 31) / 32, work = (pages > kLdsPages ? 2 * words : 0) + (rows > 1024 ? (uint64_t)pages : 0);
+  KernelWriter w(g_, slots_, "i64_t");
+  std::string args;
+  for (const uint32_t a : {now[0], now[1], next[0], next[1], op.args[2]}) args += w.arg(dense_slot(a), false) + ", ";
+  for (const int o : out) args += w.arg(o, true) + ", ";
+  args += work ? w.arg(slots_.add(SlotInfo::Temp, -1, DType::i32, work * 4), true) : "nullptr";
+  KernelStep k;
+  const std::string nm = name("fork", v);
+  k.source = "#include \"pages\"\nstruct Cfg_" + nm + " {\n  static constexpr long SEQS = " + num(seqs) + ", ROWS = " + num(rows) + ", SLOTS = " + num(slots) + ", P = " +
+             num(pages) + ", T = " + num(page) + ";\n};\nextern \"C\" __global__ void __launch_bounds__(1024) " + nm + "(" + w.params() +
+             ") {\n  accy::pages::fork<Cfg_" + nm + ">(" + args + ");\n}\n";
+  k.name = nm;
+  k.block[0] = 1024;
+  k.klass = "pages";
+  k.label = "fork:%" + std::to_string(v);
+  push(std::move(k), w);
+  for (const uint32_t u : made) finish(u);
+}
+
+void Planner::pages_compact(uint32_t v) {
+  const Op& op = g_.ops[v];
+  const Type &tt = g_.type(op.args[0]), &ht = g_.type(op.args[1]);
+  require(whole_numbers(tt, 2), op, "tables are i32 [seq, slot]");
+  require(ht.dtype == DType::i1 && ht.rank() == 1, op, "held pages are i1 [page]");
+  const int64_t pages = ht.dims[0].extent;
+  require(pages <= kMostPages, op, "more than 2^24 pages");
+  const auto calls = siblings(v, "accy.pages.compact_");
+  int64_t moves = -1;
+  for (const char* which : {"source", "target"}) {
+    const auto call = calls.find(which);
+    if (call == calls.end()) continue;
+    const Type& t = g_.ops[call->second].result;
+    require(whole_numbers(t, 1) && t.dims[0].extent <= pages && (moves < 0 || t.dims[0].extent == moves), op, "moves are i32 [move], the same of both and at most as many as pages");
+    moves = t.dims[0].extent;
+  }
+  // (a table alone: as if every page might move)
+  if (moves < 0) moves = pages;
+  int out[3] = {-1, -1, -1};
+  const char* const names[] = {"table", "source", "target"};
+  std::vector<uint32_t> made;
+  for (int i = 0; i < 3; ++i) {
+    const auto call = calls.find(names[i]);
+    if (call == calls.end()) {
+      out[i] = slots_.add(SlotInfo::Temp, -1, DType::i32, i == 0 ? tt.bytes() : (uint64_t)moves * 4);
+      continue;
+    }
+    if (i == 0) {
+      const Type& t = g_.ops[call->second].result;
+      require(whole_numbers(t, 2) && t.dims[0].extent == tt.dims[0].extent && t.dims[1].extent == tt.dims[1].extent, g_.ops[call->second], "the result is as the table");
+    }
+    out[i] = temp_slot(call->second);
+    made.push_back(call->second);
+  }
+  require(!made.empty(), op, "no result of that name");
+  const uint64_t words = (uint64_t)(pages + 31) / 32;
+  KernelWriter w(g_, slots_, "i64_t");
+  std::string args = w.arg(dense_slot(op.args[0]), false) + ", " + w.arg(dense_slot(op.args[1]), false);
+  for (const int o : out) args += ", " + w.arg(o, true);
+  args += pages > kLdsPages ? ", " + w.arg(slots_.add(SlotInfo::Temp, -1, DType::i32, 3 * words * 4), true) : ", nullptr";
+  KernelStep k;
+  const std::string nm = name("compact", v);
+  k.source = "#include \"pages\"\nstruct Cfg_" + nm + " {\n  static constexpr long ENTRIES = " + std::to_string(tt.elements()) + ", P = " + num(pages) + ", MOVES = " +
+             num(moves) + ";\n};\nextern \"C\" __global__ void __launch_bounds__(1024) " + nm + "(" + w.params() + ") {\n  accy::pages::compact<Cfg_" + nm + ">(" + args +
+             ");\n}\n";
+  k.name = nm;
+  k.block[0] = 1024;
+  k.klass = "pages";
+  k.label = "compact:%" + std::to_string(v);
+  push(std::move(k), w);
+  for (const uint32_t u : made) finish(u);
+}
+
+void Planner::pages_copy(uint32_t v) {
+  const Op& op = g_.ops[v];
+  const Type &ct = g_.type(op.args[0]), &st = g_.type(op.args[1]), &tt = g_.type(op.args[2]);
+  require(ct.rank() >= 1, op, "a cache is [page, ..]");
+  require(whole_numbers(st, 1) && whole_numbers(tt, 1) && st.dims[0].extent == tt.dims[0].extent, op, "source and target are i32 [copy]");
+  require(op.result == ct, op, "the result has the cache's type");
+  const int from = dense_slot(op.args[0]), out = updated_cache(v);
+  const int64_t n = st.dims[0].extent, pages = ct.dims[0].extent, bytes = pages ? (int64_t)(ct.bytes() / (uint64_t)pages) : 0;
+  if (n && bytes) {
+    require(pages < (int64_t(1) << 31), op, "2^31 pages or more");
+    // Lists of fork and compact name pages that differ.
+    const Op &so = g_.ops[op.args[1]], &to = g_.ops[op.args[2]];
+    auto call = [&](const Op& o, const std::string& what) { return o.kind == Kind::custom_call && o.index == 1 && o.bytes == "accy.pages." + what; };
+    const bool check = !(so.args == to.args && ((call(so, "fork_source") && call(to, "fork_target")) || (call(so, "compact_source") && call(to, "compact_target"))));
+    const bool owners = check && n > 4096;
+    int64_t W = 16;
+    while (bytes % W) W /= 2;
+    const int64_t per = 8192, parts = (bytes + per - 1) / per;
+    require(parts < 65536 && launchable((uint64_t)n, 256), op, "more workgroups than a launch takes");
+    const std::string nm = name("copy_pages", v);
+    const std::string head = "#include \"pages\"\nstruct Cfg_" + nm + " {\n  static constexpr long N = " + num(n) + ", P = " + num(pages) + ", BYTES = " + num(bytes) + ", PER = " +
+                             num(per) + ";\n  static constexpr int W = " + num(W) + ";\n  static constexpr bool CHECK = " + (check ? "true" : "false") + ", OWNERS = " +
+                             (owners ? "true" : "false") + ";\n};\n";
+    const int ss = dense_slot(op.args[1]), ts = dense_slot(op.args[2]);
+    const int aside = check ? slots_.add(SlotInfo::Temp, -1, DType::u8, (uint64_t)(n * bytes)) : -1;
+    const int flags = check ? slots_.add(SlotInfo::Temp, -1, DType::i32, (uint64_t)n * 4) : -1;
+    const int owner = owners ? slots_.add(SlotInfo::Temp, -1, DType::i32, (uint64_t)pages * 4) : -1;
+    auto launch = [&](const std::string& kernel, const std::string& call, const KernelWriter& w, uint64_t x, uint64_t y) {
+      KernelStep k;
+      // The cache's two buffers may be one, and the kernels ask whether they are.
+      std::string params = w.params();
+      for (size_t at; (at = params.find("__restrict__ ")) != std::string::npos;) params.erase(at, 13);
+      k.source = head + "extern \"C\" __global__ void __launch_bounds__(256) " + kernel + "(" + params + ") {\n  accy::pages::" + call + ";\n}\n";
+      k.name = kernel;
+      k.grid[0] = (uint32_t)x;
+      k.grid[1] = (uint32_t)y;
+      k.block[0] = 256;
+      k.klass = "pages";
+      k.label = "copy_pages:%" + std::to_string(v);
+      push(std::move(k), w);
+    };
+    for (const bool first : {true, false}) {
+      if (!owners) break;
+      KernelWriter w(g_, slots_, "i64_t");
+      const std::string s = w.arg(ss, false), t = w.arg(ts, false), o = w.arg(owner, true);
+      launch(name("claim_pages", v), std::string("claim<Cfg_") + nm + ", " + (first ? "true" : "false") + ">(" + s + ", " + t + ", " + o + ")", w, (uint64_t)(n + 255) / 256, 1);
+    }
+    for (const bool last : {false, true}) {
+      if (!last && !check) continue;
+      KernelWriter w(g_, slots_, "i64_t");
+      const std::string a = w.arg(from, false), b = w.arg(out, last), s = w.arg(ss, false), t = w.arg(ts, false), o = owners ? w.arg(owner, false) : "nullptr";
+      const std::string i = check ? w.arg(aside, !last) : "nullptr", f = check ? w.arg(flags, !last) : "nullptr";
+      launch(last ? nm : name("put_aside", v),
+             std::string(last ? "copy" : "put_aside") + "<Cfg_" + nm + ">((const u8_t*)" + a + ", (" + (last ? "" : "const ") + "u8_t*)" + b + ", " + s + ", " + t + ", " + o + ", " +
+                 (check ? std::string(last ? "(const u8_t*)" : "(u8_t*)") + i : i) + ", " + f + ")",
+             w, (uint64_t)n, (uint64_t)parts);
+    }
+  }
+  finish(v);
+}
+
+}  // namespace planning
+}  // namespace accy

@@ -19,6 +19,9 @@ extern const char* const kScatterDeviceSource;
 extern const char* const kDecodeDeviceSource;
 extern const char* const kMx4DeviceSource;
 extern const char* const kMx4ContractDeviceSource;
+extern const char* const kHeadsDeviceSource;
+extern const char* const kPagesDeviceSource;
+extern const char* const kLogitsDeviceSource;
 
 namespace {
 
@@ -66,7 +69,10 @@ std::string full_kernel_source(const std::string& body) {
                                                            {"#include \"scatter\"\n", kScatterDeviceSource},
                                                            {"#include \"decode\"\n", kDecodeDeviceSource},
                                                            {"#include \"mx4\"\n", kMx4DeviceSource},
-                                                           {"#include \"mx4_contract\"\n", kMx4ContractDeviceSource}};
+                                                           {"#include \"mx4_contract\"\n", kMx4ContractDeviceSource},
+                                                           {"#include \"heads\"\n", kHeadsDeviceSource},
+                                                           {"#include \"pages\"\n", kPagesDeviceSource},
+                                                           {"#include \"logits\"\n", kLogitsDeviceSource}};
   std::string rest = body;
   for (const auto& t : templates) {
     size_t p = rest.find(t.first);

@@ -397,8 +397,18 @@ class Value:
     def cache_values_mx4(self, slots: "Value", dim: Dim, dtype: str) -> "Value":
         return self.builder.cache_read_mx4("cache_values", self, slots, dim, dtype)
 
-    def attend_mx4(self, cache: "Value", pages: "Value", lengths: "Value") -> "Value":
-        return self.builder.attend_mx4(self, cache, pages, lengths)
+    def attend_mx4(self, cache: "Value", pages: "Value", lengths: "Value", shared=None) -> "Value":
+        return self.builder.attend_mx4(self, cache, pages, lengths, shared)
+
+    # pages of a cache, and what a model answers with (this target's custom calls)
+    def copy_pages(self, source: "Value", target: "Value") -> "Value":
+        return self.builder.copy_pages(self, source, target)
+
+    def log_probs(self, tokens: "Value", axis: str, top: int = 0) -> "LogProbs":
+        return self.builder.log_probs(self, tokens, axis, top)
+
+    def log_probs_grad(self, tokens: "Value", d_token: "Value", d_entropy: "Value", axis: str) -> "Value":
+        return self.builder.log_probs_grad(self, tokens, d_token, d_entropy, axis)
 
     def rename(self, old: str, new: str) -> "Value":
         return self.builder.rename_axis(self, old, new)
@@ -474,6 +484,57 @@ class Mx4:
         """Sum over the blocked axis of both, which is one axis: [rows of self, rows of rhs], summed in f32 and rounded to
         nearest even."""
         return self.codes.builder.contract_mx4(self, rhs, dtype)
+
+
+@dataclass(frozen=True)
+class Rotation:
+    """How the heads of a token turn with its position: pair i of a head's first 2 n dims by the angle position *
+    frequencies[i]. ``positions`` i32 [token ..], or i32 [token .., axis] with ``axes`` i32 [pair], the position that each pair goes by
+    (outside those there are: the pair does not turn); ``frequencies`` f32 [pair], n of them. Pair i is dims i and n + i
+    (``layout`` "halves") or 2 i and 2 i + 1 ("neighbours"). Angles are formed in 64 bits."""
+    positions: Value
+    frequencies: Value
+    axes: Optional[Value] = None
+    layout: str = "halves"
+
+
+@dataclass(frozen=True)
+class HeadNorm:
+    """The norm of each head before it turns: x / sqrt(mean(x^2) + eps) * gain, with gains [dim] for queries and for keys."""
+    query_gain: Value
+    key_gain: Value
+    eps: float = 1e-6
+
+
+@dataclass(frozen=True)
+class LogProbs:
+    """Of each row of logits: the log probability of the given token, the entropy, and the ``top`` largest log probabilities in
+    descending order with their tokens (none where they were not asked for)."""
+    token: Value
+    entropy: Value
+    top: Optional[Value] = None
+    top_tokens: Optional[Value] = None
+
+
+@dataclass(frozen=True)
+class ForkedPages:
+    """Page tables for the next step (``Builder.fork_pages``): ``pages`` i32 [row, slot], ``lengths`` i32 [row], the page that
+    each row copies (``source``) and to which (``target``), i32 [row], -1 for none, and ``left`` i32 [], the free pages left (below
+    zero: so many were asked for in vain)."""
+    pages: Value
+    lengths: Value
+    source: Value
+    target: Value
+    left: Value
+
+
+@dataclass(frozen=True)
+class CompactedPages:
+    """Tables with their pages moved to the lowest numbers (``Builder.compact_pages``): ``pages`` as the tables, and the moves,
+    from ``source`` to ``target``, i32 [move], -1 for none."""
+    pages: Value
+    source: Value
+    target: Value
 
 
 def mx4_specs(axis: str, *dims: Dim, **named: int) -> Tuple[Spec, Spec]:
@@ -1074,13 +1135,17 @@ class Builder:
             raise TensorError("DTypeMismatch", "slots are i32")
         return self._mx4_call(name, [cache, slots], dtype, slots.ty.dims + (cache.ty.dims[1], dim))
 
-    def attend_mx4(self, q: Value, cache: Value, pages: Value, lengths: Value) -> Value:
+    def attend_mx4(self, q: Value, cache: Value, pages: Value, lengths: Value, shared: Optional[Sequence[Value]] = None) -> Value:
         """softmax(q . k / sqrt(dim)) v over a paged cache, for the newest queries of each sequence.
 
         ``q`` [seq, head, dim] or [seq, query, head, dim]; ``pages`` i32 [seq, page slot]: key j of a sequence is row j % page
         size of page pages[j / page size]; ``lengths`` i32 [seq]: keys of each sequence, the new tokens' among them (at most
         what its pages hold). The last query sees all of them, each one before it one fewer. Query head h reads key-value
-        head h / (heads / kv_heads). Page numbers outside the cache hold no keys; a query that sees none gives 0."""
+        head h / (heads / kv_heads). Page numbers outside the cache hold no keys; a query that sees none gives 0.
+
+        ``shared`` (pages i32 [prefix, page slot], lengths i32 [prefix], of i32 [seq]): keys that several sequences have before
+        their own, each prefix read and computed once for all of its sequences. Sequence b's is prefix of[b]; outside those there are, it
+        has none. Every query of a sequence sees all of its prefix, and of its own keys what it sees without one."""
         for x in (q, pages, lengths):
             self._ensure(x)
         self._mx4_float(q.ty.dtype)
@@ -1095,7 +1160,186 @@ class Builder:
             raise TensorError("DTypeMismatch", "pages and lengths are i32")
         if pages.ty.rank != 2 or pages.ty.dims[0] != q.ty.dims[0] or lengths.ty.dims != q.ty.dims[:1]:
             raise TensorError("ShapeMismatch", "pages are [seq, page], lengths [seq]")
-        return self._mx4_call("attend", [q, cache, pages, lengths], q.ty.dtype, q.ty.dims)
+        if shared is None:
+            return self._mx4_call("attend", [q, cache, pages, lengths], q.ty.dtype, q.ty.dims)
+        if len(shared) != 3:
+            raise TensorError("InvalidDimension", "shared keys are (pages, lengths, of)")
+        for x in shared:
+            self._ensure(x)
+            if x.ty.dtype != "i32":
+                raise TensorError("DTypeMismatch", "pages, lengths and prefixes are i32")
+        if shared[0].ty.rank != 2 or shared[1].ty.dims != shared[0].ty.dims[:1] or shared[2].ty.dims != q.ty.dims[:1]:
+            raise TensorError("ShapeMismatch", "shared pages are [prefix, page], their lengths [prefix], of [seq]")
+        return self._mx4_call("attend_shared", [q, cache, self._group(pages, lengths), self._group(*shared)], q.ty.dtype, q.ty.dims)
+
+    # -- heads, pages and log probabilities: custom calls that the gfx950 target runs --
+
+    def _group(self, *operands: Value) -> Value:
+        """Several operands as one of a custom call, which takes four: a call of their own that computes nothing."""
+        return self.custom_call("accy.group", 1, operands, Type("i1", ()))
+
+    def _rotation(self, q: Value, k: Value, rotation: Rotation, norm: Optional[HeadNorm]) -> Tuple[str, List[Value]]:
+        """The calls' suffix and last operands, checked against queries [token .., head, dim] and keys [token .., kv_head, dim]."""
+        for x in (q, k, rotation.positions, rotation.frequencies):
+            self._ensure(x)
+        self._mx4_float(q.ty.dtype)
+        if k.ty.dtype != q.ty.dtype:
+            raise TensorError("DTypeMismatch", "queries and keys of one type")
+        if q.ty.rank < 2 or k.ty.rank != q.ty.rank:
+            raise TensorError("RankMismatch", "heads are [token .., head, dim]")
+        tokens = q.ty.dims[:-2]
+        if k.ty.dims[:-2] != tokens or k.ty.dims[-1] != q.ty.dims[-1]:
+            raise TensorError("ShapeMismatch", "queries and keys of the same tokens and dims")
+        positions, frequencies, axes = rotation.positions.ty, rotation.frequencies.ty, rotation.axes
+        dim = q.ty.dims[-1][1]
+        if rotation.layout not in ("halves", "neighbours"):
+            raise TensorError("InvalidDimension", f"{rotation.layout}: halves or neighbours")
+        if positions.dtype != "i32" or frequencies.dtype != "f32":
+            raise TensorError("DTypeMismatch", "positions are i32, frequencies f32")
+        if frequencies.rank != 1 or not 1 <= frequencies.shape[0] or 2 * frequencies.shape[0] > dim or not 2 <= dim <= 512:
+            raise TensorError("InvalidDimension", f"one to dim / 2 frequencies, dims up to 512: {frequencies.shape} of {dim}")
+        if axes is None:
+            if positions.dims != tokens:
+                raise TensorError("ShapeMismatch", "a position for every token")
+        else:
+            self._ensure(axes)
+            if axes.ty.dtype != "i32":
+                raise TensorError("DTypeMismatch", "axes are i32")
+            if positions.dims[:-1] != tokens or positions.rank != len(tokens) + 1 or axes.ty.dims != frequencies.dims:
+                raise TensorError("ShapeMismatch", "positions are [token .., axis], axes as the frequencies")
+        last = [self._group(rotation.positions, rotation.frequencies, *([axes] if axes is not None else []))]
+        if norm is not None:
+            for g in (norm.query_gain, norm.key_gain):
+                self._ensure(g)
+                if g.ty.dtype not in (q.ty.dtype, "f32"):
+                    raise TensorError("DTypeMismatch", f"gains are {q.ty.dtype} or f32")
+                if g.ty.shape != (dim,):
+                    raise TensorError("ShapeMismatch", "gains are [dim]")
+            if norm.query_gain.ty.dtype != norm.key_gain.ty.dtype:
+                raise TensorError("DTypeMismatch", "gains of one type")
+            last.append(self._group(norm.query_gain, norm.key_gain, self.full_float(Type("f32", ()), norm.eps)))
+        return ("" if rotation.layout == "halves" else "_neighbours"), last
+
+    def rotate_heads(self, q: Value, k: Value, rotation: Rotation, norm: Optional[HeadNorm] = None) -> Tuple[Value, Value]:
+        """Queries [token .., head, dim] and keys [token .., kv_head, dim] of a model's tokens as its attention takes them: each head
+        normalised (with ``norm``) and turned by its token's position, both in one kernel; rounded once, to nearest even."""
+        suffix, last = self._rotation(q, k, rotation, norm)
+        return tuple(self.custom_call(f"accy.heads.{name}{suffix}", 1, [q, k] + last, x.ty) for name, x in (("queries", q), ("keys", k)))
+
+    def rotate_heads_grad(self, dq: Value, dk: Value, q: Value, k: Value, rotation: Rotation, norm: Optional[HeadNorm] = None) -> Tuple[Value, ...]:
+        """The gradient of ``rotate_heads`` at q and k for the gradients dq, dk of its results: of q and k, and with ``norm`` of the
+        query and key gains (in the gains' type). Sums over tokens and heads are taken in one order, call for call."""
+        for x in (dq, dk):
+            self._ensure(x)
+        _same_type(dq.ty, q.ty)
+        _same_type(dk.ty, k.ty)
+        suffix, last = self._rotation(q, k, rotation, norm)
+        operands = [self._group(dq, dk), self._group(q, k)] + last
+        results = [("d_queries", q.ty), ("d_keys", k.ty)]
+        if norm is not None:
+            results += [("d_query_gain", norm.query_gain.ty), ("d_key_gain", norm.key_gain.ty)]
+        return tuple(self.custom_call(f"accy.heads.{name}{suffix}", 1, operands, ty) for name, ty in results)
+
+    def _table(self, table: Value, held: Value) -> None:
+        for x in (table, held):
+            self._ensure(x)
+        if table.ty.dtype != "i32" or held.ty.dtype != "i1":
+            raise TensorError("DTypeMismatch", "page tables are i32, held pages i1")
+        if table.ty.rank != 2 or held.ty.rank != 1:
+            raise TensorError("RankMismatch", "page tables are [seq, slot], held pages [page]")
+
+    def fork_pages(self, table: Value, lengths: Value, parents: Value, room: Value, held: Value, page: int) -> ForkedPages:
+        """The page tables of the next step's rows, from those of this step's sequences.
+
+        ``table`` i32 [seq, slot] and ``lengths`` i32 [seq] as in ``attend_mx4``; row r goes on as sequence parents[r] (i32 [row];
+        several rows with one parent: forked; outside those there are: the row is empty) and gets pages for room[r] (i32 [row]) more tokens,
+        as far as the table has slots. The pages that hold a sequence's tokens are shared by its rows; only a
+        last page that is partly filled belongs to one row alone: the first that has it keeps it, unless another row has it filled further than its
+        last place or it is held, and every other copies it to a page of its own (``source``, ``target``: for
+        ``copy_pages``). Free are the pages that no row keeps and that are not ``held`` (i1 [page]); they are given out in
+        ascending order, row by row, a row's copy before the pages to come. -1 stands for no page: past a row's pages, and where
+        none was free. ``page`` is the tokens of a page."""
+        self._table(table, held)
+        for x in (lengths, parents, room):
+            self._ensure(x)
+            if x.ty.dtype != "i32":
+                raise TensorError("DTypeMismatch", "lengths, parents and room are i32")
+            if x.ty.rank != 1:
+                raise TensorError("RankMismatch", "lengths are [seq], parents and room [row]")
+        if lengths.ty.dims != table.ty.dims[:1] or room.ty.dims != parents.ty.dims:
+            raise TensorError("ShapeMismatch", "lengths are [seq], room as parents")
+        if not 1 <= page < 1 << 20:
+            raise TensorError("InvalidDimension", f"{page} tokens to a page")
+        row, slot = parents.ty.dims[0], table.ty.dims[1]
+        # the size of a page as an operand, since a call has no other place for it
+        operands = [self._group(table, lengths), self._group(parents, room), held, self.full("i32", page)]
+        one = lambda name, *dims: self.custom_call(f"accy.pages.fork_{name}", 1, operands, Type("i32", tuple(dims)))
+        return ForkedPages(one("table", row, slot), one("lengths", row), one("source", row), one("target", row), one("left"))
+
+    def compact_pages(self, table: Value, held: Value, moves: Dim) -> CompactedPages:
+        """Tables whose pages lie together at the lowest numbers. Of n pages that a table names or that are ``held``, those from n on that are
+        not held move, in ascending order, to the free ones below n, as many as ``moves`` (its name and extent) has places for; what the
+        tables name is renumbered, what is no page becomes -1."""
+        self._table(table, held)
+        if not 0 <= moves[1] <= held.ty.shape[0]:
+            raise TensorError("InvalidDimension", f"{moves[1]} moves of {held.ty.shape[0]} pages")
+        one = lambda name, dims: self.custom_call(f"accy.pages.compact_{name}", 1, [table, held], Type("i32", dims))
+        return CompactedPages(one("table", table.ty.dims), one("source", (moves,)), one("target", (moves,)))
+
+    def copy_pages(self, cache: Value, source: Value, target: Value) -> Value:
+        """The cache [page, ..], of any type, with page target[i] a copy of what page source[i] held before (i32 [copy] both). A copy
+        from or to no page is none, and of two copies to one page the later one counts. Where the cache is a parameter that nothing else reads and
+        the result an output, a launch may bind both to one buffer, which is then updated in place."""
+        for x in (cache, source, target):
+            self._ensure(x)
+        if source.ty.dtype != "i32" or target.ty.dtype != "i32":
+            raise TensorError("DTypeMismatch", "pages are i32")
+        if cache.ty.rank == 0 or source.ty.rank != 1:
+            raise TensorError("RankMismatch", "caches are [page, ..], copies [copy]")
+        if source.ty.shape != target.ty.shape:
+            raise TensorError("ShapeMismatch", "a target for every source")
+        return self.custom_call("accy.pages.copy", 1, [cache, source, target], cache.ty)
+
+    def _logits(self, logits: Value, tokens: Value, axis: str) -> Tuple[Dim, ...]:
+        for x in (logits, tokens):
+            self._ensure(x)
+        self._mx4_float(logits.ty.dtype)
+        i = _find(logits.ty.dims, axis)
+        if i is None:
+            raise TensorError("AxisNotFound", axis)
+        if i != logits.ty.rank - 1:
+            raise TensorError("InvalidPermutation", f"{axis} is not the last axis")
+        if tokens.ty.dtype != "i32":
+            raise TensorError("DTypeMismatch", "tokens are i32")
+        if tokens.ty.dims != logits.ty.dims[:-1]:
+            raise TensorError("ShapeMismatch", "a token for every row of logits")
+        if not 1 <= logits.ty.shape[-1] < 1 << 30:
+            raise TensorError("InvalidDimension", axis)
+        return tokens.ty.dims
+
+    def log_probs(self, logits: Value, tokens: Value, axis: str, top: int = 0) -> LogProbs:
+        """log softmax of logits [row .., axis] at tokens i32 [row ..] (0 for a token outside the axis: padding), the entropy -sum p
+        log p of each row, and the ``top`` (up to 64) largest log probabilities with their tokens, ties to the lowest; all f32, in one pass over
+        the logits. Logits of -inf are masked: they weigh nothing, and a row of nothing else has log probabilities of -inf and the entropy 0. A
+        row with a NaN or an infinity has NaN for all of them; a NaN is no alternative (token -1 where fewer are left)."""
+        rows = self._logits(logits, tokens, axis)
+        if not 0 <= top <= min(64, logits.ty.shape[-1]):
+            raise TensorError("InvalidDimension", f"{top} alternatives")
+        one = lambda name, dtype, dims: self.custom_call(f"accy.logits.{name}", 1, [logits, tokens], Type(dtype, dims))
+        first = one("token", "f32", rows), one("entropy", "f32", rows)
+        if not top:
+            return LogProbs(*first)
+        dims = rows + (("top", top),)
+        return LogProbs(*first, one("top", "f32", dims), one("top_tokens", "i32", dims))
+
+    def log_probs_grad(self, logits: Value, tokens: Value, d_token: Value, d_entropy: Value, axis: str) -> Value:
+        """The gradient with respect to the logits of ``log_probs`` for the gradients (f32 [row ..]) of the tokens' log probabilities and of
+        the entropies. 0 where a logit is -inf, but for that of a token; a token outside the axis counts for nothing."""
+        rows = self._logits(logits, tokens, axis)
+        for x in (d_token, d_entropy):
+            self._ensure(x)
+            _same_type(x.ty, Type("f32", rows))
+        return self.custom_call("accy.logits.grad", 1, [logits, tokens, d_token, d_entropy], logits.ty)
 
     def scan(self, length: int, inits: Sequence[Value], body: Callable[["Builder", List[Value]], Sequence[Value]]) -> Value:
         """Repeat ``body`` ``length`` times carrying ``inits`` (builder.zig:899-990)."""
