@@ -1,8 +1,8 @@
 // Log probabilities of given tokens, entropies and the top alternatives of rows of logits, and the gradient.
 //
-// With m a row's maximum, y = (x - m) log2 e, l = sum 2^y and s = sum 2^y y: log p = (y - log2 l) ln 2, and the entropy is (log2 l - s /
-// l) ln 2. One pass over the row gives l, s and the alternatives: each thread keeps a maximum of its own elements, lets it follow only where
-// a batch of them has a larger one, and the threads' (m, l, s) are joined at the end. That is a conversion, a maximum, a multiply-add, an
+// With m near a row's maximum, y = (x - m) log2 e, l = sum 2^y and s = sum 2^y y: log p = (y - log2 l) ln 2, and the entropy is (log2 l - s /
+// l) ln 2. One pass over the row gives l, s and the alternatives: each thread measures from an m of its own, the maximum of its first chunk,
+// and the threads' (m, l, s) are joined at the end, measured from the row's maximum. That is a conversion, half a maximum, a multiply-add, an
 // exponential and two more operations an element, about what HBM delivers one in; so the alternatives have to come almost free.
 //
 // Alternatives: an element is compared with a bound below the row's K-th largest only where its batch's maximum reaches the bound. After the first
@@ -11,10 +11,11 @@
 // keys differ and ties go to the lowest index. A list that is full raises the bound to its own K-th key and the batch is taken
 // again (equal or ascending logits do that, a few times); at the end the keys of the list are ranked against each other.
 //
-// Rows start anywhere: chunks of 16 bytes are read on their own grid, and what lies before or after the row is masked.
+// Rows start anywhere: whole chunks of 16 bytes are read on their own grid, and the few elements before the first and after the last one
+// are a lane's each.
 //
 // C supplies DT (0 bf16, 1 f16, 2 f32), ROWS, V (elements of a row), K (alternatives, 0: none), SPLITS (workgroups of a row), NT (threads), U
-// (chunks that a thread has on their way at once).
+// (chunks that a thread holds at once).
 #pragma once
 
 namespace accy {
@@ -31,78 +32,79 @@ constexpr float LEAST = -200.0f;
 
 template <class C> struct Chunks {
   static constexpr int SIZE = C::DT == 2 ? 4 : 2, PER = 16 / SIZE;  // elements of a chunk
-  static constexpr long TOTAL = C::ROWS * C::V;
 };
 
-// The elements of a chunk as f32; those of another row are -inf, which weighs nothing.
+// The elements of a chunk as f32.
 template <class C> __device__ __forceinline__ void widen(const u32x4& w, float (&x)[Chunks<C>::PER]) {
-  if constexpr (C::DT == 2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const u32_t bits = w[i];  // (a vector's element is no object to cast the bits of)
-      x[i] = __builtin_bit_cast(float, bits);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = C::DT == 0 ? bf16_of(w[i >> 1], i) : f16_of(w[i >> 1], i);
+  for (int i = 0; i < Chunks<C>::PER; ++i) {
+    const u32_t bits = w[C::DT == 2 ? i : i >> 1];  // (a vector's element is no object to cast the bits of)
+    x[i] = C::DT == 2 ? __builtin_bit_cast(float, bits) : C::DT == 0 ? bf16_of(bits, i) : f16_of(bits, i);
   }
 }
 
-// Chunk c (of the whole buffer), of which the row has elements lo .. hi - 1; a chunk that the buffer ends in is read element by element.
-template <class C>
-__device__ __forceinline__ u32x4 read(const typename Elem<C::DT>::type* __restrict__ x, long c) {
-  typedef Chunks<C> K;
-  if (K::TOTAL % K::PER == 0 || (c + 1) * K::PER <= K::TOTAL) return *(const u32x4*)(x + c * K::PER);
-  u32x4 w = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < K::PER; ++i) {
-    if (c * K::PER + i >= K::TOTAL) continue;
-    if constexpr (C::DT == 2) w[i] = __builtin_bit_cast(u32_t, x[c * K::PER + i]);
-    else w[i >> 1] |= (u32_t)x[c * K::PER + i] << (16 * (i & 1));
-  }
-  return w;
+template <int DT> __device__ __forceinline__ float value(typename Elem<DT>::type e) {
+  if constexpr (DT == 2) return e;
+  else return DT == 0 ? bf16_to_f32(e) : f16_to_f32(e);
 }
 
-// The part of a row that belongs to split z: elements first .. end - 1 of the buffer, chunks c0 .. c1 - 1.
-struct Range {
-  long first, end, c0, c1;
+// The part of a row that belongs to split z: chunks from .. to - 1, counted from element `at` of the buffer, which `base` points to, and the
+// elements besides, `head` before the row's first whole chunk and `tail` after its last one, counted the same way. The row begins at element `lead`.
+template <class C> struct Range {
+  const typename Elem<C::DT>::type* base;
+  long at;
+  int from, to, lead, head, tail, after;
+  // The element of this thread of those besides, or -1.
+  __device__ __forceinline__ int besides() const {
+    const int i = (int)threadIdx.x;
+    return i < head ? lead + i : i < head + tail ? after + i - head : -1;
+  }
 };
-template <class C> __device__ __forceinline__ Range range_of(long row, int z) {
-  typedef Chunks<C> K;
-  const long begin = row * C::V, finish = begin + C::V, a = begin / K::PER, b = (finish + K::PER - 1) / K::PER;
-  const long per = ((b - a) + C::SPLITS - 1) / C::SPLITS;
-  Range r;
-  r.c0 = a + z * per < b ? a + z * per : b;
-  r.c1 = r.c0 + per < b ? r.c0 + per : b;
-  r.first = r.c0 * K::PER > begin ? r.c0 * K::PER : begin;
-  r.end = r.c1 * K::PER < finish ? r.c1 * K::PER : finish;
+template <class C> __device__ __forceinline__ Range<C> range_of(const typename Elem<C::DT>::type* x, long row, int z) {
+  constexpr int PER = Chunks<C>::PER;
+  const long begin = row * C::V;
+  Range<C> r;
+  r.at = begin / PER * PER;
+  r.base = x + r.at;
+  r.lead = (int)(begin - r.at);
+  const int end = r.lead + (int)C::V, first = (r.lead + PER - 1) / PER, last = end / PER > first ? end / PER : first;
+  const int per = (last - first + C::SPLITS - 1) / C::SPLITS;
+  r.from = first + z * per < last ? first + z * per : last;
+  r.to = r.from + per < last ? r.from + per : last;
+  r.after = last * PER;
+  r.head = z == 0 ? (first * PER < end ? first * PER : end) - r.lead : 0;
+  r.tail = z == C::SPLITS - 1 && end > r.after ? end - r.after : 0;
   return r;
 }
-template <class C> __device__ __forceinline__ void mask(const Range& r, long c, float (&x)[Chunks<C>::PER]) {
-  constexpr int PER = Chunks<C>::PER;
-  if (c * PER >= r.first && (c + 1) * PER <= r.end) return;
+// f(0), .., f(N - 1) with numbers that are constants from the start: an array that they index is registers, whatever stands between.
+template <int I> struct Index { static constexpr int value = I; };
+template <int N, class F> __device__ __forceinline__ void each(F f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(Index<N - 1>());
+  }
+}
+// Keeps the compiler from carrying widened elements from one pass over to the next in twice the registers.
+__device__ __forceinline__ void opaque(u32x4& w) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if (c * PER + i < r.first || c * PER + i >= r.end) x[i] = -__builtin_inff();
+  for (int i = 0; i < 4; ++i) {
+    u32_t x = w[i];
+    asm("" : "+v"(x));
+    w[i] = x;
+  }
 }
 
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
-// A thread's, or a range's: its maximum, and sums of 2^y and of 2^y y with y measured from that maximum.
+// A thread's, or a range's: sums of 2^y and of 2^y y with y measured from m, a maximum or near one.
 struct Sums {
   float m = -__builtin_inff(), l = 0.0f, s = 0.0f;
-  // The same measured from a maximum that is no smaller.
+  // The same measured from another m.
   __device__ __forceinline__ void rebase(float to) {
     const float shift = fmaxf((base_of(m) - base_of(to)) * L2E, LEAST), scale = __builtin_amdgcn_exp2f(l == 0.0f ? LEAST : shift);
     s = (s + l * shift) * scale;
     l *= scale;
     m = to;
-  }
-  // An element; base: base_of(m).
-  __device__ __forceinline__ void add(float x, float base) {
-    const float y = (x - base) * L2E, e = __builtin_amdgcn_exp2f(y);
-    l += e;
-    s = __builtin_fmaf(e, fmaxf(y, LEAST), s);
   }
   __device__ __forceinline__ void join(Sums o) {
     const float top = fmaxf(m, o.m);
@@ -113,6 +115,79 @@ struct Sums {
   }
 };
 
+// Of a thread's U chunks, `first` its first one, those before `to`.
+template <class C> __device__ __forceinline__ int present(int first, int to) {
+  const int n = (to - first + C::NT - 1) / C::NT;
+  return first >= to ? 0 : n < C::U ? n : C::U;
+}
+// Chunk c from `base`, a whole workgroup's: a row's bytes are counted in 32 bits.
+template <class C> __device__ __forceinline__ const u32x4& chunk(const typename Elem<C::DT>::type* base, int c) { return *(const u32x4*)((const u8_t*)base + (u32_t)c * 16u); }
+template <class C> __device__ __forceinline__ void fetch(const Range<C>& r, int first, int n, u32x4 (&w)[C::U]) {
+  each<C::U>([&](auto u) {
+    if (u.value < n) w[u.value] = chunk<C>(r.base, first + u.value * C::NT);
+  });
+}
+template <class C> __device__ __forceinline__ float largest(const u32x4& w) {
+  float top = -__builtin_inff(), v[Chunks<C>::PER];
+  widen<C>(w, v);
+#pragma unroll
+  for (int i = 0; i < Chunks<C>::PER; ++i) top = fmaxf(top, v[i]);
+  return top;
+}
+// One element, with care: the sums of it alone.
+__device__ __forceinline__ Sums sums_of(float x) {
+  Sums a;
+  a.m = fmaxf(x, a.m);
+  const float y = (x - base_of(a.m)) * L2E;
+  a.l = __builtin_amdgcn_exp2f(y);
+  a.s = a.l * fmaxf(y, LEAST);
+  return a;
+}
+// The first n of U chunks added to the sums; `top` becomes their maximum. They are widened once: y is measured from the m that there is, that of the
+// first chunk to begin with. Where an element lies 32 above it, or a masked one makes the quick sum of 2^y y a NaN, or m log2 e might
+// be beyond f32, they are added again with care. Returns whether they were.
+template <class C> __device__ __forceinline__ bool add(Sums& a, const u32x4 (&w)[C::U], int n, float& top) {
+  top = -__builtin_inff();
+  if (n <= 0) return false;
+  if (a.l == 0.0f) a.m = largest<C>(w[0]);
+  const float base = base_of(a.m), from = base * L2E;
+  float v[Chunks<C>::PER], dl = 0.0f, ds = 0.0f;
+  each<C::U>([&](auto u) {
+    if (u.value >= n) return;
+    widen<C>(w[u.value], v);
+#pragma unroll
+    for (int i = 0; i < Chunks<C>::PER; ++i) top = fmaxf(top, v[i]);
+#pragma unroll
+    for (int i = 0; i < Chunks<C>::PER; ++i) {
+      const float y = __builtin_fmaf(v[i], L2E, -from), e = __builtin_amdgcn_exp2f(y);
+      dl += e;
+      ds = __builtin_fmaf(e, y, ds);
+    }
+  });
+  const bool care = !(ds == ds) || !(__builtin_fabsf(base) < 0x1p+125f) || top - base > 32.0f;
+  if (care) {
+    asm volatile("");  // (a branch: computed either way it would cost as much again)
+    if (top > a.m) a.rebase(top);
+    const float base = base_of(a.m);
+    dl = ds = 0.0f;
+    each<C::U>([&](auto u) {
+      if (u.value >= n) return;
+      u32x4 again = w[u.value];
+      opaque(again);
+      widen<C>(again, v);
+#pragma unroll
+      for (int i = 0; i < Chunks<C>::PER; ++i) {
+        const float y = (v[i] - base) * L2E, e = __builtin_amdgcn_exp2f(y);
+        dl += e;
+        ds = __builtin_fmaf(e, fmaxf(y, LEAST), ds);
+      }
+    });
+  }
+  a.l += dl;
+  a.s += ds;
+  return care;
+}
+
 // The order of values, in the order of unsigned numbers: +0 and -0 are one, NaN is below all.
 __device__ __forceinline__ u32_t order(float x) {
   const u32_t b = __builtin_bit_cast(u32_t, x + 0.0f);
@@ -121,12 +196,16 @@ __device__ __forceinline__ u32_t order(float x) {
 __device__ __forceinline__ float value_of(u32_t o) { return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ u64_t key_of(float x, u32_t index) { return (u64_t)order(x) << 32 | (u32_t)~index; }
 
-// The list of a workgroup: up to CAP keys, in no order. Below the bound nothing is of interest.
+// The list of a workgroup: up to CAP keys, in no order.
 template <class C> struct List {
   static constexpr int CAP = C::K > 0 ? 1024 : 1, BEST = C::K > 0 ? C::K : 1;
-  u64_t key[CAP], best[BEST], bound;
-  u32_t share[C::NT / 64];
-  int count;
+  u64_t key[CAP], best[BEST];
+  // What up to LAID lanes of each wave lay out for the others: their chunks, which lane it is and how many chunks it has.
+  static constexpr int LAID = C::K > 0 ? 16 : 1;
+  u32x4 chunk[C::NT / 64][LAID][C::U];
+  int who[C::NT / 64][LAID];
+  u32_t share[2][C::NT / 64];
+  int count[3];
 
   // The K largest of the first n keys to `best`, in order; what is missing is 0. All threads.
   __device__ void rank(int n) {
@@ -142,146 +221,172 @@ template <class C> struct List {
   }
 };
 
-// One range: sums of all of its elements, and its K largest keys in list.best.
-template <class C>
-__device__ __forceinline__ Sums scan(const typename Elem<C::DT>::type* __restrict__ x, const Range r, long begin, List<C>& list) {
-  typedef Chunks<C> CH;
-  constexpr int PER = CH::PER, WAVES = C::NT / 64;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  Sums a;
-  if constexpr (C::K > 0) {
-    if (tid == 0) {
-      list.bound = 1ull << 32;  // everything but NaN
-      list.count = 0;
-    }
-    __syncthreads();
-  }
-  bool first = true;
-  for (long c0 = r.c0; c0 < r.c1; c0 += C::NT * C::U) {
-    u32x4 w[C::U];
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int u = 0; u < C::U; ++u) {
-      const long c = c0 + u * C::NT + tid;
-      if (c < r.c1) w[u] = read<C>(x, c);
-    }
-#pragma unroll
-    for (int u = 0; u < C::U; ++u) {
-      const long c = c0 + u * C::NT + tid;
-      if (c >= r.c1) continue;
-      float v[PER];
-      widen<C>(w[u], v);
-      mask<C>(r, c, v);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) top = fmaxf(top, v[i]);
-    }
-    if (top > a.m) a.rebase(top);
-    const float base = base_of(a.m);
-#pragma unroll
-    for (int u = 0; u < C::U; ++u) {
-      const long c = c0 + u * C::NT + tid;
-      if (c >= r.c1) continue;
-      float v[PER];
-      widen<C>(w[u], v);
-      mask<C>(r, c, v);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) a.add(v[i], base);
-    }
-    if constexpr (C::K > 0) {
-      if (first) {
-        first = false;
-        // The largest 16 bits that a share of this wave's lanes reach.
-        constexpr int SHARE = (C::K + WAVES - 1) / WAVES;
-        const u32_t mine = order(top) >> 16;
-        u32_t least = 0;
-        for (u32_t bit = 1u << 15; bit; bit >>= 1)
-          if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(mine >= (least | bit))) >= SHARE) least |= bit;
-        if (lane == 0) list.share[wave] = least;
-        __syncthreads();
-        if (tid == 0) {
-          u32_t b = list.share[0];
-          for (int i = 1; i < WAVES; ++i) b = b < list.share[i] ? b : list.share[i];
-          if (b > 0) list.bound = (u64_t)b << 48;
-        }
-        __syncthreads();
-      }
-      int before = list.count;
-      __syncthreads();
-      for (;;) {
-        const u64_t bound = list.bound;
-        if (order(top) >= (u32_t)(bound >> 32)) {
-#pragma unroll
-          for (int u = 0; u < C::U; ++u) {
-            const long c = c0 + u * C::NT + tid;
-            if (c >= r.c1) continue;
-            float v[PER];
-            widen<C>(w[u], v);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              const long at = c * PER + i;
-              const u64_t key = key_of(v[i], (u32_t)(at - begin));
-              if (key >= bound && at >= r.first && at < r.end) {
-                const int place = atomicAdd(&list.count, 1);
-                if (place < List<C>::CAP) list.key[place] = key;
-              }
-            }
-          }
-        }
-        __syncthreads();
-        const int found = list.count;
-        if (found <= List<C>::CAP) break;
-        // Full: its K-th key bounds the range's. Of what was there before the batch the keys that reach it stay, K at most, and the
-        // batch is taken again. (CAP different keys reach the old bound and K of them the new one, so that it rises by CAP - K keys every time.)
-        list.rank(List<C>::CAP);
-        const u64_t higher = list.best[C::K - 1];
-        u64_t kept[List<C>::CAP / C::NT];
-#pragma unroll
-        for (int i = 0; i < List<C>::CAP / C::NT; ++i) kept[i] = i * C::NT + tid < before ? list.key[i * C::NT + tid] : 0;
-        __syncthreads();
-        if (tid == 0) {
-          list.bound = higher;
-          list.count = 0;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < List<C>::CAP / C::NT; ++i)
-          if (kept[i] >= higher) list.key[atomicAdd(&list.count, 1)] = kept[i];
-        __syncthreads();
-        before = list.count;
-        __syncthreads();
-      }
-    }
-  }
-  if constexpr (C::K > 0) {
-    __syncthreads();
-    list.rank(list.count);
-  }
-  // the threads' sums
-  __shared__ float lds[WAVES][3];
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    Sums b;
-    b.m = __shfl_xor(a.m, o, 64);
-    b.l = __shfl_xor(a.l, o, 64);
-    b.s = __shfl_xor(a.s, o, 64);
-    a.join(b);
-  }
+// The threads' sums, and whether any of them took care: the same in all of them.
+// peak: a thread's maximum.
+template <int WAVES> __device__ __forceinline__ Sums join_threads(Sums a, float peak, bool& care, float (&lds)[WAVES][4]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  a.rebase(wave_reduce(peak, MaxOp()));
+  a.l = wave_reduce(a.l, SumOp());
+  a.s = wave_reduce(a.s, SumOp());
   if (lane == 0) {
     lds[wave][0] = a.m;
     lds[wave][1] = a.l;
     lds[wave][2] = a.s;
   }
+  const bool any = __builtin_amdgcn_ballot_w64(care) != 0;
+  if (lane == 0) lds[wave][3] = any ? 1.0f : 0.0f;
   __syncthreads();
-  a = Sums();
+  // A wave's lanes take a wave's sums each.
+  const int from = lane % WAVES;
+  a.m = lds[from][0];
+  a.l = lds[from][1];
+  a.s = lds[from][2];
+  care = __builtin_amdgcn_ballot_w64(lds[from][3] != 0.0f) != 0;
+  float top = a.m;
 #pragma unroll
-  for (int i = 0; i < WAVES; ++i) {
-    Sums b;
-    b.m = lds[i][0];
-    b.l = lds[i][1];
-    b.s = lds[i][2];
-    a.join(b);
+  for (int o = 1; o < WAVES; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  a.rebase(top);
+#pragma unroll
+  for (int o = 1; o < WAVES; o <<= 1) {
+    a.l += __shfl_xor(a.l, o, 64);
+    a.s += __shfl_xor(a.s, o, 64);
   }
   return a;
+}
+
+// The largest 16 bits that the wave's share of K lanes reach with their maxima.
+template <class C> __device__ __forceinline__ u32_t share_of(float top) {
+  constexpr int SHARE = (C::K + C::NT / 64 - 1) / (C::NT / 64);
+  const u32_t mine = order(top) >> 16;
+  u32_t least = 0;
+#pragma unroll
+  for (u32_t bit = 1u << 15; bit; bit >>= 1)
+    if (__builtin_popcountll(__builtin_amdgcn_uicmp(mine, least | bit, 35)) >= SHARE) least |= bit;  // lanes of mine >= ..
+  return least;
+}
+// The bound that all waves' shares reach together.
+template <class C> __device__ __forceinline__ u64_t bound_of(const u32_t (&share)[C::NT / 64]) {
+  u32_t b = share[0];
+#pragma unroll
+  for (int i = 1; i < C::NT / 64; ++i) b = b < share[i] ? b : share[i];
+  return b > 0 ? (u64_t)b << 48 : 1ull << 32;  // (anything but NaN)
+}
+
+// One range: sums of all of its elements, and its K largest keys in list.best. The next batch is on its way while one is worked on.
+template <class C>
+__device__ __forceinline__ Sums scan(const Range<C> r, List<C>& list) {
+  constexpr int PER = Chunks<C>::PER, WAVES = C::NT / 64;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  auto keep = [&](float v, int at, u64_t bound, int had, int turn) {
+    const u64_t key = key_of(v, (u32_t)(at - r.lead));
+    if (key < bound) return;
+    const int place = had + atomicAdd(&list.count[turn], 1);
+    if (place < List<C>::CAP) list.key[place] = key;
+  };
+  u32x4 next[C::U];
+  fetch<C>(r, r.from + tid, present<C>(r.from + tid, r.to), next);
+  const int besides = r.besides();
+  float x = 0.0f, peak = -__builtin_inff();
+  Sums a;
+  if (besides >= 0) {
+    x = value<C::DT>(r.base[besides]);
+    a = sums_of(x);
+    peak = fmaxf(peak, x);
+  }
+  if constexpr (C::K > 0) {
+    if (tid < 3) list.count[tid] = 0;
+    __syncthreads();
+  }
+  // Of the list: what is in it after the last batch, and the bound that keys have to reach; batch: counted from 0 and, in turns of three,
+  // whose counter is in use. (The counter after that is cleared before the batch's barrier, all having read it before the last one.)
+  int had = 0, batch = 0, turn = 0, rise = 0;
+  u64_t bound = 0;
+  for (int c0 = r.from; batch == 0 || c0 < r.to; c0 += C::NT * C::U, ++batch) {
+    u32x4 w[C::U];
+    each<C::U>([&](auto u) { w[u.value] = next[u.value]; });
+    const int n = present<C>(c0 + tid, r.to), following_chunk = c0 + C::NT * C::U + tid;
+    fetch<C>(r, following_chunk, present<C>(following_chunk, r.to), next);
+    float top;
+    add<C>(a, w, n, top);
+    peak = fmaxf(peak, top);
+    if constexpr (C::K > 0) {
+      // Bounds come from the threads' maxima so far: the first batch's from itself, the others' from the batches before. They rise by less and
+      // less: new ones are taken after 1, 2, 4, .. batches.
+      const bool rises = (batch & (batch + 1)) == 0;
+      if (rises) {
+        const u32_t share = share_of<C>(peak);
+        if (lane == 0) list.share[rise][wave] = share;
+      }
+      if (batch == 0) {
+        __syncthreads();
+        bound = bound_of<C>(list.share[0]);
+      }
+      const int following = turn == 2 ? 0 : turn + 1;
+      if (tid == 0) list.count[following] = 0;
+      for (;;) {
+        if (batch == 0 && besides >= 0) keep(x, besides, bound, had, turn);
+        // Lanes that reach the bound lay out their chunks, sixteen lanes at a time, and the whole wave looks through them. (A lane after the
+        // other, each waits for LDS four times over: 2048 x 50257 bf16, 20 alternatives, 81 us.)
+        u64_t lanes = __builtin_amdgcn_uicmp(order(top), (u32_t)(bound >> 32), 35);  // those where it is as large
+        while (lanes) {
+          constexpr int LAID = List<C>::LAID;
+          const int rank = __builtin_popcountll(lanes & ((1ull << lane) - 1)), count = __builtin_popcountll(lanes);
+          const bool mine = (lanes >> lane & 1) && rank < LAID;
+          if (mine) {
+            each<C::U>([&](auto u) { list.chunk[wave][rank][u.value] = w[u.value]; });
+            list.who[wave][rank] = lane | n << 8;
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+          for (int i = lane; i < (count < LAID ? count : LAID) * C::U * PER; i += 64) {
+            const int from = i / (C::U * PER), j = i % (C::U * PER), who = list.who[wave][from];
+            if (j >= (who >> 8) * PER) continue;
+            keep(value<C::DT>(((const typename Elem<C::DT>::type*)list.chunk[wave][from])[j]), (c0 + j / PER * C::NT + wave * 64 + (who & 255)) * PER + j % PER, bound, had, turn);
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          lanes &= ~__builtin_amdgcn_ballot_w64(mine);
+        }
+        __syncthreads();
+        const int found = had + list.count[turn];
+        if (found <= List<C>::CAP) {
+          had = found;
+          break;
+        }
+        // Full: its K-th key bounds the range's. Of what was there before the batch the keys that reach it stay, K at most, and the
+        // batch is taken again. (CAP different keys reach the old bound and K of them the new one, so that it rises by CAP - K keys every time.)
+        list.rank(List<C>::CAP);
+        bound = list.best[C::K - 1];
+        u64_t kept[List<C>::CAP / C::NT];
+#pragma unroll
+        for (int i = 0; i < List<C>::CAP / C::NT; ++i) kept[i] = i * C::NT + tid < had ? list.key[i * C::NT + tid] : 0;
+        if (tid == 0) list.count[turn] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < List<C>::CAP / C::NT; ++i)
+          if (kept[i] >= bound) list.key[atomicAdd(&list.count[turn], 1)] = kept[i];
+        __syncthreads();
+        had = list.count[turn];
+        __syncthreads();
+        if (tid == 0) list.count[turn] = 0;
+        __syncthreads();
+      }
+      if (rises) {
+        const u64_t higher = bound_of<C>(list.share[rise]);
+        bound = higher > bound ? higher : bound;
+        rise ^= 1;
+      }
+      turn = following;
+    }
+  }
+  if constexpr (C::K > 0) {
+    __syncthreads();
+    list.rank(had);
+  }
+  __shared__ float lds[WAVES][4];
+  bool care = false;
+  return join_threads<WAVES>(a, peak, care, lds);
 }
 
 // What a row's outputs are made of.
@@ -300,9 +405,7 @@ __device__ __forceinline__ void write(const typename Elem<C::DT>::type* __restri
     const int t = tokens[row];
     float v = 0.0f;
     if (t >= 0 && t < C::V) {
-      const typename Elem<C::DT>::type e = x[row * C::V + t];
-      if constexpr (C::DT == 2) v = log_prob(a, e);
-      else v = log_prob(a, C::DT == 0 ? bf16_to_f32(e) : f16_to_f32(e));
+      v = log_prob(a, value<C::DT>(x[row * C::V + t]));
     }
     token[row] = v;
   }
@@ -324,7 +427,7 @@ __device__ __forceinline__ void log_probs(const typename Elem<C::DT>::type* __re
                                           float* __restrict__ entropies, float* __restrict__ top, int* __restrict__ top_tokens, float* __restrict__ part) {
   __shared__ List<C> list;
   const long row = blockIdx.x;
-  const Sums a = scan<C>(x, range_of<C>(row, (int)blockIdx.y), row * C::V, list);
+  const Sums a = scan<C>(range_of<C>(x, row, (int)blockIdx.y), list);
   if constexpr (C::SPLITS == 1) {
     write<C>(x, tokens, row, a, list.best, token, entropies, top, top_tokens);
   } else {
@@ -351,14 +454,10 @@ __device__ __forceinline__ void log_probs_join(const typename Elem<C::DT>::type*
   const Part<C>* const from = (const Part<C>*)part + row * C::SPLITS;
   if constexpr (C::K > 0) {
     static_assert(C::SPLITS * C::K <= List<C>::CAP, "the splits' keys fit a list");
-    if (threadIdx.x == 0) list.count = 0;
+    // (a missing key, 0, is below all)
+    for (int i = threadIdx.x; i < C::SPLITS * C::K; i += C::NT) list.key[i] = from[i / C::K].key[i % C::K];
     __syncthreads();
-    for (int i = threadIdx.x; i < C::SPLITS * C::K; i += C::NT) {
-      const u64_t key = from[i / C::K].key[i % C::K];
-      if (key) list.key[atomicAdd(&list.count, 1)] = key;
-    }
-    __syncthreads();
-    list.rank(list.count);
+    list.rank(C::SPLITS * C::K);
   }
   write<C>(x, tokens, row, join_sums<C>(part, row), list.best, token, entropies, top, top_tokens);
 }
@@ -366,97 +465,91 @@ __device__ __forceinline__ void log_probs_join(const typename Elem<C::DT>::type*
 // ---- the gradient ----
 //
 // d x = g (1 at the token) - p (g + h (log p + H)), g and h the gradients of the token's log probability and of the entropy H: with z = log2 p,
-// p (A + B z) with A = g + h H and B = h ln 2.
+// p (A + B z) with A = -g - h H and B = -h ln 2.
 template <class C> struct Slope {
-  float base, log_l, a, b, g;  // z = (x - base) log2 e - log2 l
-  long at;                     // the token's element, or -1
+  float base, log_l, from, a, b, g;  // z = (x - base) log2 e - log2 l = x log2 e - from
+  int at;                      // the token's element counted as a Range's, or -1
 };
 template <class C>
-__device__ __forceinline__ Slope<C> slope_of(const Sums& s, long row, const int* __restrict__ tokens, const float* __restrict__ d_token,
+__device__ __forceinline__ Slope<C> slope_of(const Sums& s, long row, int lead, const int* __restrict__ tokens, const float* __restrict__ d_token,
                                              const float* __restrict__ d_entropy) {
   Slope<C> k;
   const int t = tokens[row];
   const bool inside = t >= 0 && t < C::V;
   const float h = d_entropy[row];
   k.g = inside ? d_token[row] : 0.0f;
-  k.at = inside && s.l != 0.0f ? row * C::V + t : -1;
+  k.at = inside && s.l != 0.0f ? lead + t : -1;
   k.base = base_of(s.m);
   k.log_l = s.l == 0.0f ? 0.0f : __builtin_amdgcn_logf(s.l);
-  k.a = k.g + h * entropy(s);
-  k.b = h * LN2;
+  k.from = k.base * L2E + k.log_l;
+  k.a = -k.g - h * entropy(s);
+  k.b = -h * LN2;
   return k;
-}
-template <class C> __device__ __forceinline__ float slope_at(const Slope<C>& k, float x, long at) {
-  const float z = __builtin_fmaf(x - k.base, L2E, -k.log_l);
-  const float d = __builtin_amdgcn_exp2f(z) * __builtin_fmaf(k.b, fmaxf(z, LEAST), k.a);
-  return at == k.at ? k.g - d : -d;
 }
 template <int DT> __device__ __forceinline__ typename Elem<DT>::type to_elem(float v) {
   if constexpr (DT == 0) return __builtin_bit_cast(u16_t, (__bf16)v);
   else if constexpr (DT == 1) return f32_to_f16(v);
   else return v;
 }
-// The gradient of a chunk's elements.
-template <class C>
-__device__ __forceinline__ void put(typename Elem<C::DT>::type* __restrict__ dx, const Range& r, const Slope<C>& k, long c, const u32x4& w) {
+// The gradient at an element. CARE: as in add().
+template <class C, bool CARE> __device__ __forceinline__ float slope(const Slope<C>& k, float x) {
+  const float z = CARE ? __builtin_fmaf(x - k.base, L2E, -k.log_l) : __builtin_fmaf(x, L2E, -k.from);
+  return __builtin_amdgcn_exp2f(z) * __builtin_fmaf(k.b, CARE ? fmaxf(z, LEAST) : z, k.a);
+}
+// The gradient of chunk c's elements.
+template <class C, bool CARE>
+__device__ __forceinline__ void put(typename Elem<C::DT>::type* __restrict__ to, const Slope<C>& k, int c, const u32x4& w) {
   constexpr int PER = Chunks<C>::PER;
   float v[PER];
   widen<C>(w, v);
 #pragma unroll
-  for (int i = 0; i < PER; ++i) v[i] = slope_at(k, v[i], c * PER + i);
-  if (c * PER >= r.first && (c + 1) * PER <= r.end) {
-    u32x4 o;
+  for (int i = 0; i < PER; ++i) v[i] = slope<C, CARE>(k, v[i]);
+  if (k.at >= 0 && k.at / PER == c) {
+    asm volatile("");
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (C::DT == 2) o[i] = __builtin_bit_cast(u32_t, v[i]);
-      else o[i] = (u32_t)to_elem<C::DT>(v[2 * i]) | (u32_t)to_elem<C::DT>(v[2 * i + 1]) << 16;
-    }
-    *(u32x4*)(dx + c * PER) = o;
-  } else {
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (c * PER + i >= r.first && c * PER + i < r.end) dx[c * PER + i] = to_elem<C::DT>(v[i]);
+    for (int i = 0; i < PER; ++i) v[i] += i == k.at % PER ? k.g : 0.0f;
   }
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (C::DT == 2) o[i] = __builtin_bit_cast(u32_t, v[i]);
+    else o[i] = (u32_t)to_elem<C::DT>(v[2 * i]) | (u32_t)to_elem<C::DT>(v[2 * i + 1]) << 16;
+  }
+  *(u32x4*)((u8_t*)to + (u32_t)c * 16u) = o;
+}
+template <class C> __device__ __forceinline__ void put_besides(typename Elem<C::DT>::type* __restrict__ to, const Slope<C>& k, int besides, float x) {
+  if (besides >= 0) to[besides] = to_elem<C::DT>(slope<C, true>(k, x) + (besides == k.at ? k.g : 0.0f));
 }
 
 // A row whose chunks fit the workgroup's registers, U of them a thread: read once, written once.
 template <class C>
 __device__ __forceinline__ void grad_row(const typename Elem<C::DT>::type* __restrict__ x, const int* __restrict__ tokens, const float* __restrict__ d_token,
                                          const float* __restrict__ d_entropy, typename Elem<C::DT>::type* __restrict__ dx) {
-  constexpr int PER = Chunks<C>::PER, WAVES = C::NT / 64;
-  __shared__ float tops[WAVES], ls[WAVES], ss[WAVES];
+  constexpr int WAVES = C::NT / 64;
+  __shared__ float lds[WAVES][4];
   const long row = blockIdx.x;
-  const Range r = range_of<C>(row, 0);
-  const int tid = threadIdx.x;
+  const Range<C> r = range_of<C>(x, row, 0);
+  const int first = r.from + (int)threadIdx.x, n = present<C>(first, r.to), besides = r.besides();
   u32x4 w[C::U];
-#pragma unroll
-  for (int u = 0; u < C::U; ++u)
-    if (r.c0 + u * C::NT + tid < r.c1) w[u] = read<C>(x, r.c0 + u * C::NT + tid);
+  fetch<C>(r, first, n, w);
+  float edge = 0.0f, peak;
   Sums a;
-  auto each = [&](auto f) {
-#pragma unroll
-    for (int u = 0; u < C::U; ++u) {
-      const long c = r.c0 + u * C::NT + tid;
-      if (c >= r.c1) continue;
-      float v[PER];
-      widen<C>(w[u], v);
-      mask<C>(r, c, v);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) f(v[i]);
-    }
-  };
-  each([&](float v) { a.m = fmaxf(a.m, v); });
-  a.m = block_reduce<C::NT>(a.m, MaxOp(), tops);
-  const float base = base_of(a.m);
-  each([&](float v) { a.add(v, base); });
-  a.l = block_reduce<C::NT>(a.l, SumOp(), ls);
-  a.s = block_reduce<C::NT>(a.s, SumOp(), ss);
-  const Slope<C> k = slope_of<C>(a, row, tokens, d_token, d_entropy);
-#pragma unroll
-  for (int u = 0; u < C::U; ++u) {
-    const long c = r.c0 + u * C::NT + tid;
-    if (c < r.c1) put<C>(dx, r, k, c, w[u]);
+  if (besides >= 0) {
+    edge = value<C::DT>(r.base[besides]);
+    a = sums_of(edge);
   }
+  bool care = add<C>(a, w, n, peak);
+  if (besides >= 0) peak = fmaxf(peak, edge);
+  each<C::U>([&](auto u) { opaque(w[u.value]); });
+  a = join_threads<WAVES>(a, peak, care, lds);
+  const Slope<C> k = slope_of<C>(a, row, r.lead, tokens, d_token, d_entropy);
+  typename Elem<C::DT>::type* const to = dx + r.at;
+  put_besides<C>(to, k, besides, edge);
+  each<C::U>([&](auto u) {
+    if (u.value >= n) return;
+    if (care) put<C, true>(to, k, first + u.value * C::NT, w[u.value]);
+    else put<C, false>(to, k, first + u.value * C::NT, w[u.value]);
+  });
 }
 
 // Rows that several workgroups share: the sums come from `part` (log_probs with K = 0), each workgroup writes a part of the row.
@@ -464,9 +557,12 @@ template <class C>
 __device__ __forceinline__ void grad_split(const typename Elem<C::DT>::type* __restrict__ x, const int* __restrict__ tokens, const float* __restrict__ d_token,
                                            const float* __restrict__ d_entropy, const float* __restrict__ part, typename Elem<C::DT>::type* __restrict__ dx) {
   const long row = blockIdx.x;
-  const Range r = range_of<C>(row, (int)blockIdx.y);
-  const Slope<C> k = slope_of<C>(join_sums<C>(part, row), row, tokens, d_token, d_entropy);
-  for (long c = r.c0 + threadIdx.x; c < r.c1; c += C::NT) put<C>(dx, r, k, c, read<C>(x, c));
+  const Range<C> r = range_of<C>(x, row, (int)blockIdx.y);
+  const int besides = r.besides();
+  const Slope<C> k = slope_of<C>(join_sums<C>(part, row), row, r.lead, tokens, d_token, d_entropy);
+  typename Elem<C::DT>::type* const to = dx + r.at;
+  put_besides<C>(to, k, besides, besides >= 0 ? value<C::DT>(r.base[besides]) : 0.0f);
+  for (int c = r.from + (int)threadIdx.x; c < r.to; c += C::NT) put<C, true>(to, k, c, chunk<C>(r.base, c));
 }
 
 }  // namespace logits

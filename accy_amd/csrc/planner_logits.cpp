@@ -72,8 +72,10 @@ void Planner::logits_log_probs(uint32_t v) {
     require(launchable(rows, 256), op, "more rows than a launch takes");
     const int xs = dense_slot(op.args[0]), ts = dense_slot(op.args[1]);
     const int64_t chunks = logit_chunks(V, xt.dtype), splits = logit_splits(rows, chunks, K), mine = (chunks + splits - 1) / splits;
-    // A thread's chunks in as few rounds of eight as they take, and as even.
-    const int64_t rounds = (mine + 256 * 8 - 1) / (256 * 8), u = std::max<int64_t>(1, (mine + 256 * rounds - 1) / (256 * rounds));
+    // A thread holds up to four chunks at once and has four more on their way, in as few rounds as they take and as even (us, 256 threads of 4 /
+    // 5 / 8 chunks, 512 of 4: 2048 x 50257 bf16, 20 alternatives, 66 / 67 / 71 / 85, 1024 x 50257 f32 46 / 47 / 50 / 56, 600 x 131072 bf16, five, 53
+    // / 53 / 53 / 59).
+    const int64_t rounds = (mine + 256 * 4 - 1) / (256 * 4), u = std::max<int64_t>(1, (mine + 256 * rounds - 1) / (256 * rounds));
     const std::string nm = name("log_probs", v), head = logit_config(nm, dt, rows, V, K, splits, 256, u);
     auto results = [&](KernelWriter& w) {
       std::string s;
@@ -156,7 +158,7 @@ void Planner::logits_grad(uint32_t v) {
       launch(nm, logit_config(nm, dt, rows, V, 0, 1, threads, u), "grad_row", false, -1, threads, 1);
     } else {
       const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({(int64_t)((1024 + rows - 1) / rows), chunks / 256, 64})), mine = (chunks + splits - 1) / splits;
-      const int64_t rounds = (mine + 256 * 8 - 1) / (256 * 8);
+      const int64_t rounds = (mine + 256 * 4 - 1) / (256 * 4);
       // (one split is written to the parts too: the kernels of a row's sums and of its gradient are two)
       const std::string head = logit_config(nm, dt, rows, V, 0, std::max<int64_t>(2, splits), 256, std::max<int64_t>(1, (mine + 256 * rounds - 1) / (256 * rounds)));
       const int part = slots_.add(SlotInfo::Temp, -1, DType::f32, rows * (uint64_t)std::max<int64_t>(2, splits) * logit_part(0));
