@@ -18,13 +18,14 @@ struct CheckLogits {
   static constexpr int DT = D_, K = TOP, SPLITS = S, NT = THREADS, U = CHUNKS;
   static constexpr long ROWS = 77, V = VOCAB;
 };
-template <long PAGES, long R> struct CheckFork {
+template <long PAGES, long R, bool W = false> struct CheckFork {
+  static constexpr bool WIDE = W;
   static constexpr long SEQS = 20, ROWS = R, SLOTS = 9, P = PAGES, T = 64, ENTRIES = 180, MOVES = 50;
 };
 struct CheckCopy {
   static constexpr long N = 30, P = 100, BYTES = 8704, PER = 8192;
   static constexpr int W = 16;
-  static constexpr bool CHECK = true, OWNERS = false;
+  static constexpr bool ONCE = true, CHECK = true, OWNERS = false;
 };
 
 typedef CheckHeads<0, 128, 64, 8, 8, false> Bf16Heads;
@@ -64,10 +65,14 @@ extern "C" __global__ void __launch_bounds__(1024) check_fork(const int* t, cons
 }
 extern "C" __global__ void __launch_bounds__(1024) check_fork_large(const int* t, const int* l, const int* p, const int* r, const u8_t* h, int* a, int* b, int* c,
                                                                     int* d, int* e, int* work) {
-  accy::pages::fork<CheckFork<1000000, 2000>>(t, l, p, r, h, a, b, c, d, e, work);
+  accy::pages::fork<CheckFork<1000000, 2000, true>>(t, l, p, r, h, a, b, c, d, e, work);
 }
+extern "C" __global__ void __launch_bounds__(256) check_fork_rows(const int* t, const int* work, int* a) { accy::pages::fork_rows<CheckFork<1000000, 2000, true>>(t, work, a); }
 extern "C" __global__ void __launch_bounds__(1024) check_compact(const int* t, const u8_t* h, int* a, int* b, int* c) {
   accy::pages::compact<CheckFork<1000, 20>>(t, h, a, b, c, nullptr);
+}
+extern "C" __global__ void __launch_bounds__(256) check_compact_rows(const int* t, const int* to, int* work, int* a) {
+  accy::pages::compact_rows<CheckFork<1000, 20, true>>(t, to, work, a);
 }
 extern "C" __global__ void __launch_bounds__(256) check_copy(const u8_t* from, u8_t* to, const int* s, const int* t, const u8_t* aside, const int* flags) {
   accy::pages::copy<CheckCopy>(from, to, s, t, nullptr, aside, flags);

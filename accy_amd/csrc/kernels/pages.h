@@ -95,7 +95,7 @@ template <long P> __device__ __forceinline__ u32_t held_word(const u8_t* __restr
 }
 
 // ---------------------------------------------------------------------------------------------
-// fork: C supplies SEQS, ROWS, SLOTS, P (pages), T (tokens of a page).
+// fork: C supplies SEQS, ROWS, SLOTS, P (pages), T (tokens of a page), WIDE (the tables are written by fork_rows).
 // ---------------------------------------------------------------------------------------------
 
 // What row r becomes: its parent (-1: empty), the parent's length, the slots that its tokens take and those that it is to have.
@@ -124,84 +124,103 @@ template <class C> __device__ __forceinline__ int page_at(const int* __restrict_
   return p >= 0 && p < C::P ? p : -1;
 }
 
-// `map` and `counts`: (P + 31) / 32 words each; `firsts` [P]: work space where there are more than THREADS rows.
+// What fork_rows needs of a row: the first `kept` slots are its parent's, `asked` pages from number `first` of the fresh ones follow.
+struct Row {
+  int parent, kept, first, asked;
+};
+
+// `map` and `counts`: (P + 31) / 32 words each; `firsts` [P]: work space where there are more than THREADS rows; `rows` [ROWS] and
+// `fresh` [ROWS x SLOTS]: where the tables are written by another kernel (C::WIDE).
 template <class C, bool LDS>
 __device__ __forceinline__ void fork_with(u32_t* map, int* counts, const int* __restrict__ table, const int* __restrict__ lengths,
                                           const int* __restrict__ parents, const int* __restrict__ room, const u8_t* __restrict__ held,
                                           int* __restrict__ out_table, int* __restrict__ out_lengths, int* __restrict__ source,
-                                          int* __restrict__ target, int* __restrict__ left, int* __restrict__ firsts) {
+                                          int* __restrict__ target, int* __restrict__ left, int* __restrict__ firsts, Row* __restrict__ rows,
+                                          int* __restrict__ fresh_pages) {
   constexpr long WORDS = (C::P + 31) / 32;
   constexpr int SLOTS = C::SLOTS > 0 ? (int)C::SLOTS : 1;
+  // With a thread for every row its numbers stay in registers; else they are formed again where they are needed.
+  constexpr bool ONE = C::ROWS <= THREADS;
   __shared__ int parent[THREADS], kept[THREADS], place[THREADS], sums[WAVES + 1];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto row_of = [&](long r) {
+    const Fork none = {-1, 0, 0, 0, false};
+    return r < C::ROWS ? fork_of<C>(lengths, parents, room, r) : none;
+  };
+  auto partly = [&](const Fork& f) { return f.partial ? page_at<C>(table, f.parent, f.kept - 1) : -1; };
+  Fork mine = row_of(tid);
+  int last = partly(mine);
   for (long w = tid; w < WORDS; w += THREADS) put_word<LDS>(map, w, held_word<C::P>(held, w));
   meet<LDS>();
-  // Pages that a row has filled.
+  // Pages that a row has filled: a wave takes eight rows at once, 64 slots of each.
   for (long r0 = 0; r0 < C::ROWS; r0 += THREADS) {
-    if (r0 + tid < C::ROWS) {
-      const Fork f = fork_of<C>(lengths, parents, room, r0 + tid);
-      parent[tid] = f.parent;
-      kept[tid] = f.kept - (f.partial ? 1 : 0);
-    }
+    if constexpr (!ONE) mine = row_of(r0 + tid);
+    parent[tid] = mine.parent;
+    kept[tid] = mine.kept - (mine.partial ? 1 : 0);
     __syncthreads();
-    const int n = (int)((C::ROWS - r0 < THREADS ? C::ROWS - r0 : THREADS) * C::SLOTS);
-#pragma unroll 4
-    for (int i = tid; i < n; i += THREADS) {
-      const int r = i / SLOTS, j = i % SLOTS;
-      if (j >= kept[r]) continue;
-      const int p = page_at<C>(table, parent[r], j);
-      if (p >= 0) set_bit(map, p);
+    const int n = (int)(C::ROWS - r0 < THREADS ? C::ROWS - r0 : THREADS);
+    for (int r = wave; r < n; r += 8 * WAVES) {
+      int most = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = r + i * WAVES < n && kept[r + i * WAVES] > most ? kept[r + i * WAVES] : most;
+      for (int j = lane; j < most; j += 64) {
+        int p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = r + i * WAVES;
+          p[i] = row < n && j < kept[row] ? page_at<C>(table, parent[row], j) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (p[i] >= 0) set_bit(map, p[i]);
+      }
     }
     meet<LDS>();
   }
   // Pages that a row has filled in part: whose they are. `source` says which rows copy theirs.
-  auto partly = [&](long r) {
-    const Fork f = fork_of<C>(lengths, parents, room, r);
-    return f.partial ? page_at<C>(table, f.parent, f.kept - 1) : -1;
-  };
-  if constexpr (C::ROWS <= THREADS) {
-    const int mine = tid < C::ROWS ? partly(tid) : -1;
-    place[tid] = mine;
+  bool copied = false;
+  if constexpr (ONE) {
+    place[tid] = last;
     __syncthreads();
-    bool copied = false;
-    if (mine >= 0) {
-      copied = bit<LDS>(map, mine);
-      for (int r = 0; r < tid; ++r) copied |= place[r] == mine;
+    if (last >= 0) {
+      copied = bit<LDS>(map, last);
+#pragma unroll 8
+      for (int r = 0; r < tid; ++r) copied |= place[r] == last;
     }
-    if (tid < C::ROWS) source[tid] = copied ? mine : -1;
     __syncthreads();
-    if (mine >= 0) set_bit(map, mine);
+    if (last >= 0) set_bit(map, last);
   } else {
     for (long r = tid; r < C::ROWS; r += THREADS) {
-      const int mine = partly(r);
-      if (mine >= 0) __hip_atomic_store(firsts + mine, (int)C::ROWS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = partly(row_of(r));
+      if (last >= 0) __hip_atomic_store(firsts + last, (int)C::ROWS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     meet<false>();
     for (long r = tid; r < C::ROWS; r += THREADS) {
-      const int mine = partly(r);
-      if (mine >= 0) atomicMin(firsts + mine, (int)r);
+      last = partly(row_of(r));
+      if (last >= 0) atomicMin(firsts + last, (int)r);
     }
     meet<false>();
     for (long r = tid; r < C::ROWS; r += THREADS) {
-      const int mine = partly(r);
-      source[r] = mine >= 0 && (bit<LDS>(map, mine) || __hip_atomic_load(firsts + mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != (int)r) ? mine : -1;
+      last = partly(row_of(r));
+      source[r] = last >= 0 && (bit<LDS>(map, last) || __hip_atomic_load(firsts + last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != (int)r) ? last : -1;
     }
     __syncthreads();
     for (long r = tid; r < C::ROWS; r += THREADS) {
-      const int mine = partly(r);
-      if (mine >= 0) set_bit(map, mine);
+      last = partly(row_of(r));
+      if (last >= 0) set_bit(map, last);
     }
   }
   meet<LDS>();
   // Free pages before each word.
   long from, to;
   my_words(WORDS, from, to);
-  int mine = 0, all;
-  for (long w = from; w < to; ++w) mine += __builtin_popcount(~word<LDS>(map, w));
-  int so_far = before_me(mine, sums, all);
+  int free = 0, all;
+  for (long w = from; w < to; ++w) free += __builtin_popcount(~word<LDS>(map, w));
+  const int so_far = before_me(free, sums, all);
+  int at = so_far;
   for (long w = from; w < to; ++w) {
-    put_word<LDS>((u32_t*)counts, w, (u32_t)so_far);
-    so_far += __builtin_popcount(~word<LDS>(map, w));
+    put_word<LDS>((u32_t*)counts, w, (u32_t)at);
+    at += __builtin_popcount(~word<LDS>(map, w));
   }
   meet<LDS>();
   auto fresh = [&](long k) {
@@ -217,63 +236,118 @@ __device__ __forceinline__ void fork_with(u32_t* map, int* counts, const int* __
   // The rows: their copies, and then what they are to have.
   long asked = 0;
   for (long r0 = 0; r0 < C::ROWS; r0 += THREADS) {
-    __syncthreads();
     const long r = r0 + tid;
-    Fork f = {-1, 0, 0, 0, false};
-    int old = -1, wanted = 0;
-    if (r < C::ROWS) {
-      f = fork_of<C>(lengths, parents, room, r);
-      old = source[r];
-      wanted = (old >= 0) + (f.want - f.kept);
+    int old = copied ? last : -1;
+    if constexpr (!ONE) {
+      __syncthreads();
+      mine = row_of(r);
+      old = r < C::ROWS ? source[r] : -1;
     }
+    const int wanted = (old >= 0) + (mine.want - mine.kept);
     int total;
     const long first = asked + before_me(wanted, sums, total);
+    // (the last kept slot of a row that copies is one of those to be filled)
+    const int stays = mine.kept - (old >= 0);
     if (r < C::ROWS) {
-      parent[tid] = f.parent;
-      // (the last kept slot of a row that copies is one of those to be filled)
-      kept[tid] = f.kept - (old >= 0);
-      place[tid] = (int)(first - asked);
-      out_lengths[r] = f.length;
+      out_lengths[r] = mine.length;
       const int page = old >= 0 ? fresh(first) : -1;
       source[r] = page >= 0 ? old : -1;
       target[r] = page;
+      if constexpr (C::WIDE) rows[r] = Row{mine.parent, stays, (int)first, wanted};
     }
-    __syncthreads();
-    const int n = (int)((C::ROWS - r0 < THREADS ? C::ROWS - r0 : THREADS) * C::SLOTS);
+    if constexpr (!C::WIDE) {
+      parent[tid] = mine.parent;
+      kept[tid] = stays;
+      place[tid] = (int)(first - asked);
+      __syncthreads();
+      const int n = (int)((C::ROWS - r0 < THREADS ? C::ROWS - r0 : THREADS) * C::SLOTS);
 #pragma unroll 4
-    for (int i = tid; i < n; i += THREADS) {
-      const int row = i / SLOTS, j = i % SLOTS, k = j - kept[row];
-      const int mine = (row + 1 < THREADS && r0 + row + 1 < C::ROWS ? place[row + 1] : total) - place[row];
-      int p = -1;
-      if (k < 0) p = page_at<C>(table, parent[row], j);
-      else if (k < mine) p = fresh(asked + place[row] + k);
-      out_table[r0 * C::SLOTS + i] = p;
+      for (int i = tid; i < n; i += THREADS) {
+        const int row = i / SLOTS, j = i % SLOTS, k = j - kept[row];
+        const int have = (row + 1 < THREADS && r0 + row + 1 < C::ROWS ? place[row + 1] : total) - place[row];
+        int p = -1;
+        if (k < 0) p = page_at<C>(table, parent[row], j);
+        else if (k < have) p = fresh(asked + place[row] + k);
+        out_table[r0 * C::SLOTS + i] = p;
+      }
     }
     asked += total;
   }
+  if constexpr (C::WIDE) {
+    // the pages in the order in which they are given out
+    int k = so_far;
+    for (long w = from; w < to && k < asked; ++w)
+      for (u32_t m = ~word<LDS>(map, w); m && k < asked; m &= m - 1, ++k) fresh_pages[k] = (int)(w * 32) + __builtin_ctz(m);
+    for (long k = all + (long)tid; k < asked; k += THREADS) fresh_pages[k] = -1;
+  }
   if (tid == 0) left[0] = (int)(all - asked);
 }
+// `work`: of the bitmap and its counts beyond LDS_PAGES pages, of the rows and fresh pages if C::WIDE, of `firsts`; in this order.
+template <class C> struct ForkWork {
+  static constexpr bool LDS = C::P <= LDS_PAGES;
+  static constexpr long WORDS = (C::P + 31) / 32, ROWS = LDS ? 0 : (2 * WORDS + 3) / 4 * 4, FRESH = ROWS + (C::WIDE ? 4 * C::ROWS : 0),
+                        FIRSTS = FRESH + (C::WIDE ? C::ROWS * C::SLOTS : 0);
+};
 template <class C>
 __device__ __forceinline__ void fork(const int* __restrict__ table, const int* __restrict__ lengths, const int* __restrict__ parents,
                                      const int* __restrict__ room, const u8_t* __restrict__ held, int* __restrict__ out_table,
                                      int* __restrict__ out_lengths, int* __restrict__ source, int* __restrict__ target, int* __restrict__ left,
-                                     int* __restrict__ work) {
-  constexpr long WORDS = (C::P + 31) / 32;
-  constexpr bool LDS = C::P <= LDS_PAGES;
-  __shared__ u32_t map[LDS ? WORDS + 1 : 1];
-  __shared__ int counts[LDS ? WORDS + 1 : 1];
-  int* const firsts = LDS ? work : work + 2 * WORDS;
-  fork_with<C, LDS>(LDS ? map : (u32_t*)work, LDS ? counts : work + WORDS, table, lengths, parents, room, held, out_table, out_lengths, source, target,
-                    left, firsts);
+                                     int* work) {
+  typedef ForkWork<C> W;
+  __shared__ u32_t map[W::LDS ? W::WORDS + 1 : 1];
+  __shared__ int counts[W::LDS ? W::WORDS + 1 : 1];
+  fork_with<C, W::LDS>(W::LDS ? map : (u32_t*)work, W::LDS ? counts : work + W::WORDS, table, lengths, parents, room, held, out_table, out_lengths, source,
+                       target, left, work + W::FIRSTS, (Row*)(work + W::ROWS), work + W::FRESH);
+}
+// Large tables: 1024 slots of a row to a workgroup.
+template <class C>
+__device__ __forceinline__ void fork_rows(const int* __restrict__ table, const int* __restrict__ work, int* __restrict__ out_table) {
+  typedef ForkWork<C> W;
+  const long r = blockIdx.x;
+  const Row row = ((const Row*)(work + W::ROWS))[r];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = (int)blockIdx.y * 1024 + i * 256 + (int)threadIdx.x, k = j - row.kept;
+    if (j >= C::SLOTS) break;
+    int p = -1;
+    if (k < 0) p = page_at<C>(table, row.parent, j);
+    else if (k < row.asked) p = work[W::FRESH + row.first + k];
+    out_table[r * C::SLOTS + j] = p;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
-// compact: C supplies ENTRIES (of the tables), P, MOVES.
+// compact: C supplies ENTRIES (of the tables), P, MOVES, WIDE (the tables are written by compact_rows).
 // ---------------------------------------------------------------------------------------------
+
+// The entries of the tables from `first` on, `stride` apart, with the pages that move under their new numbers: a page that moves is the k-th
+// that does by the counts. Four entries at once, since the new numbers are in memory.
+template <class C, bool LDS>
+__device__ __forceinline__ void renumber(const u32_t* used, const int* counts, int moves, const int* __restrict__ table, const int* target,
+                                         int* __restrict__ out_table, long first, long stride) {
+  for (long i = first; i < C::ENTRIES; i += 4 * stride) {
+    int p[4], k[4], to[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) p[u] = i + u * stride < C::ENTRIES ? table[i + u * stride] : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      p[u] = p[u] >= 0 && p[u] < C::P ? p[u] : -1;
+      k[u] = -1;
+      if (p[u] < 0) continue;
+      const u32_t m = word<LDS>(used, p[u] >> 5);
+      if (m >> (p[u] & 31) & 1) k[u] = (int)word<LDS>((const u32_t*)counts, p[u] >> 5) + __builtin_popcount(m & ((1u << (p[u] & 31)) - 1));
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) to[u] = k[u] >= 0 && k[u] < moves ? __hip_atomic_load(target + k[u], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : p[u];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * stride < C::ENTRIES) out_table[i + u * stride] = to[u];
+  }
+}
 
 template <class C, bool LDS>
 __device__ __forceinline__ void compact_with(u32_t* used, u32_t* busy, int* counts, const int* __restrict__ table, const u8_t* __restrict__ held,
-                                             int* __restrict__ out_table, int* __restrict__ source, int* __restrict__ target) {
+                                             int* __restrict__ out_table, int* __restrict__ source, int* __restrict__ target, int* work) {
   constexpr long WORDS = (C::P + 31) / 32;
   __shared__ int sums[WAVES + 1];
   const int tid = threadIdx.x;
@@ -315,38 +389,48 @@ __device__ __forceinline__ void compact_with(u32_t* used, u32_t* busy, int* coun
       if (hole < moves) target[hole] = (int)(w * 32) + __builtin_ctz(h);
   }
   for (long i = moves + tid; i < C::MOVES; i += THREADS) source[i] = target[i] = -1;
-  meet<false>();
-#pragma unroll 8
-  for (long i = tid; i < C::ENTRIES; i += THREADS) {
-    int p = table[i];
-    if (p < 0 || p >= C::P) {
-      p = -1;
-    } else {
-      const u32_t m = word<LDS>(used, p >> 5);
-      if (m >> (p & 31) & 1) {
-        const int k = (int)word<LDS>((const u32_t*)counts, p >> 5) + __builtin_popcount(m & ((1u << (p & 31)) - 1));
-        if (k < moves) p = __hip_atomic_load(target + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+  if (C::WIDE && tid == 0) work[0] = moves;
+  if constexpr (C::WIDE && LDS) {
+    for (long w = tid; w < WORDS; w += THREADS) {
+      work[4 + w] = (int)used[w];
+      work[4 + WORDS + w] = counts[w];
     }
-    out_table[i] = p;
+  }
+  if constexpr (!C::WIDE) {
+    meet<false>();
+    renumber<C, LDS>(used, counts, moves, table, target, out_table, tid, THREADS);
   }
 }
+// `work`: the moves, and from the fourth word on the bitmaps and counts where they are not in LDS or others read them (C::WIDE).
 template <class C>
 __device__ __forceinline__ void compact(const int* __restrict__ table, const u8_t* __restrict__ held, int* __restrict__ out_table,
-                                        int* __restrict__ source, int* __restrict__ target, int* __restrict__ work) {
+                                        int* __restrict__ source, int* __restrict__ target, int* work) {
   constexpr long WORDS = (C::P + 31) / 32;
   constexpr bool LDS = C::P <= LDS_PAGES;
   __shared__ u32_t used[LDS ? WORDS + 1 : 1], busy[LDS ? WORDS + 1 : 1];
   __shared__ int counts[LDS ? WORDS + 1 : 1];
-  compact_with<C, LDS>(LDS ? used : (u32_t*)work, LDS ? busy : (u32_t*)work + WORDS, LDS ? counts : work + 2 * WORDS, table, held, out_table, source, target);
+  compact_with<C, LDS>(LDS ? used : (u32_t*)work + 4, LDS ? busy : (u32_t*)work + 4 + 2 * WORDS, LDS ? counts : work + 4 + WORDS, table, held, out_table,
+                       source, target, work);
+}
+// Large tables: 1024 entries to a workgroup.
+template <class C>
+__device__ __forceinline__ void compact_rows(const int* __restrict__ table, const int* __restrict__ target, int* work, int* __restrict__ out_table) {
+  constexpr long WORDS = (C::P + 31) / 32;
+  renumber<C, false>((u32_t*)work + 4, work + 4 + WORDS, work[0], table, target, out_table, (long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256);
 }
 
 // ---------------------------------------------------------------------------------------------
-// copies: C supplies N (copies), P, BYTES (of a page), PER (bytes of a workgroup), W (bytes of an access), CHECK, OWNERS (the last copy to each
-// page is in a table).
+// copies: C supplies N (copies), P, BYTES (of a page), PER (bytes of a workgroup), W (bytes of an access), ONCE (with the
+// non-temporal hint), CHECK, OWNERS (the last copy to each page is in a table).
 // ---------------------------------------------------------------------------------------------
 
-template <int W> struct alignas(W) Piece { u8_t v[W]; };
+// An access of W bytes.
+typedef u32_t u32x4 __attribute__((ext_vector_type(4)));
+template <int W> struct Piece { typedef u8_t type; };
+template <> struct Piece<2> { typedef u16_t type; };
+template <> struct Piece<4> { typedef u32_t type; };
+template <> struct Piece<8> { typedef u64_t type; };
+template <> struct Piece<16> { typedef u32x4 type; };
 
 template <class C> __device__ __forceinline__ bool pair_of(const int* __restrict__ source, const int* __restrict__ target, long i, int& s, int& t) {
   s = source[i];
@@ -376,10 +460,14 @@ template <class C> __device__ __forceinline__ bool goes_to(const int* __restrict
 
 // The part blockIdx.y of a page.
 template <class C> __device__ __forceinline__ void move(const u8_t* from, u8_t* to) {
-  typedef Piece<C::W> V;
+  typedef typename Piece<C::W>::type V;
   const long begin = (long)blockIdx.y * C::PER, end = begin + C::PER < C::BYTES ? begin + C::PER : C::BYTES;
 #pragma unroll 4
-  for (long b = begin + threadIdx.x * C::W; b < end; b += 256 * C::W) *(V*)(to + b) = *(const V*)(from + b);
+  for (long b = begin + threadIdx.x * C::W; b < end; b += 256 * C::W) {
+    const V* const x = (const V*)(from + b);
+    if constexpr (C::ONCE) __builtin_nontemporal_store(__builtin_nontemporal_load(x), (V*)(to + b));
+    else *(V*)(to + b) = *x;
+  }
 }
 
 // In place: sources that are a target too, aside. aside [N][BYTES], flags [N]: whether a copy's source is there.

@@ -15,6 +15,10 @@ namespace {
 constexpr int64_t kMostPages = int64_t(1) << 24;
 constexpr int64_t kLdsPages = int64_t(1) << 17;  // LDS_PAGES of kernels/pages.h
 
+// Entries of tables that one workgroup writes as fast as another launch would (us with a copy of a few pages, one launch / two: 8 x 64 entries
+// 12 / 15, 64 x 64 14 / 15, 64 x 256 24 / 15, 128 x 256 42 / 16, 256 x 512 114 / 18).
+constexpr uint64_t kOneWorkgroup = 4096;
+
 bool whole_numbers(const Type& t, size_t rank) { return t.dtype == DType::i32 && t.rank() == rank; }
 
 }  // namespace
@@ -52,22 +56,42 @@ void Planner::pages_fork(uint32_t v) {
     made.push_back(call->second);
   }
   require(!made.empty(), op, "no result of that name");
-  const uint64_t words = (uint64_t)(pages + 31) / 32, work = (pages > kLdsPages ? 2 * words : 0) + (rows > 1024 ? (uint64_t)pages : 0);
+  // One workgroup writes small tables itself; of larger ones it leaves what each row takes to workgroups of their own.
+  const bool wide = (uint64_t)(rows * slots) > kOneWorkgroup;
+  require(launchable((uint64_t)rows, 256) && (slots + 1023) / 1024 < 65536, op, "more workgroups than a launch takes");
+  // ForkWork of kernels/pages.h
+  const uint64_t words = (uint64_t)(pages + 31) / 32, work = (pages > kLdsPages ? (2 * words + 3) / 4 * 4 : 0) + (wide ? (uint64_t)(rows * (4 + slots)) : 0) +
+                                                             (rows > 1024 ? (uint64_t)pages : 0);
+  const int table = dense_slot(now[0]), ws = work ? slots_.add(SlotInfo::Temp, -1, DType::i32, work * 4) : -1;
   KernelWriter w(g_, slots_, "i64_t");
-  std::string args;
-  for (const uint32_t a : {now[0], now[1], next[0], next[1], op.args[2]}) args += w.arg(dense_slot(a), false) + ", ";
-  for (const int o : out) args += w.arg(o, true) + ", ";
-  args += work ? w.arg(slots_.add(SlotInfo::Temp, -1, DType::i32, work * 4), true) : "nullptr";
+  std::string args = w.arg(table, false) + ", ";
+  for (const uint32_t a : {now[1], next[0], next[1], op.args[2]}) args += w.arg(dense_slot(a), false) + ", ";
+  for (size_t i = 0; i < 5; ++i) args += (i == 0 && wide ? std::string("nullptr") : w.arg(out[i], true)) + ", ";
+  args += work ? w.arg(ws, true) : "nullptr";
   KernelStep k;
   const std::string nm = name("fork", v);
-  k.source = "#include \"pages\"\nstruct Cfg_" + nm + " {\n  static constexpr long SEQS = " + num(seqs) + ", ROWS = " + num(rows) + ", SLOTS = " + num(slots) + ", P = " +
-             num(pages) + ", T = " + num(page) + ";\n};\nextern \"C\" __global__ void __launch_bounds__(1024) " + nm + "(" + w.params() +
-             ") {\n  accy::pages::fork<Cfg_" + nm + ">(" + args + ");\n}\n";
+  const std::string head = "#include \"pages\"\nstruct Cfg_" + nm + " {\n  static constexpr long SEQS = " + num(seqs) + ", ROWS = " + num(rows) + ", SLOTS = " + num(slots) +
+                           ", P = " + num(pages) + ", T = " + num(page) + ";\n  static constexpr bool WIDE = " + (wide ? "true" : "false") + ";\n};\n";
+  k.source = head + "extern \"C\" __global__ void __launch_bounds__(1024) " + nm + "(" + w.params() + ") {\n  accy::pages::fork<Cfg_" + nm + ">(" + args + ");\n}\n";
   k.name = nm;
   k.block[0] = 1024;
   k.klass = "pages";
   k.label = "fork:%" + std::to_string(v);
   push(std::move(k), w);
+  if (wide) {
+    KernelWriter rw(g_, slots_, "i64_t");
+    const std::string a = rw.arg(table, false), b = rw.arg(ws, false), c = rw.arg(out[0], true);
+    KernelStep t;
+    t.name = name("fork_rows", v);
+    t.source = head + "extern \"C\" __global__ void __launch_bounds__(256) " + t.name + "(" + rw.params() + ") {\n  accy::pages::fork_rows<Cfg_" + nm + ">(" + a + ", " + b +
+               ", " + c + ");\n}\n";
+    t.grid[0] = (uint32_t)rows;
+    t.grid[1] = (uint32_t)((slots + 1023) / 1024);
+    t.block[0] = 256;
+    t.klass = "pages";
+    t.label = "fork_rows:%" + std::to_string(v);
+    push(std::move(t), rw);
+  }
   for (const uint32_t u : made) finish(u);
 }
 
@@ -106,21 +130,37 @@ void Planner::pages_compact(uint32_t v) {
     made.push_back(call->second);
   }
   require(!made.empty(), op, "no result of that name");
-  const uint64_t words = (uint64_t)(pages + 31) / 32;
+  const uint64_t entries = tt.elements(), words = (uint64_t)(pages + 31) / 32;
+  const bool wide = entries > kOneWorkgroup;
+  const int table = dense_slot(op.args[0]);
+  const int ws = pages > kLdsPages || wide ? slots_.add(SlotInfo::Temp, -1, DType::i32, (4 + 3 * words) * 4) : -1;
   KernelWriter w(g_, slots_, "i64_t");
-  std::string args = w.arg(dense_slot(op.args[0]), false) + ", " + w.arg(dense_slot(op.args[1]), false);
-  for (const int o : out) args += ", " + w.arg(o, true);
-  args += pages > kLdsPages ? ", " + w.arg(slots_.add(SlotInfo::Temp, -1, DType::i32, 3 * words * 4), true) : ", nullptr";
+  std::string args = w.arg(table, false) + ", " + w.arg(dense_slot(op.args[1]), false);
+  for (int i = 0; i < 3; ++i) args += ", " + (i == 0 && wide ? std::string("nullptr") : w.arg(out[i], true));
+  args += ws >= 0 ? ", " + w.arg(ws, true) : ", nullptr";
   KernelStep k;
   const std::string nm = name("compact", v);
-  k.source = "#include \"pages\"\nstruct Cfg_" + nm + " {\n  static constexpr long ENTRIES = " + std::to_string(tt.elements()) + ", P = " + num(pages) + ", MOVES = " +
-             num(moves) + ";\n};\nextern \"C\" __global__ void __launch_bounds__(1024) " + nm + "(" + w.params() + ") {\n  accy::pages::compact<Cfg_" + nm + ">(" + args +
-             ");\n}\n";
+  const std::string head = "#include \"pages\"\nstruct Cfg_" + nm + " {\n  static constexpr long ENTRIES = " + std::to_string(entries) + ", P = " + num(pages) + ", MOVES = " +
+                           num(moves) + ";\n  static constexpr bool WIDE = " + (wide ? "true" : "false") + ";\n};\n";
+  k.source = head + "extern \"C\" __global__ void __launch_bounds__(1024) " + nm + "(" + w.params() + ") {\n  accy::pages::compact<Cfg_" + nm + ">(" + args + ");\n}\n";
   k.name = nm;
   k.block[0] = 1024;
   k.klass = "pages";
   k.label = "compact:%" + std::to_string(v);
   push(std::move(k), w);
+  if (wide) {
+    KernelWriter rw(g_, slots_, "i64_t");
+    const std::string a = rw.arg(table, false), b = rw.arg(out[2], false), c = rw.arg(ws, true), d = rw.arg(out[0], true);
+    KernelStep t;
+    t.name = name("compact_rows", v);
+    t.source = head + "extern \"C\" __global__ void __launch_bounds__(256) " + t.name + "(" + rw.params() + ") {\n  accy::pages::compact_rows<Cfg_" + nm + ">(" + a + ", " +
+               b + ", " + c + ", " + d + ");\n}\n";
+    t.grid[0] = grid_for(entries / 4, 256);
+    t.block[0] = 256;
+    t.klass = "pages";
+    t.label = "compact_rows:%" + std::to_string(v);
+    push(std::move(t), rw);
+  }
   for (const uint32_t u : made) finish(u);
 }
 
@@ -141,11 +181,14 @@ void Planner::pages_copy(uint32_t v) {
     const bool owners = check && n > 4096;
     int64_t W = 16;
     while (bytes % W) W /= 2;
+    // A part of a page to a workgroup (4, 8, 12, 16 KB and whole pages of 34 KB: the same to 2 %). What the caches do not hold anyway goes by them:
+    // 2990 pages of 34 KB 42 us, with the hint for loads 36, for stores 33, for both 32; a few pages may be read again at once.
+    const bool once = n * bytes >= int64_t(64) << 20;
     const int64_t per = 8192, parts = (bytes + per - 1) / per;
     require(parts < 65536 && launchable((uint64_t)n, 256), op, "more workgroups than a launch takes");
     const std::string nm = name("copy_pages", v);
     const std::string head = "#include \"pages\"\nstruct Cfg_" + nm + " {\n  static constexpr long N = " + num(n) + ", P = " + num(pages) + ", BYTES = " + num(bytes) + ", PER = " +
-                             num(per) + ";\n  static constexpr int W = " + num(W) + ";\n  static constexpr bool CHECK = " + (check ? "true" : "false") + ", OWNERS = " +
+                             num(per) + ";\n  static constexpr int W = " + num(W) + ";\n  static constexpr bool ONCE = " + (once ? "true" : "false") + ", CHECK = " + (check ? "true" : "false") + ", OWNERS = " +
                              (owners ? "true" : "false") + ";\n};\n";
     const int ss = dense_slot(op.args[1]), ts = dense_slot(op.args[2]);
     const int aside = check ? slots_.add(SlotInfo::Temp, -1, DType::u8, (uint64_t)(n * bytes)) : -1;
