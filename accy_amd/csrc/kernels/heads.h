@@ -1,7 +1,9 @@
 // Heads of queries and keys as attention takes them: each normalised, y = x / sqrt(mean(x^2) + eps) * gain, and turned by its token's
 // position: of pair i of the first 2 F dims, (a, b) becomes (a cos - b sin, b cos + a sin) of position * frequency[i]. And the gradient.
 //
-// Two numbers are read and two written for about eight operations, so a prompt's heads are bound by HBM and a step's by the launch.
+// Two numbers are read and two written for about eight operations, so a prompt's heads are bound by HBM (8192 tokens of 32 heads of 128 bf16 27 us, 5.0
+// TB/s; the gradient of 8192 x 20 x 128 31 us, 4.0 TB/s) and a step's by the launch (one token 2.3 us of kernel). The non-temporal hint gains bf16
+// rows 4 % and costs f32 rows of 80 dims half as much again.
 // A row (one head of one token) belongs to LANES adjacent lanes, so that its sum is a few shuffles, and each lane holds whole
 // pairs: W dims of a pair's first members and the W of its second (16 bytes each where the sizes allow it), which turn without
 // leaving the lane. The cosines of a token are the same for all of its heads: a workgroup forms them once for its TT tokens, a pair per
@@ -28,17 +30,24 @@ template <int DT> __device__ __forceinline__ float from_elem(typename Elem<DT>::
   else if constexpr (DT == 1) return f16_to_f32(v);
   else return v;
 }
+// W numbers as they lie in memory: one access.
+template <int BYTES> struct Bits;
+template <> struct Bits<2> { typedef u16_t type; };
+template <> struct Bits<4> { typedef u32_t type; };
+template <> struct Bits<8> { typedef u32_t type __attribute__((ext_vector_type(2))); };
+template <> struct Bits<16> { typedef u32_t type __attribute__((ext_vector_type(4))); };
+template <int DT, int W> struct Raw { typedef typename Bits<W * (DT == 2 ? 4 : 2)>::type type; };
 template <class T, int W> struct alignas(W * sizeof(T) < 16 ? W * sizeof(T) : 16) Chunk { T v[W]; };
-template <int DT, int W> __device__ __forceinline__ void load(const typename Elem<DT>::type* __restrict__ p, float* x) {
-  const Chunk<typename Elem<DT>::type, W> c = *(const Chunk<typename Elem<DT>::type, W>*)p;
+template <int DT, int W> __device__ __forceinline__ void widen(const typename Raw<DT, W>::type& raw, float* x) {
+  const Chunk<typename Elem<DT>::type, W> c = __builtin_bit_cast(Chunk<typename Elem<DT>::type, W>, raw);
 #pragma unroll
   for (int i = 0; i < W; ++i) x[i] = from_elem<DT>(c.v[i]);
 }
-template <int DT, int W> __device__ __forceinline__ void store(typename Elem<DT>::type* __restrict__ p, const float* x) {
+template <int DT, int W> __device__ __forceinline__ typename Raw<DT, W>::type narrow(const float* x) {
   Chunk<typename Elem<DT>::type, W> c;
 #pragma unroll
   for (int i = 0; i < W; ++i) c.v[i] = to_elem<DT>(x[i]);
-  *(Chunk<typename Elem<DT>::type, W>*)p = c;
+  return __builtin_bit_cast(typename Raw<DT, W>::type, c);
 }
 
 template <class C> struct Row {
@@ -79,20 +88,39 @@ __device__ __forceinline__ void turns(const int* __restrict__ positions, const f
   }
 }
 
-// One unit of a row: 2 W values, zeros where there is nothing.
-template <class C, int DT> __device__ __forceinline__ void load_unit(const typename Elem<DT>::type* __restrict__ row, int u, float (&x)[2 * C::W]) {
-  typedef Row<C> R;
+// The units of a row that are this lane's, as they lie in memory; zeros where there is nothing.
+template <class C, int DT> struct Units {
+  typedef typename Raw<DT, C::W>::type V;
+  V v[Row<C>::PER][2];
+  __device__ __forceinline__ void load(const typename Elem<DT>::type* __restrict__ row, bool here) {
+    typedef Row<C> R;
 #pragma unroll
-  for (int i = 0; i < 2 * C::W; ++i) x[i] = 0.0f;
-  if (!R::has(u)) return;
-  load<DT, C::W>(row + R::first(u), x);
-  if (R::both(u)) load<DT, C::W>(row + R::second(u), x + C::W);
-}
-template <class C> __device__ __forceinline__ void store_unit(typename Elem<C::DT>::type* __restrict__ row, int u, const float (&x)[2 * C::W]) {
+    for (int i = 0; i < R::PER; ++i) {
+      const int u = (int)(threadIdx.x % C::LANES) + i * C::LANES;
+      v[i][0] = v[i][1] = V{};
+      if (!here || !R::has(u)) continue;
+      v[i][0] = *(const V*)(row + R::first(u));
+      if (R::both(u)) v[i][1] = *(const V*)(row + R::second(u));
+    }
+  }
+  __device__ __forceinline__ void widen_to(float (&x)[Row<C>::PER][2 * C::W]) const {
+#pragma unroll
+    for (int i = 0; i < Row<C>::PER; ++i) {
+      widen<DT, C::W>(v[i][0], x[i]);
+      widen<DT, C::W>(v[i][1], x[i] + C::W);
+    }
+  }
+};
+template <class C> __device__ __forceinline__ void store_row(typename Elem<C::DT>::type* __restrict__ row, const float (&x)[Row<C>::PER][2 * C::W]) {
   typedef Row<C> R;
-  if (!R::has(u)) return;
-  store<C::DT, C::W>(row + R::first(u), x);
-  if (R::both(u)) store<C::DT, C::W>(row + R::second(u), x + C::W);
+  typedef typename Raw<C::DT, C::W>::type V;
+#pragma unroll
+  for (int i = 0; i < R::PER; ++i) {
+    const int u = (int)(threadIdx.x % C::LANES) + i * C::LANES;
+    if (!R::has(u)) continue;
+    *(V*)(row + R::first(u)) = narrow<C::DT, C::W>(x[i]);
+    if (R::both(u)) *(V*)(row + R::second(u)) = narrow<C::DT, C::W>(x[i] + C::W);
+  }
 }
 
 // The unit turned (BACK: turned back) by its cosines and sines.
@@ -136,29 +164,29 @@ template <class C, int H> __device__ __forceinline__ bool place(long t0, int row
   return t < C::TT && t0 + t < C::TOKENS;
 }
 
-// The H heads of each token of the tile, x to y. `first` has begun to load already: the rows that the workgroup starts with.
+// The first rows of the tile that are this lane's, on their way.
+template <class C, int H, int DT> __device__ __forceinline__ void start(const typename Elem<DT>::type* __restrict__ x, long t0, Units<C, DT>& next) {
+  int t;
+  long at;
+  const bool here = place<C, H>(t0, threadIdx.x / C::LANES, t, at);
+  next.load(x + (here ? at : 0), here);
+}
+
+// The H heads of each token of the tile, x to y; `next`: its first rows. The rows after are on their way while some are worked on.
 template <class C, int H>
 __device__ __forceinline__ void rotate_rows(const typename Elem<C::DT>::type* __restrict__ x, typename Elem<C::DT>::type* __restrict__ y,
                                             const float (&gain)[Row<C>::PER][2 * C::W], long t0, const float (*c)[C::F], const float (*s)[C::F],
-                                            float (&next)[Row<C>::PER][2 * C::W]) {
+                                            Units<C, C::DT>& next) {
   typedef Row<C> R;
   constexpr int AT_ONCE = 256 / C::LANES;
   const int lane = threadIdx.x % C::LANES;
   for (int row = threadIdx.x / C::LANES; row < C::TT * H; row += AT_ONCE) {
     float v[R::PER][2 * C::W];
-    int t;
-    long at;
-    const bool here = place<C, H>(t0, row, t, at);
-#pragma unroll
-    for (int u = 0; u < R::PER; ++u)
-#pragma unroll
-      for (int i = 0; i < 2 * C::W; ++i) v[u][i] = next[u][i];
-    int nt;
-    long nat;
-    if (place<C, H>(t0, row + AT_ONCE, nt, nat)) {
-#pragma unroll
-      for (int u = 0; u < R::PER; ++u) load_unit<C, C::DT>(x + nat, lane + u * C::LANES, next[u]);
-    }
+    int t, nt;
+    long at, nat;
+    const bool here = place<C, H>(t0, row, t, at), more = place<C, H>(t0, row + AT_ONCE, nt, nat);
+    next.widen_to(v);
+    if (more) next.load(x + nat, true);
     if constexpr (C::NORM) {
       float sum = 0.0f;
 #pragma unroll
@@ -173,32 +201,17 @@ __device__ __forceinline__ void rotate_rows(const typename Elem<C::DT>::type* __
     }
     if (!here) continue;
 #pragma unroll
-    for (int u = 0; u < R::PER; ++u) {
-      turn_unit<C, false>(lane + u * C::LANES, c[t], s[t], v[u]);
-      store_unit<C>(y + at, lane + u * C::LANES, v[u]);
-    }
-  }
-}
-
-template <class C, int H>
-__device__ __forceinline__ void first_rows(const typename Elem<C::DT>::type* __restrict__ x, long t0, float (&next)[Row<C>::PER][2 * C::W]) {
-  int t;
-  long at;
-#pragma unroll
-  for (int u = 0; u < Row<C>::PER; ++u)
-#pragma unroll
-    for (int i = 0; i < 2 * C::W; ++i) next[u][i] = 0.0f;
-  if (place<C, H>(t0, threadIdx.x / C::LANES, t, at)) {
-#pragma unroll
-    for (int u = 0; u < Row<C>::PER; ++u) load_unit<C, C::DT>(x + at, threadIdx.x % C::LANES + u * C::LANES, next[u]);
+    for (int u = 0; u < R::PER; ++u) turn_unit<C, false>(lane + u * C::LANES, c[t], s[t], v[u]);
+    store_row<C>(y + at, v);
   }
 }
 
 template <class C>
 __device__ __forceinline__ void load_gain(const typename Elem<C::GT>::type* __restrict__ gain, float (&g)[Row<C>::PER][2 * C::W]) {
   if constexpr (C::NORM) {
-#pragma unroll
-    for (int u = 0; u < Row<C>::PER; ++u) load_unit<C, C::GT>(gain, threadIdx.x % C::LANES + u * C::LANES, g[u]);
+    Units<C, C::GT> raw;
+    raw.load(gain, true);
+    raw.widen_to(g);
   }
 }
 
@@ -211,18 +224,19 @@ __device__ __forceinline__ void rotate(const typename Elem<C::DT>::type* __restr
   typedef Row<C> R;
   __shared__ __attribute__((aligned(16))) float c[C::TT][C::F], s[C::TT][C::F];
   const long t0 = (long)blockIdx.x * C::TT;
-  float next[R::PER][2 * C::W], gain[R::PER][2 * C::W];
-  if constexpr (C::HQ > 0) {
-    first_rows<C, C::HQ>(q, t0, next);
-    load_gain<C>(qgain, gain);
-  }
+  float gain[R::PER][2 * C::W];
+  Units<C, C::DT> queries, keys;
+  if constexpr (C::HQ > 0) start<C, C::HQ>(q, t0, queries);
+  if constexpr (C::HK > 0) start<C, C::HK>(k, t0, keys);
   turns<C>(positions, frequencies, axes, t0, c, s);
   __syncthreads();
-  if constexpr (C::HQ > 0) rotate_rows<C, C::HQ>(q, qout, gain, t0, c, s, next);
+  if constexpr (C::HQ > 0) {
+    load_gain<C>(qgain, gain);
+    rotate_rows<C, C::HQ>(q, qout, gain, t0, c, s, queries);
+  }
   if constexpr (C::HK > 0) {
-    first_rows<C, C::HK>(k, t0, next);
     load_gain<C>(kgain, gain);
-    rotate_rows<C, C::HK>(k, kout, gain, t0, c, s, next);
+    rotate_rows<C, C::HK>(k, kout, gain, t0, c, s, keys);
   }
 }
 
@@ -234,20 +248,21 @@ __device__ __forceinline__ void rotate(const typename Elem<C::DT>::type* __restr
 template <class C, int H>
 __device__ __forceinline__ void rotate_rows_grad(const typename Elem<C::DT>::type* __restrict__ dy, const typename Elem<C::DT>::type* __restrict__ x,
                                                  typename Elem<C::DT>::type* __restrict__ dx, const float (&gain)[Row<C>::PER][2 * C::W], long t0,
-                                                 const float (*c)[C::F], const float (*s)[C::F], float (&sums)[Row<C>::PER][2 * C::W]) {
+                                                 const float (*c)[C::F], const float (*s)[C::F], float (&sums)[Row<C>::PER][2 * C::W],
+                                                 Units<C, C::DT>& next_g, Units<C, C::DT>& next_x) {
   typedef Row<C> R;
   constexpr int AT_ONCE = 256 / C::LANES;
   const int lane = threadIdx.x % C::LANES;
   for (int row = threadIdx.x / C::LANES; row < C::TT * H; row += AT_ONCE) {
-    int t;
-    long at;
+    int t, nt;
+    long at, nat;
     if (!place<C, H>(t0, row, t, at)) break;  // (the lanes of a row are here or gone together)
     float g[R::PER][2 * C::W], v[R::PER][2 * C::W];
-#pragma unroll
-    for (int u = 0; u < R::PER; ++u) load_unit<C, C::DT>(dy + at, lane + u * C::LANES, g[u]);
-    if constexpr (C::NORM) {
-#pragma unroll
-      for (int u = 0; u < R::PER; ++u) load_unit<C, C::DT>(x + at, lane + u * C::LANES, v[u]);
+    next_g.widen_to(g);
+    if constexpr (C::NORM) next_x.widen_to(v);
+    if (place<C, H>(t0, row + AT_ONCE, nt, nat)) {
+      next_g.load(dy + nat, true);
+      if constexpr (C::NORM) next_x.load(x + nat, true);
     }
 #pragma unroll
     for (int u = 0; u < R::PER; ++u) turn_unit<C, true>(lane + u * C::LANES, c[t], s[t], g[u]);
@@ -271,10 +286,7 @@ __device__ __forceinline__ void rotate_rows_grad(const typename Elem<C::DT>::typ
           g[u][i] = r * __builtin_fmaf(-n, mean, g[u][i] * gain[u][i]);
         }
     }
-    if (dx) {
-#pragma unroll
-      for (int u = 0; u < R::PER; ++u) store_unit<C>(dx + at, lane + u * C::LANES, g[u]);
-    }
+    if (dx) store_row<C>(dx + at, g);
   }
 }
 
@@ -322,11 +334,20 @@ __device__ __forceinline__ void rotate_grad(const typename Elem<C::DT>::type* __
 #pragma unroll
     for (int i = 0; i < 2 * C::W; ++i) sums[0][u][i] = sums[1][u][i] = 0.0f;
   for (long t0 = (long)blockIdx.x * C::TT; t0 < C::TOKENS; t0 += (long)gridDim.x * C::TT) {
+    Units<C, C::DT> gq, xq, gk, xk;
+    if constexpr (C::HQ > 0) {
+      start<C, C::HQ>(dq, t0, gq);
+      if constexpr (C::NORM) start<C, C::HQ>(q, t0, xq);
+    }
+    if constexpr (C::HK > 0) {
+      start<C, C::HK>(dk, t0, gk);
+      if constexpr (C::NORM) start<C, C::HK>(k, t0, xk);
+    }
     __syncthreads();
     turns<C>(positions, frequencies, axes, t0, c, s);
     __syncthreads();
-    if constexpr (C::HQ > 0) rotate_rows_grad<C, C::HQ>(dq, q, qout, gains[0], t0, c, s, sums[0]);
-    if constexpr (C::HK > 0) rotate_rows_grad<C, C::HK>(dk, k, kout, gains[1], t0, c, s, sums[1]);
+    if constexpr (C::HQ > 0) rotate_rows_grad<C, C::HQ>(dq, q, qout, gains[0], t0, c, s, sums[0], gq, xq);
+    if constexpr (C::HK > 0) rotate_rows_grad<C, C::HK>(dk, k, kout, gains[1], t0, c, s, sums[1], gk, xk);
   }
   if constexpr (C::NORM) {
     if (part) {
@@ -336,25 +357,26 @@ __device__ __forceinline__ void rotate_grad(const typename Elem<C::DT>::type* __
   }
 }
 
-// The workgroups' sums, 64 dims and sixteen strands of them to a workgroup of 1024; blockIdx.y: queries, keys.
+// The workgroups' sums, 32 dims and 32 strands of them to a workgroup of 1024; blockIdx.y: queries, keys.
 template <class C, int GROUPS>
 __device__ __forceinline__ void gain_sums(const float* __restrict__ part, typename Elem<C::GT>::type* __restrict__ qgain,
                                           typename Elem<C::GT>::type* __restrict__ kgain) {
-  __shared__ float lds[16][64];
-  const int d = blockIdx.x * 64 + (threadIdx.x & 63), strand = threadIdx.x >> 6;
+  __shared__ float lds[32][33];
+  const int lane = threadIdx.x & 31, d = blockIdx.x * 32 + lane, strand = threadIdx.x >> 5;
   typename Elem<C::GT>::type* const to = blockIdx.y ? kgain : qgain;
   float sum = 0.0f;
   if (d < C::D) {
-#pragma unroll 8
-    for (int g = strand; g < GROUPS; g += 16) sum += part[((long)g * 2 + blockIdx.y) * C::D + d];
+#pragma unroll 16
+    for (int g = strand; g < GROUPS; g += 32) sum += part[((long)g * 2 + blockIdx.y) * C::D + d];
   }
-  lds[strand][threadIdx.x & 63] = sum;
+  lds[strand][lane] = sum;
   __syncthreads();
-  if (strand != 0 || d >= C::D || !to) return;
-  sum = 0.0f;
+  // a row of lanes each adds up a dim
+  sum = lds[lane][strand];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sum += lds[i][threadIdx.x & 63];
-  to[d] = to_elem<C::GT>(sum);
+  for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor(sum, o, 64);
+  const int mine = blockIdx.x * 32 + strand;
+  if (lane == 0 && mine < C::D && to) to[mine] = to_elem<C::GT>(sum);
 }
 
 }  // namespace heads

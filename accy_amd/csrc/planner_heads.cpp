@@ -85,12 +85,17 @@ bool Planner::heads(uint32_t v) {
     const int64_t units = F / W + (D - 2 * F + 2 * W - 1) / (2 * W);
     int64_t lanes = 1;
     while (lanes < 64 && lanes < units) lanes *= 2;
-    // Tokens of a workgroup: more than one while that leaves eight workgroups for every CU; their cosines and sines fit 16 KB.
+    // Tokens of a workgroup's tile: more than one while tiles are left for every CU, the tile's rows are no more than a few rounds of the workgroup's
+    // lanes, and the tile's cosines and sines fit 16 KB. The gradient's workgroups, two to a CU, walk over the tiles (us, tiles at least / rounds / workgroups:
+    // 4001 x 15 heads of 96 f32 2048 / 4 / 1024 22.5, 1024 / 4 / 512 23.0, 512 / 8 / 512 20.2, 8192 x 20 x 128 bf16 36.3, 32.8, 31.3, 16000 x 5 x 256
+    // bf16 40.7, 34.6, 32.9); without it 1024 / 4, 2048 / 4, 1024 / 8 and 512 / 8 are within 2 % for 8192 x 32 x 128 bf16, 27.3, and 3000 x 32 x 80
+    // f32 takes 12.6, 13.9, 12.7, 13.0.
     const int64_t rows = (int64_t)(out[0] >= 0 || grad ? hq : 0) + (int64_t)(out[1] >= 0 || grad ? hk : 0);
+    const uint64_t least = grad ? 512 : 1024;
     int64_t tt = 1;
-    while (tt < 16 && tokens / (uint64_t)(2 * tt) >= 2048 && 2 * tt * F * 8 <= 16384 && tt * rows < 4 * 256 / lanes) tt *= 2;
+    while (tt < 16 && tokens / (uint64_t)(2 * tt) >= least && 2 * tt * F * 8 <= 16384 && tt * rows < (grad ? 8 : 4) * 256 / lanes) tt *= 2;
     const uint64_t tiles = (tokens + (uint64_t)tt - 1) / (uint64_t)tt;
-    const uint64_t groups = grad ? std::max<uint64_t>(1, std::min<uint64_t>(tiles, 1024)) : tiles;
+    const uint64_t groups = grad ? std::max<uint64_t>(1, std::min<uint64_t>(tiles, 512)) : tiles;
     require(launchable(groups, 256), op, "more workgroups than a launch takes");
     const std::string nm = name(grad ? "heads_grad" : "heads", v);
     char e[64];
@@ -100,7 +105,7 @@ bool Planner::heads(uint32_t v) {
     const std::string head = "#include \"heads\"\nstruct Cfg_" + nm + " {\n  static constexpr int DT = " + num(dt) + ", GT = " + num(gt) + ", D = " + num(D) + ", F = " +
                              num(F) + ", HQ = " + num(grad || out[0] >= 0 ? (int64_t)hq : 0) + ", HK = " + num(grad || out[1] >= 0 ? (int64_t)hk : 0) +
                              ", AXES = " + num(several ? std::max<int64_t>(1, last(pt)) : 0) + ", W = " + num(W) + ", LANES = " + num(lanes) + ", TT = " + num(tt) +
-                             ";\n  static constexpr bool NEIGHBOURS = " + (neighbours ? "true" : "false") + ", NORM = " + (norm ? "true" : "false") +
+                             ";\n  static constexpr bool NEIGHBOURS = " + (neighbours ? "true" : "false") + ", NORM = " + (norm ? "true" : "false")  +
                              ";\n  static constexpr long TOKENS = " + std::to_string(tokens) + ";\n  static constexpr float EPS = " + eps_text + ";\n};\n";
     require(!several || last(pt) > 0 || tokens == 0, op, "positions without an axis");
     KernelWriter w(g_, slots_, "i64_t");
@@ -139,7 +144,7 @@ bool Planner::heads(uint32_t v) {
       s.name = name("heads_gain", v);
       s.source = head + "extern \"C\" __global__ void __launch_bounds__(1024) " + s.name + "(" + sw.params() + ") {\n  accy::heads::gain_sums<Cfg_" + nm + ", " +
                  std::to_string(groups) + ">(" + p + ", " + a + ", " + b + ");\n}\n";
-      s.grid[0] = (uint32_t)((D + 63) / 64);
+      s.grid[0] = (uint32_t)((D + 31) / 32);
       s.grid[1] = 2;
       s.block[0] = 1024;
       s.klass = "heads";

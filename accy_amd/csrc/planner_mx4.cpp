@@ -522,10 +522,13 @@ void Planner::mx4_attend(uint32_t v) {
     // Up to three workgroups share a CU. Fewer sequences and heads than 256 are split along their keys till 512 workgroups are at
     // work (8 x 16 heads x 4096 keys of 128 bf16: 31.5 us in 1, 20.9 in 2, 18.5 in 4, 18.7 in 6 and 8 splits), more of them till
     // uneven lengths even out (48 x 8 x 16000: 155 in 1, 119 to 125 in 2 to 8), each split with four steps of every wave at least.
-    const int64_t steps = (maxp * c.tokens + 31) / 32, want = wgs >= 256 ? 1024 : 512;
+    // Beside shared keys one workgroup a CU is enough: the prefixes' are at work too (64 x 4 heads x 1024 own keys behind 8192 shared ones 27.8 us
+    // in 1, 30.0 in 2).
+    const int64_t steps = (maxp * c.tokens + 31) / 32, want = shared ? 256 : wgs >= 256 ? 1024 : 512;
     const int64_t splits = opt_.allow_split ? std::max<int64_t>(1, std::min<int64_t>({(want + wgs - 1) / wgs, steps / 16, 64})) : 1;
     require(launchable((uint64_t)wgs, 256), op, "more workgroups than a launch takes");
-    // A prefix's rows, sixteen to a workgroup, against its keys: split till two workgroups are at work on every CU.
+    // A prefix's rows, sixteen to a workgroup, against its keys: split till two workgroups are at work on every CU (us, till 256 / 512 / 768 / 1024
+    // workgroups: 64 x 4 heads x 4 rows, 8192 shared keys of 128 bf16, 33.9 / 27.8 / 32.8 / 32.4, 128 x 8 x 4 x 16384 129 / 106 / 111 / 110).
     const int64_t prefix_groups = shared ? seqs * Q * G / 16 + prefixes : 0, prefix_steps = (prefix_maxp * c.tokens + 31) / 32;
     const int64_t rows = std::max<int64_t>(1, (seqs * Q * G + 15) / 16);
     const int64_t prefix_splits = !shared ? 0 : opt_.allow_split ? std::max<int64_t>(1, std::min<int64_t>({(512 + H * rows - 1) / (H * rows), prefix_steps / 16, 64})) : 1;
