@@ -20,7 +20,7 @@ struct CheckLogits {
 };
 template <long PAGES, long R, bool W = false> struct CheckFork {
   static constexpr bool WIDE = W;
-  static constexpr long SEQS = 20, ROWS = R, SLOTS = 9, P = PAGES, T = 64, ENTRIES = 180, MOVES = 50;
+  static constexpr long SEQS = 20, ROWS = R, SLOTS = 9, P = PAGES, T = 64, NEW = 2, ENTRIES = 180, MOVES = 50;
 };
 struct CheckCopy {
   static constexpr long N = 30, P = 100, BYTES = 8704, PER = 8192;
@@ -60,12 +60,12 @@ extern "C" __global__ void __launch_bounds__(256) check_grad_split(const u16_t* 
 }
 
 extern "C" __global__ void __launch_bounds__(1024) check_fork(const int* t, const int* l, const int* p, const int* r, const u8_t* h, int* a, int* b, int* c,
-                                                              int* d, int* e) {
-  accy::pages::fork<CheckFork<1000, 20>>(t, l, p, r, h, a, b, c, d, e, nullptr);
+                                                              int* d, int* e, int* s) {
+  accy::pages::fork<CheckFork<1000, 20>>(t, l, p, r, h, a, b, c, d, e, s, nullptr);
 }
 extern "C" __global__ void __launch_bounds__(1024) check_fork_large(const int* t, const int* l, const int* p, const int* r, const u8_t* h, int* a, int* b, int* c,
-                                                                    int* d, int* e, int* work) {
-  accy::pages::fork<CheckFork<1000000, 2000, true>>(t, l, p, r, h, a, b, c, d, e, work);
+                                                                    int* d, int* e, int* s, int* work) {
+  accy::pages::fork<CheckFork<1000000, 2000, true>>(t, l, p, r, h, a, b, c, d, e, s, work);
 }
 extern "C" __global__ void __launch_bounds__(256) check_fork_rows(const int* t, const int* work, int* a) { accy::pages::fork_rows<CheckFork<1000000, 2000, true>>(t, work, a); }
 extern "C" __global__ void __launch_bounds__(1024) check_compact(const int* t, const u8_t* h, int* a, int* b, int* c) {

@@ -30,12 +30,13 @@ template <int DT> __device__ __forceinline__ float from_elem(typename Elem<DT>::
   else if constexpr (DT == 1) return f16_to_f32(v);
   else return v;
 }
-// W numbers as they lie in memory: one access.
+// W numbers as they lie in memory: one access (two of 32 bytes).
 template <int BYTES> struct Bits;
 template <> struct Bits<2> { typedef u16_t type; };
 template <> struct Bits<4> { typedef u32_t type; };
 template <> struct Bits<8> { typedef u32_t type __attribute__((ext_vector_type(2))); };
 template <> struct Bits<16> { typedef u32_t type __attribute__((ext_vector_type(4))); };
+template <> struct Bits<32> { typedef u32_t type __attribute__((ext_vector_type(8), aligned(16))); };  // gains of f32 beside 16-bit heads
 template <int DT, int W> struct Raw { typedef typename Bits<W * (DT == 2 ? 4 : 2)>::type type; };
 template <class T, int W> struct alignas(W * sizeof(T) < 16 ? W * sizeof(T) : 16) Chunk { T v[W]; };
 template <int DT, int W> __device__ __forceinline__ void widen(const typename Raw<DT, W>::type& raw, float* x) {

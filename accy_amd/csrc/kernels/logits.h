@@ -101,7 +101,8 @@ struct Sums {
   float m = -__builtin_inff(), l = 0.0f, s = 0.0f;
   // The same measured from another m.
   __device__ __forceinline__ void rebase(float to) {
-    const float shift = fmaxf((base_of(m) - base_of(to)) * L2E, LEAST), scale = __builtin_amdgcn_exp2f(l == 0.0f ? LEAST : shift);
+    // (a sum of nothing is measured from nothing: its shift may be beyond f32)
+    const float shift = l == 0.0f ? 0.0f : fmaxf((base_of(m) - base_of(to)) * L2E, LEAST), scale = __builtin_amdgcn_exp2f(shift);
     s = (s + l * shift) * scale;
     l *= scale;
     m = to;

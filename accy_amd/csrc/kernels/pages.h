@@ -95,7 +95,7 @@ template <long P> __device__ __forceinline__ u32_t held_word(const u8_t* __restr
 }
 
 // ---------------------------------------------------------------------------------------------
-// fork: C supplies SEQS, ROWS, SLOTS, P (pages), T (tokens of a page), WIDE (the tables are written by fork_rows).
+// fork: C supplies SEQS, ROWS, SLOTS, P (pages), T (tokens of a page), NEW (tokens of a row whose slots are asked for), WIDE (the tables are written by fork_rows).
 // ---------------------------------------------------------------------------------------------
 
 // What row r becomes: its parent (-1: empty), the parent's length, the slots that its tokens take and those that it is to have.
@@ -135,8 +135,8 @@ template <class C, bool LDS>
 __device__ __forceinline__ void fork_with(u32_t* map, int* counts, const int* __restrict__ table, const int* __restrict__ lengths,
                                           const int* __restrict__ parents, const int* __restrict__ room, const u8_t* __restrict__ held,
                                           int* __restrict__ out_table, int* __restrict__ out_lengths, int* __restrict__ source,
-                                          int* __restrict__ target, int* __restrict__ left, int* __restrict__ firsts, Row* __restrict__ rows,
-                                          int* __restrict__ fresh_pages) {
+                                          int* __restrict__ target, int* __restrict__ left, int* __restrict__ slots, int* __restrict__ firsts,
+                                          Row* __restrict__ rows, int* __restrict__ fresh_pages) {
   constexpr long WORDS = (C::P + 31) / 32;
   constexpr int SLOTS = C::SLOTS > 0 ? (int)C::SLOTS : 1;
   // With a thread for every row its numbers stay in registers; else they are formed again where they are needed.
@@ -254,6 +254,17 @@ __device__ __forceinline__ void fork_with(u32_t* map, int* counts, const int* __
       source[r] = page >= 0 ? old : -1;
       target[r] = page;
       if constexpr (C::WIDE) rows[r] = Row{mine.parent, stays, (int)first, wanted};
+      // the slots of the row's next tokens, those that it has room for
+      const int more = C::NEW > 0 ? room[r] : 0;
+      for (int i = 0; i < C::NEW; ++i) {
+        const long token = (long)mine.length + i;
+        int p = -1;
+        if (mine.parent >= 0 && i < more && token < C::SLOTS * C::T) {
+          const int k = (int)(token / C::T) - stays;
+          p = k < 0 ? page_at<C>(table, mine.parent, (int)(token / C::T)) : fresh(first + k);
+        }
+        slots[r * C::NEW + i] = p < 0 ? -1 : (int)(p * C::T + token % C::T);
+      }
     }
     if constexpr (!C::WIDE) {
       parent[tid] = mine.parent;
@@ -292,12 +303,12 @@ template <class C>
 __device__ __forceinline__ void fork(const int* __restrict__ table, const int* __restrict__ lengths, const int* __restrict__ parents,
                                      const int* __restrict__ room, const u8_t* __restrict__ held, int* __restrict__ out_table,
                                      int* __restrict__ out_lengths, int* __restrict__ source, int* __restrict__ target, int* __restrict__ left,
-                                     int* work) {
+                                     int* __restrict__ slots, int* work) {
   typedef ForkWork<C> W;
   __shared__ u32_t map[W::LDS ? W::WORDS + 1 : 1];
   __shared__ int counts[W::LDS ? W::WORDS + 1 : 1];
   fork_with<C, W::LDS>(W::LDS ? map : (u32_t*)work, W::LDS ? counts : work + W::WORDS, table, lengths, parents, room, held, out_table, out_lengths, source,
-                       target, left, work + W::FIRSTS, (Row*)(work + W::ROWS), work + W::FRESH);
+                       target, left, slots, work + W::FIRSTS, (Row*)(work + W::ROWS), work + W::FRESH);
 }
 // Large tables: 1024 slots of a row to a workgroup.
 template <class C>

@@ -101,10 +101,21 @@ void Planner::mark_custom_operands() {
 }
 
 // The cache's own buffer may be the result's where the caller hands it in, gets it back, and nothing else of the program
-// reads what was in it; else the whole cache is copied first. Returns the result's slot.
+// reads what was in it; else the whole cache is copied first. A result that only another update reads is that one's buffer already. Returns the
+// result's slot.
 int Planner::updated_cache(uint32_t v) {
   const Op& op = g_.ops[v];
+  uint32_t end = v;
+  while (!is_output_[end] && users_[end].size() == 1) {
+    const uint32_t u = users_[end][0];
+    const Op& uo = g_.ops[u];
+    const bool update = uo.kind == Kind::custom_call && uo.index == 1 && (uo.bytes == "accy.mx4.cache_write" || uo.bytes == "accy.pages.copy");
+    if (!update || uo.args.empty() || uo.args[0] != end || !(uo.result == op.result)) break;
+    end = u;
+  }
+  if (end != v && slots_.slot_of[v] < 0) slots_.slot_of[v] = temp_slot(end);
   const int old = dense_slot(op.args[0]), out = temp_slot(v);
+  if (old == out) return out;
   Step copy;
   copy.type = Step::Copy;
   copy.copy.src = old;

@@ -1,8 +1,8 @@
 // Custom calls on the pages of a cache (kernels/pages.h), "accy.pages.<name>":
 //
-//   fork_table, fork_lengths, fork_source, fork_target, fork_left(group(table, lengths), group(parents, room), held, page)
+//   fork_table, fork_lengths, fork_source, fork_target, fork_left, fork_slots(group(table, lengths), group(parents, room), held, page)
 //       table i32 [seq, slot], lengths i32 [seq], parents, room i32 [row], held i1 [page], page an i32 constant -> i32 [row, slot], [row], [row],
-//       [row], []: planned as one kernel
+//       [row], [], [row] or [row, token]: planned as one kernel
 //   compact_table, compact_source, compact_target(table, held)   table i32 [seq, slot], held i1 [page] -> as the table, i32 [move] twice
 //   copy(cache, source, target)   cache [page, ..], i32 [copy] twice -> the cache
 #include "planner_custom.hpp"
@@ -36,13 +36,25 @@ void Planner::pages_fork(uint32_t v) {
   require(page >= 1 && page < (1 << 20), op, "the size of a page is an i32 constant of 1 to 2^20");
   const int64_t seqs = tt.dims[0].extent, slots = tt.dims[1].extent, rows = pt.dims[0].extent, pages = ht.dims[0].extent;
   require(pages <= kMostPages, op, "more than 2^24 pages");
+  require(pages < (int64_t(1) << 31) / page && slots < (int64_t(1) << 31) / page, op, "2^31 slots or more");
   require(slots < (int64_t(1) << 31) && rows < (int64_t(1) << 31) && rows * std::max<int64_t>(1, slots) < (int64_t(1) << 31), op, "2^31 entries or more");
   const auto calls = siblings(v, "accy.pages.fork_");
-  const char* const names[] = {"table", "lengths", "source", "target", "left"};
-  std::vector<int> out(5, -1);
+  const char* const names[] = {"table", "lengths", "source", "target", "left", "slots"};
+  std::vector<int> out(6, -1);
   std::vector<uint32_t> made;
-  for (size_t i = 0; i < 5; ++i) {
+  int64_t tokens = 0;  // of a row, whose slots are asked for
+  for (size_t i = 0; i < 6; ++i) {
     const auto call = calls.find(names[i]);
+    if (i == 5) {
+      if (call == calls.end()) break;
+      const Type& t = g_.ops[call->second].result;
+      require((whole_numbers(t, 1) || whole_numbers(t, 2)) && t.dims[0].extent == rows && (t.rank() == 1 || (last(t) >= 1 && last(t) <= 1024)),
+              g_.ops[call->second], "the result is i32 [row] or [row, token], of up to 1024 tokens");
+      tokens = t.rank() == 1 ? 1 : last(t);
+      out[i] = temp_slot(call->second);
+      made.push_back(call->second);
+      break;
+    }
     const uint64_t bytes = i == 0 ? (uint64_t)(rows * slots) * 4 : i == 4 ? 4 : (uint64_t)rows * 4;
     if (call == calls.end()) {
       out[i] = slots_.add(SlotInfo::Temp, -1, DType::i32, bytes);  // what nobody reads is written all the same
@@ -66,12 +78,12 @@ void Planner::pages_fork(uint32_t v) {
   KernelWriter w(g_, slots_, "i64_t");
   std::string args = w.arg(table, false) + ", ";
   for (const uint32_t a : {now[1], next[0], next[1], op.args[2]}) args += w.arg(dense_slot(a), false) + ", ";
-  for (size_t i = 0; i < 5; ++i) args += (i == 0 && wide ? std::string("nullptr") : w.arg(out[i], true)) + ", ";
+  for (size_t i = 0; i < 6; ++i) args += ((i == 0 && wide) || out[i] < 0 ? std::string("nullptr") : w.arg(out[i], true)) + ", ";
   args += work ? w.arg(ws, true) : "nullptr";
   KernelStep k;
   const std::string nm = name("fork", v);
   const std::string head = "#include \"pages\"\nstruct Cfg_" + nm + " {\n  static constexpr long SEQS = " + num(seqs) + ", ROWS = " + num(rows) + ", SLOTS = " + num(slots) +
-                           ", P = " + num(pages) + ", T = " + num(page) + ";\n  static constexpr bool WIDE = " + (wide ? "true" : "false") + ";\n};\n";
+                           ", P = " + num(pages) + ", T = " + num(page) + ", NEW = " + num(tokens) + ";\n  static constexpr bool WIDE = " + (wide ? "true" : "false") + ";\n};\n";
   k.source = head + "extern \"C\" __global__ void __launch_bounds__(1024) " + nm + "(" + w.params() + ") {\n  accy::pages::fork<Cfg_" + nm + ">(" + args + ");\n}\n";
   k.name = nm;
   k.block[0] = 1024;

@@ -519,13 +519,15 @@ class LogProbs:
 @dataclass(frozen=True)
 class ForkedPages:
     """Page tables for the next step (``Builder.fork_pages``): ``pages`` i32 [row, slot], ``lengths`` i32 [row], the page that
-    each row copies (``source``) and to which (``target``), i32 [row], -1 for none, and ``left`` i32 [], the free pages left (below
-    zero: so many were asked for in vain)."""
+    each row copies (``source``) and to which (``target``), i32 [row], -1 for none, ``left`` i32 [], the free pages left (below
+    zero: so many were asked for in vain), and ``slots`` i32 [row] or [row, token], where in the cache the keys and values of each row's next tokens go
+    (-1: no page, or no room asked for)."""
     pages: Value
     lengths: Value
     source: Value
     target: Value
     left: Value
+    slots: Value
 
 
 @dataclass(frozen=True)
@@ -1248,8 +1250,8 @@ class Builder:
         if table.ty.rank != 2 or held.ty.rank != 1:
             raise TensorError("RankMismatch", "page tables are [seq, slot], held pages [page]")
 
-    def fork_pages(self, table: Value, lengths: Value, parents: Value, room: Value, held: Value, page: int) -> ForkedPages:
-        """The page tables of the next step's rows, from those of this step's sequences.
+    def fork_pages(self, table: Value, lengths: Value, parents: Value, room: Value, held: Value, page: int, tokens: int = 1) -> ForkedPages:
+        """The page tables of the next step's rows, from those of this step's sequences, and the slots of each row's next ``tokens`` tokens.
 
         ``table`` i32 [seq, slot] and ``lengths`` i32 [seq] as in ``attend_mx4``; row r goes on as sequence parents[r] (i32 [row];
         several rows with one parent: forked; outside those there are: the row is empty) and gets pages for room[r] (i32 [row]) more tokens,
@@ -1270,11 +1272,14 @@ class Builder:
             raise TensorError("ShapeMismatch", "lengths are [seq], room as parents")
         if not 1 <= page < 1 << 20:
             raise TensorError("InvalidDimension", f"{page} tokens to a page")
+        if not 1 <= tokens <= 1024:
+            raise TensorError("InvalidDimension", f"slots of {tokens} tokens")
         row, slot = parents.ty.dims[0], table.ty.dims[1]
         # the size of a page as an operand, since a call has no other place for it
         operands = [self._group(table, lengths), self._group(parents, room), held, self.full("i32", page)]
         one = lambda name, *dims: self.custom_call(f"accy.pages.fork_{name}", 1, operands, Type("i32", tuple(dims)))
-        return ForkedPages(one("table", row, slot), one("lengths", row), one("source", row), one("target", row), one("left"))
+        return ForkedPages(one("table", row, slot), one("lengths", row), one("source", row), one("target", row), one("left"),
+                           one("slots", row) if tokens == 1 else one("slots", row, ("token", tokens)))
 
     def compact_pages(self, table: Value, held: Value, moves: Dim) -> CompactedPages:
         """Tables whose pages lie together at the lowest numbers. Of n pages that a table names or that are ``held``, those from n on that are

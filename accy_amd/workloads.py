@@ -332,6 +332,42 @@ def decoder_step_mx4_program(seqs: int = 64, model: int = 2048, heads: int = 16,
     return T.define("decoder_step_mx4", specs, body)
 
 
+def answers_step_mx4_program(seqs: int = 64, rows: int = 64, model: int = 2048, heads: int = 16, kv_heads: int = 4, hd: int = 128, vocab: int = 32000,
+                             pages: int = 4096, page: int = 64, slots: int = 64, prefixes: int = 1, prefix_pages: int = 128, top: int = 5,
+                             dtype: str = "bf16") -> T.Program:
+    """One token of each of ``rows`` answers to a few prompts, from their pages to their log probabilities: page tables forked from
+    the last step's ``seqs`` sequences and the partly filled pages that they share copied, an attention layer (norms of its heads, rotation by position, the new
+    keys and values into the cache, attention over the prompts' shared pages and the answers' own), and the log probabilities of given tokens.
+
+    Inputs: x [row, model], the norm's gains, Wq, Wk, Wv, Wo (codes and scales each), the query and key heads' gains, positions, frequencies, the last
+    norm's gains, the vocabulary's weights (codes and scales), the cache, the page table, lengths, parents, room, the held pages (the prompts' among
+    them), the prompts' pages and lengths, each row's prompt, the tokens. Outputs: log probabilities, entropies, the top alternatives and their tokens, the new
+    page table, the lengths with this token, and the cache, which may be the input cache's buffer."""
+    def body(b: T.Builder, args: List[T.Value]) -> List[T.Value]:
+        x, g, wq, wk, wv, wo = args[0], args[1], *(b.mx4(args[i], args[i + 1], n) for i, n in ((2, "model"), (4, "model"), (6, "model"), (8, "att")))
+        qg, kg, positions, frequencies, g2, head = *args[10:15], b.mx4(args[15], args[16], "model")
+        cache, table, lengths, parents, room, held, prefix_table, prefix_lengths, of, tokens = args[17:]
+        now = b.fork_pages(table, lengths, parents, room, held, page)
+        cache = cache.copy_pages(now.source, now.target)
+        h = rms_norm(b, x, g, "model", dtype).quantize_mx4("model")
+        q, k = b.rotate_heads(h.contract(wq, dtype), h.contract(wk, dtype), T.Rotation(positions, frequencies), T.HeadNorm(qg, kg))
+        cache = cache.cache_write_mx4(k, h.contract(wv, dtype), now.slots)
+        grown = now.lengths.add(b.full("i32", 1, ("row", rows)))
+        o = q.attend_mx4(cache, now.pages, grown, shared=(prefix_table, prefix_lengths, of))
+        y = x.add(o.merge(("head", "dim"), "att").quantize_mx4("att").contract(wo, dtype))
+        logits = rms_norm(b, y, g2, "model", dtype).quantize_mx4("model").contract(head, "f32")
+        p = logits.log_probs(tokens, "vocab", top=top)
+        return [p.token, p.entropy, p.top, p.top_tokens, now.pages, grown, cache]
+    kv = T.mx4_specs("model", kv_head=kv_heads, dim=hd, model=model)
+    row = T.spec("i32", row=rows)
+    specs = [T.spec(dtype, row=rows, model=model), T.spec(dtype, model=model), *T.mx4_specs("model", head=heads, dim=hd, model=model), *kv, *kv,
+             *T.mx4_specs("att", model=model, att=heads * hd), T.spec(dtype, dim=hd), T.spec(dtype, dim=hd), row, T.spec("f32", pair=hd // 2),
+             T.spec(dtype, model=model), *T.mx4_specs("model", vocab=vocab, model=model), T.cache_mx4_spec(pages, kv_heads, hd, page),
+             T.spec("i32", seq=seqs, slot=slots), T.spec("i32", seq=seqs), row, row, T.spec("i1", page=pages),
+             T.spec("i32", prefix=prefixes, prefix_page=prefix_pages), T.spec("i32", prefix=prefixes), row, row]
+    return T.define("answers_step_mx4", specs, body)
+
+
 CONFIGS: Dict[str, dict] = {
     "c1-tone": dict(program=tone_program, inputs=tone_inputs, kw=dict(guesses=8192, points=16384)),
     "c2-lse": dict(program=logsumexp_program, inputs=logsumexp_inputs, kw=dict(rows=32768, features=8192)),
