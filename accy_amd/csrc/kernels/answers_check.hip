@@ -17,6 +17,7 @@ template <int D_, long VOCAB, int TOP, int S, int THREADS, int CHUNKS>
 struct CheckLogits {
   static constexpr int DT = D_, K = TOP, SPLITS = S, NT = THREADS, U = CHUNKS;
   static constexpr long ROWS = 77, V = VOCAB;
+  static constexpr bool ONCE = S == 1;
 };
 template <long PAGES, long R, bool W = false> struct CheckFork {
   static constexpr bool WIDE = W;

@@ -15,7 +15,7 @@
 // are a lane's each.
 //
 // C supplies DT (0 bf16, 1 f16, 2 f32), ROWS, V (elements of a row), K (alternatives, 0: none), SPLITS (workgroups of a row), NT (threads), U
-// (chunks that a thread holds at once).
+// (chunks that a thread holds at once), ONCE (with the non-temporal hint).
 #pragma once
 
 namespace accy {
@@ -107,13 +107,6 @@ struct Sums {
     l *= scale;
     m = to;
   }
-  __device__ __forceinline__ void join(Sums o) {
-    const float top = fmaxf(m, o.m);
-    rebase(top);
-    o.rebase(top);
-    l += o.l;
-    s += o.s;
-  }
 };
 
 // Of a thread's U chunks, `first` its first one, those before `to`.
@@ -125,7 +118,10 @@ template <class C> __device__ __forceinline__ int present(int first, int to) {
 template <class C> __device__ __forceinline__ const u32x4& chunk(const typename Elem<C::DT>::type* base, int c) { return *(const u32x4*)((const u8_t*)base + (u32_t)c * 16u); }
 template <class C> __device__ __forceinline__ void fetch(const Range<C>& r, int first, int n, u32x4 (&w)[C::U]) {
   each<C::U>([&](auto u) {
-    if (u.value < n) w[u.value] = chunk<C>(r.base, first + u.value * C::NT);
+    if (u.value < n) {
+      if constexpr (C::ONCE) w[u.value] = __builtin_nontemporal_load(&chunk<C>(r.base, first + u.value * C::NT));
+      else w[u.value] = chunk<C>(r.base, first + u.value * C::NT);
+    }
   });
 }
 template <class C> __device__ __forceinline__ float largest(const u32x4& w) {
@@ -438,12 +434,16 @@ __device__ __forceinline__ void log_probs(const typename Elem<C::DT>::type* __re
   }
 }
 
-// A row's parts joined, in split order.
+// A row's parts joined, a lane's each (there are 64 at most): the same in all threads.
 template <class C> __device__ __forceinline__ Sums join_sums(const float* __restrict__ part, long row) {
+  static_assert(C::SPLITS <= 64, "a wave holds a row's parts");
   const Part<C>* const from = (const Part<C>*)part + row * C::SPLITS;
+  const int lane = threadIdx.x & 63;
   Sums a;
-#pragma unroll 4
-  for (int z = 0; z < C::SPLITS; ++z) a.join(from[z].a);
+  if (lane < C::SPLITS) a = from[lane].a;
+  a.rebase(wave_reduce(a.m, MaxOp()));
+  a.l = wave_reduce(a.l, SumOp());
+  a.s = wave_reduce(a.s, SumOp());
   return a;
 }
 template <class C>
@@ -453,14 +453,30 @@ __device__ __forceinline__ void log_probs_join(const typename Elem<C::DT>::type*
   __shared__ List<C> list;
   const long row = blockIdx.x;
   const Part<C>* const from = (const Part<C>*)part + row * C::SPLITS;
+  const Sums a = join_sums<C>(part, row);
   if constexpr (C::K > 0) {
     static_assert(C::SPLITS * C::K <= List<C>::CAP, "the splits' keys fit a list");
-    // (a missing key, 0, is below all)
-    for (int i = threadIdx.x; i < C::SPLITS * C::K; i += C::NT) list.key[i] = from[i / C::K].key[i % C::K];
+    // Keys below what K of the threads' largest reach are left out before the others are ranked (512 keys 5 us otherwise).
+    constexpr int KEYS = C::SPLITS * C::K;
+    const int tid = threadIdx.x;
+    float most = -__builtin_inff();
+    for (int i = tid; i < KEYS; i += C::NT) {
+      const u64_t key = from[i / C::K].key[i % C::K];
+      if (key) most = fmaxf(most, value_of((u32_t)(key >> 32)));
+    }
+    const u32_t share = share_of<C>(most);
+    if ((tid & 63) == 0) list.share[0][tid >> 6] = share;
+    if (tid == 0) list.count[0] = 0;
     __syncthreads();
-    list.rank(C::SPLITS * C::K);
+    const u64_t bound = bound_of<C>(list.share[0]);
+    for (int i = tid; i < KEYS; i += C::NT) {
+      const u64_t key = from[i / C::K].key[i % C::K];
+      if (key >= bound) list.key[atomicAdd(&list.count[0], 1)] = key;
+    }
+    __syncthreads();
+    list.rank(list.count[0]);
   }
-  write<C>(x, tokens, row, join_sums<C>(part, row), list.best, token, entropies, top, top_tokens);
+  write<C>(x, tokens, row, a, list.best, token, entropies, top, top_tokens);
 }
 
 // ---- the gradient ----
@@ -516,7 +532,9 @@ __device__ __forceinline__ void put(typename Elem<C::DT>::type* __restrict__ to,
     if constexpr (C::DT == 2) o[i] = __builtin_bit_cast(u32_t, v[i]);
     else o[i] = (u32_t)to_elem<C::DT>(v[2 * i]) | (u32_t)to_elem<C::DT>(v[2 * i + 1]) << 16;
   }
-  *(u32x4*)((u8_t*)to + (u32_t)c * 16u) = o;
+  u32x4* const at = (u32x4*)((u8_t*)to + (u32_t)c * 16u);
+  if constexpr (C::ONCE) __builtin_nontemporal_store(o, at);
+  else *at = o;
 }
 template <class C> __device__ __forceinline__ void put_besides(typename Elem<C::DT>::type* __restrict__ to, const Slope<C>& k, int besides, float x) {
   if (besides >= 0) to[besides] = to_elem<C::DT>(slope<C, true>(k, x) + (besides == k.at ? k.g : 0.0f));

@@ -634,7 +634,7 @@ class Planner {
   int64_t logit_chunks(int64_t vocab, DType d) const;
   int64_t logit_splits(uint64_t rows, int64_t chunks, int64_t k) const;
   uint64_t logit_part(int64_t k) const;
-  std::string logit_config(const std::string& nm, int dt, uint64_t rows, int64_t vocab, int64_t k, int64_t splits, int64_t threads, int64_t u) const;
+  std::string logit_config(const std::string& nm, int dt, uint64_t rows, int64_t vocab, int64_t k, int64_t splits, int64_t threads, int64_t u, bool once) const;
 
   void mx4_quantize(uint32_t v);
   void mx4_values(uint32_t v);

@@ -18,6 +18,11 @@ bool rows_only(const Type& t, DType d, const Type& logits) {
   return true;
 }
 
+// Logits that the caches do not hold are read, and their gradient written, past them (us without / with the hint: gradients of 1001 x 50257 f16 55.4 / 49.8,
+// 512 x 50257 f32 50.6 / 42.8, 2048 x 32000 bf16 52.6 / 50.2; log probabilities 2048 x 50257 bf16 66.1 / 65.1, 1024 x 50257 f32 46.3 / 44.6, but 600
+// x 8000 bf16 9.1 / 9.5, 64 x 50257 13.8 / 14.3).
+bool past_caches(const Type& logits) { return logits.bytes() >= uint64_t(64) << 20; }
+
 }  // namespace
 
 // Chunks of a row at most: rows of whole chunks start on one, others anywhere.
@@ -26,9 +31,9 @@ int64_t Planner::logit_chunks(int64_t vocab, DType d) const {
   return vocab % per == 0 ? vocab / per : (vocab + 2 * per - 2) / per;
 }
 
-std::string Planner::logit_config(const std::string& nm, int dt, uint64_t rows, int64_t vocab, int64_t k, int64_t splits, int64_t threads, int64_t u) const {
+std::string Planner::logit_config(const std::string& nm, int dt, uint64_t rows, int64_t vocab, int64_t k, int64_t splits, int64_t threads, int64_t u, bool once) const {
   return "#include \"logits\"\nstruct Cfg_" + nm + " {\n  static constexpr int DT = " + num(dt) + ", K = " + num(k) + ", SPLITS = " + num(splits) + ", NT = " +
-         num(threads) + ", U = " + num(u) + ";\n  static constexpr long ROWS = " + std::to_string(rows) + ", V = " + num(vocab) + ";\n};\n";
+         num(threads) + ", U = " + num(u) + ";\n  static constexpr long ROWS = " + std::to_string(rows) + ", V = " + num(vocab) + ";\n  static constexpr bool ONCE = " + (once ? "true" : "false") + ";\n};\n";
 }
 
 // Workgroups of a row: one where there are rows enough, else till four workgroups for every CU are at work, each with a chunk for every
@@ -76,7 +81,7 @@ void Planner::logits_log_probs(uint32_t v) {
     // 5 / 8 chunks, 512 of 4: 2048 x 50257 bf16, 20 alternatives, 66 / 67 / 71 / 85, 1024 x 50257 f32 46 / 47 / 50 / 56, 600 x 131072 bf16, five, 53
     // / 53 / 53 / 59).
     const int64_t rounds = (mine + 256 * 4 - 1) / (256 * 4), u = std::max<int64_t>(1, (mine + 256 * rounds - 1) / (256 * rounds));
-    const std::string nm = name("log_probs", v), head = logit_config(nm, dt, rows, V, K, splits, 256, u);
+    const std::string nm = name("log_probs", v), head = logit_config(nm, dt, rows, V, K, splits, 256, u, past_caches(xt));
     auto results = [&](KernelWriter& w) {
       std::string s;
       for (int i = 0; i < 4; ++i) s += std::string(i ? ", " : "") + (out[i] >= 0 ? w.arg(out[i], true) : std::string("nullptr"));
@@ -130,6 +135,8 @@ void Planner::logits_grad(uint32_t v) {
     int slots[4];
     for (size_t i = 0; i < 4; ++i) slots[i] = dense_slot(op.args[i]);
     const int64_t chunks = logit_chunks(V, xt.dtype);
+    // Rows stay in the registers of one workgroup where there are rows for every CU (or they are short), in as few threads as hold them in eight chunks
+    // each: 1001 x 50257 f16 55 us with 1024 threads, 58 with 512, 69 with 256. Other rows are read twice, by several workgroups.
     int64_t threads = 256;
     while (threads < 1024 && (chunks + threads - 1) / threads > 8) threads *= 2;
     const int64_t u = (chunks + threads - 1) / threads;
@@ -155,12 +162,12 @@ void Planner::logits_grad(uint32_t v) {
       push(std::move(k), w);
     };
     if (u <= 16 && (rows >= 256 || chunks <= 512)) {
-      launch(nm, logit_config(nm, dt, rows, V, 0, 1, threads, u), "grad_row", false, -1, threads, 1);
+      launch(nm, logit_config(nm, dt, rows, V, 0, 1, threads, u, past_caches(xt)), "grad_row", false, -1, threads, 1);
     } else {
       const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({(int64_t)((1024 + rows - 1) / rows), chunks / 256, 64})), mine = (chunks + splits - 1) / splits;
       const int64_t rounds = (mine + 256 * 4 - 1) / (256 * 4);
       // (one split is written to the parts too: the kernels of a row's sums and of its gradient are two)
-      const std::string head = logit_config(nm, dt, rows, V, 0, std::max<int64_t>(2, splits), 256, std::max<int64_t>(1, (mine + 256 * rounds - 1) / (256 * rounds)));
+      const std::string head = logit_config(nm, dt, rows, V, 0, std::max<int64_t>(2, splits), 256, std::max<int64_t>(1, (mine + 256 * rounds - 1) / (256 * rounds)), false);
       const int part = slots_.add(SlotInfo::Temp, -1, DType::f32, rows * (uint64_t)std::max<int64_t>(2, splits) * logit_part(0));
       launch(name("log_probs_sums", v), head, "log_probs", true, part, 256, std::max<int64_t>(2, splits));
       launch(nm, head, "grad_split", false, part, 256, std::max<int64_t>(2, splits));
