@@ -27,7 +27,7 @@ void Planner::custom(uint32_t v) {
     const std::string pages = after("accy.pages.");
     if (pages == "copy") return operands(3), pages_copy(v);
     if (pages.compare(0, 5, "fork_") == 0) return operands(4), pages_fork(v);
-    if (pages.compare(0, 8, "compact_") == 0) return operands(2), pages_compact(v);
+    if (pages.compare(0, 8, "compact_") == 0) return operands(3), pages_compact(v);
     const std::string logits = after("accy.logits.");
     if (logits == "grad") return operands(4), logits_grad(v);
     if (logits == "token" || logits == "entropy" || logits == "top" || logits == "top_tokens") return operands(2), logits_log_probs(v);

@@ -626,6 +626,7 @@ class Planner {
   int updated_cache(uint32_t v);
 
   bool heads(uint32_t v);
+  int64_t whole_constant(uint32_t v) const;
   void pages_copy(uint32_t v);
   void pages_fork(uint32_t v);
   void pages_compact(uint32_t v);

@@ -506,6 +506,7 @@ void Planner::mx4_attend(uint32_t v) {
     require(oft.dtype == DType::i32 && oft.rank() == 1 && oft.dims[0].extent == seqs, op, "prefixes of sequences are i32 [seq]");
     require(prefix_maxp < (int64_t(1) << 31) / c.tokens, op, "a prefix has fewer than 2^31 keys");
     require(prefixes >= 1 && prefixes <= 1024, op, "1 to 1024 prefixes");  // their counts lie in a stage of LDS
+    require(seqs < (int64_t(1) << 31) / std::max<int64_t>(1, Q * G), op, "2^31 query rows of a key-value head or more");
   }
   const int out = temp_slot(v);
   const uint64_t nel = op.result.elements();

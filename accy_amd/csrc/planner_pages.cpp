@@ -3,7 +3,8 @@
 //   fork_table, fork_lengths, fork_source, fork_target, fork_left, fork_slots(group(table, lengths), group(parents, room), held, page)
 //       table i32 [seq, slot], lengths i32 [seq], parents, room i32 [row], held i1 [page], page an i32 constant -> i32 [row, slot], [row], [row],
 //       [row], [], [row] or [row, token]: planned as one kernel
-//   compact_table, compact_source, compact_target(table, held)   table i32 [seq, slot], held i1 [page] -> as the table, i32 [move] twice
+//   compact_table, compact_source, compact_target(table, held, moves)   table i32 [seq, slot], held i1 [page], moves an i32 constant -> as the table,
+//       i32 [move] twice
 //   copy(cache, source, target)   cache [page, ..], i32 [copy] twice -> the cache
 #include "planner_custom.hpp"
 
@@ -23,6 +24,14 @@ bool whole_numbers(const Type& t, size_t rank) { return t.dtype == DType::i32 &&
 
 }  // namespace
 
+// An operand that is an i32 constant, -1 where it is none.
+int64_t Planner::whole_constant(uint32_t v) const {
+  const Op& op = g_.ops[v];
+  int32_t n = -1;
+  if (op.kind == Kind::constant && op.result.dtype == DType::i32 && op.result.rank() == 0 && op.bytes.size() >= 4) std::memcpy(&n, op.bytes.data(), 4);
+  return n;
+}
+
 void Planner::pages_fork(uint32_t v) {
   const Op& op = g_.ops[v];
   const std::vector<uint32_t> now = grouped(op, op.args[0], 2, 2), next = grouped(op, op.args[1], 2, 2);
@@ -30,9 +39,7 @@ void Planner::pages_fork(uint32_t v) {
   require(whole_numbers(tt, 2) && whole_numbers(lt, 1) && lt.dims[0].extent == tt.dims[0].extent, op, "tables are i32 [seq, slot], lengths i32 [seq]");
   require(whole_numbers(pt, 1) && whole_numbers(rt, 1) && pt.dims[0].extent == rt.dims[0].extent, op, "parents and room are i32 [row]");
   require(ht.dtype == DType::i1 && ht.rank() == 1, op, "held pages are i1 [page]");
-  const Op& size = g_.ops[op.args[3]];
-  int32_t page = 0;
-  if (size.kind == Kind::constant && size.result.dtype == DType::i32 && size.result.rank() == 0 && size.bytes.size() >= 4) std::memcpy(&page, size.bytes.data(), 4);
+  const int64_t page = whole_constant(op.args[3]);
   require(page >= 1 && page < (1 << 20), op, "the size of a page is an i32 constant of 1 to 2^20");
   const int64_t seqs = tt.dims[0].extent, slots = tt.dims[1].extent, rows = pt.dims[0].extent, pages = ht.dims[0].extent;
   require(pages <= kMostPages, op, "more than 2^24 pages");
@@ -115,16 +122,8 @@ void Planner::pages_compact(uint32_t v) {
   const int64_t pages = ht.dims[0].extent;
   require(pages <= kMostPages, op, "more than 2^24 pages");
   const auto calls = siblings(v, "accy.pages.compact_");
-  int64_t moves = -1;
-  for (const char* which : {"source", "target"}) {
-    const auto call = calls.find(which);
-    if (call == calls.end()) continue;
-    const Type& t = g_.ops[call->second].result;
-    require(whole_numbers(t, 1) && t.dims[0].extent <= pages && (moves < 0 || t.dims[0].extent == moves), op, "moves are i32 [move], the same of both and at most as many as pages");
-    moves = t.dims[0].extent;
-  }
-  // (a table alone: as if every page might move)
-  if (moves < 0) moves = pages;
+  const int64_t moves = whole_constant(op.args[2]);
+  require(moves >= 0 && moves <= pages, op, "the number of moves is an i32 constant, at most as many as pages");
   int out[3] = {-1, -1, -1};
   const char* const names[] = {"table", "source", "target"};
   std::vector<uint32_t> made;
@@ -134,10 +133,9 @@ void Planner::pages_compact(uint32_t v) {
       out[i] = slots_.add(SlotInfo::Temp, -1, DType::i32, i == 0 ? tt.bytes() : (uint64_t)moves * 4);
       continue;
     }
-    if (i == 0) {
-      const Type& t = g_.ops[call->second].result;
-      require(whole_numbers(t, 2) && t.dims[0].extent == tt.dims[0].extent && t.dims[1].extent == tt.dims[1].extent, g_.ops[call->second], "the result is as the table");
-    }
+    const Type& t = g_.ops[call->second].result;
+    if (i == 0) require(whole_numbers(t, 2) && t.dims[0].extent == tt.dims[0].extent && t.dims[1].extent == tt.dims[1].extent, g_.ops[call->second], "the result is as the table");
+    else require(whole_numbers(t, 1) && t.dims[0].extent == moves, g_.ops[call->second], "the result is i32 [move]");
     out[i] = temp_slot(call->second);
     made.push_back(call->second);
   }

@@ -1145,7 +1145,7 @@ class Builder:
         what its pages hold). The last query sees all of them, each one before it one fewer. Query head h reads key-value
         head h / (heads / kv_heads). Page numbers outside the cache hold no keys; a query that sees none gives 0.
 
-        ``shared`` (pages i32 [prefix, page slot], lengths i32 [prefix], of i32 [seq]): keys that several sequences have before
+        ``shared`` (pages i32 [prefix, page slot], lengths i32 [prefix], of i32 [seq]; 1 to 1024 prefixes): keys that several sequences have before
         their own, each prefix read and computed once for all of its sequences. Sequence b's is prefix of[b]; outside those there are, it
         has none. Every query of a sequence sees all of its prefix, and of its own keys what it sees without one."""
         for x in (q, pages, lengths):
@@ -1172,6 +1172,8 @@ class Builder:
                 raise TensorError("DTypeMismatch", "pages, lengths and prefixes are i32")
         if shared[0].ty.rank != 2 or shared[1].ty.dims != shared[0].ty.dims[:1] or shared[2].ty.dims != q.ty.dims[:1]:
             raise TensorError("ShapeMismatch", "shared pages are [prefix, page], their lengths [prefix], of [seq]")
+        if not 1 <= shared[0].ty.shape[0] <= 1024:
+            raise TensorError("InvalidDimension", f"{shared[0].ty.shape[0]} prefixes (1 to 1024)")
         return self._mx4_call("attend_shared", [q, cache, self._group(pages, lengths), self._group(*shared)], q.ty.dtype, q.ty.dims)
 
     # -- heads, pages and log probabilities: custom calls that the gfx950 target runs --
@@ -1260,7 +1262,7 @@ class Builder:
         last place or it is held, and every other copies it to a page of its own (``source``, ``target``: for
         ``copy_pages``). Free are the pages that no row keeps and that are not ``held`` (i1 [page]); they are given out in
         ascending order, row by row, a row's copy before the pages to come. -1 stands for no page: past a row's pages, and where
-        none was free. ``page`` is the tokens of a page."""
+        none was free. ``page`` is the tokens of a page; of at most 2^24 pages."""
         self._table(table, held)
         for x in (lengths, parents, room):
             self._ensure(x)
@@ -1288,12 +1290,14 @@ class Builder:
         self._table(table, held)
         if not 0 <= moves[1] <= held.ty.shape[0]:
             raise TensorError("InvalidDimension", f"{moves[1]} moves of {held.ty.shape[0]} pages")
-        one = lambda name, dims: self.custom_call(f"accy.pages.compact_{name}", 1, [table, held], Type("i32", dims))
+        operands = [table, held, self.full("i32", moves[1])]  # the moves as an operand too: the table alone depends on them
+        one = lambda name, dims: self.custom_call(f"accy.pages.compact_{name}", 1, operands, Type("i32", dims))
         return CompactedPages(one("table", table.ty.dims), one("source", (moves,)), one("target", (moves,)))
 
     def copy_pages(self, cache: Value, source: Value, target: Value) -> Value:
         """The cache [page, ..], of any type, with page target[i] a copy of what page source[i] held before (i32 [copy] both). A copy
-        from or to no page is none, and of two copies to one page the later one counts. Where the cache is a parameter that nothing else reads and
+        from or to no page is none, and of two copies to one page the later one counts (lists of ``fork_pages`` and ``compact_pages`` have none such;
+        for others the program keeps a workspace of all copies' bytes). Where the cache is a parameter that nothing else reads and
         the result an output, a launch may bind both to one buffer, which is then updated in place."""
         for x in (cache, source, target):
             self._ensure(x)

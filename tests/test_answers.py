@@ -117,9 +117,12 @@ F32 = lambda *e: ("f32", e)  # noqa: E731
     ("pages.copy", [F32(3, 2), I32(2), I32(2)], [(0,), (1,), (2,)], F32(4, 2), "cache's type"),
     ("pages.fork_table", [I32(3, 2), I32(3), I32(4), ("i1", (9,)), I32()], [(0, 1), (2, 2), (3,), (4,)], I32(4, 2), "i32 constant"),
     ("pages.fork_table", [I32(3, 2), I32(3), I32(4), ("i1", (9,)), I32()], [(0,), (2, 2), (3,), (4,)], I32(4, 2), "group of 2"),
-    ("pages.compact_table", [I32(3, 2), ("i1", (9,))], [(0,), (1,)], I32(3, 3), "as the table"),
-    ("pages.compact_source", [I32(3, 2), ("i1", (9,))], [(0,), (1,)], I32(10), "as many as pages"),
-    ("pages.compact_source", [I32(3, 2), ("i1", ((1 << 24) + 1,))], [(0,), (1,)], I32(10), "2^24 pages"),
+    ("pages.compact_table", [I32(3, 2), ("i1", (9,)), 5], [(0,), (1,), (2,)], I32(3, 3), "as the table"),
+    ("pages.compact_source", [I32(3, 2), ("i1", (9,)), 5], [(0,), (1,), (2,)], I32(4), "i32 [move]"),
+    ("pages.compact_source", [I32(3, 2), ("i1", (9,)), 10], [(0,), (1,), (2,)], I32(10), "as many as pages"),
+    ("pages.compact_target", [I32(3, 2), ("i1", (9,)), I32()], [(0,), (1,), (2,)], I32(9), "i32 constant"),
+    ("pages.compact_target", [I32(3, 2), ("i1", (9,))], [(0,), (1,)], I32(9), "3 operands"),
+    ("pages.compact_source", [I32(3, 2), ("i1", ((1 << 24) + 1,)), 5], [(0,), (1,), (2,)], I32(5), "2^24 pages"),
     ("logits.token", [F32(3, 9), I32(3)], [(0,), (1,)], F32(3, 1), "f32 [row"),
     ("logits.top", [F32(3, 9), I32(3)], [(0,), (1,)], F32(3, 10), "1 to 64 alternatives"),
     ("logits.top_tokens", [F32(3, 9), I32(3)], [(0,), (1,)], F32(3, 2), "of tokens i32"),
@@ -134,9 +137,10 @@ def test_planning_refuses_what_the_wire_may_carry(call, operands, groups, result
     dims = lambda i, e: [(f"a{i}_{j}", n) for j, n in enumerate(e)]  # noqa: E731
 
     def body(b, a):
+        a = [a.pop(0) if isinstance(o, tuple) else b.full("i32", o) for a in [list(a)] for o in operands]
         args = [a[g[0]] if len(g) == 1 else b._group(*(a[i] for i in g)) for g in groups]
         return b.custom_call(f"accy.{call}", 1, args, T.Type(result[0], tuple(dims("r", result[1]))))
-    prog = T.define("bad", [T.spec(d, *dims(i, e)) for i, (d, e) in enumerate(operands)], body)
+    prog = T.define("bad", [T.spec(o[0], *dims(i, o[1])) for i, o in enumerate(operands) if isinstance(o, tuple)], body)
     with pytest.raises(hip.HipError) as e:
         hip.plan_source(prog)
     assert e.value.status == hip.COMPILE_FAILED and reason in e.value.message and f"accy.{call}" in e.value.message
@@ -243,7 +247,7 @@ def _grad_want(dy, x, gain, angle, pairs, layout, norm, eps):
 
 HEADS = [(1, 1, 1, 2, 1, 0, "halves"), (1, 16, 4, 128, 64, 0, "halves"), (3, 5, 1, 10, 3, 0, "neighbours"), (7, 12, 3, 96, 32, 3, "neighbours"),
          (2, 3, 2, 80, 20, 2, "halves"), (65, 2, 2, 64, 32, 1, "halves"), (33, 4, 1, 256, 128, 0, "neighbours"), (5, 1, 3, 250, 125, 0, "halves"),
-         (2, 2, 1, 512, 255, 4, "halves"), (4500, 1, 1, 24, 8, 0, "neighbours"), (2100, 3, 2, 32, 16, 0, "halves")]
+         (2, 2, 1, 512, 255, 4, "halves"), (4, 2, 1, 7, 3, 0, "halves"), (3, 0, 2, 32, 16, 0, "halves"), (3, 2, 0, 32, 12, 0, "neighbours"), (4500, 1, 1, 24, 8, 0, "neighbours"), (2100, 3, 2, 32, 16, 0, "halves")]
 
 
 def _heads_inputs(tokens, hq, hk, dim, pairs, axes, dtype, gains, rng):
@@ -524,7 +528,7 @@ def fork_want(table, lengths, parents, room, held, page, tokens):
 
 
 FORKS = [(1, 1, 1, 1, 32), (4, 6, 5, 40, 64), (8, 8, 64, 300, 64), (3, 40, 9, 64, 1), (5, 300, 20, 900, 16), (20, 7, 700, 3000, 64), (6, 1100, 3, 5000, 32), (9, 30, 4, 140000, 64),
-         (4, 1500, 5, 135000, 7), (2, 3, 0, 10, 32), (0, 4, 3, 10, 32)]
+         (4, 1500, 5, 135000, 7), (2, 3, 0, 10, 32), (0, 4, 3, 10, 32), (3, 0, 4, 10, 32), (2, 3, 4, 0, 32)]
 
 
 @pytest.mark.gpu
@@ -534,8 +538,8 @@ def test_fork_pages(seqs, rows, slots, pages, page):
     LDS holds; large tables, which other workgroups write."""
     rng = np.random.default_rng(rows + pages)
     for case in range(3):
-        table = rng.integers(0, pages, (seqs, slots)).astype(np.int32)
-        if case:  # pages of their own but for a beginning, as in earnest
+        table = rng.integers(0, max(pages, 1), (seqs, slots)).astype(np.int32)
+        if case and pages:  # pages of their own but for a beginning, as in earnest
             table[...] = rng.permutation(max(pages, seqs * slots))[:seqs * slots].reshape(seqs, slots) % pages
             table[:, :slots // 3] = table[:1, :slots // 3]
         else:
@@ -573,7 +577,7 @@ def compact_want(table, held, moves):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("seqs,slots,pages,moves", [(1, 1, 1, 1), (4, 6, 40, 10), (8, 64, 3000, 600), (100, 90, 20000, 20000), (7, 9, 140000, 50), (3, 0, 10, 4), (5, 5, 30, 0), (9, 600, 200000, 4000)])
+@pytest.mark.parametrize("seqs,slots,pages,moves", [(1, 1, 1, 1), (4, 6, 40, 10), (8, 64, 3000, 600), (100, 90, 20000, 20000), (7, 9, 140000, 50), (3, 0, 10, 4), (5, 5, 30, 0), (9, 600, 200000, 4000), (2, 3, 0, 0)])
 def test_compact_pages(seqs, slots, pages, moves):
     rng = np.random.default_rng(pages)
     for case in range(2):
@@ -586,7 +590,19 @@ def test_compact_pages(seqs, slots, pages, moves):
             assert np.array_equal(got, want)
     if slots:
         alone = hip_run(T.define("table", [T.spec("i32", seq=seqs, slot=slots), T.spec("i1", page=pages)], lambda b, a: b.compact_pages(*a, ("move", moves)).pages), [table, held])[0]
-        assert np.array_equal(alone, compact_want(table, held, pages)[0])
+        assert np.array_equal(alone, compact_want(table, held, moves)[0])
+
+
+@pytest.mark.gpu
+def test_compact_pages_of_two_numbers_of_moves():
+    """Results of two calls on one table that differ in their moves alone, each by its own."""
+    rng = np.random.default_rng(3)
+    table, held = rng.integers(0, 400, (6, 20)).astype(np.int32), rng.random(400) < 0.1
+    prog = T.define("compact", [T.spec("i32", seq=6, slot=20), T.spec("i1", page=400)],
+                    lambda b, a: [v for x, y in [(b.compact_pages(*a, ("move", 9)), b.compact_pages(*a, ("move", 70)))] for v in (x.pages, y.source, y.pages, x.target)])
+    few, many = compact_want(table, held, 9), compact_want(table, held, 70)
+    for got, want in zip(hip_run(prog, [table, held]), (few[0], many[1], many[0], few[2])):
+        assert np.array_equal(got, want)
 
 
 def copied(cache, source, target):
