@@ -475,6 +475,25 @@ def test_log_probs_gradient(rows, n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,n", [(3, 512), (260, 9000), (2, 20011)])
+def test_log_probs_of_a_chunk_far_below(rows, n, dtype):
+    """Logits near -2.5e38, whose distance from the maximum is beyond the type in powers of two, in chunks whose own maximum is -4e37 or -1e19."""
+    x = np.random.default_rng(n).standard_normal((rows, n))
+    for r, high in ((0, -4e37), (1, -1e19)):
+        x[r, 16:32] = -2.5e38
+        x[r, 16:32:4] = high
+        x[r, 40] = high
+    x = floats(x, dtype)
+    tokens = np.full(rows, 17, np.int32)
+    say(f"far below {rows} {n} {dtype}")
+    _check_log_probs(x[2:], tokens[2:], 3, dtype)
+    _check_grad(x[2:], tokens[2:], dtype)
+    _check_log_probs(x[:2], tokens[:2], 3, dtype)
+    _check_grad(x, tokens, dtype)
+
+
+@pytest.mark.gpu
 def test_log_probs_without_rows_and_of_a_vector():
     got = hip_run(T.define("p", [T.spec("f32", row=0, vocab=9), T.spec("i32", row=0)], lambda b, a: a[0].log_probs(a[1], "vocab", top=2).top), [np.zeros((0, 9), np.float32), np.zeros(0, np.int32)])[0]
     assert got.shape == (0, 2)
