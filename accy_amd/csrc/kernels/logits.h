@@ -4,7 +4,7 @@
 // l) ln 2. One pass over the row gives l, s and the alternatives: each thread measures from an m of its own, the maximum of its first chunk,
 // and the threads' (m, l, s) are joined at the end, measured from the row's maximum. That is a conversion, half a maximum, a multiply-add, an
 // exponential and two more operations an element, more than HBM delivers one in; so the alternatives have to come almost free
-// (2048 x 50257 bf16 62 us, 3.3 TB/s, with 20 alternatives; 8 x 32000 f32 in 31 parts a row 5.7 us of kernel and 6.1 of the parts' join). The
+// (2048 x 50257 bf16 55-58 us, 3.7 TB/s, with 20 alternatives, 49 with one; 8 x 32000 f32 in 31 parts a row 5.7 us of kernel and 6.1 of the parts' join). The
 // gradient reads a row once and writes it: 1001 x 50257 f16 48 us, 4.2 TB/s.
 //
 // Alternatives: an element is compared with a bound below the row's K-th largest only where its batch's maximum reaches the bound. After the first
@@ -143,9 +143,9 @@ __device__ __forceinline__ Sums sums_of(float x) {
   return a;
 }
 // The first n of U chunks added to the sums; `top` becomes their maximum. They are widened once: y is measured from the m that there is, that of the
-// first chunk to begin with. Where an element lies 32 above it, or a masked one makes the quick sum of 2^y y a NaN, or m is so
-// large that it counts beside the largest numbers (y measured from another thread's m might be beyond f32 where this one's is not), they are added again
-// with care. Returns whether they were.
+// first chunk to begin with. Where an element lies 32 above it (or it is that of nothing but masked elements), or m is so large that it counts beside
+// the largest numbers, they are added again with care. Returns whether they were. (Masked elements cost one
+// maximum each; when they made the batch one to be added again, 2048 x 50257 bf16, a third of every seventh row masked, took 66 us instead of 61.)
 template <class C> __device__ __forceinline__ bool add(Sums& a, const u32x4 (&w)[C::U], int n, float& top) {
   top = -__builtin_inff();
   if (n <= 0) return false;
@@ -161,10 +161,10 @@ template <class C> __device__ __forceinline__ bool add(Sums& a, const u32x4 (&w)
     for (int i = 0; i < Chunks<C>::PER; ++i) {
       const float y = __builtin_fmaf(v[i], L2E, -from), e = __builtin_amdgcn_exp2f(y);
       dl += e;
-      ds = __builtin_fmaf(e, y, ds);
+      ds = __builtin_fmaf(e, fmaxf(y, LEAST), ds);
     }
   });
-  const bool care = !(ds == ds) || !(__builtin_fabsf(base) < 0x1p+60f) || top - base > 32.0f;
+  const bool care = !(__builtin_fabsf(base) < 0x1p+60f) || top - a.m > 32.0f;
   if (care) {
     asm volatile("");  // (a branch: computed either way it would cost as much again)
     if (top > a.m) a.rebase(top);
@@ -214,6 +214,7 @@ template <class C> struct List {
     for (int i = threadIdx.x; i < n; i += C::NT) {
       const u64_t mine = key[i];
       int above = 0;
+#pragma unroll 4  // (eight: 84 registers in place of 72, a workgroup to a CU less, 2048 x 50257 bf16 62 us in place of 58)
       for (int j = 0; j < n; ++j) above += key[j] > mine;
       if (above < BEST) best[above] = mine;
     }
@@ -514,7 +515,7 @@ template <int DT> __device__ __forceinline__ typename Elem<DT>::type to_elem(flo
 // The gradient at an element. CARE: as in add().
 template <class C, bool CARE> __device__ __forceinline__ float slope(const Slope<C>& k, float x) {
   const float z = CARE ? __builtin_fmaf(x - k.base, L2E, -k.log_l) : __builtin_fmaf(x, L2E, -k.from);
-  return __builtin_amdgcn_exp2f(z) * __builtin_fmaf(k.b, CARE ? fmaxf(z, LEAST) : z, k.a);
+  return __builtin_amdgcn_exp2f(z) * __builtin_fmaf(k.b, fmaxf(z, LEAST), k.a);
 }
 // The gradient of chunk c's elements.
 template <class C, bool CARE>

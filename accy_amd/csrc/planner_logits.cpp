@@ -78,8 +78,8 @@ void Planner::logits_log_probs(uint32_t v) {
     const int xs = dense_slot(op.args[0]), ts = dense_slot(op.args[1]);
     const int64_t chunks = logit_chunks(V, xt.dtype), splits = logit_splits(rows, chunks, K), mine = (chunks + splits - 1) / splits;
     // A thread holds up to four chunks at once and has four more on their way, in as few rounds as they take and as even (us, 256 threads of 4 /
-    // 5 / 8 chunks, 512 of 4: 2048 x 50257 bf16, 20 alternatives, 66 / 67 / 71 / 85, 1024 x 50257 f32 46 / 47 / 50 / 56, 600 x 131072 bf16, five, 53
-    // / 53 / 53 / 59).
+    // 3 / 2 chunks: 2048 x 50257 bf16, 20 alternatives, 58 / 59 / 64, 1024 x 50257 f32 42 / 45 / 50; in an earlier form 256 threads of 4 / 5 / 8 chunks
+    // and 512 of 4: 66 / 67 / 71 / 85, 46 / 47 / 50 / 56, 600 x 131072 bf16, five, 53 / 53 / 53 / 59).
     const int64_t rounds = (mine + 256 * 4 - 1) / (256 * 4), u = std::max<int64_t>(1, (mine + 256 * rounds - 1) / (256 * rounds));
     const std::string nm = name("log_probs", v), head = logit_config(nm, dt, rows, V, K, splits, 256, u, past_caches(xt));
     auto results = [&](KernelWriter& w) {
