@@ -2,7 +2,7 @@
 // position: of pair i of the first 2 F dims, (a, b) becomes (a cos - b sin, b cos + a sin) of position * frequency[i]. And the gradient.
 //
 // Two numbers are read and two written for about eight operations, so a prompt's heads are bound by HBM (8192 tokens of 32 heads of 128 bf16 27 us, 5.0
-// TB/s; the gradient of 8192 x 20 x 128 31 us, 4.0 TB/s) and a step's by the launch (one token 2.3 us of kernel). The non-temporal hint gains bf16
+// TB/s; the gradient of 8192 x 20 x 128 31 us, 4.0 TB/s) and a step's by the launch (one token 3.4 us of kernel in a call of 8). The non-temporal hint gains bf16
 // rows 4 % and costs f32 rows of 80 dims half as much again.
 // A row (one head of one token) belongs to LANES adjacent lanes, so that its sum is a few shuffles, and each lane holds whole
 // pairs: W dims of a pair's first members and the W of its second (16 bytes each where the sizes allow it), which turn without

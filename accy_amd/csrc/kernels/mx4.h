@@ -786,9 +786,9 @@ __device__ __forceinline__ void attend(const typename Elem<C::DT>::type* __restr
 
 // With keys that sequences share: a wave's step of 32 keys costs about 1840 cycles for its sixteen rows, 210 VALU and 32 matrix instructions one
 // after the other for the most part, whoever's rows they are; what is saved is the steps of rows that would be alone (64 sequences of 4 rows to
-// a head over 8192 shared keys: 28 us, 110 by themselves). (32 rows to a wave, keys and values widened once for both sixteens: 256 registers, two
-// workgroups to a CU, 33 us against 28.) The first workgroups take the prefixes, the rows of all of a prefix's sequences together, the others
-// each sequence's own keys. Every row's parts are joined by the next kernel.
+// each of 4 heads of 128 over 8192 shared keys and up to 1024 of their own: a call 25 us, 62 with all of the keys each one's own). (32 rows to a
+// wave, keys and values widened once for both sixteens: 256 registers, two workgroups to a CU, 33 us against 28.) The first workgroups take the
+// prefixes, the rows of all of a prefix's sequences together, the others each sequence's own keys. Every row's parts are joined by the next kernel.
 template <class C>
 __device__ __forceinline__ void attend_shared(const typename Elem<C::DT>::type* __restrict__ Q, const u8_t* __restrict__ cache,
                                               const int* __restrict__ pages, const int* __restrict__ lengths, const int* __restrict__ prefix_pages,

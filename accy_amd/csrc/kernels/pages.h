@@ -3,11 +3,12 @@
 // fork and compact are counting: which pages are in use is a bitmap (a bit a page), the k-th free page the k-th bit that is clear, found by
 // the words' running counts. One workgroup of 1024 threads does either in a few passes over the tables, the bitmaps in LDS (beyond
 // LDS_PAGES pages in memory), so that a call is one launch; what bounds it is the way to memory and back of each pass and what one
-// CU reads and writes, the tables. No order of atomics shows: bits are set, and ties go to the lowest row or page.
+// CU reads and writes, the tables (us of kernel: 8 rows of 64 slots 7.0, 256 of 512 among 16384 pages 14.6 and 4.0 for the rows' tables by themselves, compaction
+// of 64 x 256 slots 8.6 and 4.7). No order of atomics shows: bits are set, and ties go to the lowest row or page.
 //
-// copies are bound by HBM. Source and target pages of fork and compact differ from each other and are all different, so that their
-// copies need no check (C::CHECK false); of other lists the last copy to a page counts, and in place a page that is the source of one
-// copy and the target of another is kept aside first.
+// copies are bound by HBM (about 3000 pages of 34 KB 40 us, 5.2 TB/s). Source and target pages of fork and compact differ from each other
+// and are all different, so that their copies need no check (C::CHECK false); of other lists the last copy to a page counts, and in place a page
+// that is the source of one copy and the target of another is kept aside first.
 #pragma once
 
 namespace accy {
