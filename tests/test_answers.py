@@ -662,6 +662,39 @@ def test_copy_pages(dtype, shape, n):
     stream.destroy()
 
 
+@pytest.mark.gpu
+def test_copies_of_pages_one_after_the_other():
+    """Three in a row over one buffer, in place and into another; a cache that is its own lists, and one read again after it was copied, stay what they were."""
+    rng = np.random.default_rng(5)
+    cache = rng.integers(0, 250, (40, 3, 17)).astype(np.uint8)
+    lists = [rng.integers(-1, 41, n).astype(np.int32) for n in (25, 25, 60, 60, 5, 5)]
+    want = cache
+    for i in (0, 2, 4):
+        want = copied(want, *lists[i:i + 2])
+    specs = [T.spec("u8", page=40, r=3, c=17), *[T.spec("i32", **{f"copy{i // 2}": len(x)}) for i, x in enumerate(lists)]]
+    prog = T.define("row", specs, lambda b, a: a[0].copy_pages(*a[1:3]).copy_pages(*a[3:5]).copy_pages(*a[5:7]))
+    say("copies in a row")
+    assert np.array_equal(hip_run(prog, [cache, *lists])[0], want)
+    stream, bufs = hip.Stream(), [hip.DeviceBuffer.from_array(x) for x in (cache, *lists)]
+    with hip.Hip(prog) as ex:
+        for _ in range(2):
+            bufs[0].upload(cache)
+            ex.launch_device([b.ptr for b in bufs], [bufs[0].ptr], stream.handle)
+            stream.synchronize()
+            assert np.array_equal(bufs[0].download(np.empty_like(cache)), want)
+    stream.destroy()
+    numbers, other = rng.permutation(64).astype(np.int32), rng.permutation(64).astype(np.int32)
+    one = copied(numbers, numbers, other)
+    prog = T.define("own", [T.spec("i32", page=64)] * 2, lambda b, a: [a[0].copy_pages(a[0], a[1]).copy_pages(b.full("i32", 3, ("page", 64)), a[1]), a[0].copy_pages(a[1], a[0])])
+    say("a cache as its own lists")
+    got = hip_run(prog, [numbers, other])
+    assert np.array_equal(got[0], copied(one, np.full(64, 3, np.int32), other)) and np.array_equal(got[1], copied(numbers, other, numbers))
+    first = lambda b, a: a[0].copy_pages(a[0], a[1])  # noqa: E731
+    prog = T.define("again", [T.spec("i32", page=64)] * 2, lambda b, a: [v for c in [first(b, a)] for v in (c.copy_pages(c, a[1]), c.copy_pages(a[1], c))])
+    got = hip_run(prog, [numbers, other])
+    assert np.array_equal(got[0], copied(one, one, other)) and np.array_equal(got[1], copied(one, other, one))
+
+
 # ---- attention with shared keys ----
 
 def shared_attention(q, cache, pages, lengths, prefix_pages, prefix_lengths, of):
