@@ -403,6 +403,7 @@ __device__ __forceinline__ void compact_with(u32_t* used, u32_t* busy, int* coun
   for (long i = moves + tid; i < C::MOVES; i += THREADS) source[i] = target[i] = -1;
   if (C::WIDE && tid == 0) work[0] = moves;
   if constexpr (C::WIDE && LDS) {
+    meet<LDS>();  // (past 32 pages a thread, words are others' than those that wrote them)
     for (long w = tid; w < WORDS; w += THREADS) {
       work[4 + w] = (int)used[w];
       work[4 + WORDS + w] = counts[w];

@@ -613,6 +613,32 @@ def test_compact_pages(seqs, slots, pages, moves):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("pages", [32768, 32769, 40000, 65536, 131071, 131072, 131073])
+def test_large_tables_among_pages_of_several_words_a_thread(pages):
+    """Bitmaps of more words than a workgroup has threads, up to where they leave LDS, and tables that another kernel writes: the counts
+    that it reads are those of all words. Pages in use, holes and moves lie in words all over; rows forked from the same tables."""
+    rng = np.random.default_rng(pages)
+    for used, held_share, moves in ((pages // 4, 0.02, 9000), (pages, 0.4, 700)):
+        table = rng.integers(0, used, (64, 256)).astype(np.int32) * (pages // used)
+        table[rng.random(table.shape) < 0.05] = -1
+        held = rng.random(pages) < held_share
+        prog = T.define("compact", [T.spec("i32", seq=64, slot=256), T.spec("i1", page=pages)],
+                        lambda b, a: [v for c in [b.compact_pages(*a, ("move", moves))] for v in (c.pages, c.source, c.target)])
+        want = compact_want(table, held, moves)
+        assert len(np.unique(want[1] // 32)) > 90 and (want[0] != table).any()
+        say(f"compact 64 x 256 of {pages}")
+        for got, w in zip(hip_run(prog, [table, held]), want):
+            assert np.array_equal(got, w)
+        ins = [table, rng.integers(0, 256 * 16 + 1, 64).astype(np.int32), rng.integers(-1, 65, 40).astype(np.int32), rng.integers(0, 400, 40).astype(np.int32), held]
+        row = T.spec("i32", row=40)
+        prog = T.define("fork", [T.spec("i32", seq=64, slot=256), T.spec("i32", seq=64), row, row, T.spec("i1", page=pages)],
+                        lambda b, a: [v for f in [b.fork_pages(*a, 16, tokens=2)] for v in (f.pages, f.lengths, f.source, f.target, f.left, f.slots)])
+        say(f"fork 64 x 256 of {pages}")
+        for got, w in zip(hip_run(prog, ins), fork_want(*ins, 16, 2)):
+            assert np.array_equal(got, w)
+
+
+@pytest.mark.gpu
 def test_compact_pages_of_two_numbers_of_moves():
     """Results of two calls on one table that differ in their moves alone, each by its own."""
     rng = np.random.default_rng(3)
