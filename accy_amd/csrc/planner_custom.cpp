@@ -50,8 +50,9 @@ std::vector<uint32_t> Planner::grouped(const Op& op, uint32_t a, size_t least, s
   return group.args;
 }
 
-// The live calls of one set with v's operands (v among them), each name once: name -> operation. They are one kernel's.
-std::map<std::string, uint32_t> Planner::siblings(uint32_t v, const std::string& prefix, const std::string& suffix) const {
+// The live calls of one set with v's operands (v among them) that `fits` takes, each name once: name -> operation. They are one kernel's. `fits` sees
+// them in order, v first.
+std::map<std::string, uint32_t> Planner::siblings(uint32_t v, const std::string& prefix, const std::string& suffix, const std::function<bool(const Op&)>& fits) const {
   const Op& op = g_.ops[v];
   std::map<std::string, uint32_t> found;
   for (uint32_t u = v; u < g_.ops.size(); ++u) {
@@ -59,6 +60,7 @@ std::map<std::string, uint32_t> Planner::siblings(uint32_t v, const std::string&
     if (!live_[u] || done_[u] || uo.kind != Kind::custom_call || uo.index != 1 || uo.args != op.args) continue;
     if (uo.bytes.size() < prefix.size() + suffix.size() || uo.bytes.compare(0, prefix.size(), prefix) != 0) continue;
     if (uo.bytes.compare(uo.bytes.size() - suffix.size(), suffix.size(), suffix) != 0) continue;
+    if (fits && !fits(uo)) continue;
     found.emplace(uo.bytes.substr(prefix.size(), uo.bytes.size() - prefix.size() - suffix.size()), u);
   }
   return found;

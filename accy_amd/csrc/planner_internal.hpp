@@ -622,7 +622,8 @@ class Planner {
 
   void group(uint32_t v);
   std::vector<uint32_t> grouped(const Op& op, uint32_t a, size_t least, size_t most) const;
-  std::map<std::string, uint32_t> siblings(uint32_t v, const std::string& prefix, const std::string& suffix = "") const;
+  std::map<std::string, uint32_t> siblings(uint32_t v, const std::string& prefix, const std::string& suffix = "",
+                                           const std::function<bool(const Op&)>& fits = nullptr) const;
   int updated_cache(uint32_t v);
 
   bool heads(uint32_t v);

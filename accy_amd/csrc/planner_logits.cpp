@@ -52,11 +52,16 @@ void Planner::logits_log_probs(uint32_t v) {
   const int64_t V = last(xt);
   require(V >= 1 && V < (int64_t(1) << 30), op, "1 to 2^30 logits to a row");
   const uint64_t rows = tt.elements();
-  const auto calls = siblings(v, "accy.logits.");
+  // As many alternatives as v asks for, or else the first call that asks for some; calls for another number are kernels of their own.
+  int64_t K = 0;
+  const auto calls = siblings(v, "accy.logits.", "", [&](const Op& o) {
+    if (o.bytes != "accy.logits.top" && o.bytes != "accy.logits.top_tokens") return true;
+    if (!K) K = last(o.result);
+    return last(o.result) == K;
+  });
   int out[4] = {-1, -1, -1, -1};
   const char* const names[] = {"token", "entropy", "top", "top_tokens"};
   std::vector<uint32_t> made;
-  int64_t K = 0;
   for (int i = 0; i < 4; ++i) {
     const auto call = calls.find(names[i]);
     if (call == calls.end()) continue;
@@ -67,8 +72,6 @@ void Planner::logits_log_probs(uint32_t v) {
       require(rt.dtype == (i == 2 ? DType::f32 : DType::i32) && rt.rank() == xt.rank() && same_rows(rt, xt), g_.ops[call->second],
               "the result is f32, of tokens i32, [row .., top]");
       require(last(rt) >= 1 && last(rt) <= 64 && last(rt) <= V, g_.ops[call->second], "1 to 64 alternatives, as many as there are logits");
-      if (K && last(rt) != K) continue;  // another number of alternatives: a call of its own
-      K = last(rt);
     }
     out[i] = temp_slot(call->second);
     made.push_back(call->second);

@@ -6,6 +6,7 @@ reciprocal square root, exponential or logarithm by 2^-22 at most, a sum of n te
 """
 import ctypes
 import random
+import re
 
 import numpy as np
 import pytest
@@ -173,6 +174,26 @@ def test_results_of_one_call_are_one_kernel():
     step = W.answers_step_mx4_program(8, 8, 128, 4, 2, 64, 300, 40, 32, 6, 2, 3, 4)
     assert _labels(step) == ["fork", "copy_pages", "row", "quantize", "mx4", "mx4", "heads", "mx4", "cache_write", "mx4_attend", "mx4_join", "quantize", "mx4", "row",
                              "quantize", "mx4", "log_probs"]
+
+
+ALTERNATIVES = [((1, 5), ("x.top_tokens", "y.top")), ((5, 3), ("x.top_tokens", "y.top")), ((2, 4), ("y.top", "x.top_tokens", "y.top_tokens", "x.token")), ((4, 2), ("x.top", "y.top_tokens")),
+                ((3, 7), ("x.entropy", "y.top_tokens", "x.top")), ((6, 6), ("x.top", "y.top_tokens", "y.top"))]
+
+
+def _two_numbers_program(numbers, names, rows=3, vocab=40):
+    def body(b, a):
+        both = dict(zip("xy", (a[0].log_probs(a[1], "vocab", top=n) for n in numbers)))
+        return [getattr(both[n[0]], n[2:]) for n in names]
+    return T.define("two", [T.spec("f32", row=rows, vocab=vocab), T.spec("i32", row=rows)], body)
+
+
+@pytest.mark.parametrize("numbers,names", ALTERNATIVES)
+def test_every_result_of_two_numbers_of_alternatives_has_a_kernel(numbers, names):
+    """Results of two calls on the same logits that differ in their alternatives alone: each is written, by a kernel of its own number."""
+    source = hip.plan_source(_two_numbers_program(numbers, names))
+    # (results are the pointers of a kernel that are not const)
+    results = [len(re.findall(r"(?<!const )(?:float|int|i32_t)\* __restrict__ a\d+", line)) for line in source.splitlines() if "__global__" in line]
+    assert sum(results) == len(names), source
 
 
 def test_every_mutated_program_gets_a_status():
@@ -431,6 +452,26 @@ def _hard_rows(n, dtype):
             "infinity": np.where(np.arange(n) == n - 2, np.inf, base), "all nan": np.full(n, np.nan), "few": np.where(np.arange(n) < 3, 1.0, np.nan),
             "negative": -100 - np.abs(base), "two heights": np.where(np.arange(n) < n // 2, -5.0, 30000.0), "bottom": np.full(n, -50000.0)}
     return np.stack([np.asarray(v, np.float64) for v in rows.values()])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("numbers,names", ALTERNATIVES)
+@pytest.mark.parametrize("rows,vocab", [(3, 40), (2, 9000)])
+def test_results_of_two_numbers_of_alternatives(rows, vocab, numbers, names):
+    rng = np.random.default_rng(vocab)
+    x, tokens = rng.standard_normal((rows, vocab)).astype(np.float32), rng.integers(0, vocab, rows).astype(np.int32)
+    token, entropy, logp = _log_probs_want(x.astype(np.float64), tokens)
+    order = np.argsort(-x, axis=1, kind="stable")
+    say(f"two numbers {numbers} {names} {rows} {vocab}")
+    for got, name in zip(hip_run(_two_numbers_program(numbers, names, rows, vocab), [x, tokens]), names):
+        best = order[:, :numbers[name[0] == "y"]]
+        want = {"token": token, "entropy": entropy, "top": np.take_along_axis(logp, best, 1), "top_tokens": best}[name[2:]]
+        if name[2:] == "top_tokens":
+            assert np.array_equal(got, want)
+            continue
+        # as in _check_log_probs
+        tol = _steps(x)[:, None] * (4 * (2 + np.log(vocab + 1)) if name[2:] == "entropy" else 1)
+        assert_within(got.reshape(rows, -1), want.reshape(rows, -1), tol + 2 * E24 * np.abs(want.reshape(rows, -1)), name)
 
 
 @pytest.mark.gpu
