@@ -81,7 +81,10 @@ void Planner::process(uint32_t v) {
     case Kind::scatter_add: scatter_add(v); break;
     case Kind::scan: scan(v); break;
     case Kind::projection: break;  // written by its scan's loop step
-    case Kind::custom_call: custom(v); break;
+    case Kind::custom_call:
+      custom(v);
+      if (!done_[v]) fail(Err::Unsupported, "custom_call " + op.bytes + ": no kernel writes its result");
+      break;
     case Kind::sparse_cross_entropy:  // expanded before planning
       fail(Err::Unsupported, std::string(kind_name(op.kind)) + " is not supported by the HIP target");
     default:

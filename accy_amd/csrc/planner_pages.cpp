@@ -74,7 +74,7 @@ void Planner::pages_fork(uint32_t v) {
     out[i] = temp_slot(call->second);
     made.push_back(call->second);
   }
-  require(!made.empty(), op, "no result of that name");
+  require(std::find(made.begin(), made.end(), v) != made.end(), op, "no result of that name");
   // One workgroup writes small tables itself; of larger ones it leaves what each row takes to workgroups of their own.
   const bool wide = (uint64_t)(rows * slots) > kOneWorkgroup;
   require(launchable((uint64_t)rows, 256) && (slots + 1023) / 1024 < 65536, op, "more workgroups than a launch takes");
@@ -139,7 +139,7 @@ void Planner::pages_compact(uint32_t v) {
     out[i] = temp_slot(call->second);
     made.push_back(call->second);
   }
-  require(!made.empty(), op, "no result of that name");
+  require(std::find(made.begin(), made.end(), v) != made.end(), op, "no result of that name");
   const uint64_t entries = tt.elements(), words = (uint64_t)(pages + 31) / 32;
   const bool wide = entries > kOneWorkgroup;
   const int table = dense_slot(op.args[0]);

@@ -147,6 +147,22 @@ def test_planning_refuses_what_the_wire_may_carry(call, operands, groups, result
     assert e.value.status == hip.COMPILE_FAILED and reason in e.value.message and f"accy.{call}" in e.value.message
 
 
+@pytest.mark.parametrize("name", ["fork_page", "fork_", "fork_tables", "compact_left", "compact_"])
+def test_a_name_that_is_none_is_refused_beside_those_that_are(name):
+    """A call of a set without such a result, on the operands of one that there is: neither may be passed over."""
+    def body(b, a):
+        fork = name.startswith("fork")
+        args = [b._group(a[0], a[1]), b._group(a[2], a[2]), a[3], b.full("i32", 64)] if fork else [a[0], a[3], b.full("i32", 5)]
+        there = "fork_lengths" if fork else "compact_source"
+        calls = [b.custom_call(f"accy.pages.{n}", 1, args, T.Type("i32", (("row", 5),))) for n in (name, there)]
+        return calls if first else calls[::-1]
+    for first in (True, False):
+        prog = T.define("p", [T.spec("i32", seq=4, slot=7), T.spec("i32", seq=4), T.spec("i32", row=5), T.spec("i1", page=30)], body)
+        with pytest.raises(hip.HipError) as e:
+            hip.plan_source(prog)
+        assert e.value.status == hip.COMPILE_FAILED and f"accy.pages.{name}" in e.value.message
+
+
 def test_groups_are_operands_only():
     spec = [T.spec("f32", r=2)]
     for body in (lambda b, a: b._group(a[0], a[0]), lambda b, a: b.broadcast(b._group(a[0], a[0]), [("r", 2)]),
