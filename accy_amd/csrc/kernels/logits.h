@@ -96,15 +96,24 @@ __device__ __forceinline__ void opaque(u32x4& w) {
   }
 }
 
+// y = (x - base) log2 e as one multiply-add an element, x L2E - base L2E, takes base L2E rounded, and is off by that rounding, the same for all
+// elements of a thread: rest_of(base), which is itself a number. A thread's sums are of such y's, and the rest leaves them where the threads' are
+// joined. From FAR on it is beyond 1: there it is none, and y is formed from x - base.
+constexpr float FAR = 0x1p+24f;
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+__device__ __forceinline__ bool is_far(float base) { return !(__builtin_fabsf(base) < FAR); }
+__device__ __forceinline__ float rest_of(float base) { return is_far(base) ? 0.0f : __builtin_fmaf(base, L2E, -(base * L2E)); }
+// With care: the same from x - base, whose rounding is that of a difference.
+__device__ __forceinline__ float careful(float x, float base, float rest) { return __builtin_fmaf(x - base, L2E, rest); }
 
 // A thread's, or a range's: sums of 2^y and of 2^y y with y measured from m, a maximum or near one.
 struct Sums {
   float m = -__builtin_inff(), l = 0.0f, s = 0.0f;
-  // The same measured from another m.
-  __device__ __forceinline__ void rebase(float to) {
+  // The same measured from another m, with y's that are larger by `more`.
+  __device__ __forceinline__ void rebase(float to, float more = 0.0f) {
+#pragma clang fp contract(off)  // (the rest of an element that is alone in its row leaves 0 behind)
     // (a sum of nothing is measured from nothing: its shift may be beyond f32)
-    const float shift = l == 0.0f ? 0.0f : fmaxf((base_of(m) - base_of(to)) * L2E, LEAST), scale = __builtin_amdgcn_exp2f(shift);
+    const float shift = l == 0.0f ? 0.0f : fmaxf(careful(base_of(m), base_of(to), more), LEAST), scale = __builtin_amdgcn_exp2f(shift);
     s = (s + l * shift) * scale;
     l *= scale;
     m = to;
@@ -137,14 +146,14 @@ template <class C> __device__ __forceinline__ float largest(const u32x4& w) {
 __device__ __forceinline__ Sums sums_of(float x) {
   Sums a;
   a.m = fmaxf(x, a.m);
-  const float y = (x - base_of(a.m)) * L2E;
+  const float y = careful(x, base_of(a.m), rest_of(base_of(a.m)));
   a.l = __builtin_amdgcn_exp2f(y);
   a.s = a.l * fmaxf(y, LEAST);
   return a;
 }
 // The first n of U chunks added to the sums; `top` becomes their maximum. They are widened once: y is measured from the m that there is, that of the
-// first chunk to begin with. Where an element lies 32 above it (or it is that of nothing but masked elements), or m is so large that it counts beside
-// the largest numbers, they are added again with care. Returns whether they were. (Masked elements cost one
+// first chunk to begin with. Where an element lies 32 above it (or it is that of nothing but masked elements), or m is far from 0, they are added
+// again with care. Returns whether they were. (Masked elements cost one
 // maximum each; when they made the batch one to be added again, 2048 x 50257 bf16, a third of every seventh row masked, took 66 us instead of 61.)
 template <class C> __device__ __forceinline__ bool add(Sums& a, const u32x4 (&w)[C::U], int n, float& top) {
   top = -__builtin_inff();
@@ -164,20 +173,22 @@ template <class C> __device__ __forceinline__ bool add(Sums& a, const u32x4 (&w)
       ds = __builtin_fmaf(e, fmaxf(y, LEAST), ds);
     }
   });
-  const bool care = !(__builtin_fabsf(base) < 0x1p+60f) || top - a.m > 32.0f;
+  const bool care = is_far(base) || top - a.m > 32.0f;
   if (care) {
     asm volatile("");  // (a branch: computed either way it would cost as much again)
-    if (top > a.m) a.rebase(top);
-    const float base = base_of(a.m);
+    if (top > a.m) a.rebase(top, rest_of(top) - rest_of(base_of(a.m)));
+    float base = base_of(a.m);
+    const float rest = rest_of(base);
     dl = ds = 0.0f;
     each<C::U>([&](auto u) {
       if (u.value >= n) return;
       u32x4 again = w[u.value];
-      opaque(again);
+      if constexpr (C::DT != 2) opaque(again);
+      asm("" : "+v"(base), "+v"(dl), "+v"(ds));  // (chunk after chunk: f32 rows of 13 fill the registers otherwise)
       widen<C>(again, v);
 #pragma unroll
       for (int i = 0; i < Chunks<C>::PER; ++i) {
-        const float y = (v[i] - base) * L2E, e = __builtin_amdgcn_exp2f(y);
+        const float y = careful(v[i], base, rest), e = __builtin_amdgcn_exp2f(y);
         dl += e;
         ds = __builtin_fmaf(e, fmaxf(y, LEAST), ds);
       }
@@ -226,7 +237,7 @@ template <class C> struct List {
 // peak: a thread's maximum.
 template <int WAVES> __device__ __forceinline__ Sums join_threads(Sums a, float peak, bool& care, float (&lds)[WAVES][4]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  a.rebase(wave_reduce(peak, MaxOp()));
+  a.rebase(wave_reduce(peak, MaxOp()), -rest_of(base_of(a.m)));
   a.l = wave_reduce(a.l, SumOp());
   a.s = wave_reduce(a.s, SumOp());
   if (lane == 0) {
@@ -485,11 +496,17 @@ __device__ __forceinline__ void log_probs_join(const typename Elem<C::DT>::type*
 
 // ---- the gradient ----
 //
-// d x = g (1 at the token) - p (g + h (log p + H)), g and h the gradients of the token's log probability and of the entropy H: with z = log2 p,
-// p (A + B z) with A = -g - h H and B = -h ln 2.
+// d x = g (1 at the token) - p (g + h (log p + H)), g and h the gradients of the token's log probability and of the entropy H: p is 2^y / l and log p +
+// H is (y - s / l) ln 2, so that this is 2^y (A + B y) with A = (h ln 2 s / l - g) / l and B = -h ln 2 / l.
 template <class C> struct Slope {
-  float base, log_l, from, a, b, g;  // z = (x - base) log2 e - log2 l = x log2 e - from
+  float base, a, b, g;
   int at;                      // the token's element counted as a Range's, or -1
+  // For y's with the rest of the base: what it adds leaves A and 2^y.
+  __device__ __forceinline__ void with_rest() {
+    const float rest = rest_of(base), scale = __builtin_amdgcn_exp2f(-rest);
+    a = (a - b * rest) * scale;
+    b *= scale;
+  }
 };
 template <class C>
 __device__ __forceinline__ Slope<C> slope_of(const Sums& s, long row, int lead, const int* __restrict__ tokens, const float* __restrict__ d_token,
@@ -497,14 +514,12 @@ __device__ __forceinline__ Slope<C> slope_of(const Sums& s, long row, int lead, 
   Slope<C> k;
   const int t = tokens[row];
   const bool inside = t >= 0 && t < C::V;
-  const float h = d_entropy[row];
+  const float h = d_entropy[row], by = s.l == 0.0f ? 0.0f : 1.0f / s.l;
   k.g = inside ? d_token[row] : 0.0f;
   k.at = inside && s.l != 0.0f ? lead + t : -1;
   k.base = base_of(s.m);
-  k.log_l = s.l == 0.0f ? 0.0f : __builtin_amdgcn_logf(s.l);
-  k.from = k.base * L2E + k.log_l;
-  k.a = -k.g - h * entropy(s);
-  k.b = -h * LN2;
+  k.a = (h * LN2 * (s.s * by) - k.g) * by;
+  k.b = -h * LN2 * by;
   return k;
 }
 template <int DT> __device__ __forceinline__ typename Elem<DT>::type to_elem(float v) {
@@ -512,10 +527,10 @@ template <int DT> __device__ __forceinline__ typename Elem<DT>::type to_elem(flo
   else if constexpr (DT == 1) return f32_to_f16(v);
   else return v;
 }
-// The gradient at an element. CARE: as in add().
+// The gradient at an element. CARE: as in add(); without, the slope is one with_rest().
 template <class C, bool CARE> __device__ __forceinline__ float slope(const Slope<C>& k, float x) {
-  const float z = CARE ? __builtin_fmaf(x - k.base, L2E, -k.log_l) : __builtin_fmaf(x, L2E, -k.from);
-  return __builtin_amdgcn_exp2f(z) * __builtin_fmaf(k.b, fmaxf(z, LEAST), k.a);
+  const float y = CARE ? careful(x, k.base, 0.0f) : __builtin_fmaf(x, L2E, -(k.base * L2E));
+  return __builtin_amdgcn_exp2f(y) * __builtin_fmaf(k.b, fmaxf(y, LEAST), k.a);
 }
 // The gradient of chunk c's elements.
 template <class C, bool CARE>
@@ -565,9 +580,11 @@ __device__ __forceinline__ void grad_row(const typename Elem<C::DT>::type* __res
   if (besides >= 0) peak = fmaxf(peak, edge);
   each<C::U>([&](auto u) { opaque(w[u.value]); });
   a = join_threads<WAVES>(a, peak, care, lds);
-  const Slope<C> k = slope_of<C>(a, row, r.lead, tokens, d_token, d_entropy);
+  Slope<C> k = slope_of<C>(a, row, r.lead, tokens, d_token, d_entropy);
+  care = __builtin_amdgcn_ballot_w64(care || is_far(k.base)) != 0;  // (an edge's; one for all, as it is)
   typename Elem<C::DT>::type* const to = dx + r.at;
   put_besides<C>(to, k, besides, edge);
+  if (!care) k.with_rest();
   each<C::U>([&](auto u) {
     if (u.value >= n) return;
     if (care) put<C, true>(to, k, first + u.value * C::NT, w[u.value]);

@@ -550,6 +550,86 @@ def test_log_probs_of_a_chunk_far_below(rows, n, dtype):
     _check_grad(x, tokens, dtype)
 
 
+def _steps_of_weight(x):
+    """As _steps, but for the logits' own size: a softmax depends on differences from the maximum alone, and those are formed with one rounding, so
+    that what counts of them is the mean over the row's probabilities (a sum's relative error) and, beside a result, the result's own size."""
+    with np.errstate(all="ignore"):
+        bad = ~(np.isfinite(x) | np.isneginf(x)).all(-1) | np.isneginf(x).all(-1)
+        x = np.where(bad[:, None], 0.0, x)
+        far = x.max(-1, keepdims=True) - x
+        p = np.exp(-far)
+        mean = (p * np.where(p > 0, far, 0.0)).sum(-1) / p.sum(-1)
+    return E24 * (200 + x.shape[-1] / 2048 + 4 * mean + 8 * np.log(x.shape[-1] + 1))
+
+
+def _check_large(x, tokens, top, dtype):
+    """log_probs and its gradient with tolerances that do not grow with the logits."""
+    rows, n = x.shape
+    spec = [T.spec(dtype, row=rows, vocab=n), T.spec("i32", row=rows)]
+    prog = T.define("log_probs", spec, lambda b, a: [v for p in [a[0].log_probs(a[1], "vocab", top=top)] for v in (p.token, p.entropy, p.top, p.top_tokens)])
+    got = hip_run(prog, [x, tokens])
+    v = wide(x, dtype)
+    token, entropy, logp = _log_probs_want(v, tokens)
+    tol = _steps_of_weight(v)
+    best = np.argsort(-v, axis=1, kind="stable")[:, :top]
+    assert np.array_equal(got[3], best)
+    # (beyond f32 a log probability is -inf)
+    least = lambda w: np.where(w < -3.4028235e38, -np.inf, w)  # noqa: E731
+    assert_within(got[0], least(token), tol + 2 * E24 * np.abs(token), "token")
+    assert_within(got[1], entropy, 4 * tol * (2 + np.log(n + 1)), "entropy")
+    want = np.take_along_axis(logp, best, 1)
+    assert_within(got[2], least(want), tol[:, None] + 2 * E24 * np.abs(want), "top")
+    rng = np.random.default_rng(rows)
+    a, h = (rng.standard_normal(rows).astype(np.float32) for _ in range(2))
+    prog = T.define("grad", spec + [T.spec("f32", row=rows)] * 2, lambda b, x: x[0].log_probs_grad(*x[1:], "vocab"))
+    got = wide(hip_run(prog, [x, tokens, a, h])[0], dtype)
+    want, size = _grad_logits_want(v, tokens, a.astype(np.float64), h.astype(np.float64))
+    assert_within(got, want, HALF_STEP[dtype] * np.abs(want) + 8 * (tol * (2 + np.log(n + 1)))[:, None] * size + (2.0 ** -25 if dtype == "f16" else 1e-37), "gradient")
+
+
+def _shifted_rows(n, dtype):
+    """Ordinary rows at a distance from 0, rows of one large value, and ordinary rows of which a third, or whole stretches at the beginning, in the middle or at
+    the ends, are masked with a large finite value."""
+    rng = np.random.default_rng(n)
+    offsets = [1e3, -1e3, 3e4, -3e4] + ([] if dtype == "f16" else [1e5, -1e5, 1e6, -1e7, 1e7, 2.0 ** 24, -2.0 ** 24, 1e8, -1e8, 1e10, -1e10, 1e12, -1e12])
+    base, rows = rng.standard_normal(n) * 2.5, []
+    for o in offsets:
+        rows += [base + o, np.full(n, o), np.where(np.arange(n) % 3 == 0, base, -abs(o))]
+        rows += [np.where(part, base, -abs(o)) for part in (np.arange(n) >= n // 2, np.arange(n) < n // 2, np.abs(np.arange(n) - n // 2) > n // 4, np.arange(n) == n // 2)]
+        # the largest ones alone in what lies beside the whole chunks
+        rows += [np.where((np.arange(n) == 0) | (np.arange(n) == n - 1), base + abs(o), base + abs(o) - 3)]
+    return np.stack(rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,copies", [(7, 1), (100, 1), (2501, 1), (12001, 1), (40003, 1), (2501, 40), (12001, 10)])
+def test_log_probs_do_not_depend_on_a_shift(n, copies, dtype):
+    """Rows at distances of 1e3 to 1e12 from 0, and masks of -1e3 to -1e12: in a few rows (several workgroups each), in a workgroup's registers, and in more than 512."""
+    rows = _shifted_rows(n, dtype)
+    x = floats(np.tile(rows, (max(1, -(-copies * 32 // len(rows))) if copies > 1 else 1, 1)), dtype)
+    tokens = (np.arange(len(x)).astype(np.int32) * 7) % n
+    say(f"shifted {len(x)} {n} {dtype}")
+    _check_large(x, tokens, min(n, 5), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shift", [0.0, 1e5, -1e7])
+def test_the_gradient_of_a_row_does_not_depend_on_how_many_there_are(shift):
+    """One row by itself, in two kernels, and among 300, in one kernel: the same but for roundings."""
+    rng = np.random.default_rng(9)
+    x = (rng.standard_normal((300, 20011)) * 2.5 + shift).astype(np.float32)
+    tokens, a, h = rng.integers(0, 20011, 300).astype(np.int32), *(rng.standard_normal(300).astype(np.float32) for _ in range(2))
+
+    def grad(rows):
+        spec = [T.spec("f32", row=rows, vocab=20011), T.spec("i32", row=rows), *[T.spec("f32", row=rows)] * 2]
+        return hip_run(T.define("grad", spec, lambda b, v: v[0].log_probs_grad(*v[1:], "vocab")), [x[:rows], tokens[:rows], a[:rows], h[:rows]])[0]
+    say(f"gradient alone and among others, {shift}")
+    alone, among = grad(1).astype(np.float64), grad(300)[:1].astype(np.float64)
+    _, size = _grad_logits_want(x[:1].astype(np.float64), tokens[:1], a[:1].astype(np.float64), h[:1].astype(np.float64))
+    assert_within(among, alone, 16 * (_steps_of_weight(x[:1].astype(np.float64)) * (2 + np.log(20012)))[:, None] * size + 1e-37)
+
+
 @pytest.mark.gpu
 def test_log_probs_without_rows_and_of_a_vector():
     got = hip_run(T.define("p", [T.spec("f32", row=0, vocab=9), T.spec("i32", row=0)], lambda b, a: a[0].log_probs(a[1], "vocab", top=2).top), [np.zeros((0, 9), np.float32), np.zeros(0, np.int32)])[0]
