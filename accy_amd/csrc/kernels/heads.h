@@ -7,8 +7,9 @@
 // A row (one head of one token) belongs to LANES adjacent lanes, so that its sum is a few shuffles, and each lane holds whole
 // pairs: W dims of a pair's first members and the W of its second (16 bytes each where the sizes allow it), which turn without
 // leaving the lane. The cosines of a token are the same for all of its heads: a workgroup forms them once for its TT tokens, a pair per
-// thread, while its first rows are on their way. Angles: the turns position * frequency / 2 pi in 64 bits, whose fraction
-// is exact to 2^-30 for every 32-bit position, then f32 polynomials on an eighth of a turn.
+// thread, while its first rows are on their way. Angles: the turns position * frequency / 2 pi in two 64-bit numbers, whose fraction
+// is off by 2^-50 at most up to 2^50 turns, which positions of 32 bits do not reach below frequencies of millions, then f32 polynomials on an eighth
+// of a turn. (One 64-bit number is off by 2^-52 of the turns: 2^-23 at the largest positions and a frequency of 1.)
 //
 // C supplies DT (elements: 0 bf16, 1 f16, 2 f32), GT (gains), D, F, HQ, HK (heads of queries and keys), TOKENS, AXES (positions per
 // token, 0: one without axes), NEIGHBOURS (pairs 2 i, 2 i + 1, else i, F + i), NORM, EPS, W, LANES, TT.
@@ -62,8 +63,12 @@ template <class C> struct Row {
 };
 
 __device__ __forceinline__ void turn(int position, float frequency, float& c, float& s) {
-  double t = (double)position * ((double)frequency * 0.15915494309189535);
-  t -= __builtin_rint(t);
+  // Twice a product and what its rounding left out, 1 / 2 pi in two numbers.
+  constexpr double HI = 0x1.45f306dc9c883p-3, LO = -0x1.6b01ec5417056p-57;
+  const double f = frequency, p = position, rate = f * HI, rate_lo = __builtin_fma(f, HI, -rate) + f * LO;
+  double t = p * rate;
+  const double t_lo = __builtin_fma(p, rate, -t) + p * rate_lo;
+  t = (t - __builtin_rint(t)) + t_lo;
   const double k = __builtin_rint(t * 4.0);
   const float r = (float)((t - k * 0.25) * 6.283185307179586);
   const u32_t q = (u32_t)(int)k;

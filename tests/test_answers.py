@@ -7,6 +7,7 @@ reciprocal square root, exponential or logarithm by 2^-22 at most, a sum of n te
 import ctypes
 import random
 import re
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -353,6 +354,37 @@ def _differences(f, at, grads, step=1e-5):
             lo[i][j] -= step
             hi[i][j] += step
             assert abs((f(*hi) - f(*lo)) / (2 * step) - g[j]) <= 1e-7 * (1 + np.abs(g).max())
+
+
+def _turns_exactly(position, freq):
+    """cos and sin of position * freq for whole positions and f32 frequencies, reduced in fractions with 80 digits of pi."""
+    pi = Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899")
+    turns = np.array([[float((lambda t: t - round(t))(int(p) * Fraction(float(f)) / (2 * pi))) for f in freq] for p in position])
+    return np.cos(2 * np.pi * turns), np.sin(2 * np.pi * turns)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["halves", "neighbours"])
+def test_heads_of_far_positions_and_of_fast_pairs(layout):
+    """Every 32-bit position is exact, at frequencies from 1e-4 to 2e4. A cosine is off by its argument's rounding, an ulp and a half of the polynomial
+    and the rounding of the reduced angle, 4 steps of 2^-24; two products and a sum are 3 more."""
+    position = np.array([2 ** 31 - 1, -2 ** 31, 2 ** 31 - 2, 2 ** 30 + 12345, -1999999999, 123456789, 16777217, -99999, 1, 0], np.int32)
+    freq = np.float32([1, 0.7, 0.999, 0.1, 1e-4, 3.3, 10, 100.1, 1000.7, 19999.9])
+    rng = np.random.default_rng(4)
+    q, k = (rng.standard_normal((10, h, 22)).astype(np.float32) for h in (3, 1))
+    c, s = (x[:, None] for x in _turns_exactly(position, freq))
+    say(f"far positions {layout}")
+    got = hip_run(_heads_program(10, 3, 1, 22, 10, 0, layout, "f32", False), [q, k, position, freq])
+    back = hip_run(_grad_program(10, 3, 1, 22, 10, 0, layout, "f32", False), [q, k, q, k, position, freq])
+    for x, there, here in zip((q, k), got, back):
+        x = x.astype(np.float64)
+        a, b = _pairs(x, 10, layout)
+        size = np.abs(a) + np.abs(b)
+        for y, sign in ((there, 1), (here, -1)):
+            ya, yb = _pairs(y.astype(np.float64), 10, layout)
+            assert_within(ya, a * c - sign * b * s, 7 * E24 * size, "first of a pair")
+            assert_within(yb, b * c + sign * a * s, 7 * E24 * size, "second of a pair")
+            assert np.array_equal(y[..., 20:], x[..., 20:].astype(np.float32))
 
 
 @pytest.mark.gpu
