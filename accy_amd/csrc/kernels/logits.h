@@ -96,6 +96,9 @@ __device__ __forceinline__ void opaque(u32x4& w) {
   }
 }
 
+// What a chunk makes of these is there before the next chunk begins: the compiler would begin with all of a row's chunks, and put some aside in memory.
+__device__ __forceinline__ void in_order(float& a, float& b, float& c, float& d) { asm("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d)); }
+
 // y = (x - base) log2 e as one multiply-add an element, x L2E - base L2E, takes base L2E rounded, and is off by that rounding, the same for all
 // elements of a thread: rest_of(base), which is itself a number. A thread's sums are of such y's, and the rest leaves them where the threads' are
 // joined. From FAR on it is beyond 1: there it is none, and y is formed from x - base.
@@ -159,10 +162,11 @@ template <class C> __device__ __forceinline__ bool add(Sums& a, const u32x4 (&w)
   top = -__builtin_inff();
   if (n <= 0) return false;
   if (a.l == 0.0f) a.m = largest<C>(w[0]);
-  const float base = base_of(a.m), from = base * L2E;
-  float v[Chunks<C>::PER], dl = 0.0f, ds = 0.0f;
+  const float base = base_of(a.m);
+  float v[Chunks<C>::PER], dl = 0.0f, ds = 0.0f, from = base * L2E;
   each<C::U>([&](auto u) {
     if (u.value >= n) return;
+    if constexpr (C::U > 4) in_order(from, dl, ds, top);
     widen<C>(w[u.value], v);
 #pragma unroll
     for (int i = 0; i < Chunks<C>::PER; ++i) top = fmaxf(top, v[i]);
@@ -177,14 +181,13 @@ template <class C> __device__ __forceinline__ bool add(Sums& a, const u32x4 (&w)
   if (care) {
     asm volatile("");  // (a branch: computed either way it would cost as much again)
     if (top > a.m) a.rebase(top, rest_of(top) - rest_of(base_of(a.m)));
-    float base = base_of(a.m);
-    const float rest = rest_of(base);
+    float base = base_of(a.m), rest = rest_of(base);
     dl = ds = 0.0f;
     each<C::U>([&](auto u) {
       if (u.value >= n) return;
       u32x4 again = w[u.value];
+      if constexpr (C::U > 4) in_order(base, dl, ds, rest);
       if constexpr (C::DT != 2) opaque(again);
-      asm("" : "+v"(base), "+v"(dl), "+v"(ds));  // (chunk after chunk: f32 rows of 13 fill the registers otherwise)
       widen<C>(again, v);
 #pragma unroll
       for (int i = 0; i < Chunks<C>::PER; ++i) {

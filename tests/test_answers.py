@@ -663,6 +663,27 @@ def test_the_gradient_of_a_row_does_not_depend_on_how_many_there_are(shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,dtype", [(65536, "f16"), (90103, "bf16"), (106496, "f16"), (131072, "bf16"), (131063, "f16"), (65531, "f32"), (151936, "bf16"), (180215, "f16"), (90112, "f32"), (200001, "bf16")])
+def test_log_probs_gradient_of_long_rows(n, dtype):
+    """Rows that fill a workgroup's registers, whole chunks and not, and longer ones: four different rows 64 times over, each the same wherever it lies."""
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((4, n)) * 2.5
+    x[1, ::3], x[2] = -np.inf, x[2] + 300
+    x = floats(x, dtype)
+    tokens, a, h = np.array([n - 1, 4, 0, -1], np.int32), *(rng.standard_normal(4).astype(np.float32) for _ in range(2))
+    spec = [T.spec(dtype, row=256, vocab=n), T.spec("i32", row=256), *[T.spec("f32", row=256)] * 2]
+    say(f"gradient 256 {n} {dtype}")
+    got = hip_run(T.define("grad", spec, lambda b, v: v[0].log_probs_grad(*v[1:], "vocab")), [np.tile(v, (64, 1)[:v.ndim]) for v in (x, tokens, a, h)])[0].reshape(64, 4, n)
+    v = wide(x, dtype)
+    want, size = _grad_logits_want(v, tokens, a.astype(np.float64), h.astype(np.float64))
+    tol = HALF_STEP[dtype] * np.abs(want) + 8 * (_steps_of_weight(v) * (2 + np.log(n + 1)))[:, None] * size + (2.0 ** -25 if dtype == "f16" else 1e-37)
+    # (a row's place decides which of its elements are whole chunks': eight rows on, the same again)
+    for first in (0, 1):
+        assert_within(wide(got[first], dtype), want, tol, "gradient")
+        assert (got[first] == got[first::2]).all()
+
+
+@pytest.mark.gpu
 def test_log_probs_without_rows_and_of_a_vector():
     got = hip_run(T.define("p", [T.spec("f32", row=0, vocab=9), T.spec("i32", row=0)], lambda b, a: a[0].log_probs(a[1], "vocab", top=2).top), [np.zeros((0, 9), np.float32), np.zeros(0, np.int32)])[0]
     assert got.shape == (0, 2)
