@@ -50,9 +50,9 @@ def test_log_probabilities_use_no_scratch(tmp_path):
                 [_logits_grad(*s, d) for s in ((1001, 50257), (300, 1031), (8, 50257), (512, 65500)) for d in ("bf16", "f16", "f32")], tmp_path)
 
 
-@pytest.mark.parametrize("chunks", [8, 11, 13, 16])
+@pytest.mark.parametrize("chunks", [8, 11, 13, 16, 17, 19, 22])
 def test_the_gradient_of_rows_that_fill_the_registers_uses_no_scratch(tmp_path, chunks):
-    """Rows of 8 to 16 chunks of 16 bytes for each of 1024 threads, whole ones and such that start anywhere, in the registers of one workgroup."""
+    """Rows of 8 to 22 chunks of 16 bytes for each of 1024 threads, whole ones and such that start anywhere, in the registers of one workgroup."""
     used = _no_scratch([_logits_grad(300, chunks * 1024 * per - less, d) for d, per in (("bf16", 8), ("f16", 8), ("f32", 4)) for less in (0, per + 1)], tmp_path)
     assert [label for label, _ in used] == ["log_probs_grad"] * 6
 
