@@ -156,11 +156,11 @@ __device__ __forceinline__ Sums sums_of(float x) {
 }
 // The first n of U chunks added to the sums; `top` becomes their maximum. They are widened once: y is measured from the m that there is, that of the
 // first chunk to begin with. Where an element lies 32 above it (or it is that of nothing but masked elements), or m is far from 0, they are added
-// again with care. Returns whether they were. (Masked elements cost one
+// again with care. (Masked elements cost one
 // maximum each; when they made the batch one to be added again, 2048 x 50257 bf16, a third of every seventh row masked, took 66 us instead of 61.)
-template <class C> __device__ __forceinline__ bool add(Sums& a, const u32x4 (&w)[C::U], int n, float& top) {
+template <class C> __device__ __forceinline__ void add(Sums& a, const u32x4 (&w)[C::U], int n, float& top) {
   top = -__builtin_inff();
-  if (n <= 0) return false;
+  if (n <= 0) return;
   if (a.l == 0.0f) a.m = largest<C>(w[0]);
   const float base = base_of(a.m);
   float v[Chunks<C>::PER], dl = 0.0f, ds = 0.0f, from = base * L2E;
@@ -177,8 +177,7 @@ template <class C> __device__ __forceinline__ bool add(Sums& a, const u32x4 (&w)
       ds = __builtin_fmaf(e, fmaxf(y, LEAST), ds);
     }
   });
-  const bool care = is_far(base) || top - a.m > 32.0f;
-  if (care) {
+  if (is_far(base) || top - a.m > 32.0f) {
     asm volatile("");  // (a branch: computed either way it would cost as much again)
     if (top > a.m) a.rebase(top, rest_of(top) - rest_of(base_of(a.m)));
     float base = base_of(a.m), rest = rest_of(base);
@@ -199,7 +198,6 @@ template <class C> __device__ __forceinline__ bool add(Sums& a, const u32x4 (&w)
   }
   a.l += dl;
   a.s += ds;
-  return care;
 }
 
 // The order of values, in the order of unsigned numbers: +0 and -0 are one, NaN is below all.
@@ -236,9 +234,8 @@ template <class C> struct List {
   }
 };
 
-// The threads' sums, and whether any of them took care: the same in all of them.
-// peak: a thread's maximum.
-template <int WAVES> __device__ __forceinline__ Sums join_threads(Sums a, float peak, bool& care, float (&lds)[WAVES][4]) {
+// The threads' sums: the same in all of them. peak: a thread's maximum.
+template <int WAVES> __device__ __forceinline__ Sums join_threads(Sums a, float peak, float (&lds)[WAVES][3]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   a.rebase(wave_reduce(peak, MaxOp()), -rest_of(base_of(a.m)));
   a.l = wave_reduce(a.l, SumOp());
@@ -248,15 +245,12 @@ template <int WAVES> __device__ __forceinline__ Sums join_threads(Sums a, float 
     lds[wave][1] = a.l;
     lds[wave][2] = a.s;
   }
-  const bool any = __builtin_amdgcn_ballot_w64(care) != 0;
-  if (lane == 0) lds[wave][3] = any ? 1.0f : 0.0f;
   __syncthreads();
   // A wave's lanes take a wave's sums each.
   const int from = lane % WAVES;
   a.m = lds[from][0];
   a.l = lds[from][1];
   a.s = lds[from][2];
-  care = __builtin_amdgcn_ballot_w64(lds[from][3] != 0.0f) != 0;
   float top = a.m;
 #pragma unroll
   for (int o = 1; o < WAVES; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
@@ -399,9 +393,8 @@ __device__ __forceinline__ Sums scan(const Range<C> r, List<C>& list) {
     __syncthreads();
     list.rank(had);
   }
-  __shared__ float lds[WAVES][4];
-  bool care = false;
-  return join_threads<WAVES>(a, peak, care, lds);
+  __shared__ float lds[WAVES][3];
+  return join_threads<WAVES>(a, peak, lds);
 }
 
 // What a row's outputs are made of.
@@ -504,12 +497,6 @@ __device__ __forceinline__ void log_probs_join(const typename Elem<C::DT>::type*
 template <class C> struct Slope {
   float base, a, b, g;
   int at;                      // the token's element counted as a Range's, or -1
-  // For y's with the rest of the base: what it adds leaves A and 2^y.
-  __device__ __forceinline__ void with_rest() {
-    const float rest = rest_of(base), scale = __builtin_amdgcn_exp2f(-rest);
-    a = (a - b * rest) * scale;
-    b *= scale;
-  }
 };
 template <class C>
 __device__ __forceinline__ Slope<C> slope_of(const Sums& s, long row, int lead, const int* __restrict__ tokens, const float* __restrict__ d_token,
@@ -530,19 +517,19 @@ template <int DT> __device__ __forceinline__ typename Elem<DT>::type to_elem(flo
   else if constexpr (DT == 1) return f32_to_f16(v);
   else return v;
 }
-// The gradient at an element. CARE: as in add(); without, the slope is one with_rest().
-template <class C, bool CARE> __device__ __forceinline__ float slope(const Slope<C>& k, float x) {
-  const float y = CARE ? careful(x, k.base, 0.0f) : __builtin_fmaf(x, L2E, -(k.base * L2E));
+// The gradient at an element.
+template <class C> __device__ __forceinline__ float slope(const Slope<C>& k, float x) {
+  const float y = (x - k.base) * L2E;
   return __builtin_amdgcn_exp2f(y) * __builtin_fmaf(k.b, fmaxf(y, LEAST), k.a);
 }
 // The gradient of chunk c's elements.
-template <class C, bool CARE>
+template <class C>
 __device__ __forceinline__ void put(typename Elem<C::DT>::type* __restrict__ to, const Slope<C>& k, int c, const u32x4& w) {
   constexpr int PER = Chunks<C>::PER;
   float v[PER];
   widen<C>(w, v);
 #pragma unroll
-  for (int i = 0; i < PER; ++i) v[i] = slope<C, CARE>(k, v[i]);
+  for (int i = 0; i < PER; ++i) v[i] = slope<C>(k, v[i]);
   if (k.at >= 0 && k.at / PER == c) {
     asm volatile("");
 #pragma unroll
@@ -559,7 +546,7 @@ __device__ __forceinline__ void put(typename Elem<C::DT>::type* __restrict__ to,
   else *at = o;
 }
 template <class C> __device__ __forceinline__ void put_besides(typename Elem<C::DT>::type* __restrict__ to, const Slope<C>& k, int besides, float x) {
-  if (besides >= 0) to[besides] = to_elem<C::DT>(slope<C, true>(k, x) + (besides == k.at ? k.g : 0.0f));
+  if (besides >= 0) to[besides] = to_elem<C::DT>(slope<C>(k, x) + (besides == k.at ? k.g : 0.0f));
 }
 
 // A row whose chunks fit the workgroup's registers, U of them a thread: read once, written once.
@@ -567,7 +554,7 @@ template <class C>
 __device__ __forceinline__ void grad_row(const typename Elem<C::DT>::type* __restrict__ x, const int* __restrict__ tokens, const float* __restrict__ d_token,
                                          const float* __restrict__ d_entropy, typename Elem<C::DT>::type* __restrict__ dx) {
   constexpr int WAVES = C::NT / 64;
-  __shared__ float lds[WAVES][4];
+  __shared__ float lds[WAVES][3];
   const long row = blockIdx.x;
   const Range<C> r = range_of<C>(x, row, 0);
   const int first = r.from + (int)threadIdx.x, n = present<C>(first, r.to), besides = r.besides();
@@ -579,19 +566,15 @@ __device__ __forceinline__ void grad_row(const typename Elem<C::DT>::type* __res
     edge = value<C::DT>(r.base[besides]);
     a = sums_of(edge);
   }
-  bool care = add<C>(a, w, n, peak);
+  add<C>(a, w, n, peak);
   if (besides >= 0) peak = fmaxf(peak, edge);
   each<C::U>([&](auto u) { opaque(w[u.value]); });
-  a = join_threads<WAVES>(a, peak, care, lds);
-  Slope<C> k = slope_of<C>(a, row, r.lead, tokens, d_token, d_entropy);
-  care = __builtin_amdgcn_ballot_w64(care || is_far(k.base)) != 0;  // (an edge's; one for all, as it is)
+  a = join_threads<WAVES>(a, peak, lds);
+  const Slope<C> k = slope_of<C>(a, row, r.lead, tokens, d_token, d_entropy);
   typename Elem<C::DT>::type* const to = dx + r.at;
   put_besides<C>(to, k, besides, edge);
-  if (!care) k.with_rest();
   each<C::U>([&](auto u) {
-    if (u.value >= n) return;
-    if (care) put<C, true>(to, k, first + u.value * C::NT, w[u.value]);
-    else put<C, false>(to, k, first + u.value * C::NT, w[u.value]);
+    if (u.value < n) put<C>(to, k, first + u.value * C::NT, w[u.value]);
   });
 }
 
@@ -605,7 +588,7 @@ __device__ __forceinline__ void grad_split(const typename Elem<C::DT>::type* __r
   const Slope<C> k = slope_of<C>(join_sums<C>(part, row), row, r.lead, tokens, d_token, d_entropy);
   typename Elem<C::DT>::type* const to = dx + r.at;
   put_besides<C>(to, k, besides, besides >= 0 ? value<C::DT>(r.base[besides]) : 0.0f);
-  for (int c = r.from + (int)threadIdx.x; c < r.to; c += C::NT) put<C, true>(to, k, c, chunk<C>(r.base, c));
+  for (int c = r.from + (int)threadIdx.x; c < r.to; c += C::NT) put<C>(to, k, c, chunk<C>(r.base, c));
 }
 
 }  // namespace logits

@@ -646,6 +646,20 @@ def test_log_probs_do_not_depend_on_a_shift(n, copies, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(12, 5), (12, 700), (260, 9001), (6, 20011)])
+def test_a_certain_token_has_an_entropy_whose_gradient_is_none(rows, n):
+    """Rows in which one logit lies 1000 above all others, wherever that is: its probability is 1, the entropy 0 and the entropy's gradient none at all."""
+    at = np.arange(rows) % n
+    x = np.resize(np.float32([0, 0.3, 7.1, -300.7, 3000.1, -1e5 - 0.3]), rows)[:, None] - np.full(n, 1000, np.float32)
+    x[np.arange(rows), at] += 1000
+    tokens, zero, h = np.full(rows, -1, np.int32), np.zeros(rows, np.float32), np.linspace(-3, 2, rows).astype(np.float32)
+    spec = [T.spec("f32", row=rows, vocab=n), T.spec("i32", row=rows), *[T.spec("f32", row=rows)] * 2]
+    say(f"certain {rows} {n}")
+    got = hip_run(T.define("grad", spec, lambda b, v: v[0].log_probs_grad(*v[1:], "vocab")), [x, tokens, zero, h])[0]
+    assert not got.any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shift", [0.0, 1e5, -1e7])
 def test_the_gradient_of_a_row_does_not_depend_on_how_many_there_are(shift):
     """One row by itself, in two kernels, and among 300, in one kernel: the same but for roundings."""
