@@ -260,6 +260,8 @@ template <int WAVES> __device__ __forceinline__ Sums join_threads(Sums a, float 
     a.l += __shfl_xor(a.l, o, 64);
     a.s += __shfl_xor(a.s, o, 64);
   }
+  // The maximum's own 2^y is 1: a sum below it is so by its roundings alone, and would make a log probability one above 0.
+  if (a.l > 0.0f && a.l < 1.0f) a.l = 1.0f;
   return a;
 }
 
@@ -402,7 +404,11 @@ __device__ __forceinline__ float log_prob(const Sums& a, float x) {
   if (a.l == 0.0f) return -__builtin_inff();
   return (x - base_of(a.m)) - __builtin_amdgcn_logf(a.l) * LN2;
 }
-__device__ __forceinline__ float entropy(const Sums& a) { return a.l == 0.0f ? 0.0f : (__builtin_amdgcn_logf(a.l) - a.s / a.l) * LN2; }
+// A difference of numbers up to 46 (where a thread's m lies 32 below its maximum): off by some 2^-24 of that, and below 0 for nothing but that.
+__device__ __forceinline__ float entropy(const Sums& a) {
+  const float h = a.l == 0.0f ? 0.0f : (__builtin_amdgcn_logf(a.l) - a.s / a.l) * LN2;
+  return h < 0.0f ? 0.0f : h;
+}
 
 template <class C>
 __device__ __forceinline__ void write(const typename Elem<C::DT>::type* __restrict__ x, const int* __restrict__ tokens, long row, const Sums& a,

@@ -660,6 +660,26 @@ def test_a_certain_token_has_an_entropy_whose_gradient_is_none(rows, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,n", [(600, 20011), (9, 9001), (600, 70)])
+def test_entropies_of_peaked_rows(rows, n, dtype):
+    """One logit 12 to 40 above the others: entropies near 0, none below, and no log probability above 0. A thread's sum of 2^y y may be of y up to 46, from an m 32 lower in units of log 2: the
+    sum's roundings, one of y, three where it is measured from another maximum, and log2 l's, are 2^-24 of that each, times ln 2."""
+    rng = np.random.default_rng(rows + n)
+    x = rng.standard_normal((rows, n)) * 2.5
+    x[np.arange(rows), rng.integers(0, n, rows)] = x.max(-1) + rng.uniform(12, 40, rows)
+    x = floats(x, dtype)
+    tokens = np.zeros(rows, np.int32)
+    say(f"peaked {rows} {n} {dtype}")
+    got, top = hip_run(T.define("p", [T.spec(dtype, row=rows, vocab=n), T.spec("i32", row=rows)],
+                                lambda b, a: [v for p in [a[0].log_probs(a[1], "vocab", top=1)] for v in (p.entropy, p.top)]), [x, tokens])
+    _, want, logp = _log_probs_want(wide(x, dtype), tokens)
+    assert (got >= 0).all() and (top <= 0).all()
+    assert_within(top[:, 0], logp.max(-1), _steps_of_weight(wide(x, dtype)) + 2 * E24 * np.abs(logp.max(-1)), "top")
+    assert_within(got, want, 6 * 46 * E24 * np.log(2) + 2 * E24 * want, "entropy")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shift", [0.0, 1e5, -1e7])
 def test_the_gradient_of_a_row_does_not_depend_on_how_many_there_are(shift):
     """One row by itself, in two kernels, and among 300, in one kernel: the same but for roundings."""
