@@ -1167,3 +1167,70 @@ def test_answers_step_captured_into_hip_graphs(scratch, in_place):
         for h in handles:
             s.release(h)
         stream.destroy()
+
+
+def _training_programs():
+    """Gradients of heads and of logits in both of their forms, and pages moved, copied in any order and twice to one page."""
+    rng = np.random.default_rng(12)
+    heads = _heads_specs(300, 3, 2, 48, 16, 2, "bf16", True)
+    logits = lambda rows, n, dtype: [T.spec(dtype, **{f"r{n}": rows, f"v{n}": n}), T.spec("i32", **{f"r{n}": rows}), *[T.spec("f32", **{f"r{n}": rows})] * 2]  # noqa: E731
+
+    def train(b, a):
+        grads = list(b.rotate_heads_grad(*a[:4], *_operands(b, a[4:9], 2, "neighbours", True, 1e-5)))
+        return grads + [a[9].log_probs_grad(*a[10:13], "v700"), a[13].log_probs_grad(*a[14:17], "v20011"), a[13].log_probs(a[14], "v20011", top=3).top]
+    q, k, position, freq, axis, gain = _heads_inputs(300, 3, 2, 48, 16, 2, "bf16", "bf16", rng)
+    ins = [q[::-1].copy(), k[::-1].copy(), q, k, position, freq, axis, *gain]
+    for rows, n, dtype in ((270, 700, "f16"), (3, 20011, "f32")):
+        ins += [floats(rng.standard_normal((rows, n)) * 2, dtype), rng.integers(0, n, rows).astype(np.int32), *(rng.standard_normal(rows).astype(np.float32) for _ in range(2))]
+    yield T.define("train", heads[:2] + heads + logits(270, 700, "f16") + logits(3, 20011, "f32"), train), ins
+    table, held = rng.integers(-1, 900, (70, 64)).astype(np.int32), rng.random(900) < 0.1
+    cache, lists = rng.integers(0, 256, (900, 3, 40)).astype(np.uint8), [rng.integers(-1, 901, n).astype(np.int32) for n in (50, 50, 5000, 5000)]
+
+    def pages(b, a):
+        c = b.compact_pages(a[0], a[1], ("move", 300))
+        return [c.pages, c.source, c.target, a[2].copy_pages(c.source, c.target).copy_pages(a[3], a[4]).copy_pages(a[5], a[6])]
+    yield T.define("pages", [T.spec("i32", seq=70, slot=64), T.spec("i1", page=900), T.spec("u8", page=900, r=3, c=40),
+                             *[T.spec("i32", **{f"copy{len(x)}": len(x)}) for x in lists]], pages), [table, held, cache, *lists]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scratch", [False, True])
+def test_gradients_and_moved_pages_captured_into_hip_graphs(scratch):
+    """Two programs captured and replayed in turn on one stream, each run eagerly on another between its replays."""
+    rt, s, stream, other = _hip_runtime(), hip.Session(), hip.Stream(), hip.Stream()
+    progs = list(_training_programs())
+    refs = [hip_run(*p) for p in progs]
+    table, held, cache, *lists = progs[1][1]
+    moved = compact_want(table, held, 300)
+    want = copied(copied(copied(cache, *moved[1:]), *lists[:2]), *lists[2:])
+    assert all(np.array_equal(g, w) for g, w in zip(refs[1], (*moved, want)))
+    handles, bounds, graphs, exes = [s.compile(p) for p, _ in progs], [_Bound(*p) for p in progs], [], []
+    try:
+        for h, bound, ref in zip(handles, bounds, refs):
+            bound.call(h, scratch, stream)
+            stream.synchronize()
+            _same(bound.read(), ref)
+            graphs.append(_capture(rt, stream, lambda: bound.call(h, scratch, stream)))
+            exes.append(ctypes.c_void_p())
+            assert rt.hipGraphInstantiate(ctypes.byref(exes[-1]), graphs[-1], None, None, 0) == 0
+        for r in range(3):
+            for i in (0, 1):
+                say(f"replay {r} of {i}, scratch={scratch}")
+                bounds[i].clear()
+                assert rt.hipGraphLaunch(exes[i], ctypes.c_void_p(stream.handle)) == 0
+                stream.synchronize()
+                _same(bounds[i].read(), refs[i])
+                bounds[i].clear()
+                bounds[i].call(handles[i], scratch, other)
+                other.synchronize()
+                _same(bounds[i].read(), refs[i])
+        for exe, graph in zip(exes, graphs):
+            rt.hipGraphExecDestroy(exe)
+            rt.hipGraphDestroy(graph)
+    finally:
+        for b in bounds:
+            b.free()
+        for h in handles:
+            s.release(h)
+        stream.destroy()
+        other.destroy()
