@@ -4,8 +4,8 @@
 // l) ln 2. One pass over the row gives l, s and the alternatives: each thread measures from an m of its own, the maximum of its first chunk,
 // and the threads' (m, l, s) are joined at the end, measured from the row's maximum. That is a conversion, half a maximum, a multiply-add, an
 // exponential and two more operations an element, more than HBM delivers one in; so the alternatives have to come almost free
-// (2048 x 50257 bf16 55-58 us, 3.7 TB/s, with 20 alternatives, 49 with one; 8 x 32000 f32 in 31 parts a row 5.7 us of kernel and 6.1 of the parts' join). The
-// gradient reads a row once and writes it: 1001 x 50257 f16 48 us, 4.2 TB/s.
+// (2048 x 50257 bf16 55-58 us, 3.7 TB/s, with 20 alternatives, 49 with one; 8 x 32000 f32 in 31 parts a row 5.2 us of kernel and 6.4 of the parts' join). The
+// gradient reads a row once and writes it: 1001 x 50257 f16 47 us, 4.3 TB/s.
 //
 // Alternatives: an element is compared with a bound below the row's K-th largest only where its batch's maximum reaches the bound. After the first
 // batch each wave takes the largest bound that a quarter (its share of K) of its lanes' maxima reach, and the least of the waves' bounds stands

@@ -141,7 +141,7 @@ void Planner::logits_grad(uint32_t v) {
     // Rows stay in the registers of one workgroup where there are rows for every CU (or they are short), in as few threads as hold them in eight chunks
     // each: 1001 x 50257 f16 55 us with 1024 threads, 58 with 512, 69 with 256. Other rows are read twice, by several workgroups. 22 chunks are as
     // many as 128 registers hold of every type beside what else they do, and so far one reading is the faster one (us, in registers / read twice: 1024 x
-    // 139264 bf16, 17 chunks, 109 / 180, 1024 x 151936 126 / 199, 300 x 151936 50 / 58, 1024 x 180215 f16 160 / 250, 512 x 69632 f32 52 / 90, 256 x 90107 38 / 55).
+    // 139264 bf16, 17 chunks, 110 / 180, 1024 x 151936 127 / 199, 300 x 151936 51 / 58, 1024 x 180215 f16 160 / 250, 512 x 69632 f32 51 / 90, 256 x 90107 38 / 55).
     int64_t threads = 256;
     while (threads < 1024 && (chunks + threads - 1) / threads > 8) threads *= 2;
     const int64_t u = (chunks + threads - 1) / threads;
