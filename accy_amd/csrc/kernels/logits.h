@@ -114,10 +114,9 @@ struct Sums {
   float m = -__builtin_inff(), l = 0.0f, s = 0.0f;
   // The same measured from another m, with y's that are larger by `more`.
   __device__ __forceinline__ void rebase(float to, float more = 0.0f) {
-#pragma clang fp contract(off)  // (the rest of an element that is alone in its row leaves 0 behind)
     // (a sum of nothing is measured from nothing: its shift may be beyond f32)
     const float shift = l == 0.0f ? 0.0f : fmaxf(careful(base_of(m), base_of(to), more), LEAST), scale = __builtin_amdgcn_exp2f(shift);
-    s = (s + l * shift) * scale;
+    s = (s + l * shift) * scale;  // (no multiply-add: the rest of an element that is alone in its row leaves 0 behind)
     l *= scale;
     m = to;
   }
